@@ -32,6 +32,7 @@ import torch
 from . import _lib
 from ._lib import RasterizerError, on_device as _on, stream_of as _stream
 from .ssim import fused_ssim
+from .tokens import axial_frequencies, axial_rotary, layer_norm, packed_attention
 
 __all__ = [
     "project_points",
@@ -67,6 +68,10 @@ __all__ = [
     "set_blend_waves",
     "check_forward_order",
     "fused_ssim",
+    "layer_norm",
+    "axial_rotary",
+    "axial_frequencies",
+    "packed_attention",
     "RasterizerError",
 ]
 

@@ -86,6 +86,23 @@ class GsGatherTensor(ctypes.Structure):
     _fields_ = [("src", _P), ("dst", _P), ("delta", _P), ("width", _I32), ("zero_fresh", _I32)]
 
 
+class GsRotaryTensor(ctypes.Structure):
+    """include/gs_rasterizer.h GsRotaryTensor."""
+
+    _fields_ = [("x", _P), ("y", _P), ("x_token", _I64), ("x_head", _I64), ("y_token", _I64),
+                ("y_head", _I64), ("heads", _I32)]
+
+
+class GsAttention(ctypes.Structure):
+    """include/gs_rasterizer.h GsAttention."""
+
+    _fields_ = [("rows_q", _I64), ("rows_k", _I64), ("q_row", _I64), ("q_head", _I64),
+                ("k_row", _I64), ("k_head", _I64), ("v_row", _I64), ("v_head", _I64),
+                ("offsets_q", _P), ("offsets_k", _P), ("lengths_k", _P), ("sequences", _I32),
+                ("heads_q", _I32), ("heads_k", _I32), ("dim", _I32), ("type", _I32),
+                ("causal", _I32), ("scale", _F)]
+
+
 SIGNATURES.update({
     "gs_adam_step": [ctypes.POINTER(GsAdamTensor), _I32, ctypes.c_double, ctypes.c_double,
                      ctypes.c_double, _P],
@@ -96,6 +113,17 @@ SIGNATURES.update({
     "gs_ssim_forward": [_P] * 4 + [_I32] * 5 + [_F] + [_P] * 5 + [_F, _P, _P, _SZ, _P],
     "gs_ssim_forward_noalloc": [_P] * 4 + [_I32] * 5 + [_F] + [_P] * 5 + [_F, _P, _P],
     "gs_ssim_backward": [_P] * 5 + [_I32] * 4 + [_F] + [_P] * 3 + [_F, _P, _P, _P],
+    "gs_layer_norm_forward": [_P, _I64, _P, _P, _I64, _I32, _F, _I32, _I32, _P, _P, _P],
+    "gs_layer_norm_backward_workspace_size": [_I64, _I32, _PSZ],
+    "gs_layer_norm_backward": [_P, _I64, _P, _I64, _P, _P, _I64, _I32, _I32, _I32]
+    + [_P] * 4 + [_SZ, _P],
+    "gs_axial_rotary": [ctypes.POINTER(GsRotaryTensor), _I32, _P, _I64, _I32, _P,
+                        ctypes.POINTER(_I32), _I32, _I64, _I32, _I32, _I32, _I32, _P],
+    "gs_attention_forward_workspace_size": [ctypes.POINTER(GsAttention), _PSZ],
+    "gs_attention_forward": [ctypes.POINTER(GsAttention)] + [_P] * 6 + [_SZ, _P],
+    "gs_attention_backward_workspace_size": [ctypes.POINTER(GsAttention), _PSZ],
+    "gs_attention_backward": [ctypes.POINTER(GsAttention)] + [_P] * 6 + [_I64, _I64]
+    + [_P] * 4 + [_SZ, _P],
 })
 
 _lib = None

@@ -676,6 +676,99 @@ int gs_rasterize_work(const int32_t *indexing_offset, const int32_t *gaussian_id
                       float transmittance_threshold, float chi_squared_threshold,
                       uint64_t *visited, uint64_t *composited, hipStream_t stream);
 
+/* ------------------------------------------------------ patch-network operators
+ *
+ * Operators of a network that predicts Gaussians from posed images (tokens are
+ * image patches): layer norm, rotary positions of several axes, attention over
+ * packed sequences.  No counterpart in the reference.  Element types are
+ * GS_F32, GS_F16 and GS_BF16; sums, statistics and gradients of weights are
+ * accumulated in float.  Strides are in elements; the innermost dimension is
+ * contiguous.
+ */
+enum { GS_F32 = 0, GS_F16 = 1, GS_BF16 = 2 };
+enum { GS_POS_I32 = 0, GS_POS_I64 = 1, GS_POS_F32 = 2 };
+enum { GS_MAX_AXES = 4, GS_MAX_HEAD_DIM = 128 };
+
+/*
+ * gs_layer_norm_forward: y = (x - mean) / sqrt(var + eps) * weight + bias over
+ *   each row of `channels` elements; rows x_stride apart, y contiguous.  weight
+ *   and bias (weight_type) may be NULL.  stats, when set, receives (mean,
+ *   1 / sqrt(var + eps)) a row for the backward.
+ * gs_layer_norm_backward: any of grad_x, grad_weight, grad_bias may be NULL;
+ *   what is set is overwritten.  The weight's gradients are summed over the rows
+ *   in an order that depends on the sizes alone.
+ */
+int gs_layer_norm_forward(const void *x, int64_t x_stride, const void *weight, const void *bias,
+                          int64_t rows, int32_t channels, float eps, int32_t type,
+                          int32_t weight_type, void *y, float *stats, hipStream_t stream);
+int gs_layer_norm_backward_workspace_size(int64_t rows, int32_t channels, size_t *bytes);
+int gs_layer_norm_backward(const void *grad_y, int64_t grad_y_stride, const void *x,
+                           int64_t x_stride, const void *weight, const float *stats, int64_t rows,
+                           int32_t channels, int32_t type, int32_t weight_type, void *grad_x,
+                           void *grad_weight, void *grad_bias, void *workspace,
+                           size_t workspace_bytes, hipStream_t stream);
+
+/* One tensor of gs_axial_rotary: `heads` heads a token, read at x and written at y (y == x with
+ * the same strides turns it in place; otherwise the two must not overlap). */
+typedef struct {
+    const void *x;
+    void *y;
+    int64_t x_token, x_head, y_token, y_head; /* strides, elements */
+    int32_t heads;
+} GsRotaryTensor;
+
+/*
+ * gs_axial_rotary: turns pair p of every head of token t by the angle
+ *   positions[t][axis(p)] * frequencies[p], times -1 when inverse is set (the
+ *   gradient's pass).  sections (host memory, `axes` entries) gives how many of
+ *   the P = sum(sections) pairs go to each axis, in order; a pair is elements
+ *   (p, p + P) of a head, or (2 p, 2 p + 1) when interleaved.  Elements from 2 P
+ *   to dim are copied.  positions rows are position_stride apart.
+ */
+int gs_axial_rotary(const GsRotaryTensor *tensors, int32_t n_tensors, const void *positions,
+                    int64_t position_stride, int32_t position_type, const float *frequencies,
+                    const int32_t *sections, int32_t axes, int64_t tokens, int32_t dim,
+                    int32_t type, int32_t interleaved, int32_t inverse, hipStream_t stream);
+
+/*
+ * Attention over packed sequences.  Sequence b has the queries offsets_q[b] to
+ * offsets_q[b + 1] of q and the keys from offsets_k[b] to offsets_k[b + 1] of k
+ * and v, or only the first lengths_k[b] of these where lengths_k is set (a cache
+ * that is not full).  Offsets and lengths are device memory, rise from at least
+ * 0 and are clamped to the tensors' rows.  heads_q is a multiple of heads_k:
+ * query head h reads key head h / (heads_q / heads_k).  causal: query i of a
+ * sequence's Lq sees keys j <= i + Lk - Lq, else every key.  A query that sees
+ * no key, and a row of no sequence, has output 0 and log-sum -infinity, and
+ * sends no gradient.
+ * dim is a multiple of 8 and at most GS_MAX_HEAD_DIM, type GS_F16 or GS_BF16;
+ * q, k, v and grad_out are 16-byte aligned with strides that are multiples of 8
+ * (GS_ERR_UNSUPPORTED otherwise).  Outputs are contiguous (rows, heads, dim).
+ */
+typedef struct {
+    int64_t rows_q, rows_k;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head; /* strides, elements */
+    const int32_t *offsets_q, *offsets_k, *lengths_k;
+    int32_t sequences, heads_q, heads_k, dim, type, causal;
+    float scale;
+} GsAttention;
+
+/*
+ * gs_attention_forward: out = softmax(scale q k^T) v; log_sum, when set, receives
+ *   the natural logarithm of each softmax's denominator, (rows_q, heads_q).
+ * gs_attention_backward: gradients of q, k and v from out, log_sum and grad_out;
+ *   every row is written.  Deterministic: no atomics.
+ */
+int gs_attention_forward_workspace_size(const GsAttention *a, size_t *bytes);
+int gs_attention_forward(const GsAttention *a, const void *q, const void *k, const void *v,
+                         void *out, float *log_sum, void *workspace, size_t workspace_bytes,
+                         hipStream_t stream);
+int gs_attention_backward_workspace_size(const GsAttention *a, size_t *bytes);
+int gs_attention_backward(const GsAttention *a, const void *q, const void *k, const void *v,
+                          const void *out, const float *log_sum, const void *grad_out,
+                          int64_t grad_out_row, int64_t grad_out_head, void *grad_q, void *grad_k,
+                          void *grad_v, void *workspace, size_t workspace_bytes,
+                          hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
