@@ -1,0 +1,231 @@
+// What the attention kernels share: sequences in packed rows, tiles of rows in LDS,
+// and matrix products over them.
+//
+// A tile holds rows of one head, DIM elements each (the head's dimension rounded up,
+// zeros behind it), in 16-byte chunks.  It is read two ways: along a row, 8 elements
+// a lane, as an operand that contracts over the dimension; and down the rows, 4 rows
+// a lane, by the LDS's transposed read, as one that contracts over the rows.  The
+// chunks of a row are permuted by an exclusive or with a function of the row, so that
+// eight lanes at a time meet all 64 banks either way.
+//
+// Products are v_mfma_f32_32x32x16: lane l gives column l % 32 of an operand and 8 of
+// its 16 contracted places (half l / 32); of the 32x32 result it holds column l % 32
+// and the rows (r & 3) + 8 (r >> 2) + 4 (l / 32).  A result is used again as an operand
+// without leaving its lane: registers 8 s to 8 s + 7 hold 8 of the rows 16 s to
+// 16 s + 15, and the other operand is read in the same order of rows.
+#pragma once
+
+#include "element.h"
+
+namespace gs {
+
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+using i16x4 = __attribute__((ext_vector_type(4))) short;
+template <typename T>
+struct Vec {
+    using x2 = __attribute__((ext_vector_type(2))) T;
+    using x4 = __attribute__((ext_vector_type(4))) T;
+    using x8 = __attribute__((ext_vector_type(8))) T;
+};
+typedef __attribute__((address_space(3))) char lds_char;
+
+__device__ __forceinline__ f32x16 mfma(Vec<bf16>::x8 a, Vec<bf16>::x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(Vec<f16>::x8 a, Vec<f16>::x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// Rounds to nearest even.
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::x8 pack8(const float *v) {
+    typename Vec<T>::x8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (T)v[i];
+    return r;
+}
+
+// The sum and the maximum of a column's two halves, in both.
+__device__ __forceinline__ float half_sum(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_bit_cast(float, (uint32_t)s[0]) + __builtin_bit_cast(float, (uint32_t)s[1]);
+}
+__device__ __forceinline__ float half_max(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)s[0]),
+                 __builtin_bit_cast(float, (uint32_t)s[1]));
+}
+
+// Row of a 32x32 result that a lane of half h holds in register r.
+__device__ __forceinline__ constexpr int result_row(int r, int h) {
+    return (r & 3) + 8 * (r >> 2) + 4 * h;
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// ---------------------------------------------------------------- sequences
+// Sequence s = 1 .. sequences; 0 and sequences + 1 hold the rows before the first
+// offset and after the last, and have no keys, so that every row is in one.  Offsets
+// are clamped to the tensors, whatever they say.
+__device__ __forceinline__ int clamp_row(int64_t v, int64_t low, int64_t high) {
+    return (int)(v < low ? low : v > high ? high : v);
+}
+
+__device__ __forceinline__ int2 rows_of(const int32_t *offsets, int sequences, int64_t rows, int s) {
+    int2 r;
+    r.x = s == 0 ? 0 : clamp_row(offsets[s - 1], 0, rows);
+    r.y = s > sequences ? (int)rows : clamp_row(offsets[s], r.x, rows);
+    return r;
+}
+
+struct Span {
+    int q0, lq;  // first query row, number of queries
+    int k0, lk;  // first key row, number of keys that count
+    int k1;      // end of the key rows
+};
+
+__device__ __forceinline__ Span span_of(const GsAttention &a, int s) {
+    const int2 q = rows_of(a.offsets_q, a.sequences, a.rows_q, s);
+    const int2 k = rows_of(a.offsets_k, a.sequences, a.rows_k, s);
+    Span p;
+    p.q0 = uniform(q.x);
+    p.lq = uniform(q.y - q.x);
+    p.k0 = uniform(k.x);
+    p.k1 = uniform(k.y);
+    int n = s == 0 || s > a.sequences ? 0 : k.y - k.x;
+    if (n > 0 && a.lengths_k) n = clamp_row(a.lengths_k[s - 1], 0, n);
+    p.lk = uniform(n);
+    return p;
+}
+
+// The sequence and the tile in it of a launch's tile number, tiles of `size` units,
+// `units` units a row; counted from the back, so that the tiles that see most under a
+// causal mask start first.  Every lane of a wave calls it.  False: no such tile.
+__device__ __forceinline__ bool find_tile(const int32_t *offsets, int sequences, int64_t rows,
+                                          int units, int size, int number, int *sequence,
+                                          int *tile) {
+    const int lane = __lane_id(), all = sequences + 2;
+    int total = 0, sum = 0;
+    for (int first = 0; first < all; first += kWave) {
+        const int s = first + lane;
+        int n = 0;
+        if (s < all) {
+            const int2 r = rows_of(offsets, sequences, rows, s);
+            n = (int)(((int64_t)(r.y - r.x) * units + size - 1) / size);
+        }
+        sum = n;
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const int t = __shfl_up(sum, o, kWave);
+            if (lane >= o) sum += t;
+        }
+        total += __shfl(sum, kWave - 1, kWave);
+    }
+    int want = total - 1 - number;
+    if (want < 0) return false;
+    // `sum` holds the last group's running count; the groups before it are counted again
+    for (int first = 0; first < all; first += kWave) {
+        if (all > kWave) {
+            const int s = first + lane;
+            int n = 0;
+            if (s < all) {
+                const int2 r = rows_of(offsets, sequences, rows, s);
+                n = (int)(((int64_t)(r.y - r.x) * units + size - 1) / size);
+            }
+            sum = n;
+#pragma unroll
+            for (int o = 1; o < kWave; o <<= 1) {
+                const int t = __shfl_up(sum, o, kWave);
+                if (lane >= o) sum += t;
+            }
+        }
+        const uint64_t after = __ballot(sum > want);
+        if (after) {
+            const int l = __ffsll((unsigned long long)after) - 1;
+            const int before = l ? __shfl(sum, l - 1, kWave) : 0;
+            *sequence = uniform(first + l);
+            *tile = uniform(want - before);
+            return true;
+        }
+        want -= __shfl(sum, kWave - 1, kWave);
+    }
+    return false;
+}
+
+// -------------------------------------------------------------------- tiles
+template <typename T, int DIM, int ROWS, int WAVES>
+struct Tile {
+    static constexpr int kChunks = DIM / 8;                      // of a row
+    static constexpr int kBytes = ROWS * DIM * 2;
+    static constexpr int kCopies = ROWS * kChunks / (64 * WAVES);  // a wave's, 1 KiB each
+    static_assert(ROWS * kChunks % (64 * WAVES) == 0, "whole waves of chunks");
+    using x8 = typename Vec<T>::x8;
+
+    // Row r's chunk c lies at chunk c ^ swizzle(r); the same for row r + 8.
+    static __device__ __forceinline__ constexpr int swizzle(int r) {
+        return DIM == 128 ? (r & 7) << 1
+               : DIM == 64 ? ((r >> 1) & 3) << 1
+                           : (r >> 2) & 1;
+    }
+
+    // Byte offsets, from the tile's first row in memory, of the chunks that this lane
+    // copies; past every bound where the chunk lies behind the dimension.
+    struct Copy {
+        uint32_t from[kCopies];
+    };
+    static __device__ __forceinline__ Copy copy_of(int wave, int64_t stride, int dim) {
+        Copy c;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int at = (i * WAVES + wave) * 64 + __lane_id();
+            const int row = at / kChunks, chunk = (at % kChunks) ^ swizzle(row);
+            c.from[i] = chunk * 8 < dim ? (uint32_t)(row * (int)stride + chunk * 8) * 2u
+                                        : 0x80000000u;
+        }
+        return c;
+    }
+
+    // Starts this wave's part of the copy of `rows` rows (the rest become zeros) into
+    // LDS.  The descriptor's bound ends behind the last row: what lies past it is
+    // read as zeros, and not touched.
+    static __device__ __forceinline__ void start(const Copy &c, int wave, const T *first,
+                                                 int64_t stride, int rows, int dim,
+                                                 lds_char *tile) {
+        const int n = rows < ROWS ? rows : ROWS;
+        const int bytes = n > 0 ? ((n - 1) * (int)stride + dim) * 2 : 0;
+        const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)first, 0, bytes, 0x00027000);
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                from, (__attribute__((address_space(3))) void *)(tile + (i * WAVES + wave) * 1024),
+                16, c.from[i], 0, 0, 0);
+    }
+
+    // Operand that contracts over the dimension: row `base` + l % 32, places 16 s + 8 (l / 32).
+    static __device__ __forceinline__ x8 along(const lds_char *tile, int base, int s) {
+        const int l = __lane_id(), row = l & 31;
+        const int chunk = (2 * s + (l >> 5)) ^ swizzle(row);
+        return *(const __attribute__((address_space(3))) x8 *)(tile + base * DIM * 2 +
+                                                                row * DIM * 2 + chunk * 16);
+    }
+
+    // Operand that contracts over rows base .. base + 15 in the order of a result's
+    // registers: column 32 d + l % 32, rows base + 4 (l / 32) + 0..3 and + 8..11.
+    static __device__ __forceinline__ x8 down(const lds_char *tile, int base, int d) {
+        const int l = __lane_id();
+        const int row = 4 * (l >> 5) + ((l & 15) >> 2);
+        const int chunk = (4 * d + ((l >> 4) & 1) * 2 + ((l & 3) >> 1)) ^ swizzle(row);
+        const lds_char *p = tile + base * DIM * 2 + row * DIM * 2 + chunk * 16 + (l & 1) * 8;
+        const int next = 8 * DIM * 2;
+        typedef __attribute__((address_space(3))) i16x4 lds_x4;
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_x4 *)p);
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_x4 *)(p + next));
+        const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_bit_cast(x8, both);
+    }
+};
+
+}  // namespace gs
