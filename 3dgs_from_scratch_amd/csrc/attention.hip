@@ -5,6 +5,7 @@
 // with dk and dv summed over the query heads of a group.  Scores, softmax
 // statistics and sums are in float.
 
+#include <initializer_list>
 #include <type_traits>
 
 #include "attention_tile.h"
@@ -77,28 +78,28 @@ __device__ __forceinline__ bool not_finite(const lds_char *tile, int base, int r
     return __ballot(m >= (std::is_same<T, bf16>::value ? 0x7f80 : 0x7c00)) != 0;
 }
 
-// acc += V^T P^T over `groups` groups of 16 keys where V holds infinities or NaN that some
-// columns do not see: a key at a time, added to the columns that see it.  last: the last key
-// a column sees, from `base`.
-template <typename T, int DIM, typename VTile>
+// acc += X^T P over `groups` groups of 16 rows of a tile X that holds infinities or NaN in
+// rows that some columns do not see: a row at a time, added where `sees` says so.
+template <typename T, int DIM, typename XTile, typename Sees>
 __device__ __forceinline__ void add_seen(f32x16 *acc, const lds_char *tile, int base,
-                                         const typename Vec<T>::x8 *p, int groups, int last) {
+                                         const typename Vec<T>::x8 *p, int groups, Sees sees) {
     const int half = __lane_id() >> 5;
 #pragma unroll 1
-    for (int key = 0; key < 16 * groups; ++key) {
-        const int g = key >> 4;
+    for (int row = 0; row < 16 * groups; ++row) {
+        const int g = row >> 4;
         const auto only = [&](typename Vec<T>::x8 x) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (result_row(j, half) != (key & 15)) x[j] = (T)0.0f;
+                if (result_row(j, half) != (row & 15)) x[j] = (T)0.0f;
             return x;
         };
         const auto weights = only(g == 0 ? p[0] : g == 1 ? p[1] : g == 2 ? p[2] : p[3]);
+        const bool seen = sees(base + row);
 #pragma unroll
         for (int d = 0; d < DIM / 32; ++d) {
-            const f32x16 one = mfma(only(VTile::down(tile, base + 16 * g, d)), weights, f32x16{});
+            const f32x16 one = mfma(only(XTile::down(tile, base + 16 * g, d)), weights, f32x16{});
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[d][r] += key <= last ? one[r] : 0.0f;
+            for (int r = 0; r < 16; ++r) acc[d][r] += seen ? one[r] : 0.0f;
         }
     }
 }
@@ -141,7 +142,7 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
     const int kh = blockIdx.x % a.heads_k, group = a.heads_q / a.heads_k;
     int sequence, number;
     if (!find_tile(a.offsets_q, a.sequences, a.rows_q, group, F::kRows, blockIdx.x / a.heads_k,
-                   &sequence, &number))
+                   true, &sequence, &number))
         return;
     const Span p = span_of(a, sequence);
     const int lane = __lane_id(), half = lane >> 5, wave = uniform(threadIdx.x / kWave);
@@ -249,7 +250,8 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
         }
         if constexpr (kMasks)
             if (split_keys) {
-                add_seen<T, DIM, KTile>(acc, vt, base, weights, 2 * F::kSub, last - key0);
+                add_seen<T, DIM, KTile>(acc, vt, base, weights, 2 * F::kSub,
+                                        [&](int at) { return t * F::kKeys + at <= last; });
                 return;
             }
 #pragma unroll
@@ -367,101 +369,276 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
 }
 
 // ---------------------------------------------------------------- gradients
-__device__ __forceinline__ int sequence_of(const int32_t *offsets, int sequences, int64_t row) {
-    int s = 0;
-    while (s <= sequences && row >= offsets[s]) ++s;
-    return s;
-}
+// Two launches, neither with atomics: the queries' gradients, a workgroup a tile of
+// packed rows as in the forward, which also leaves each row's log-sum (in the exponent
+// of two) and delta for the second; then the keys' and values', a workgroup a tile of
+// keys, over all the queries of all heads of the group.  Scores are computed again in
+// both: seven products in all where one launch with atomics needs five.
+constexpr int kBackRows = 64;             // of a tile in LDS
+constexpr int kBackOwn = 32 * kWaves;     // rows or keys of a workgroup
 
-template <typename T>
-__global__ __launch_bounds__(64) void attention_dq_kernel(
+template <typename T, int DIM>
+__global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
     GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
     const T *__restrict__ out, const float *__restrict__ log_sum, const T *__restrict__ go,
-    int64_t go_row, int64_t go_head, T *__restrict__ dq, float *__restrict__ delta) {
-    const int64_t row = blockIdx.x;
-    const int head = blockIdx.y, kh = head / (a.heads_q / a.heads_k), lane = threadIdx.x;
-    const int s = sequence_of(a.offsets_q, a.sequences, row);
-    const Span p = span_of(a, s);
-    const int64_t keys = p.lk, i = row - p.q0, lq = p.lq;
-    const int64_t seen = a.causal ? clamp_row(i + keys - lq + 1, 0, keys) : keys;
-    const bool one = lane < a.dim, two = lane + 64 < a.dim;
-    const T *qr = q + row * a.q_row + head * a.q_head;
-    const T *gr = go + row * go_row + head * go_head;
-    const int64_t at = row * a.heads_q + head;
-    const float q0 = one ? to_float(qr[lane]) * a.scale : 0.0f;
-    const float q1 = two ? to_float(qr[lane + 64]) * a.scale : 0.0f;
-    const float g0 = one ? to_float(gr[lane]) : 0.0f, g1 = two ? to_float(gr[lane + 64]) : 0.0f;
-    const float d = wave_sum(fmaf(g0, one ? to_float(out[at * a.dim + lane]) : 0.0f,
-                                  g1 * (two ? to_float(out[at * a.dim + lane + 64]) : 0.0f)));
-    if (lane == 0) delta[at] = d;
-    const float l = log_sum[at];
-    float s0 = 0.0f, s1 = 0.0f;
-    for (int64_t j = 0; j < seen && l != -INFINITY; ++j) {
-        const T *kr = k + (p.k0 + j) * a.k_row + kh * a.k_head;
-        const T *vr = v + (p.k0 + j) * a.v_row + kh * a.v_head;
-        const float k0 = one ? to_float(kr[lane]) : 0.0f, k1 = two ? to_float(kr[lane + 64]) : 0.0f;
-        const float w = expf(wave_sum(fmaf(k0, q0, k1 * q1)) - l);
-        const float gp = wave_sum(fmaf(g0, one ? to_float(vr[lane]) : 0.0f,
-                                       g1 * (two ? to_float(vr[lane + 64]) : 0.0f)));
-        const float ds = w * (gp - d);
-        s0 = fmaf(ds, k0, s0);
-        s1 = fmaf(ds, k1, s1);
+    int64_t go_row, int64_t go_head, T *__restrict__ dq, float *__restrict__ row_log,
+    float *__restrict__ row_delta) {
+    using KTile = Tile<T, DIM, kBackRows, kWaves>;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * KTile::kBytes];
+    lds_char *const tiles = (lds_char *)lds;
+
+    const int kh = blockIdx.x % a.heads_k, group = a.heads_q / a.heads_k;
+    int sequence, number;
+    if (!find_tile(a.offsets_q, a.sequences, a.rows_q, group, kBackOwn, blockIdx.x / a.heads_k,
+                   true, &sequence, &number))
+        return;
+    const Span p = span_of(a, sequence);
+    const int lane = __lane_id(), half = lane >> 5, wave = uniform(threadIdx.x / kWave);
+    const int rows = p.lq * group;
+    const int row0 = number * kBackOwn + 32 * wave, row = row0 + (lane & 31);
+    const bool real = row < rows;
+    const int query = (real ? row : rows - 1) / group;
+    const int head = kh * group + (real ? row - query * group : 0);
+    const int64_t at = (int64_t)(p.q0 + query) * a.heads_q + head;
+
+    const int shift = a.causal ? p.lk - p.lq : p.lk;
+    const int last = a.causal ? min(query + shift, p.lk - 1) : p.lk - 1;
+    const int all_see = a.causal ? min(number * kBackOwn / group + shift, p.lk - 1) : p.lk - 1;
+    const int wave_last =
+        a.causal ? min(min(row0 + 31, rows - 1) / group + shift, p.lk - 1) : p.lk - 1;
+    const int block_end = min(number * kBackOwn + kBackOwn, rows) - 1;
+    const int seen = a.causal ? min(block_end / group + shift, p.lk - 1) + 1 : p.lk;
+    const int end_tile = seen > 0 ? (seen + kBackRows - 1) / kBackRows : 0;
+
+    RowOperand<T, DIM> qr, gr;
+    qr.load(real ? q + (int64_t)(p.q0 + query) * a.q_row + (int64_t)head * a.q_head : nullptr,
+            a.dim, false);
+    gr.load(real ? go + (int64_t)(p.q0 + query) * go_row + (int64_t)head * go_head : nullptr,
+            a.dim, false);
+    float delta = 0.0f;
+    {
+        RowOperand<T, DIM> o;
+        o.load(real ? out + at * a.dim : nullptr, a.dim, false);
+#pragma unroll
+        for (int s = 0; s < DIM / 16; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                delta = fmaf(to_float(gr.x[s][i]), to_float(o.x[s][i]), delta);
     }
-    T *dst = dq + at * a.dim;
-    if (one) dst[lane] = from_float<T>(s0 * a.scale);
-    if (two) dst[lane + 64] = from_float<T>(s1 * a.scale);
+    delta = half_sum(delta);
+    // a row that saw nothing has no weights: exp2(x - infinity) = 0
+    const float given = real ? log_sum[at] : -INFINITY;
+    const float log2_sum = given == -INFINITY ? INFINITY : given * kLog2e;
+    if (real && half == 0) {
+        const int64_t to = (int64_t)head * a.rows_q + p.q0 + query;
+        row_log[to] = log2_sum;
+        row_delta[to] = delta;
+    }
+
+    const float c = a.scale * kLog2e;
+    const auto copy_k = KTile::copy_of(wave, a.k_row, a.dim);
+    const auto copy_v = KTile::copy_of(wave, a.v_row, a.dim);
+    const auto fetch = [&](int t) {
+        lds_char *to = tiles + (t & 1) * 2 * KTile::kBytes;
+        const int64_t key = p.k0 + (int64_t)t * kBackRows;
+        KTile::start(copy_k, wave, k + key * a.k_row + kh * a.k_head, a.k_row,
+                     p.lk - t * kBackRows, a.dim, to);
+        KTile::start(copy_v, wave, v + key * a.v_row + kh * a.v_head, a.v_row,
+                     p.lk - t * kBackRows, a.dim, to + KTile::kBytes);
+    };
+
+    f32x16 acc[DIM / 32];
+#pragma unroll
+    for (int d = 0; d < DIM / 32; ++d) acc[d] = f32x16{};
+
+    const auto step = [&](int t, auto masks) {
+        constexpr bool kMasks = decltype(masks)::value;
+        __syncthreads();  // tile t is in LDS, and tile t - 1 has been read
+        if (t + 1 < end_tile) fetch(t + 1);
+        const lds_char *kt = tiles + (t & 1) * 2 * KTile::kBytes, *vt = kt + KTile::kBytes;
+        const int key0 = t * kBackRows;
+        if (kMasks && key0 > wave_last) return;
+        bool split_keys = false;
+        if constexpr (kMasks)
+            if (a.causal) split_keys = not_finite<T, DIM>(kt, 0, kBackRows);
+#pragma unroll
+        for (int n = 0; n < kBackRows / 32; ++n) {
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int i = 0; i < DIM / 16; ++i) s = mfma(KTile::along(kt, 32 * n, i), qr.x[i], s);
+#pragma unroll
+            for (int i = 0; i < DIM / 16; ++i) dp = mfma(KTile::along(vt, 32 * n, i), gr.x[i], dp);
+            float ds[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -log2_sum)) * (dp[r] - delta);
+                if (kMasks && key0 + 32 * n + result_row(r, half) > last) ds[r] = 0.0f;
+            }
+            const typename Vec<T>::x8 x[4] = {pack8<T>(ds), pack8<T>(ds + 8)};
+            if constexpr (kMasks)
+                if (split_keys) {
+                    add_seen<T, DIM, KTile>(acc, kt, 32 * n, x, 2,
+                                            [&](int i) { return key0 + i <= last; });
+                    continue;
+                }
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int d = 0; d < DIM / 32; ++d)
+                    acc[d] = mfma(KTile::down(kt, 32 * n + 16 * g, d), x[g], acc[d]);
+        }
+    };
+    if (end_tile > 0) fetch(0);
+    int t = 0;
+    for (const int whole = min(end_tile, (all_see + 1) / kBackRows); t < whole; ++t)
+        step(t, std::false_type{});
+    for (; t < end_tile; ++t) step(t, std::true_type{});
+    store_columns<T, DIM>(acc, a.scale, real ? dq + at * a.dim : nullptr, a.dim);
 }
 
-template <typename T>
-__global__ __launch_bounds__(64) void attention_dkv_kernel(
+template <typename T, int DIM>
+__global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_kernel(
     GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-    const float *__restrict__ log_sum, const T *__restrict__ go, int64_t go_row, int64_t go_head,
-    const float *__restrict__ delta, T *__restrict__ dk, T *__restrict__ dv) {
-    const int64_t row = blockIdx.x;
-    const int kh = blockIdx.y, group = a.heads_q / a.heads_k, lane = threadIdx.x;
-    const int s = sequence_of(a.offsets_k, a.sequences, row);
-    const Span p = span_of(a, s);
-    const int64_t keys = p.lk, j = row - p.k0, lq = p.lq;
-    int64_t first = a.causal ? j + lq - keys : 0;
-    if (first < 0) first = 0;
-    if (j >= keys) first = lq;
-    const bool one = lane < a.dim, two = lane + 64 < a.dim;
-    const T *kr = k + row * a.k_row + kh * a.k_head, *vr = v + row * a.v_row + kh * a.v_head;
-    const float k0 = one ? to_float(kr[lane]) * a.scale : 0.0f;
-    const float k1 = two ? to_float(kr[lane + 64]) * a.scale : 0.0f;
-    const float v0 = one ? to_float(vr[lane]) : 0.0f, v1 = two ? to_float(vr[lane + 64]) : 0.0f;
-    float dk0 = 0.0f, dk1 = 0.0f, dv0 = 0.0f, dv1 = 0.0f;
-    for (int64_t i = first; i < lq; ++i)
-        for (int g = 0; g < group; ++g) {
-            const int64_t r = p.q0 + i, head = kh * group + g, at = r * a.heads_q + head;
-            const float l = log_sum[at];
-            if (l == -INFINITY) continue;
-            const T *qr = q + r * a.q_row + head * a.q_head;
-            const T *gr = go + r * go_row + head * go_head;
-            const float q0 = one ? to_float(qr[lane]) : 0.0f;
-            const float q1 = two ? to_float(qr[lane + 64]) : 0.0f;
-            const float g0 = one ? to_float(gr[lane]) : 0.0f;
-            const float g1 = two ? to_float(gr[lane + 64]) : 0.0f;
-            const float w = expf(wave_sum(fmaf(k0, q0, k1 * q1)) - l);
-            const float ds = w * (wave_sum(fmaf(g0, v0, g1 * v1)) - delta[at]);
-            dk0 = fmaf(ds, q0, dk0);
-            dk1 = fmaf(ds, q1, dk1);
-            dv0 = fmaf(w, g0, dv0);
-            dv1 = fmaf(w, g1, dv1);
+    const T *__restrict__ go, int64_t go_row, int64_t go_head, const float *__restrict__ row_log,
+    const float *__restrict__ row_delta, T *__restrict__ dk, T *__restrict__ dv) {
+    using QTile = Tile<T, DIM, kBackRows, kWaves>;
+    constexpr int kFloats = kBackRows * 4;                         // bytes of one float a row
+    constexpr int kStage = 2 * QTile::kBytes + 1024;               // Q, dout, log-sums, deltas
+    static_assert(2 * kFloats <= 1024, "a tile's rows");
+    __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+    lds_char *const tiles = (lds_char *)lds;
+
+    const int kh = blockIdx.x % a.heads_k, group = a.heads_q / a.heads_k;
+    int sequence, number;
+    if (!find_tile(a.offsets_k, a.sequences, a.rows_k, 1, kBackOwn, blockIdx.x / a.heads_k, false,
+                   &sequence, &number))
+        return;
+    const Span p = span_of(a, sequence);
+    const int lane = __lane_id(), half = lane >> 5, wave = uniform(threadIdx.x / kWave);
+    const int block_key = number * kBackOwn;
+    const int key = block_key + 32 * wave + (lane & 31);  // in the sequence
+    const bool real = key < p.k1 - p.k0, counts = key < p.lk;
+
+    // queries from `first` on see some key of the workgroup, from `whole` on all of them
+    const int shift = a.causal ? p.lk - p.lq : p.lk;
+    const int end_key = min(block_key + kBackOwn, p.lk);
+    const int first = a.causal ? max(block_key - shift, 0) : 0;
+    const int whole = a.causal ? max(end_key - 1 - shift, 0) : 0;
+    const int first_tile = first / kBackRows;
+    const int end_tile = block_key < p.lk ? (p.lq + kBackRows - 1) / kBackRows : 0;
+    const int per_head = max(end_tile - first_tile, 0), steps = per_head * group;
+    const int own_first = a.causal ? key - shift : 0;  // the first query that sees this key
+
+    const T *key_row = counts ? k + (int64_t)(p.k0 + key) * a.k_row + (int64_t)kh * a.k_head : nullptr;
+    const T *value_row = counts ? v + (int64_t)(p.k0 + key) * a.v_row + (int64_t)kh * a.v_head : nullptr;
+    RowOperand<T, DIM> kr, vr;
+    kr.load(key_row, a.dim, false);
+    vr.load(value_row, a.dim, false);
+
+    const float c = a.scale * kLog2e;
+    const auto copy_q = QTile::copy_of(wave, a.q_row, a.dim);
+    const auto copy_g = QTile::copy_of(wave, go_row, a.dim);
+    const auto fetch = [&](int i, int head, int t) {
+        lds_char *to = tiles + (i & 1) * kStage;
+        const int64_t row = p.q0 + (int64_t)t * kBackRows;
+        const int present = p.lq - t * kBackRows;
+        QTile::start(copy_q, wave, q + row * a.q_row + head * a.q_head, a.q_row, present, a.dim, to);
+        QTile::start(copy_g, wave, go + row * go_row + head * go_head, go_row, present, a.dim,
+                     to + QTile::kBytes);
+        const int64_t f = head * a.rows_q + row;
+        if (wave < 2)
+            QTile::start_floats((wave == 0 ? row_log : row_delta) + f, present,
+                                to + 2 * QTile::kBytes + wave * kFloats);
+    };
+
+    f32x16 gk[DIM / 32], gv[DIM / 32];
+#pragma unroll
+    for (int d = 0; d < DIM / 32; ++d) gk[d] = gv[d] = f32x16{};
+
+    const auto step = [&](int i, int t, auto masks) {
+        constexpr bool kMasks = decltype(masks)::value;
+        const lds_char *qt = tiles + (i & 1) * kStage, *gt = qt + QTile::kBytes;
+        const lds_char *logs = gt + QTile::kBytes, *deltas = logs + kFloats;
+        const int query0 = t * kBackRows;
+        bool split_rows = false;
+        if constexpr (kMasks)
+            split_rows = not_finite<T, DIM>(qt, 0, kBackRows) || not_finite<T, DIM>(gt, 0, kBackRows);
+#pragma unroll kMasks ? 1 : 2
+        for (int n = 0; n < kBackRows / 32; ++n) {
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int j = 0; j < DIM / 16; ++j) s = mfma(QTile::along(qt, 32 * n, j), kr.x[j], s);
+#pragma unroll
+            for (int j = 0; j < DIM / 16; ++j) dp = mfma(QTile::along(gt, 32 * n, j), vr.x[j], dp);
+            float w[16], ds[16];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                using lds_f4 = const __attribute__((address_space(3))) f32x4;
+                const f32x4 l = *(lds_f4 *)(logs + (32 * n + result_row(4 * g, half)) * 4);
+                const f32x4 e = *(lds_f4 *)(deltas + (32 * n + result_row(4 * g, half)) * 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = 4 * g + j;
+                    w[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -l[j]));
+                    ds[r] = w[r] * (dp[r] - e[j]);
+                    if (kMasks && query0 + 32 * n + result_row(r, half) < own_first)
+                        w[r] = ds[r] = 0.0f;
+                }
+            }
+            const typename Vec<T>::x8 pw[4] = {pack8<T>(w), pack8<T>(w + 8)};
+            const typename Vec<T>::x8 pd[4] = {pack8<T>(ds), pack8<T>(ds + 8)};
+            if constexpr (kMasks)
+                if (split_rows) {
+                    const auto sees = [&](int row) { return query0 + row >= own_first; };
+                    add_seen<T, DIM, QTile>(gv, gt, 32 * n, pw, 2, sees);
+                    add_seen<T, DIM, QTile>(gk, qt, 32 * n, pd, 2, sees);
+                    continue;
+                }
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int d = 0; d < DIM / 32; ++d) {
+                    gv[d] = mfma(QTile::down(gt, 32 * n + 16 * g, d), pw[g], gv[d]);
+                    gk[d] = mfma(QTile::down(qt, 32 * n + 16 * g, d), pd[g], gk[d]);
+                }
         }
-    const int64_t at = (row * a.heads_k + kh) * a.dim;
-    if (one) {
-        dk[at + lane] = from_float<T>(dk0 * a.scale);
-        dv[at + lane] = from_float<T>(dv0);
+    };
+    int head = kh * group, t = first_tile;
+    if (steps > 0) fetch(0, head, t);
+    for (int i = 0; i < steps; ++i) {
+        __syncthreads();  // tile i is in LDS, and tile i - 1 has been read
+        const int now = t;
+        if (++t == end_tile) {
+            t = first_tile;
+            ++head;
+        }
+        if (i + 1 < steps) fetch(i + 1, head, t);
+        if (now * kBackRows >= whole)
+            step(i, now, std::false_type{});
+        else
+            step(i, now, std::true_type{});
     }
-    if (two) {
-        dk[at + lane + 64] = from_float<T>(dk1 * a.scale);
-        dv[at + lane + 64] = from_float<T>(dv1);
+    // keys past the length that counts have no gradient
+    if (__ballot(!counts)) {
+#pragma unroll
+        for (int d = 0; d < DIM / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                gk[d][r] = counts ? gk[d][r] : 0.0f;
+                gv[d][r] = counts ? gv[d][r] : 0.0f;
+            }
     }
+    const int64_t at = ((int64_t)(p.k0 + key) * a.heads_k + kh) * a.dim;
+    store_columns<T, DIM>(gk, a.scale, real ? dk + at : nullptr, a.dim);
+    store_columns<T, DIM>(gv, 1.0f, real ? dv + at : nullptr, a.dim);
 }
 
 constexpr int64_t kMaxRows = 0x7fffffffLL - 65536;  // row numbers stay in 32 bits
-constexpr int64_t kMaxStride = 1 << 23;             // and byte offsets in a tile
+constexpr int64_t kMaxStride = 1 << 23;             // and a tile's byte offsets in 31
+
+// Rows that a tile can be copied from: byte offsets fit, and a row past the last one lies
+// wholly behind the copy's bound.
+static bool tile_stride(int64_t stride, int dim) { return stride >= dim && stride <= kMaxStride; }
 
 static int check_attention(const GsAttention *a) {
     if (!a || a->rows_q < 0 || a->rows_k < 0 || a->sequences < 0 || a->heads_q < 1 ||
@@ -473,7 +650,8 @@ static int check_attention(const GsAttention *a) {
     if (!element_type(a->type)) return GS_ERR_INVALID_ARGUMENT;
     if (a->type == GS_F32 || a->dim % 8 != 0 || a->dim > GS_MAX_HEAD_DIM ||
         a->rows_q > kMaxRows / (a->heads_q / a->heads_k) || a->rows_k > kMaxRows ||
-        a->k_row > kMaxStride || a->v_row > kMaxStride ||
+        !tile_stride(a->q_row, a->dim) || !tile_stride(a->k_row, a->dim) ||
+        !tile_stride(a->v_row, a->dim) ||
         (a->q_row | a->q_head | a->k_row | a->k_head | a->v_row | a->v_head) % 8 != 0)
         return GS_ERR_UNSUPPORTED;
     return GS_OK;
@@ -582,7 +760,7 @@ extern "C" int gs_attention_backward_workspace_size(const GsAttention *a, size_t
     const int st = check_attention(a);
     if (st) return st;
     if (!bytes) return GS_ERR_INVALID_ARGUMENT;
-    *bytes = (size_t)a->rows_q * a->heads_q * sizeof(float);
+    *bytes = (size_t)a->rows_q * a->heads_q * 2 * sizeof(float);
     return GS_OK;
 }
 
@@ -599,26 +777,35 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
     if (a->rows_q > 0 && (!q || !out || !log_sum || !grad_out || !grad_q || !workspace))
         return GS_ERR_INVALID_ARGUMENT;
     if (a->rows_k > 0 && (!k || !v || !grad_k || !grad_v)) return GS_ERR_INVALID_ARGUMENT;
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(grad_out) ||
-        (grad_out_row | grad_out_head) % 8 != 0)
+    for (const void *x : {q, k, v, out, grad_out, (const void *)grad_q, (const void *)grad_k,
+                          (const void *)grad_v})
+        if (!aligned16(x)) return GS_ERR_UNSUPPORTED;
+    if ((grad_out_row | grad_out_head) % 8 != 0 || !tile_stride(grad_out_row, a->dim))
         return GS_ERR_UNSUPPORTED;
     if (workspace_bytes < need) return GS_ERR_WORKSPACE_TOO_SMALL;
-    const auto launch = [&](auto t) {
+    const int64_t group = a->heads_q / a->heads_k;
+    const int64_t blocks_q = (a->rows_q * group / kBackOwn + a->sequences + 2) * a->heads_k;
+    const int64_t blocks_k = (a->rows_k / kBackOwn + a->sequences + 2) * a->heads_k;
+    if (blocks_q > 0x7fffffffLL || blocks_k > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
+    float *row_log = (float *)workspace, *row_delta = row_log + a->rows_q * a->heads_q;
+    const auto launch = [&](auto t, auto d) {
         using T = decltype(t);
+        constexpr int kDim = decltype(d)::value;
         if (a->rows_q > 0) {
-            hipLaunchKernelGGL((attention_dq_kernel<T>), dim3((unsigned)a->rows_q, a->heads_q),
-                               dim3(64), 0, stream, *a, (const T *)q, (const T *)k, (const T *)v,
-                               (const T *)out, log_sum, (const T *)grad_out, grad_out_row,
-                               grad_out_head, (T *)grad_q, (float *)workspace);
+            hipLaunchKernelGGL((attention_dq_kernel<T, kDim>), dim3((unsigned)blocks_q),
+                               dim3(64 * kWaves), 0, stream, *a, (const T *)q, (const T *)k,
+                               (const T *)v, (const T *)out, log_sum, (const T *)grad_out,
+                               grad_out_row, grad_out_head, (T *)grad_q, row_log, row_delta);
             const int s = launch_status();
             if (s) return s;
         }
         if (a->rows_k > 0)
-            hipLaunchKernelGGL((attention_dkv_kernel<T>), dim3((unsigned)a->rows_k, a->heads_k),
-                               dim3(64), 0, stream, *a, (const T *)q, (const T *)k, (const T *)v,
-                               log_sum, (const T *)grad_out, grad_out_row, grad_out_head,
-                               (const float *)workspace, (T *)grad_k, (T *)grad_v);
+            hipLaunchKernelGGL((attention_dkv_kernel<T, kDim>), dim3((unsigned)blocks_k),
+                               dim3(64 * kWaves), 0, stream, *a, (const T *)q, (const T *)k,
+                               (const T *)v, (const T *)grad_out, grad_out_row, grad_out_head,
+                               row_log, row_delta, (T *)grad_k, (T *)grad_v);
         return launch_status();
     };
-    return a->type == GS_F16 ? launch(f16{}) : launch(bf16{});
+    return a->type == GS_F16 ? with_tile(a->dim, [&](auto d) { return launch(f16{}, d); })
+                             : with_tile(a->dim, [&](auto d) { return launch(bf16{}, d); });
 }

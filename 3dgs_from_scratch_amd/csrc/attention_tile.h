@@ -20,6 +20,7 @@
 namespace gs {
 
 using f32x16 = __attribute__((ext_vector_type(16))) float;
+using f32x4 = __attribute__((ext_vector_type(4))) float;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 using i16x4 = __attribute__((ext_vector_type(4))) short;
 template <typename T>
@@ -102,11 +103,12 @@ __device__ __forceinline__ Span span_of(const GsAttention &a, int s) {
 }
 
 // The sequence and the tile in it of a launch's tile number, tiles of `size` units,
-// `units` units a row; counted from the back, so that the tiles that see most under a
-// causal mask start first.  Every lane of a wave calls it.  False: no such tile.
+// `units` units a row.  Counted from the back on request: under a causal mask the last
+// queries see most, and should start first.  Every lane of a wave calls it.  False: no
+// such tile.
 __device__ __forceinline__ bool find_tile(const int32_t *offsets, int sequences, int64_t rows,
-                                          int units, int size, int number, int *sequence,
-                                          int *tile) {
+                                          int units, int size, int number, bool from_back,
+                                          int *sequence, int *tile) {
     const int lane = __lane_id(), all = sequences + 2;
     int total = 0, sum = 0;
     for (int first = 0; first < all; first += kWave) {
@@ -124,8 +126,8 @@ __device__ __forceinline__ bool find_tile(const int32_t *offsets, int sequences,
         }
         total += __shfl(sum, kWave - 1, kWave);
     }
-    int want = total - 1 - number;
-    if (want < 0) return false;
+    if (number >= total) return false;
+    int want = from_back ? total - 1 - number : number;
     // `sum` holds the last group's running count; the groups before it are counted again
     for (int first = 0; first < all; first += kWave) {
         if (all > kWave) {
@@ -202,6 +204,16 @@ struct Tile {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 from, (__attribute__((address_space(3))) void *)(tile + (i * WAVES + wave) * 1024),
                 16, c.from[i], 0, 0, 0);
+    }
+
+    // Starts the copy of one float a row (64 rows, `present` of them in memory, the rest
+    // become zeros); one wave does it.
+    static __device__ __forceinline__ void start_floats(const float *first, int present,
+                                                        lds_char *to) {
+        const int n = present < 0 ? 0 : present < 64 ? present : 64;
+        const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)first, 0, n * 4, 0x00027000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            from, (__attribute__((address_space(3))) void *)to, 4, __lane_id() * 4, 0, 0, 0);
     }
 
     // Operand that contracts over the dimension: row `base` + l % 32, places 16 s + 8 (l / 32).

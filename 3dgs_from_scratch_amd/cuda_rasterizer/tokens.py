@@ -37,6 +37,7 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 MAX_AXES = 4
 MAX_HEAD_DIM = 128
+_MAX_STRIDE = 1 << 23  # elements from a row to the next
 
 
 def _check(what: str, name: str, t, dims: int | None = None, types=_TYPES, device=None):
@@ -260,10 +261,12 @@ def axial_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
 
 # ------------------------------------------------------------------- attention
 def _laid_out(t: torch.Tensor) -> torch.Tensor:
-    """t where the kernels can read it in 16-byte pieces, else a contiguous copy."""
+    """t where the kernels can read its rows in 16-byte pieces, else a contiguous copy."""
     s = t.stride()
-    return t if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0 \
-        else t.clone(memory_format=torch.contiguous_format)
+    if (s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.shape[2] <= s[0] <= _MAX_STRIDE
+            and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _problem(q, k, v, offsets_q, offsets_k, lengths_k, causal, scale):

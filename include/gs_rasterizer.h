@@ -741,8 +741,9 @@ int gs_axial_rotary(const GsRotaryTensor *tensors, int32_t n_tensors, const void
  * no key, and a row of no sequence, has output 0 and log-sum -infinity, and
  * sends no gradient.
  * dim is a multiple of 8 and at most GS_MAX_HEAD_DIM, type GS_F16 or GS_BF16;
- * q, k, v and grad_out are 16-byte aligned with strides that are multiples of 8
- * (GS_ERR_UNSUPPORTED otherwise).  Outputs are contiguous (rows, heads, dim).
+ * q, k, v and grad_out are 16-byte aligned with strides that are multiples of 8,
+ * row strides from dim to 2^23 (GS_ERR_UNSUPPORTED otherwise).  Outputs are 16-byte
+ * aligned and contiguous (rows, heads, dim).
  */
 typedef struct {
     int64_t rows_q, rows_k;
