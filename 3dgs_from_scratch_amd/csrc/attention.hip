@@ -465,9 +465,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
         for (int n = 0; n < kBackRows / 32; ++n) {
             f32x16 s = {}, dp = {};
 #pragma unroll
-            for (int i = 0; i < DIM / 16; ++i) s = mfma(KTile::along(kt, 32 * n, i), qr.x[i], s);
-#pragma unroll
-            for (int i = 0; i < DIM / 16; ++i) dp = mfma(KTile::along(vt, 32 * n, i), gr.x[i], dp);
+            for (int i = 0; i < DIM / 16; ++i) {
+                s = mfma(KTile::along(kt, 32 * n, i), qr.x[i], s);
+                dp = mfma(KTile::along(vt, 32 * n, i), gr.x[i], dp);
+            }
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -526,7 +527,7 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
     const int whole = a.causal ? max(end_key - 1 - shift, 0) : 0;
     const int first_tile = first / kBackRows;
     const int end_tile = block_key < p.lk ? (p.lq + kBackRows - 1) / kBackRows : 0;
-    const int per_head = max(end_tile - first_tile, 0), steps = per_head * group;
+    const int whole_tile = min((whole + kBackRows - 1) / kBackRows, end_tile);
     const int own_first = a.causal ? key - shift : 0;  // the first query that sees this key
 
     const T *key_row = counts ? k + (int64_t)(p.k0 + key) * a.k_row + (int64_t)kh * a.k_head : nullptr;
@@ -567,9 +568,10 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
         for (int n = 0; n < kBackRows / 32; ++n) {
             f32x16 s = {}, dp = {};
 #pragma unroll
-            for (int j = 0; j < DIM / 16; ++j) s = mfma(QTile::along(qt, 32 * n, j), kr.x[j], s);
-#pragma unroll
-            for (int j = 0; j < DIM / 16; ++j) dp = mfma(QTile::along(gt, 32 * n, j), vr.x[j], dp);
+            for (int j = 0; j < DIM / 16; ++j) {
+                s = mfma(QTile::along(qt, 32 * n, j), kr.x[j], s);
+                dp = mfma(QTile::along(gt, 32 * n, j), vr.x[j], dp);
+            }
             float w[16], ds[16];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -603,20 +605,39 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
                 }
         }
     };
-    int head = kh * group, t = first_tile;
-    if (steps > 0) fetch(0, head, t);
-    for (int i = 0; i < steps; ++i) {
+    // of every head of the group the tiles with queries that do not see all the keys, then
+    // of every head the others
+    const int part = max(whole_tile - first_tile, 0) * group;
+    const int steps = max(end_tile - first_tile, 0) * group;
+    const auto place = [&](int i, int *tile) {  // the head and tile of a step
+        const int from = i < part ? first_tile : whole_tile;
+        const int per_head = (i < part ? whole_tile : end_tile) - from;
+        const int j = i < part ? i : i - part;
+        *tile = from + j % per_head;
+        return kh * group + j / per_head;
+    };
+    const auto begin = [&](int i) {
         __syncthreads();  // tile i is in LDS, and tile i - 1 has been read
-        const int now = t;
-        if (++t == end_tile) {
-            t = first_tile;
-            ++head;
+        if (i + 1 < steps) {
+            int tile;
+            const int head = place(i + 1, &tile);
+            fetch(i + 1, head, tile);
         }
-        if (i + 1 < steps) fetch(i + 1, head, t);
-        if (now * kBackRows >= whole)
-            step(i, now, std::false_type{});
-        else
-            step(i, now, std::true_type{});
+    };
+    int tile;
+    if (steps > 0) {
+        const int head = place(0, &tile);
+        fetch(0, head, tile);
+    }
+    int i = 0;
+    for (; i < part; ++i) {
+        begin(i);
+        place(i, &tile);
+        step(i, tile, std::true_type{});
+    }
+    for (; i < steps; ++i) {
+        begin(i);
+        step(i, 0, std::false_type{});
     }
     // keys past the length that counts have no gradient
     if (__ballot(!counts)) {

@@ -158,6 +158,15 @@ __device__ __forceinline__ bool find_tile(const int32_t *offsets, int sequences,
 }
 
 // -------------------------------------------------------------------- tiles
+// Four rows of the column that this lane gets of its 16 lanes' 4 x 16 block.  Without the
+// restrict the compiler takes any copy to LDS that is under way for one to this address,
+// and waits for the next tile's before the first such read of this one (forward 3%,
+// keys' gradients 40%); the barrier at a tile's start is what orders them.
+typedef __attribute__((address_space(3))) i16x4 lds_x4;
+__device__ __forceinline__ i16x4 transposed(const lds_x4 *__restrict__ p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_x4 *)p);
+}
+
 template <typename T, int DIM, int ROWS, int WAVES>
 struct Tile {
     static constexpr int kChunks = DIM / 8;                      // of a row
@@ -210,7 +219,7 @@ struct Tile {
     // become zeros); one wave does it.
     static __device__ __forceinline__ void start_floats(const float *first, int present,
                                                         lds_char *to) {
-        const int n = present < 0 ? 0 : present < 64 ? present : 64;
+        const int n = uniform(present < 0 ? 0 : present < 64 ? present : 64);
         const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)first, 0, n * 4, 0x00027000);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
             from, (__attribute__((address_space(3))) void *)to, 4, __lane_id() * 4, 0, 0, 0);
@@ -232,9 +241,7 @@ struct Tile {
         const int chunk = (4 * d + ((l >> 4) & 1) * 2 + ((l & 3) >> 1)) ^ swizzle(row);
         const lds_char *p = tile + base * DIM * 2 + row * DIM * 2 + chunk * 16 + (l & 1) * 8;
         const int next = 8 * DIM * 2;
-        typedef __attribute__((address_space(3))) i16x4 lds_x4;
-        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_x4 *)p);
-        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_x4 *)(p + next));
+        const i16x4 lo = transposed((const lds_x4 *)p), hi = transposed((const lds_x4 *)(p + next));
         const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         return __builtin_bit_cast(x8, both);
     }
