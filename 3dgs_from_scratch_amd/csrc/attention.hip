@@ -63,45 +63,91 @@ __device__ __forceinline__ void store_columns(const f32x16 *acc, float factor, T
     }
 }
 
-// Whether `rows` rows of a tile hold an infinity or a NaN; the same in every lane.
-template <typename T, int DIM>
-__device__ __forceinline__ bool not_finite(const lds_char *tile, int base, int rows) {
+// Infinities and NaN in rows of a tile that some columns do not see: their weights there are
+// 0, but 0 times them is no 0.  Tiles at a causal edge are looked through for such rows; where
+// there are any, the product takes zeros for these values, and a second one finds the sums
+// that such a value belongs to, which become NaN.
+template <typename T>
+__device__ __forceinline__ bool not_finite(uint32_t bits) {
+    constexpr uint32_t kInfinity = std::is_same<T, bf16>::value ? 0x7f80 : 0x7c00;
+    return (bits & 0x7fff) >= kInfinity;
+}
+
+// The rows from `base` on, ROWS of them, that hold such a value: a bit each, in every lane.
+template <typename T, int DIM, int ROWS>
+__device__ __forceinline__ uint64_t rows_not_finite(const lds_char *tile, int base) {
     using u16x8 = __attribute__((ext_vector_type(8))) uint16_t;
+    constexpr int kChunks = DIM / 8;
+    const int row = __lane_id() % ROWS;
+    const lds_char *p = tile + (base + row) * DIM * 2;
+    int chunk = row % kChunks;  // each lane begins elsewhere: other banks
     u16x8 most = {};
-    for (int at = __lane_id() * 16; at < rows * DIM * 2; at += 1024) {
-        const u16x8 x = *(const __attribute__((address_space(3))) u16x8 *)(tile + base * DIM * 2 + at);
+    for (int i = 0; i < kChunks; ++i) {
+        const u16x8 x = *(const __attribute__((address_space(3))) u16x8 *)(p + chunk * 16);
         most = __builtin_elementwise_max(most, x & (uint16_t)0x7fff);
+        chunk = chunk + 1 == kChunks ? 0 : chunk + 1;
     }
     uint16_t m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = most[i] > m ? most[i] : m;
-    return __ballot(m >= (std::is_same<T, bf16>::value ? 0x7f80 : 0x7c00)) != 0;
+    const uint64_t found = __ballot(not_finite<T>(m));
+    return ROWS == 64 ? found : found & 0xffffffffull;
 }
 
-// acc += X^T P over `groups` groups of 16 rows of a tile X that holds infinities or NaN in
-// rows that some columns do not see: a row at a time, added where `sees` says so.
+// acc += X^T P over 32 rows of a tile X from `base`, P in two operands of 16 rows.
+template <typename T, int DIM, typename XTile>
+__device__ __forceinline__ void add_product(f32x16 *acc, const lds_char *tile, int base,
+                                            const typename Vec<T>::x8 *p) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int d = 0; d < DIM / 32; ++d)
+            acc[d] = mfma(XTile::down(tile, base + 16 * g, d), p[g], acc[d]);
+}
+
+// The same where the rows hold infinities or NaN; sees(i): whether the lane's column sees row
+// base + i.
 template <typename T, int DIM, typename XTile, typename Sees>
-__device__ __forceinline__ void add_seen(f32x16 *acc, const lds_char *tile, int base,
-                                         const typename Vec<T>::x8 *p, int groups, Sees sees) {
+__device__ __forceinline__ void add_product_seen(f32x16 *acc, const lds_char *tile, int base,
+                                                 const typename Vec<T>::x8 *p, Sees sees) {
+    using x8 = typename Vec<T>::x8;
     const int half = __lane_id() >> 5;
 #pragma unroll 1
-    for (int row = 0; row < 16 * groups; ++row) {
-        const int g = row >> 4;
-        const auto only = [&](typename Vec<T>::x8 x) {
+    for (int g = 0; g < 2; ++g) {
+        const x8 weights = g ? p[1] : p[0];
+        x8 seen;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (result_row(j, half) != (row & 15)) x[j] = (T)0.0f;
-            return x;
-        };
-        const auto weights = only(g == 0 ? p[0] : g == 1 ? p[1] : g == 2 ? p[2] : p[3]);
-        const bool seen = sees(base + row);
+        for (int j = 0; j < 8; ++j) seen[j] = (T)(sees(16 * g + result_row(j, half)) ? 1.0f : 0.0f);
 #pragma unroll
         for (int d = 0; d < DIM / 32; ++d) {
-            const f32x16 one = mfma(only(XTile::down(tile, base + 16 * g, d)), weights, f32x16{});
+            x8 x = XTile::down(tile, base + 16 * g, d), bad;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[d][r] += seen ? one[r] : 0.0f;
+            for (int j = 0; j < 8; ++j) {
+                const bool b = not_finite<T>(__builtin_bit_cast(uint16_t, (T)x[j]));
+                bad[j] = (T)(b ? 1.0f : 0.0f);
+                x[j] = b ? (T)0.0f : x[j];
+            }
+            acc[d] = mfma(x, weights, acc[d]);
+            const f32x16 count = mfma(bad, seen, f32x16{});
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] = count[r] > 0.0f ? NAN : acc[d][r];
         }
     }
+}
+
+// The same, not rounded, for a sum that is joined later.
+template <int DIM>
+__device__ __forceinline__ void store_partial(const f32x16 *acc, float *row, int dim) {
+    const int half = __lane_id() >> 5;
+#pragma unroll
+    for (int d = 0; d < DIM / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int column = 32 * d + result_row(4 * g, half);
+            if (row && column < dim)
+                *(float4 *)(row + column) = make_float4(acc[d][4 * g], acc[d][4 * g + 1],
+                                                        acc[d][4 * g + 2], acc[d][4 * g + 3]);
+        }
 }
 
 // Forward.  A workgroup takes a tile of packed rows of one key head (row r of a
@@ -112,6 +158,17 @@ __device__ __forceinline__ void add_seen(f32x16 *acc, const lds_char *tile, int 
 // that follow a new maximum none.  K and V go from memory into LDS beside the work on
 // the tile before.  BY_KEYS: a few rows only; the waves share the rows and split the
 // keys of a tile, and join at the end.
+// A workgroup's place in its launch: splits of a tile next to each other, so that the longest
+// tiles start first, and key heads innermost: workgroups go to the eight XCDs in turn, and
+// with 8 or a divisor of 8 key heads an XCD's L2 holds one of them.
+struct Place {
+    int kh, split, tile;
+};
+__device__ __forceinline__ Place place_of(int heads_k, int splits) {
+    const int rest = blockIdx.x / heads_k;
+    return {(int)blockIdx.x % heads_k, rest % splits, rest / splits};
+}
+
 template <typename T, int DIM, bool BY_KEYS>
 struct Forward {
     static constexpr int kSub = BY_KEYS ? 1 : 2;                    // 32-key parts of a wave
@@ -138,10 +195,10 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
     __shared__ __attribute__((aligned(1024))) char lds[F::kLds];
     lds_char *const tiles = (lds_char *)lds;
 
-    // key heads next to each other: with 8 or a divisor of 8 of them, an XCD's L2 holds one
-    const int kh = blockIdx.x % a.heads_k, group = a.heads_q / a.heads_k;
+    const Place at_grid = place_of(a.heads_k, partial.splits);
+    const int kh = at_grid.kh, split = at_grid.split, group = a.heads_q / a.heads_k;
     int sequence, number;
-    if (!find_tile(a.offsets_q, a.sequences, a.rows_q, group, F::kRows, blockIdx.x / a.heads_k,
+    if (!find_tile(a.offsets_q, a.sequences, a.rows_q, group, F::kRows, at_grid.tile,
                    true, &sequence, &number))
         return;
     const Span p = span_of(a, sequence);
@@ -166,7 +223,7 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
     // this split's tiles
     const int tiles_all = seen > 0 ? (seen + F::kKeys - 1) / F::kKeys : 0;
     const int share = (tiles_all + partial.splits - 1) / partial.splits;
-    const int first_tile = min((int)blockIdx.y * share, tiles_all);
+    const int first_tile = min(split * share, tiles_all);
     const int end_tile = min(first_tile + share, tiles_all);
 
     const bool negate = a.scale < 0.0f;
@@ -208,11 +265,9 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
             for (int i = 0; i < DIM / 16; ++i)
                 s[n] = mfma(KTile::along(kt, base + 32 * n, i), qr.x[i], s[n]);
         }
-        bool split_keys = false;
+        uint64_t found = 0;
         if constexpr (kMasks) {
-            // 0 times an infinity is no 0: a value that some rows of the tile do not see
-            // must not meet their weights
-            if (a.causal) split_keys = not_finite<T, DIM>(vt, base, 32 * F::kSub);
+            if (a.causal) found = rows_not_finite<T, DIM, 32 * F::kSub>(vt, base);
 #pragma unroll
             for (int n = 0; n < F::kSub; ++n)
 #pragma unroll
@@ -236,7 +291,7 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
             for (int d = 0; d < DIM / 32; ++d) acc[d] *= keep;
         }
         const float minus = top == -INFINITY ? 0.0f : -top;
-        typename Vec<T>::x8 weights[4] = {};  // (2 kSub are used)
+        typename Vec<T>::x8 weights[2 * F::kSub];
 #pragma unroll
         for (int n = 0; n < F::kSub; ++n) {
             float w[16];
@@ -248,17 +303,15 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
             weights[2 * n] = pack8<T>(w);
             weights[2 * n + 1] = pack8<T>(w + 8);
         }
-        if constexpr (kMasks)
-            if (split_keys) {
-                add_seen<T, DIM, KTile>(acc, vt, base, weights, 2 * F::kSub,
-                                        [&](int at) { return t * F::kKeys + at <= last; });
-                return;
-            }
 #pragma unroll
-        for (int g = 0; g < 2 * F::kSub; ++g)
-#pragma unroll
-            for (int d = 0; d < DIM / 32; ++d)
-                acc[d] = mfma(KTile::down(vt, base + 16 * g, d), weights[g], acc[d]);
+        for (int n = 0; n < F::kSub; ++n) {
+            const uint32_t part = (uint32_t)(found >> (32 * n));
+            if (kMasks && part)
+                add_product_seen<T, DIM, KTile>(acc, vt, base + 32 * n, weights + 2 * n,
+                                                [&](int i) { return key0 + 32 * n + i <= last; });
+            else
+                add_product<T, DIM, KTile>(acc, vt, base + 32 * n, weights + 2 * n);
+        }
     };
     if (first_tile < end_tile) fetch(first_tile);
     int t = first_tile;
@@ -305,20 +358,10 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
     }
 
     if (partial.splits > 1) {
-        const int64_t slot = (int64_t)blockIdx.y * a.rows_q * a.heads_q + at;
+        const int64_t slot = (int64_t)split * a.rows_q * a.heads_q + at;
         if (real && half == 0) partial.max_sum[slot] = make_float2(top, sum);
-        if (real && top != -INFINITY) {
-#pragma unroll
-            for (int d = 0; d < DIM / 32; ++d)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int column = 32 * d + result_row(4 * g, half);
-                    if (column < a.dim)
-                        *(float4 *)(partial.sums + slot * a.dim + column) =
-                            make_float4(acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2],
-                                        acc[d][4 * g + 3]);
-                }
-        }
+        store_partial<DIM>(acc, real && top != -INFINITY ? partial.sums + slot * a.dim : nullptr,
+                           a.dim);
         return;
     }
     // a row that saw nothing: zeros, whatever met them
@@ -382,14 +425,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
     GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
     const T *__restrict__ out, const float *__restrict__ log_sum, const T *__restrict__ go,
     int64_t go_row, int64_t go_head, T *__restrict__ dq, float *__restrict__ row_log,
-    float *__restrict__ row_delta) {
+    float *__restrict__ row_delta, float *__restrict__ partial, int splits) {
     using KTile = Tile<T, DIM, kBackRows, kWaves>;
     __shared__ __attribute__((aligned(1024))) char lds[4 * KTile::kBytes];
     lds_char *const tiles = (lds_char *)lds;
 
-    const int kh = blockIdx.x % a.heads_k, group = a.heads_q / a.heads_k;
+    const Place at_grid = place_of(a.heads_k, splits);
+    const int kh = at_grid.kh, split = at_grid.split, group = a.heads_q / a.heads_k;
     int sequence, number;
-    if (!find_tile(a.offsets_q, a.sequences, a.rows_q, group, kBackOwn, blockIdx.x / a.heads_k,
+    if (!find_tile(a.offsets_q, a.sequences, a.rows_q, group, kBackOwn, at_grid.tile,
                    true, &sequence, &number))
         return;
     const Span p = span_of(a, sequence);
@@ -408,7 +452,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
         a.causal ? min(min(row0 + 31, rows - 1) / group + shift, p.lk - 1) : p.lk - 1;
     const int block_end = min(number * kBackOwn + kBackOwn, rows) - 1;
     const int seen = a.causal ? min(block_end / group + shift, p.lk - 1) + 1 : p.lk;
-    const int end_tile = seen > 0 ? (seen + kBackRows - 1) / kBackRows : 0;
+    const int tiles_all = seen > 0 ? (seen + kBackRows - 1) / kBackRows : 0;
+    const int share = (tiles_all + splits - 1) / splits;  // this split's tiles
+    const int first_tile = min(split * share, tiles_all);
+    const int end_tile = min(first_tile + share, tiles_all);
 
     RowOperand<T, DIM> qr, gr;
     qr.load(real ? q + (int64_t)(p.q0 + query) * a.q_row + (int64_t)head * a.q_head : nullptr,
@@ -429,7 +476,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
     // a row that saw nothing has no weights: exp2(x - infinity) = 0
     const float given = real ? log_sum[at] : -INFINITY;
     const float log2_sum = given == -INFINITY ? INFINITY : given * kLog2e;
-    if (real && half == 0) {
+    if (real && half == 0 && split == 0) {
         const int64_t to = (int64_t)head * a.rows_q + p.q0 + query;
         row_log[to] = log2_sum;
         row_delta[to] = delta;
@@ -458,9 +505,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
         const lds_char *kt = tiles + (t & 1) * 2 * KTile::kBytes, *vt = kt + KTile::kBytes;
         const int key0 = t * kBackRows;
         if (kMasks && key0 > wave_last) return;
-        bool split_keys = false;
-        if constexpr (kMasks)
-            if (a.causal) split_keys = not_finite<T, DIM>(kt, 0, kBackRows);
+        uint64_t found = 0;
+        if (kMasks && a.causal) found = rows_not_finite<T, DIM, kBackRows>(kt, 0);
 #pragma unroll
         for (int n = 0; n < kBackRows / 32; ++n) {
             f32x16 s = {}, dp = {};
@@ -475,33 +521,34 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
                 ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -log2_sum)) * (dp[r] - delta);
                 if (kMasks && key0 + 32 * n + result_row(r, half) > last) ds[r] = 0.0f;
             }
-            const typename Vec<T>::x8 x[4] = {pack8<T>(ds), pack8<T>(ds + 8)};
-            if constexpr (kMasks)
-                if (split_keys) {
-                    add_seen<T, DIM, KTile>(acc, kt, 32 * n, x, 2,
-                                            [&](int i) { return key0 + i <= last; });
-                    continue;
-                }
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int d = 0; d < DIM / 32; ++d)
-                    acc[d] = mfma(KTile::down(kt, 32 * n + 16 * g, d), x[g], acc[d]);
+            const typename Vec<T>::x8 x[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
+            const uint32_t part = (uint32_t)(found >> (32 * n));
+            if (kMasks && part)
+                add_product_seen<T, DIM, KTile>(acc, kt, 32 * n, x, [&](int i) {
+                    return key0 + 32 * n + i <= last;
+                });
+            else
+                add_product<T, DIM, KTile>(acc, kt, 32 * n, x);
         }
     };
-    if (end_tile > 0) fetch(0);
-    int t = 0;
+    if (first_tile < end_tile) fetch(first_tile);
+    int t = first_tile;
     for (const int whole = min(end_tile, (all_see + 1) / kBackRows); t < whole; ++t)
         step(t, std::false_type{});
     for (; t < end_tile; ++t) step(t, std::true_type{});
-    store_columns<T, DIM>(acc, a.scale, real ? dq + at * a.dim : nullptr, a.dim);
+    if (splits > 1)
+        store_partial<DIM>(acc, real ? partial + ((int64_t)split * a.rows_q * a.heads_q + at) * a.dim
+                                     : nullptr, a.dim);
+    else
+        store_columns<T, DIM>(acc, a.scale, real ? dq + at * a.dim : nullptr, a.dim);
 }
 
 template <typename T, int DIM>
 __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_kernel(
     GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
     const T *__restrict__ go, int64_t go_row, int64_t go_head, const float *__restrict__ row_log,
-    const float *__restrict__ row_delta, T *__restrict__ dk, T *__restrict__ dv) {
+    const float *__restrict__ row_delta, T *__restrict__ dk, T *__restrict__ dv,
+    float *__restrict__ partial, int splits) {
     using QTile = Tile<T, DIM, kBackRows, kWaves>;
     constexpr int kFloats = kBackRows * 4;                         // bytes of one float a row
     constexpr int kStage = 2 * QTile::kBytes + 1024;               // Q, dout, log-sums, deltas
@@ -509,9 +556,10 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
     __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
     lds_char *const tiles = (lds_char *)lds;
 
-    const int kh = blockIdx.x % a.heads_k, group = a.heads_q / a.heads_k;
+    const Place at_grid = place_of(a.heads_k, splits);
+    const int kh = at_grid.kh, split = at_grid.split, group = a.heads_q / a.heads_k;
     int sequence, number;
-    if (!find_tile(a.offsets_k, a.sequences, a.rows_k, 1, kBackOwn, blockIdx.x / a.heads_k, false,
+    if (!find_tile(a.offsets_k, a.sequences, a.rows_k, 1, kBackOwn, at_grid.tile, false,
                    &sequence, &number))
         return;
     const Span p = span_of(a, sequence);
@@ -558,13 +606,16 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
 
     const auto step = [&](int i, int t, auto masks) {
         constexpr bool kMasks = decltype(masks)::value;
+        constexpr int kUnroll = kMasks ? 1 : 2;
         const lds_char *qt = tiles + (i & 1) * kStage, *gt = qt + QTile::kBytes;
         const lds_char *logs = gt + QTile::kBytes, *deltas = logs + kFloats;
         const int query0 = t * kBackRows;
-        bool split_rows = false;
-        if constexpr (kMasks)
-            split_rows = not_finite<T, DIM>(qt, 0, kBackRows) || not_finite<T, DIM>(gt, 0, kBackRows);
-#pragma unroll kMasks ? 1 : 2
+        uint64_t found_q = 0, found_g = 0;
+        if constexpr (kMasks) {
+            found_q = rows_not_finite<T, DIM, kBackRows>(qt, 0);
+            found_g = rows_not_finite<T, DIM, kBackRows>(gt, 0);
+        }
+#pragma unroll kUnroll
         for (int n = 0; n < kBackRows / 32; ++n) {
             f32x16 s = {}, dp = {};
 #pragma unroll
@@ -587,28 +638,28 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
                         w[r] = ds[r] = 0.0f;
                 }
             }
-            const typename Vec<T>::x8 pw[4] = {pack8<T>(w), pack8<T>(w + 8)};
-            const typename Vec<T>::x8 pd[4] = {pack8<T>(ds), pack8<T>(ds + 8)};
-            if constexpr (kMasks)
-                if (split_rows) {
-                    const auto sees = [&](int row) { return query0 + row >= own_first; };
-                    add_seen<T, DIM, QTile>(gv, gt, 32 * n, pw, 2, sees);
-                    add_seen<T, DIM, QTile>(gk, qt, 32 * n, pd, 2, sees);
-                    continue;
-                }
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int d = 0; d < DIM / 32; ++d) {
-                    gv[d] = mfma(QTile::down(gt, 32 * n + 16 * g, d), pw[g], gv[d]);
-                    gk[d] = mfma(QTile::down(qt, 32 * n + 16 * g, d), pd[g], gk[d]);
-                }
+            const typename Vec<T>::x8 pw[2] = {pack8<T>(w), pack8<T>(w + 8)};
+            const typename Vec<T>::x8 pd[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
+            const auto sees = [&](int i) { return query0 + 32 * n + i >= own_first; };
+            const uint32_t part_q = (uint32_t)(found_q >> (32 * n));
+            const uint32_t part_g = (uint32_t)(found_g >> (32 * n));
+            if (kMasks && part_g)
+                add_product_seen<T, DIM, QTile>(gv, gt, 32 * n, pw, sees);
+            else
+                add_product<T, DIM, QTile>(gv, gt, 32 * n, pw);
+            if (kMasks && part_q)
+                add_product_seen<T, DIM, QTile>(gk, qt, 32 * n, pd, sees);
+            else
+                add_product<T, DIM, QTile>(gk, qt, 32 * n, pd);
         }
     };
     // of every head of the group the tiles with queries that do not see all the keys, then
     // of every head the others
     const int part = max(whole_tile - first_tile, 0) * group;
-    const int steps = max(end_tile - first_tile, 0) * group;
+    const int steps_all = max(end_tile - first_tile, 0) * group;
+    const int share = (steps_all + splits - 1) / splits;  // this split's steps
+    const int first_step = min(split * share, steps_all);
+    const int steps = min(first_step + share, steps_all);
     const auto place = [&](int i, int *tile) {  // the head and tile of a step
         const int from = i < part ? first_tile : whole_tile;
         const int per_head = (i < part ? whole_tile : end_tile) - from;
@@ -624,13 +675,12 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
             fetch(i + 1, head, tile);
         }
     };
-    int tile;
-    if (steps > 0) {
-        const int head = place(0, &tile);
-        fetch(0, head, tile);
+    int tile, i = first_step;
+    if (i < steps) {
+        const int head = place(i, &tile);
+        fetch(i, head, tile);
     }
-    int i = 0;
-    for (; i < part; ++i) {
+    for (; i < min(part, steps); ++i) {
         begin(i);
         place(i, &tile);
         step(i, tile, std::true_type{});
@@ -650,8 +700,31 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
             }
     }
     const int64_t at = ((int64_t)(p.k0 + key) * a.heads_k + kh) * a.dim;
+    if (splits > 1) {
+        const int64_t size = a.rows_k * a.heads_k * a.dim;
+        float *to = partial + split * size + at;
+        store_partial<DIM>(gk, real ? to : nullptr, a.dim);
+        store_partial<DIM>(gv, real ? to + splits * size : nullptr, a.dim);
+        return;
+    }
     store_columns<T, DIM>(gk, a.scale, real ? dk + at : nullptr, a.dim);
     store_columns<T, DIM>(gv, 1.0f, real ? dv + at : nullptr, a.dim);
+}
+
+// Sums of splits, rounded: the y-th of the launch's outputs, four elements a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_sum_kernel(const float *__restrict__ partial,
+                                                            int64_t size, int splits, float scale0,
+                                                            float scale1, T *__restrict__ out0,
+                                                            T *__restrict__ out1) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= size) return;
+    const float *p = partial + (int64_t)blockIdx.y * splits * size + i;
+    f32x4 sum = *(const f32x4 *)p;
+    for (int s = 1; s < splits; ++s) sum += *(const f32x4 *)(p + s * size);
+    sum *= blockIdx.y ? scale1 : scale0;
+    const typename Vec<T>::x4 o = {(T)sum[0], (T)sum[1], (T)sum[2], (T)sum[3]};
+    *(typename Vec<T>::x4 *)((blockIdx.y ? out1 : out0) + i) = o;
 }
 
 constexpr int64_t kMaxRows = 0x7fffffffLL - 65536;  // row numbers stay in 32 bits
@@ -706,6 +779,46 @@ static ForwardPlan plan_forward(const GsAttention &a) {
     return f;
 }
 
+// How a backward is launched.  A launch of fewer workgroups than fill the card three times
+// (two of a SIMD's four waves fit at up to 64 dimensions in the keys' launch, one above)
+// splits its sums.
+struct BackwardPlan {
+    int64_t tiles_q, tiles_k;
+    int splits_q, splits_k;
+};
+
+static int backward_splits(int64_t busy, int64_t slots, int64_t steps) {
+    if (busy < 1 || busy >= slots) return 1;
+    const int64_t want = (slots + busy - 1) / busy, most = steps / 8;
+    const int64_t splits = want < most ? want : most;
+    return (int)(splits < 1 ? 1 : splits > 8 ? 8 : splits);
+}
+
+static BackwardPlan plan_backward(const GsAttention &a) {
+    const int64_t group = a.heads_q / a.heads_k, packed = a.rows_q * group;
+    const int64_t sequences = a.sequences > 0 ? a.sequences : 1, see = a.causal ? 2 : 1;
+    BackwardPlan b;
+    b.tiles_q = packed / kBackOwn + a.sequences + 2;
+    b.tiles_k = a.rows_k / kBackOwn + a.sequences + 2;
+    b.splits_q = backward_splits((packed + kBackOwn - 1) / kBackOwn * a.heads_k, 512,
+                                 a.rows_k / sequences / kBackRows / see);
+    b.splits_k = backward_splits((a.rows_k + kBackOwn - 1) / kBackOwn * a.heads_k,
+                                 a.dim > 64 ? 768 : 1024,
+                                 packed / sequences / kBackRows / see);
+    return b;
+}
+
+static size_t backward_partials(const GsAttention &a, const BackwardPlan &b) {
+    const size_t q = b.splits_q > 1 ? (size_t)b.splits_q * a.rows_q * a.heads_q * a.dim : 0;
+    const size_t k = b.splits_k > 1 ? (size_t)b.splits_k * a.rows_k * a.heads_k * a.dim * 2 : 0;
+    return (q > k ? q : k) * sizeof(float);
+}
+
+// Bytes of the row log-sums and deltas, a multiple of 16.
+static size_t backward_rows(const GsAttention &a) {
+    return ((size_t)a.rows_q * a.heads_q * 2 * sizeof(float) + 15) / 16 * 16;
+}
+
 static size_t partial_bytes(const GsAttention &a, int splits) {
     if (splits == 1) return 0;
     return (size_t)splits * a.rows_q * a.heads_q * (a.dim * sizeof(float) + sizeof(float2));
@@ -715,7 +828,7 @@ template <typename T, int DIM>
 static int launch_forward(const GsAttention &a, const ForwardPlan &f, const void *q, const void *k,
                           const void *v, void *out, float *log_sum, const Partial &partial,
                           hipStream_t stream) {
-    const dim3 grid((unsigned)(f.tiles * a.heads_k), f.splits);
+    const dim3 grid((unsigned)(f.tiles * a.heads_k * f.splits));
     if (f.by_keys)
         hipLaunchKernelGGL((attention_kernel<T, DIM, true>), grid, dim3(64 * kWaves), 0, stream, a,
                            (const T *)q, (const T *)k, (const T *)v, (T *)out, log_sum, partial);
@@ -760,7 +873,7 @@ extern "C" int gs_attention_forward(const GsAttention *a, const void *q, const v
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
         return GS_ERR_UNSUPPORTED;
     const ForwardPlan f = plan_forward(*a);
-    if (f.tiles * a->heads_k > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
+    if (f.tiles * a->heads_k * f.splits > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
     const size_t need = partial_bytes(*a, f.splits);
     if (need && !workspace) return GS_ERR_INVALID_ARGUMENT;
     if (workspace_bytes < need) return GS_ERR_WORKSPACE_TOO_SMALL;
@@ -781,7 +894,7 @@ extern "C" int gs_attention_backward_workspace_size(const GsAttention *a, size_t
     const int st = check_attention(a);
     if (st) return st;
     if (!bytes) return GS_ERR_INVALID_ARGUMENT;
-    *bytes = (size_t)a->rows_q * a->heads_q * 2 * sizeof(float);
+    *bytes = backward_rows(*a) + backward_partials(*a, plan_backward(*a));
     return GS_OK;
 }
 
@@ -804,27 +917,41 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
     if ((grad_out_row | grad_out_head) % 8 != 0 || !tile_stride(grad_out_row, a->dim))
         return GS_ERR_UNSUPPORTED;
     if (workspace_bytes < need) return GS_ERR_WORKSPACE_TOO_SMALL;
-    const int64_t group = a->heads_q / a->heads_k;
-    const int64_t blocks_q = (a->rows_q * group / kBackOwn + a->sequences + 2) * a->heads_k;
-    const int64_t blocks_k = (a->rows_k / kBackOwn + a->sequences + 2) * a->heads_k;
+    const BackwardPlan b = plan_backward(*a);
+    const int64_t blocks_q = b.tiles_q * a->heads_k * b.splits_q;
+    const int64_t blocks_k = b.tiles_k * a->heads_k * b.splits_k;
     if (blocks_q > 0x7fffffffLL || blocks_k > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
     float *row_log = (float *)workspace, *row_delta = row_log + a->rows_q * a->heads_q;
+    float *partial = (float *)((char *)workspace + backward_rows(*a));
     const auto launch = [&](auto t, auto d) {
         using T = decltype(t);
         constexpr int kDim = decltype(d)::value;
+        const dim3 block(64 * kWaves);
+        const auto join = [&](int64_t size, int splits, int outputs, float scale0, T *out0, T *out1) {
+            hipLaunchKernelGGL((attention_sum_kernel<T>), dim3((unsigned)((size / 4 + 255) / 256), outputs),
+                               dim3(256), 0, stream, (const float *)partial, size, splits, scale0,
+                               1.0f, out0, out1);
+        };
         if (a->rows_q > 0) {
             hipLaunchKernelGGL((attention_dq_kernel<T, kDim>), dim3((unsigned)blocks_q),
-                               dim3(64 * kWaves), 0, stream, *a, (const T *)q, (const T *)k,
-                               (const T *)v, (const T *)out, log_sum, (const T *)grad_out,
-                               grad_out_row, grad_out_head, (T *)grad_q, row_log, row_delta);
+                               block, 0, stream, *a, (const T *)q, (const T *)k, (const T *)v,
+                               (const T *)out, log_sum, (const T *)grad_out, grad_out_row,
+                               grad_out_head, (T *)grad_q, row_log, row_delta, partial, b.splits_q);
+            if (b.splits_q > 1)
+                join(a->rows_q * a->heads_q * a->dim, b.splits_q, 1, a->scale, (T *)grad_q,
+                     (T *)nullptr);
             const int s = launch_status();
             if (s) return s;
         }
-        if (a->rows_k > 0)
+        if (a->rows_k > 0) {
             hipLaunchKernelGGL((attention_dkv_kernel<T, kDim>), dim3((unsigned)blocks_k),
-                               dim3(64 * kWaves), 0, stream, *a, (const T *)q, (const T *)k,
-                               (const T *)v, (const T *)grad_out, grad_out_row, grad_out_head,
-                               row_log, row_delta, (T *)grad_k, (T *)grad_v);
+                               block, 0, stream, *a, (const T *)q, (const T *)k, (const T *)v,
+                               (const T *)grad_out, grad_out_row, grad_out_head, row_log, row_delta,
+                               (T *)grad_k, (T *)grad_v, partial, b.splits_k);
+            if (b.splits_k > 1)
+                join(a->rows_k * a->heads_k * a->dim, b.splits_k, 2, a->scale, (T *)grad_k,
+                     (T *)grad_v);
+        }
         return launch_status();
     };
     return a->type == GS_F16 ? with_tile(a->dim, [&](auto d) { return launch(f16{}, d); })

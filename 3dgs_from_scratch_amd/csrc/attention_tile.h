@@ -245,6 +245,13 @@ struct Tile {
         const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         return __builtin_bit_cast(x8, both);
     }
+
+    // One element.
+    static __device__ __forceinline__ uint16_t bits(const lds_char *tile, int row, int column) {
+        const int chunk = (column >> 3) ^ swizzle(row);
+        return *(const __attribute__((address_space(3))) uint16_t *)(tile + row * DIM * 2 +
+                                                                      chunk * 16 + (column & 7) * 2);
+    }
 };
 
 }  // namespace gs
