@@ -587,8 +587,9 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
     const float c = a.scale * kLog2e;
     const auto copy_q = QTile::copy_of(wave, a.q_row, a.dim);
     const auto copy_g = QTile::copy_of(wave, go_row, a.dim);
-    const auto fetch = [&](int i, int head, int t) {
+    const auto fetch = [&](int i) {
         lds_char *to = tiles + (i & 1) * kStage;
+        const int t = end_tile - 1 - i / group, head = kh * group + i % group;
         const int64_t row = p.q0 + (int64_t)t * kBackRows;
         const int present = p.lq - t * kBackRows;
         QTile::start(copy_q, wave, q + row * a.q_row + head * a.q_head, a.q_row, present, a.dim, to);
@@ -604,12 +605,12 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
 #pragma unroll
     for (int d = 0; d < DIM / 32; ++d) gk[d] = gv[d] = f32x16{};
 
-    const auto step = [&](int i, int t, auto masks) {
+    const auto step = [&](int i, auto masks) {
         constexpr bool kMasks = decltype(masks)::value;
         constexpr int kUnroll = kMasks ? 1 : 2;
         const lds_char *qt = tiles + (i & 1) * kStage, *gt = qt + QTile::kBytes;
         const lds_char *logs = gt + QTile::kBytes, *deltas = logs + kFloats;
-        const int query0 = t * kBackRows;
+        const int query0 = (end_tile - 1 - i / group) * kBackRows;
         uint64_t found_q = 0, found_g = 0;
         if constexpr (kMasks) {
             found_q = rows_not_finite<T, DIM, kBackRows>(qt, 0);
@@ -653,41 +654,27 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
                 add_product<T, DIM, QTile>(gk, qt, 32 * n, pd);
         }
     };
-    // of every head of the group the tiles with queries that do not see all the keys, then
-    // of every head the others
-    const int part = max(whole_tile - first_tile, 0) * group;
+    // from the last tile back, every head of the group in turn: workgroups that start together
+    // read the same tiles at the same time, also where a causal mask gives them different
+    // first ones; the tiles with queries that do not see all the keys come last
+    const int whole_steps = max(end_tile - whole_tile, 0) * group;
     const int steps_all = max(end_tile - first_tile, 0) * group;
     const int share = (steps_all + splits - 1) / splits;  // this split's steps
     const int first_step = min(split * share, steps_all);
     const int steps = min(first_step + share, steps_all);
-    const auto place = [&](int i, int *tile) {  // the head and tile of a step
-        const int from = i < part ? first_tile : whole_tile;
-        const int per_head = (i < part ? whole_tile : end_tile) - from;
-        const int j = i < part ? i : i - part;
-        *tile = from + j % per_head;
-        return kh * group + j / per_head;
-    };
     const auto begin = [&](int i) {
         __syncthreads();  // tile i is in LDS, and tile i - 1 has been read
-        if (i + 1 < steps) {
-            int tile;
-            const int head = place(i + 1, &tile);
-            fetch(i + 1, head, tile);
-        }
+        if (i + 1 < steps) fetch(i + 1);
     };
-    int tile, i = first_step;
-    if (i < steps) {
-        const int head = place(i, &tile);
-        fetch(i, head, tile);
-    }
-    for (; i < min(part, steps); ++i) {
+    int i = first_step;
+    if (i < steps) fetch(i);
+    for (; i < min(whole_steps, steps); ++i) {
         begin(i);
-        place(i, &tile);
-        step(i, tile, std::true_type{});
+        step(i, std::false_type{});
     }
     for (; i < steps; ++i) {
         begin(i);
-        step(i, 0, std::false_type{});
+        step(i, std::true_type{});
     }
     // keys past the length that counts have no gradient
     if (__ballot(!counts)) {
