@@ -27,10 +27,62 @@ inline int with_element(int32_t type, F f) {
     }
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = kWave / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+// v of the lane that differs in the bits of a pattern, within 16 lanes.
+template <int PATTERN>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                                         0, __builtin_bit_cast(int, v), PATTERN, 0xf, 0xf, true));
+}
+
+// The sum over LANES (16 or 64) neighbouring lanes, in each: quad permutations, the
+// mirrors of 8 and of 16 lanes, then exchanges of 16 and of 32 lanes.  No LDS.
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float v) {
+    static_assert(LANES == 16 || LANES == 64, "a row of lanes or a wave");
+    v += dpp<0xb1>(v);
+    v += dpp<0x4e>(v);
+    v += dpp<0x141>(v);
+    v += dpp<0x140>(v);
+    if constexpr (LANES == 64) {
+        uint32_t u = __builtin_bit_cast(uint32_t, v);
+        const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        v = __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
+        u = __builtin_bit_cast(uint32_t, v);
+        const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        v = __builtin_bit_cast(float, (uint32_t)b[0]) + __builtin_bit_cast(float, (uint32_t)b[1]);
+    }
     return v;
+}
+
+__device__ __forceinline__ float wave_sum(float v) { return lane_sum<kWave>(v); }
+
+// N neighbouring elements, read or written as one access.
+template <typename T, int N>
+struct Pack {
+    typedef T type __attribute__((ext_vector_type(N)));
+};
+template <typename T>
+struct Pack<T, 1> {
+    typedef T type;
+};
+template <typename T, int N>
+__device__ __forceinline__ void load_floats(const T *p, float *v) {
+    const auto x = *(const typename Pack<T, N>::type *)p;
+    if constexpr (N == 1)
+        v[0] = to_float(x);
+    else
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = to_float((T)x[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_floats(T *p, const float *v) {
+    typename Pack<T, N>::type x;
+    if constexpr (N == 1)
+        x = from_float<T>(v[0]);
+    else
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = from_float<T>(v[i]);
+    *(typename Pack<T, N>::type *)p = x;
 }
 
 }  // namespace gs

@@ -3,93 +3,281 @@
 //   dx = r (g - mean(g) - h mean(g h)) with g = dy w,  dw = sum dy h,  db = sum dy
 // the means over a row's channels, the sums over the rows.  All arithmetic is in
 // float; an output is rounded once.
+//
+// Bound by memory: forward reads x and writes y, backward reads x and dy and writes dx,
+// each once.  A row is held in the registers of 16 lanes, a wave or a workgroup, so the
+// variance is taken of differences to the mean without a second read; the backward
+// keeps the weight's sums of its rows in registers too, joins its waves in LDS, and a
+// second launch adds up the workgroups' sums in an order that the sizes alone give.
+
+#include <initializer_list>
+#include <type_traits>
 
 #include "element.h"
 
 namespace gs {
 
 constexpr int kNormBlock = 256;
-constexpr int kNormSplits = 512;  // most row ranges of the weight's gradient
+constexpr int kNormGroups = 1024;  // most workgroups of a backward
 
-// The sums of a and b over the workgroup, in every thread.
-__device__ __forceinline__ float2 block_sum2(float a, float b) {
-    __shared__ float2 part[kNormBlock / kWave];
-    a = wave_sum(a);
-    b = wave_sum(b);
-    __syncthreads();  // an earlier call's values have been read
-    if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = make_float2(a, b);
-    __syncthreads();
-    float2 s = part[0];
+// How a row lies in registers: LANES lanes, SLOTS packs of VEC elements in each; pack i of
+// lane l is number i * LANES + l of the row.
+template <int LANES_, int SLOTS_, int VEC_>
+struct Shape {
+    static constexpr int kLanes = LANES_, kSlots = SLOTS_, kVec = VEC_;
+    static constexpr int kRows = kNormBlock / kLanes;  // of a workgroup at a time
+    static constexpr int kHeld = kSlots * kVec;
+};
+
+// The sums of two values over a row's lanes, in all of them.
+template <int LANES>
+__device__ __forceinline__ float2 row_sum(float a, float b) {
+    if constexpr (LANES <= kWave) {
+        return make_float2(lane_sum<LANES>(a), lane_sum<LANES>(b));
+    } else {
+        __shared__ float2 part[LANES / kWave];
+        a = lane_sum<kWave>(a);
+        b = lane_sum<kWave>(b);
+        __syncthreads();  // an earlier call's values have been read
+        if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = make_float2(a, b);
+        __syncthreads();
+        float2 s = part[0];
 #pragma unroll
-    for (int w = 1; w < kNormBlock / kWave; ++w) {
-        s.x += part[w].x;
-        s.y += part[w].y;
+        for (int w = 1; w < LANES / kWave; ++w) {
+            s.x += part[w].x;
+            s.y += part[w].y;
+        }
+        return s;
     }
-    return s;
 }
 
-template <typename T, typename W>
+// A weight or bias vector of any of the types, or nothing.
+struct Weights {
+    const void *p;
+    int32_t type;
+};
+
+template <int VEC>
+__device__ __forceinline__ void load_weights(const Weights &w, int at, float none, float *v) {
+    if (!w.p) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = none;
+    } else if (w.type == GS_F32) {
+        load_floats<float, VEC>((const float *)w.p + at, v);
+    } else if (w.type == GS_F16) {
+        load_floats<f16, VEC>((const f16 *)w.p + at, v);
+    } else {
+        load_floats<bf16, VEC>((const bf16 *)w.p + at, v);
+    }
+}
+
+// The lane's packs of a row; zeros past its end.
+template <typename S, typename T>
+__device__ __forceinline__ void load_row(const T *row, int lane, int channels, float *v) {
+#pragma unroll
+    for (int i = 0; i < S::kSlots; ++i) {
+        const int at = (i * S::kLanes + lane) * S::kVec;
+        if (at < channels) {
+            load_floats<T, S::kVec>(row + at, v + i * S::kVec);
+        } else {
+#pragma unroll
+            for (int j = 0; j < S::kVec; ++j) v[i * S::kVec + j] = 0.0f;
+        }
+    }
+}
+
+template <typename T, typename S>
 __global__ __launch_bounds__(kNormBlock) void layer_norm_kernel(
-    const T *__restrict__ x, int64_t x_stride, const W *__restrict__ weight,
-    const W *__restrict__ bias, int64_t rows, int channels, float eps, T *__restrict__ y,
-    float2 *__restrict__ stats) {
+    const T *__restrict__ x, int64_t x_stride, Weights weight, Weights bias, int64_t rows,
+    int channels, float eps, T *__restrict__ y, float2 *__restrict__ stats) {
+    const int lane = threadIdx.x % S::kLanes;
+    const int64_t first = (int64_t)blockIdx.x * S::kRows + threadIdx.x / S::kLanes;
+    const float n = (float)channels;
+    // (rows a workgroup long: all its threads leave the loop together)
+    for (int64_t row = first; row < rows; row += (int64_t)gridDim.x * S::kRows) {
+        float v[S::kHeld];
+        load_row<S>(x + row * x_stride, lane, channels, v);
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::kHeld; ++i) s += v[i];
+        const float mean = row_sum<S::kLanes>(s, 0.0f).x / n;
+        float q = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::kSlots; ++i)
+            if ((i * S::kLanes + lane) * S::kVec < channels) {
+#pragma unroll
+                for (int j = 0; j < S::kVec; ++j) {
+                    float &d = v[i * S::kVec + j];
+                    d -= mean;
+                    q = fmaf(d, d, q);
+                }
+            }
+        const float r = 1.0f / sqrtf(row_sum<S::kLanes>(q, 0.0f).x / n + eps);
+#pragma unroll
+        for (int i = 0; i < S::kSlots; ++i) {
+            const int at = (i * S::kLanes + lane) * S::kVec;
+            if (at >= channels) continue;
+            float w[S::kVec], b[S::kVec];
+            load_weights<S::kVec>(weight, at, 1.0f, w);
+            load_weights<S::kVec>(bias, at, 0.0f, b);
+#pragma unroll
+            for (int j = 0; j < S::kVec; ++j) w[j] = fmaf(v[i * S::kVec + j] * r, w[j], b[j]);
+            store_floats<T, S::kVec>(y + row * channels + at, w);
+        }
+        if (stats && lane == 0) stats[row] = make_float2(mean, r);
+    }
+}
+
+// partial[workgroup][0..1][channel]: the workgroup's sums of dy h and of dy.
+template <typename T, typename S, bool SUMS>
+__global__ __launch_bounds__(kNormBlock) void layer_norm_backward_kernel(
+    const T *__restrict__ dy, int64_t dy_stride, const T *__restrict__ x, int64_t x_stride,
+    Weights weight, const float2 *__restrict__ stats, int64_t rows, int channels,
+    T *__restrict__ dx, float *__restrict__ partial) {
+    const int lane = threadIdx.x % S::kLanes, group = threadIdx.x / S::kLanes;
+    const float n = (float)channels;
+    float w[S::kHeld], sum_w[SUMS ? S::kHeld : 1], sum_b[SUMS ? S::kHeld : 1];
+#pragma unroll
+    for (int i = 0; i < S::kSlots; ++i) {
+        const int at = (i * S::kLanes + lane) * S::kVec;
+        load_weights<S::kVec>(at < channels ? weight : Weights{nullptr, GS_F32}, at, 1.0f,
+                              w + i * S::kVec);
+    }
+    if constexpr (SUMS)
+#pragma unroll
+        for (int i = 0; i < S::kHeld; ++i) sum_w[i] = sum_b[i] = 0.0f;
+    for (int64_t row = (int64_t)blockIdx.x * S::kRows + group; row < rows;
+         row += (int64_t)gridDim.x * S::kRows) {
+        float g[S::kHeld], h[S::kHeld];
+        load_row<S>(dy + row * dy_stride, lane, channels, g);
+        load_row<S>(x + row * x_stride, lane, channels, h);
+        const float2 st = stats[row];
+        float a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::kHeld; ++i) {
+            h[i] = (h[i] - st.x) * st.y;
+            if constexpr (SUMS) {
+                sum_w[i] = fmaf(g[i], h[i], sum_w[i]);
+                sum_b[i] += g[i];
+            }
+            g[i] *= w[i];
+            a += g[i];  // (both are 0 past the row's end: g is)
+            b = fmaf(g[i], h[i], b);
+        }
+        if (!dx) continue;
+        const float2 m = row_sum<S::kLanes>(a, b);
+        const float ma = m.x / n, mb = m.y / n;
+#pragma unroll
+        for (int i = 0; i < S::kSlots; ++i) {
+            const int at = (i * S::kLanes + lane) * S::kVec;
+            if (at >= channels) continue;
+#pragma unroll
+            for (int j = 0; j < S::kVec; ++j) {
+                const int e = i * S::kVec + j;
+                g[e] = st.y * (g[e] - ma - h[e] * mb);
+            }
+            store_floats<T, S::kVec>(dx + row * channels + at, g + i * S::kVec);
+        }
+    }
+    if constexpr (SUMS) {
+        // the workgroup's rows of lanes, one pack after another
+        __shared__ float joined[S::kRows > 1 ? 2 * kNormBlock * S::kVec : 1];
+        float *to = partial + (int64_t)blockIdx.x * 2 * channels;
+#pragma unroll
+        for (int i = 0; i < S::kSlots; ++i) {
+            const int at = (i * S::kLanes + lane) * S::kVec;
+            if constexpr (S::kRows > 1) {
+                __syncthreads();  // the pack before has been read
+#pragma unroll
+                for (int j = 0; j < S::kVec; ++j) {
+                    joined[(2 * j) * kNormBlock + threadIdx.x] = sum_w[i * S::kVec + j];
+                    joined[(2 * j + 1) * kNormBlock + threadIdx.x] = sum_b[i * S::kVec + j];
+                }
+                __syncthreads();
+                if (group == 0 && at < channels) {
+#pragma unroll
+                    for (int j = 0; j < S::kVec; ++j) {
+                        float a = 0.0f, b = 0.0f;
+                        for (int r = 0; r < S::kRows; ++r) {
+                            a += joined[(2 * j) * kNormBlock + r * S::kLanes + lane];
+                            b += joined[(2 * j + 1) * kNormBlock + r * S::kLanes + lane];
+                        }
+                        to[at + j] = a;
+                        to[channels + at + j] = b;
+                    }
+                }
+            } else if (at < channels) {
+#pragma unroll
+                for (int j = 0; j < S::kVec; ++j) {
+                    to[at + j] = sum_w[i * S::kVec + j];
+                    to[channels + at + j] = sum_b[i * S::kVec + j];
+                }
+            }
+        }
+    }
+}
+
+// Rows too long for registers: the row is read once for each of the mean, the variance
+// and the output.
+template <typename T>
+__global__ __launch_bounds__(kNormBlock) void layer_norm_long_kernel(
+    const T *__restrict__ x, int64_t x_stride, Weights weight, Weights bias, int64_t rows,
+    int channels, float eps, T *__restrict__ y, float2 *__restrict__ stats) {
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *xr = x + row * x_stride;
-        T *yr = y + row * channels;
         float s = 0.0f;
         for (int c = threadIdx.x; c < channels; c += kNormBlock) s += to_float(xr[c]);
-        const float mean = block_sum2(s, 0.0f).x / (float)channels;
+        const float mean = row_sum<kNormBlock>(s, 0.0f).x / (float)channels;
         float q = 0.0f;
         for (int c = threadIdx.x; c < channels; c += kNormBlock) {
             const float d = to_float(xr[c]) - mean;
             q = fmaf(d, d, q);
         }
-        const float r = 1.0f / sqrtf(block_sum2(q, 0.0f).x / (float)channels + eps);
+        const float r = 1.0f / sqrtf(row_sum<kNormBlock>(q, 0.0f).x / (float)channels + eps);
         for (int c = threadIdx.x; c < channels; c += kNormBlock) {
-            const float h = (to_float(xr[c]) - mean) * r;
-            yr[c] = from_float<T>(fmaf(h, weight ? to_float(weight[c]) : 1.0f,
-                                       bias ? to_float(bias[c]) : 0.0f));
+            float w, b;
+            load_weights<1>(weight, c, 1.0f, &w);
+            load_weights<1>(bias, c, 0.0f, &b);
+            y[row * channels + c] = from_float<T>(fmaf((to_float(xr[c]) - mean) * r, w, b));
         }
         if (stats && threadIdx.x == 0) stats[row] = make_float2(mean, r);
     }
 }
 
-template <typename T, typename W>
-__global__ __launch_bounds__(kNormBlock) void layer_norm_dx_kernel(
+template <typename T>
+__global__ __launch_bounds__(kNormBlock) void layer_norm_long_dx_kernel(
     const T *__restrict__ dy, int64_t dy_stride, const T *__restrict__ x, int64_t x_stride,
-    const W *__restrict__ weight, const float2 *__restrict__ stats, int64_t rows, int channels,
+    Weights weight, const float2 *__restrict__ stats, int64_t rows, int channels,
     T *__restrict__ dx) {
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *xr = x + row * x_stride, *gr = dy + row * dy_stride;
         const float2 st = stats[row];
-        float a = 0.0f, b = 0.0f;
+        float a = 0.0f, b = 0.0f, w;
         for (int c = threadIdx.x; c < channels; c += kNormBlock) {
-            const float g = to_float(gr[c]) * (weight ? to_float(weight[c]) : 1.0f);
+            load_weights<1>(weight, c, 1.0f, &w);
+            const float g = to_float(gr[c]) * w;
             a += g;
             b = fmaf(g, (to_float(xr[c]) - st.x) * st.y, b);
         }
-        const float2 m = block_sum2(a, b);
+        const float2 m = row_sum<kNormBlock>(a, b);
         const float ma = m.x / (float)channels, mb = m.y / (float)channels;
         for (int c = threadIdx.x; c < channels; c += kNormBlock) {
-            const float g = to_float(gr[c]) * (weight ? to_float(weight[c]) : 1.0f);
+            load_weights<1>(weight, c, 1.0f, &w);
+            const float g = to_float(gr[c]) * w;
             const float h = (to_float(xr[c]) - st.x) * st.y;
             dx[row * channels + c] = from_float<T>(st.y * (g - ma - h * mb));
         }
     }
 }
 
-// partial[split][0..1][channel]: sums of dy h and of dy over the split's rows.
 template <typename T>
-__global__ __launch_bounds__(kNormBlock) void layer_norm_dw_kernel(
+__global__ __launch_bounds__(kNormBlock) void layer_norm_long_sums_kernel(
     const T *__restrict__ dy, int64_t dy_stride, const T *__restrict__ x, int64_t x_stride,
-    const float2 *__restrict__ stats, int64_t rows, int channels, int64_t split_rows,
-    float *__restrict__ partial) {
+    const float2 *__restrict__ stats, int64_t rows, int channels, float *__restrict__ partial) {
     const int c = blockIdx.x * kNormBlock + threadIdx.x;
     if (c >= channels) return;
-    const int64_t first = blockIdx.y * split_rows;
-    const int64_t last = first + split_rows < rows ? first + split_rows : rows;
     float w = 0.0f, b = 0.0f;
-    for (int64_t row = first; row < last; ++row) {
+    for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
         const float2 st = stats[row];
         const float g = to_float(dy[row * dy_stride + c]);
         w = fmaf(g, (to_float(x[row * x_stride + c]) - st.x) * st.y, w);
@@ -100,27 +288,86 @@ __global__ __launch_bounds__(kNormBlock) void layer_norm_dw_kernel(
     p[channels] = b;
 }
 
-template <typename W>
-__global__ __launch_bounds__(kNormBlock) void layer_norm_join_kernel(
-    const float *__restrict__ partial, int splits, int channels, W *__restrict__ dw,
-    W *__restrict__ db) {
-    const int c = blockIdx.x * kNormBlock + threadIdx.x;
-    if (c >= channels) return;
-    float w = 0.0f, b = 0.0f;
-    for (int s = 0; s < splits; ++s) {
-        w += partial[(int64_t)s * 2 * channels + c];
-        b += partial[(int64_t)s * 2 * channels + channels + c];
+// The sums of the workgroups' sums: 16 columns of the 2 * channels a workgroup, in 16
+// groups of workgroups each.
+__global__ __launch_bounds__(256) void layer_norm_join_kernel(const float *__restrict__ partial,
+                                                              int groups, int channels,
+                                                              int32_t type, void *__restrict__ dw,
+                                                              void *__restrict__ db) {
+    __shared__ float part[16][17];
+    const int across = threadIdx.x % 16, down = threadIdx.x / 16;
+    const int c = blockIdx.x * 16 + across;
+    float s = 0.0f;
+    if (c < 2 * channels)
+        for (int g = down; g < groups; g += 16) s += partial[(int64_t)g * 2 * channels + c];
+    part[down][across] = s;
+    __syncthreads();
+    if (down || c >= 2 * channels) return;
+    s = 0.0f;
+#pragma unroll
+    for (int g = 0; g < 16; ++g) s += part[g][across];
+    void *out = c < channels ? dw : db;
+    const int at = c < channels ? c : c - channels;
+    if (!out) return;
+    if (type == GS_F32)
+        ((float *)out)[at] = s;
+    else if (type == GS_F16)
+        ((f16 *)out)[at] = from_float<f16>(s);
+    else
+        ((bf16 *)out)[at] = from_float<bf16>(s);
+}
+
+// Rows of lanes and packs for a number of channels.  VEC is 16 bytes where the channels,
+// the strides and the addresses allow it, else one element.  A row of 16 lanes where
+// that is enough, else a wave, else a workgroup; f gets the shape, or void if the row does
+// not fit in registers.
+template <int VEC, typename F>
+static int with_shape(int channels, F f) {
+    const int packs = (channels + VEC - 1) / VEC;
+    if (packs <= 16) return f(Shape<16, 1, VEC>{});
+    if (packs <= 32) return f(Shape<16, 2, VEC>{});
+    if (packs <= 64) return f(Shape<64, 1, VEC>{});
+    if (packs <= 128) return f(Shape<64, 2, VEC>{});
+    if (packs <= 192) return f(Shape<64, 3, VEC>{});
+    if (packs <= 256) return f(Shape<64, 4, VEC>{});
+    if constexpr (VEC == 1) {
+        if (packs <= 512) return f(Shape<64, 8, VEC>{});
+        if (packs <= 1024) return f(Shape<64, 16, VEC>{});
+        if (packs <= 4096) return f(Shape<256, 16, VEC>{});
+    } else {
+        if (packs <= 512) return f(Shape<256, 2, VEC>{});
+        if (packs <= 1024) return f(Shape<256, 4, VEC>{});
     }
-    if (dw) dw[c] = from_float<W>(w);
-    if (db) db[c] = from_float<W>(b);
+    return f(0);
 }
 
-static int norm_splits(int64_t rows) {
-    const int64_t s = (rows + 15) / 16;
-    return (int)(s < kNormSplits ? s : kNormSplits);
+template <typename T, typename F>
+static int with_shape(int channels, bool wide, F f) {
+    return wide ? with_shape<16 / sizeof(T)>(channels, f) : with_shape<1>(channels, f);
 }
 
-static unsigned norm_grid(int64_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); }
+static bool wide_access(int size, int channels, std::initializer_list<int64_t> strides,
+                        std::initializer_list<const void *> pointers) {
+    const int vec = 16 / size;
+    if (channels % vec) return false;
+    for (int64_t s : strides)
+        if (s % vec) return false;
+    for (const void *p : pointers)
+        if ((uintptr_t)p % 16) return false;
+    return true;
+}
+
+// Workgroups of a backward: as many as the rows give, at most kNormGroups, and at least
+// four rows a row of lanes where there are more.
+static int norm_groups(int64_t rows) {
+    const int64_t g = (rows + 15) / 16;
+    return (int)(g < kNormGroups ? g : kNormGroups);
+}
+
+static unsigned norm_grid(int64_t rows, int at_once) {
+    const int64_t g = (rows + at_once - 1) / at_once;
+    return (unsigned)(g < 65536 ? g : 65536);
+}
 
 }  // namespace gs
 
@@ -135,13 +382,20 @@ extern "C" int gs_layer_norm_forward(const void *x, int64_t x_stride, const void
         return GS_ERR_INVALID_ARGUMENT;
     if (rows == 0) return GS_OK;
     if (!x || !y) return GS_ERR_INVALID_ARGUMENT;
+    const bool wide = wide_access(element_size(type), channels, {x_stride}, {x, y, weight, bias});
     return with_element(type, [&](auto t) {
-        return with_element(weight_type, [&](auto w) {
-            using T = decltype(t);
-            using W = decltype(w);
-            hipLaunchKernelGGL((layer_norm_kernel<T, W>), dim3(norm_grid(rows)), dim3(kNormBlock),
-                               0, stream, (const T *)x, x_stride, (const W *)weight,
-                               (const W *)bias, rows, channels, eps, (T *)y, (float2 *)stats);
+        using T = decltype(t);
+        return with_shape<T>(channels, wide, [&](auto shape) {
+            using S = decltype(shape);
+            const Weights w = {weight, weight_type}, b = {bias, weight_type};
+            if constexpr (std::is_same<S, int>::value)
+                hipLaunchKernelGGL((layer_norm_long_kernel<T>), dim3(norm_grid(rows, 1)),
+                                   dim3(kNormBlock), 0, stream, (const T *)x, x_stride, w, b, rows,
+                                   channels, eps, (T *)y, (float2 *)stats);
+            else
+                hipLaunchKernelGGL((layer_norm_kernel<T, S>), dim3(norm_grid(rows, S::kRows)),
+                                   dim3(kNormBlock), 0, stream, (const T *)x, x_stride, w, b, rows,
+                                   channels, eps, (T *)y, (float2 *)stats);
             return launch_status();
         });
     });
@@ -150,7 +404,7 @@ extern "C" int gs_layer_norm_forward(const void *x, int64_t x_stride, const void
 extern "C" int gs_layer_norm_backward_workspace_size(int64_t rows, int32_t channels,
                                                      size_t *bytes) {
     if (rows < 0 || channels <= 0 || !bytes) return GS_ERR_INVALID_ARGUMENT;
-    *bytes = (size_t)norm_splits(rows) * 2 * channels * sizeof(float);
+    *bytes = (size_t)norm_groups(rows) * 2 * channels * sizeof(float);
     return GS_OK;
 }
 
@@ -165,39 +419,53 @@ extern "C" int gs_layer_norm_backward(const void *grad_y, int64_t grad_y_stride,
         return GS_ERR_INVALID_ARGUMENT;
     if (rows > 0 && (!grad_y || !x || !stats)) return GS_ERR_INVALID_ARGUMENT;
     const bool sums = grad_weight || grad_bias;
-    const int splits = norm_splits(rows);
+    const int groups = norm_groups(rows);
     if (sums && rows > 0) {
         if (!workspace) return GS_ERR_INVALID_ARGUMENT;
-        if (workspace_bytes < (size_t)splits * 2 * channels * sizeof(float))
+        if (workspace_bytes < (size_t)groups * 2 * channels * sizeof(float))
             return GS_ERR_WORKSPACE_TOO_SMALL;
     }
-    return with_element(type, [&](auto t) {
-        return with_element(weight_type, [&](auto w) {
+    if (rows > 0 && (sums || grad_x)) {
+        const bool wide = wide_access(element_size(type), channels, {x_stride, grad_y_stride},
+                                      {x, grad_y, grad_x, weight});
+        const int st = with_element(type, [&](auto t) {
             using T = decltype(t);
-            using W = decltype(w);
-            const dim3 block(kNormBlock);
-            int st = GS_OK;
-            if (grad_x && rows > 0) {
-                hipLaunchKernelGGL((layer_norm_dx_kernel<T, W>), dim3(norm_grid(rows)), block, 0,
-                                   stream, (const T *)grad_y, grad_y_stride, (const T *)x,
-                                   x_stride, (const W *)weight, (const float2 *)stats, rows,
-                                   channels, (T *)grad_x);
-                if ((st = launch_status())) return st;
-            }
-            if (!sums) return st;
-            const int columns = ceil_div(channels, kNormBlock);
-            if (splits > 0) {
-                const int64_t split_rows = (rows + splits - 1) / splits;
-                hipLaunchKernelGGL((layer_norm_dw_kernel<T>), dim3(columns, splits), block, 0,
-                                   stream, (const T *)grad_y, grad_y_stride, (const T *)x,
-                                   x_stride, (const float2 *)stats, rows, channels, split_rows,
-                                   (float *)workspace);
-                if ((st = launch_status())) return st;
-            }
-            hipLaunchKernelGGL((layer_norm_join_kernel<W>), dim3(columns), block, 0, stream,
-                               (const float *)workspace, splits, channels, (W *)grad_weight,
-                               (W *)grad_bias);
-            return launch_status();
+            return with_shape<T>(channels, wide, [&](auto shape) {
+                using S = decltype(shape);
+                const Weights w = {weight, weight_type};
+                const dim3 block(kNormBlock);
+                float *partial = (float *)workspace;
+                if constexpr (std::is_same<S, int>::value) {
+                    if (grad_x)
+                        hipLaunchKernelGGL((layer_norm_long_dx_kernel<T>), dim3(norm_grid(rows, 1)),
+                                           block, 0, stream, (const T *)grad_y, grad_y_stride,
+                                           (const T *)x, x_stride, w, (const float2 *)stats, rows,
+                                           channels, (T *)grad_x);
+                    if (sums)
+                        hipLaunchKernelGGL((layer_norm_long_sums_kernel<T>),
+                                           dim3(ceil_div(channels, kNormBlock), groups), block, 0,
+                                           stream, (const T *)grad_y, grad_y_stride, (const T *)x,
+                                           x_stride, (const float2 *)stats, rows, channels, partial);
+                } else if (sums) {
+                    hipLaunchKernelGGL((layer_norm_backward_kernel<T, S, true>), dim3(groups), block,
+                                       0, stream, (const T *)grad_y, grad_y_stride, (const T *)x,
+                                       x_stride, w, (const float2 *)stats, rows, channels,
+                                       (T *)grad_x, partial);
+                } else {
+                    hipLaunchKernelGGL((layer_norm_backward_kernel<T, S, false>),
+                                       dim3(norm_grid(rows, S::kRows)), block, 0, stream,
+                                       (const T *)grad_y, grad_y_stride, (const T *)x, x_stride, w,
+                                       (const float2 *)stats, rows, channels, (T *)grad_x,
+                                       (float *)nullptr);
+                }
+                return launch_status();
+            });
         });
-    });
+        if (st) return st;
+    }
+    if (!sums) return GS_OK;
+    hipLaunchKernelGGL(layer_norm_join_kernel, dim3(ceil_div(2 * (int64_t)channels, 16)), dim3(256),
+                       0, stream, (const float *)workspace, rows > 0 ? groups : 0, channels,
+                       weight_type, grad_weight, grad_bias);
+    return launch_status();
 }
