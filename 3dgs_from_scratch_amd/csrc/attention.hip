@@ -250,7 +250,7 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
 
     const auto step = [&](int t, auto masks) {
         constexpr bool kMasks = decltype(masks)::value;
-        __syncthreads();  // tile t is in LDS, and tile t - 1 has been read
+        copies_done();  // tile t is in LDS, and tile t - 1 has been read
         if (t + 1 < end_tile) fetch(t + 1);
         const lds_char *kt = tiles + (t & 1) * 2 * KTile::kBytes, *vt = kt + KTile::kBytes;
         const int base = BY_KEYS ? 32 * wave : 0;  // of this wave's keys in the tile
@@ -500,7 +500,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
 
     const auto step = [&](int t, auto masks) {
         constexpr bool kMasks = decltype(masks)::value;
-        __syncthreads();  // tile t is in LDS, and tile t - 1 has been read
+        copies_done();  // tile t is in LDS, and tile t - 1 has been read
         if (t + 1 < end_tile) fetch(t + 1);
         const lds_char *kt = tiles + (t & 1) * 2 * KTile::kBytes, *vt = kt + KTile::kBytes;
         const int key0 = t * kBackRows;
@@ -663,7 +663,7 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
     const int first_step = min(split * share, steps_all);
     const int steps = min(first_step + share, steps_all);
     const auto begin = [&](int i) {
-        __syncthreads();  // tile i is in LDS, and tile i - 1 has been read
+        copies_done();  // tile i is in LDS, and tile i - 1 has been read
         if (i + 1 < steps) fetch(i + 1);
     };
     int i = first_step;

@@ -158,10 +158,18 @@ __device__ __forceinline__ bool find_tile(const int32_t *offsets, int sequences,
 }
 
 // -------------------------------------------------------------------- tiles
+// The workgroup's copies into LDS that were started before are done, and its reads of LDS
+// too.  A barrier alone does not wait for copies: to the compiler they are loads whose
+// results nobody has asked for.
+__device__ __forceinline__ void copies_done() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 // Four rows of the column that this lane gets of its 16 lanes' 4 x 16 block.  Without the
 // restrict the compiler takes any copy to LDS that is under way for one to this address,
-// and waits for the next tile's before the first such read of this one (forward 3%,
-// keys' gradients 40%); the barrier at a tile's start is what orders them.
+// and waits for the next tile's before the first such read of this one; copies_done() at a
+// tile's start is what orders them.
 typedef __attribute__((address_space(3))) i16x4 lds_x4;
 __device__ __forceinline__ i16x4 transposed(const lds_x4 *__restrict__ p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_x4 *)p);

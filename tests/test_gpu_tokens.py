@@ -400,6 +400,32 @@ def test_attention_over_a_cache(gpu, new, causal, dim):
                         causal=causal, go=go)
 
 
+def test_attention_over_long_caches(gpu):
+    """A gigabyte of cache, so that copies of tiles wait for memory; the same twice over."""
+    lengths = [30_000, 32_640, 3, 2500, 18_967, 7600, 21_404, 8160]
+    slab, n = 32_640, len(lengths)
+    lk = torch.tensor(lengths, dtype=torch.int32, device=gpu)
+    for dtype in TYPES[1:]:
+        q, k, v, _ = attention_inputs(gpu, n, n * slab, 16, 8, 128, dtype)
+        args = (q, k, v, offsets_of([1] * n, gpu), offsets_of([slab] * n, gpu), lk)
+        first = check_attention(*args, causal=True)[0]
+        for _ in range(5):
+            assert torch.equal(cr.packed_attention(*args, causal=True), first)
+
+
+def test_attention_twice_over(gpu):
+    """Many workgroups at work: the same values every time, gradients too."""
+    q, k, v, go = attention_inputs(gpu, 9000, 9000, 8, 2, 128, torch.bfloat16)
+    at = offsets_of([4000, 5000], gpu)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    first = None
+    for _ in range(4):
+        out = cr.packed_attention(*leaves, at, causal=True)
+        got = (out.detach(), *torch.autograd.grad(out, leaves, go))
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
 def test_attention_rows_of_no_sequence(gpu):
     q, k, v, go = attention_inputs(gpu, 150, 150, 2, 2, 64, torch.float16)
     k[:9], v[140:], k[145:] = math.nan, math.nan, math.inf
