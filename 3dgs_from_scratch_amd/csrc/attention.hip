@@ -39,11 +39,22 @@ struct RowOperand {
     }
 };
 
-// One 32x32 result of a wave's 32 columns, DIM rows: written as 16-bit rows of the
-// columns' own addresses.
+// 32x32 results of a wave's 32 columns, DIM rows in all, written as 16-bit rows of the
+// columns' own addresses (none where that is null); with_rest: to `rest` what the rounding
+// took away.  Every lane calls it, with the same with_rest.
 template <typename T, int DIM>
-__device__ __forceinline__ void store_columns(const f32x16 *acc, float factor, T *row, int dim) {
+__device__ __forceinline__ void store_columns(const f32x16 *acc, float factor, T *row, int dim,
+                                              bool with_rest = false, T *rest = nullptr) {
     const int h = __lane_id() >> 5;
+    // a half holds rows 4 h + 0..3 and 8 + 4 h + 0..3; after the exchange half h holds
+    // 8 h + 0..7
+    const auto put = [&](T *to, const float *v, int at) {
+        const u32x4 w = __builtin_bit_cast(u32x4, pack8<T>(v));
+        const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+        const auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+        const u32x4 o = {(uint32_t)a[0], (uint32_t)b[0], (uint32_t)a[1], (uint32_t)b[1]};
+        if (to && at < dim) *(u32x4 *)(to + at) = o;
+    };
 #pragma unroll
     for (int d = 0; d < DIM / 32; ++d) {
 #pragma unroll
@@ -51,14 +62,13 @@ __device__ __forceinline__ void store_columns(const f32x16 *acc, float factor, T
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = acc[d][8 * g + i] * factor;
-            const u32x4 w = __builtin_bit_cast(u32x4, pack8<T>(v));
-            // a half holds rows 4 h + 0..3 and 8 + 4 h + 0..3; after the exchange
-            // half h holds 8 h + 0..7
-            const auto lo = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
-            const auto hi = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-            const u32x4 o = {(uint32_t)lo[0], (uint32_t)hi[0], (uint32_t)lo[1], (uint32_t)hi[1]};
             const int at = 32 * d + 16 * g + 8 * h;
-            if (row && at < dim) *(u32x4 *)(row + at) = o;
+            put(row, v, at);
+            if (with_rest) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] -= to_float(from_float<T>(v[i]));
+                put(rest, v, at);
+            }
         }
     }
 }
@@ -189,7 +199,7 @@ struct Partial {
 template <typename T, int DIM, bool BY_KEYS>
 __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel(
     GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-    T *__restrict__ out, float *__restrict__ log_sum, Partial partial) {
+    T *__restrict__ out, T *__restrict__ out_rest, float *__restrict__ log_sum, Partial partial) {
     using F = Forward<T, DIM, BY_KEYS>;
     using KTile = typename F::KTile;
     __shared__ __attribute__((aligned(1024))) char lds[F::kLds];
@@ -372,7 +382,8 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[d][r] = none ? 0.0f : acc[d][r];
     }
-    store_columns<T, DIM>(acc, none ? 1.0f : 1.0f / sum, real ? out + at * a.dim : nullptr, a.dim);
+    store_columns<T, DIM>(acc, none ? 1.0f : 1.0f / sum, real ? out + at * a.dim : nullptr, a.dim,
+                          out_rest != nullptr, real && out_rest ? out_rest + at * a.dim : nullptr);
     if (log_sum && real && half == 0)
         log_sum[at] = none ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
@@ -381,6 +392,7 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
 template <typename T>
 __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int dim, Partial partial,
                                                              T *__restrict__ out,
+                                                             T *__restrict__ out_rest,
                                                              float *__restrict__ log_sum) {
     const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
     if (row >= rows) return;
@@ -403,10 +415,16 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
         y = fmaf(o.y, w, y);
     }
     const bool none = top == -INFINITY;
-    const float r = none ? 0.0f : 1.0f / sum;
+    const float r = 1.0f / sum;
     if (in) {
-        const typename Vec<T>::x2 o = {(T)(x * r), (T)(y * r)};
+        x = none ? 0.0f : x * r;
+        y = none ? 0.0f : y * r;
+        const typename Vec<T>::x2 o = {(T)x, (T)y};
         *(typename Vec<T>::x2 *)(out + row * dim + 2 * lane) = o;
+        if (out_rest) {
+            const typename Vec<T>::x2 e = {(T)(x - to_float((T)o[0])), (T)(y - to_float((T)o[1]))};
+            *(typename Vec<T>::x2 *)(out_rest + row * dim + 2 * lane) = e;
+        }
     }
     if (log_sum && lane == 0) log_sum[row] = none ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
@@ -423,8 +441,8 @@ constexpr int kBackOwn = 32 * kWaves;     // rows or keys of a workgroup
 template <typename T, int DIM>
 __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
     GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-    const T *__restrict__ out, const float *__restrict__ log_sum, const T *__restrict__ go,
-    int64_t go_row, int64_t go_head, T *__restrict__ dq, float *__restrict__ row_log,
+    const T *__restrict__ out, const T *__restrict__ out_rest, const float *__restrict__ log_sum,
+    const T *__restrict__ go, int64_t go_row, int64_t go_head, T *__restrict__ dq, float *__restrict__ row_log,
     float *__restrict__ row_delta, float *__restrict__ partial, int splits) {
     using KTile = Tile<T, DIM, kBackRows, kWaves>;
     __shared__ __attribute__((aligned(1024))) char lds[4 * KTile::kBytes];
@@ -462,10 +480,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
             a.dim, false);
     gr.load(real ? go + (int64_t)(p.q0 + query) * go_row + (int64_t)head * go_head : nullptr,
             a.dim, false);
+    // delta of the output before it was rounded: the rounded one's error in delta is shared by
+    // all of a row's score gradients, and where these nearly cancel it is most of theirs
     float delta = 0.0f;
-    {
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        const T *from = part ? out_rest : out;
         RowOperand<T, DIM> o;
-        o.load(real ? out + at * a.dim : nullptr, a.dim, false);
+        o.load(real ? from + at * a.dim : nullptr, a.dim, false);
 #pragma unroll
         for (int s = 0; s < DIM / 16; ++s)
 #pragma unroll
@@ -813,20 +835,22 @@ static size_t partial_bytes(const GsAttention &a, int splits) {
 
 template <typename T, int DIM>
 static int launch_forward(const GsAttention &a, const ForwardPlan &f, const void *q, const void *k,
-                          const void *v, void *out, float *log_sum, const Partial &partial,
-                          hipStream_t stream) {
+                          const void *v, void *out, void *out_rest, float *log_sum,
+                          const Partial &partial, hipStream_t stream) {
     const dim3 grid((unsigned)(f.tiles * a.heads_k * f.splits));
     if (f.by_keys)
         hipLaunchKernelGGL((attention_kernel<T, DIM, true>), grid, dim3(64 * kWaves), 0, stream, a,
-                           (const T *)q, (const T *)k, (const T *)v, (T *)out, log_sum, partial);
+                           (const T *)q, (const T *)k, (const T *)v, (T *)out, (T *)out_rest, log_sum,
+                           partial);
     else
         hipLaunchKernelGGL((attention_kernel<T, DIM, false>), grid, dim3(64 * kWaves), 0, stream, a,
-                           (const T *)q, (const T *)k, (const T *)v, (T *)out, log_sum, partial);
+                           (const T *)q, (const T *)k, (const T *)v, (T *)out, (T *)out_rest, log_sum,
+                           partial);
     int st = launch_status();
     if (st || f.splits == 1) return st;
     const int64_t rows = a.rows_q * a.heads_q;
     hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0,
-                       stream, rows, a.dim, partial, (T *)out, log_sum);
+                       stream, rows, a.dim, partial, (T *)out, (T *)out_rest, log_sum);
     return launch_status();
 }
 
@@ -851,13 +875,13 @@ extern "C" int gs_attention_forward_workspace_size(const GsAttention *a, size_t 
 }
 
 extern "C" int gs_attention_forward(const GsAttention *a, const void *q, const void *k,
-                                    const void *v, void *out, float *log_sum, void *workspace,
-                                    size_t workspace_bytes, hipStream_t stream) {
+                                    const void *v, void *out, void *out_rest, float *log_sum,
+                                    void *workspace, size_t workspace_bytes, hipStream_t stream) {
     const int st = check_attention(a);
     if (st) return st;
     if (a->rows_q == 0) return GS_OK;
     if (!q || !out || (a->rows_k > 0 && (!k || !v))) return GS_ERR_INVALID_ARGUMENT;
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(out_rest))
         return GS_ERR_UNSUPPORTED;
     const ForwardPlan f = plan_forward(*a);
     if (f.tiles * a->heads_k * f.splits > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
@@ -870,8 +894,8 @@ extern "C" int gs_attention_forward(const GsAttention *a, const void *q, const v
     partial.max_sum = (float2 *)((float *)workspace + (size_t)f.splits * a->rows_q * a->heads_q * a->dim);
     const auto launch = [&](auto t) {
         return with_tile(a->dim, [&](auto d) {
-            return launch_forward<decltype(t), decltype(d)::value>(*a, f, q, k, v, out, log_sum,
-                                                                   partial, stream);
+            return launch_forward<decltype(t), decltype(d)::value>(
+                *a, f, q, k, v, out, out_rest, log_sum, partial, stream);
         });
     };
     return a->type == GS_F16 ? launch(f16{}) : launch(bf16{});
@@ -886,8 +910,9 @@ extern "C" int gs_attention_backward_workspace_size(const GsAttention *a, size_t
 }
 
 extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const void *k,
-                                     const void *v, const void *out, const float *log_sum,
-                                     const void *grad_out, int64_t grad_out_row,
+                                     const void *v, const void *out, const void *out_rest,
+                                     const float *log_sum, const void *grad_out,
+                                     int64_t grad_out_row,
                                      int64_t grad_out_head, void *grad_q, void *grad_k,
                                      void *grad_v, void *workspace, size_t workspace_bytes,
                                      hipStream_t stream) {
@@ -895,10 +920,10 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
     int st = gs_attention_backward_workspace_size(a, &need);
     if (st) return st;
     if (grad_out_row < 0 || grad_out_head < 0) return GS_ERR_INVALID_ARGUMENT;
-    if (a->rows_q > 0 && (!q || !out || !log_sum || !grad_out || !grad_q || !workspace))
+    if (a->rows_q > 0 && (!q || !out || !out_rest || !log_sum || !grad_out || !grad_q || !workspace))
         return GS_ERR_INVALID_ARGUMENT;
     if (a->rows_k > 0 && (!k || !v || !grad_k || !grad_v)) return GS_ERR_INVALID_ARGUMENT;
-    for (const void *x : {q, k, v, out, grad_out, (const void *)grad_q, (const void *)grad_k,
+    for (const void *x : {q, k, v, out, out_rest, grad_out, (const void *)grad_q, (const void *)grad_k,
                           (const void *)grad_v})
         if (!aligned16(x)) return GS_ERR_UNSUPPORTED;
     if ((grad_out_row | grad_out_head) % 8 != 0 || !tile_stride(grad_out_row, a->dim))
@@ -922,8 +947,9 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
         if (a->rows_q > 0) {
             hipLaunchKernelGGL((attention_dq_kernel<T, kDim>), dim3((unsigned)blocks_q),
                                block, 0, stream, *a, (const T *)q, (const T *)k, (const T *)v,
-                               (const T *)out, log_sum, (const T *)grad_out, grad_out_row,
-                               grad_out_head, (T *)grad_q, row_log, row_delta, partial, b.splits_q);
+                               (const T *)out, (const T *)out_rest, log_sum, (const T *)grad_out,
+                               grad_out_row, grad_out_head, (T *)grad_q, row_log, row_delta, partial,
+                               b.splits_q);
             if (b.splits_q > 1)
                 join(a->rows_q * a->heads_q * a->dim, b.splits_q, 1, a->scale, (T *)grad_q,
                      (T *)nullptr);

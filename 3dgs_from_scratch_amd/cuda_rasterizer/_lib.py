@@ -120,9 +120,9 @@ SIGNATURES.update({
     "gs_axial_rotary": [ctypes.POINTER(GsRotaryTensor), _I32, _P, _I64, _I32, _P,
                         ctypes.POINTER(_I32), _I32, _I64, _I32, _I32, _I32, _I32, _P],
     "gs_attention_forward_workspace_size": [ctypes.POINTER(GsAttention), _PSZ],
-    "gs_attention_forward": [ctypes.POINTER(GsAttention)] + [_P] * 6 + [_SZ, _P],
+    "gs_attention_forward": [ctypes.POINTER(GsAttention)] + [_P] * 7 + [_SZ, _P],
     "gs_attention_backward_workspace_size": [ctypes.POINTER(GsAttention), _PSZ],
-    "gs_attention_backward": [ctypes.POINTER(GsAttention)] + [_P] * 6 + [_I64, _I64]
+    "gs_attention_backward": [ctypes.POINTER(GsAttention)] + [_P] * 7 + [_I64, _I64]
     + [_P] * 4 + [_SZ, _P],
 })
 

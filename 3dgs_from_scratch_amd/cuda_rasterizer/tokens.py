@@ -277,12 +277,14 @@ def _problem(q, k, v, offsets_q, offsets_k, lengths_k, causal, scale):
 
 
 def attention_forward(q, k, v, offsets_q, offsets_k, lengths_k, causal: bool, scale: float,
-                      with_log_sum: bool = True):
-    """(out, log_sum) of checked inputs (see packed_attention); log_sum is what
-    attention_backward reads, None without with_log_sum."""
+                      with_log_sum: bool = True, with_rest: bool = True):
+    """(out, out_rest, log_sum) of checked inputs (see packed_attention).  out_rest is
+    what rounding took from out; attention_backward reads it and log_sum.  None for
+    what is not asked for."""
     q, k, v = _laid_out(q), _laid_out(k), _laid_out(v)
     dev = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    rest = torch.empty(q.shape, dtype=q.dtype, device=dev) if with_rest else None
     log_sum = (torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if with_log_sum else None)
     a = _problem(q, k, v, offsets_q, offsets_k, lengths_k, causal, scale)
     lib = _lib.load()
@@ -290,13 +292,13 @@ def attention_forward(q, k, v, offsets_q, offsets_k, lengths_k, causal: bool, sc
         ws, size = _workspace(lib.gs_attention_forward_workspace_size, ctypes.byref(a), device=dev)
         ev = _lib.timer.record("attention_forward", dev)
         _lib.check(lib.gs_attention_forward(
-            ctypes.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+            ctypes.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(rest),
             _ptr(log_sum), _ptr(ws), size, _lib.stream_of(dev)), "attention_forward")
         _lib.timer.stop(ev, dev)
-    return out, log_sum
+    return out, rest, log_sum
 
 
-def attention_backward(grad_out, q, k, v, out, log_sum, offsets_q, offsets_k, lengths_k,
+def attention_backward(grad_out, q, k, v, out, out_rest, log_sum, offsets_q, offsets_k, lengths_k,
                        causal: bool, scale: float):
     """(grad_q, grad_k, grad_v), contiguous, of attention_forward's out."""
     _check("packed_attention", "grad_out", grad_out, 3, (q.dtype,), q.device)
@@ -313,8 +315,8 @@ def attention_backward(grad_out, q, k, v, out, log_sum, offsets_q, offsets_k, le
         ev = _lib.timer.record("attention_backward", dev)
         _lib.check(lib.gs_attention_backward(
             ctypes.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-            log_sum.data_ptr(), go.data_ptr(), go.stride(0), go.stride(1), gq.data_ptr(),
-            gk.data_ptr(), gv.data_ptr(), _ptr(ws), size, _lib.stream_of(dev)),
+            out_rest.data_ptr(), log_sum.data_ptr(), go.data_ptr(), go.stride(0), go.stride(1),
+            gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _ptr(ws), size, _lib.stream_of(dev)),
             "attention_backward")
         _lib.timer.stop(ev, dev)
     return gq, gk, gv
@@ -323,8 +325,9 @@ def attention_backward(grad_out, q, k, v, out, log_sum, offsets_q, offsets_k, le
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets_q, offsets_k, lengths_k, causal, scale):
-        out, log_sum = attention_forward(q, k, v, offsets_q, offsets_k, lengths_k, causal, scale)
-        ctx.save_for_backward(q, k, v, out, log_sum, offsets_q, offsets_k, lengths_k)
+        args = offsets_q, offsets_k, lengths_k
+        out, rest, log_sum = attention_forward(q, k, v, *args, causal, scale)
+        ctx.save_for_backward(q, k, v, out, rest, log_sum, *args)
         ctx.how = (causal, scale)
         ctx.mark_non_differentiable(log_sum)
         return out, log_sum
@@ -396,5 +399,5 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets_
     if _differentiable(q, k, v):
         out, log_sum = _PackedAttention.apply(*args)
     else:
-        out, log_sum = attention_forward(*args, with_log_sum=return_log_sum)
+        out, _, log_sum = attention_forward(*args, with_log_sum=return_log_sum, with_rest=False)
     return (out, log_sum) if return_log_sum else out

@@ -755,20 +755,21 @@ typedef struct {
 
 /*
  * gs_attention_forward: out = softmax(scale q k^T) v; log_sum, when set, receives
- *   the natural logarithm of each softmax's denominator, (rows_q, heads_q).
- * gs_attention_backward: gradients of q, k and v from out, log_sum and grad_out;
- *   every row is written.  Deterministic: no atomics.
+ *   the natural logarithm of each softmax's denominator, (rows_q, heads_q), and
+ *   out_rest, laid out as out, what rounding took from out.
+ * gs_attention_backward: gradients of q, k and v from out, out_rest, log_sum and
+ *   grad_out; every row is written.  Deterministic: no atomics.
  */
 int gs_attention_forward_workspace_size(const GsAttention *a, size_t *bytes);
 int gs_attention_forward(const GsAttention *a, const void *q, const void *k, const void *v,
-                         void *out, float *log_sum, void *workspace, size_t workspace_bytes,
-                         hipStream_t stream);
+                         void *out, void *out_rest, float *log_sum, void *workspace,
+                         size_t workspace_bytes, hipStream_t stream);
 int gs_attention_backward_workspace_size(const GsAttention *a, size_t *bytes);
 int gs_attention_backward(const GsAttention *a, const void *q, const void *k, const void *v,
-                          const void *out, const float *log_sum, const void *grad_out,
-                          int64_t grad_out_row, int64_t grad_out_head, void *grad_q, void *grad_k,
-                          void *grad_v, void *workspace, size_t workspace_bytes,
-                          hipStream_t stream);
+                          const void *out, const void *out_rest, const float *log_sum,
+                          const void *grad_out, int64_t grad_out_row, int64_t grad_out_head,
+                          void *grad_q, void *grad_k, void *grad_v, void *workspace,
+                          size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -611,5 +611,5 @@ def test_attention_refusals(gpu):
     leaf = q.clone().requires_grad_(True)
     out = cr.packed_attention(leaf, k, v, at)
     with pytest.raises(RuntimeError, match="grad_out"):
-        tokens.attention_backward(out.float(), q, k, v, out, out[..., 0].float(), at, at, None,
+        tokens.attention_backward(out.float(), q, k, v, out, out, out[..., 0].float(), at, at, None,
                                   False, 0.125)

@@ -121,19 +121,20 @@ def test_entry_points_reject_on_the_host():
             (dict(dim=136), -4), (dict(k_row=60), -4), (dict(rows_k=2**31), -4)):
         a = ctypes.byref(_attention_problem(**changes))
         assert forward_size(a, ctypes.byref(size)) == status, changes
-        assert lib.gs_attention_forward(a, some, some, some, some, None, None, 0, None) == status
-        assert lib.gs_attention_backward(a, some, some, some, some, some, some, 64, 64, some, some,
-                                         some, some, 1 << 40, None) == status
+        assert lib.gs_attention_forward(a, some, some, some, some, None, None, None, 0,
+                                        None) == status
+        assert lib.gs_attention_backward(a, *([some] * 7), 64, 64, some, some, some, some, 1 << 40,
+                                         None) == status
     a = ctypes.byref(_attention_problem())
-    assert lib.gs_attention_forward(a, None, some, some, some, None, None, 0, None) == -1
-    assert lib.gs_attention_forward(a, odd, some, some, some, None, None, 0, None) == -4
+    assert lib.gs_attention_forward(a, None, some, some, some, None, None, None, 0, None) == -1
+    assert lib.gs_attention_forward(a, odd, some, some, some, None, None, None, 0, None) == -4
     assert lib.gs_attention_backward_workspace_size(a, ctypes.byref(size)) == 0
-    assert lib.gs_attention_backward(a, some, some, some, some, some, some, 64, 64, some, some,
-                                     some, some, size.value - 1, None) == -2
-    assert lib.gs_attention_backward(a, some, some, some, some, some, some, 60, 64, some, some,
-                                     some, some, size.value, None) == -4
+    assert lib.gs_attention_backward(a, *([some] * 7), 64, 64, some, some, some, some,
+                                     size.value - 1, None) == -2
+    assert lib.gs_attention_backward(a, *([some] * 7), 60, 64, some, some, some, some, size.value,
+                                     None) == -4
     assert lib.gs_attention_forward(ctypes.byref(_attention_problem(rows_q=0)), None, None, None,
-                                    None, None, None, 0, None) == 0
+                                    None, None, None, None, 0, None) == 0
 
 
 def test_python_layer_refuses_cpu_tensors_and_other_things():
