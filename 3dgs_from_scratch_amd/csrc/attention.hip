@@ -147,7 +147,7 @@ __device__ __forceinline__ void add_product_seen(f32x16 *acc, const lds_char *ti
 
 // The same, not rounded, for a sum that is joined later.
 template <int DIM>
-__device__ __forceinline__ void store_partial(const f32x16 *acc, float *row, int dim) {
+__device__ __forceinline__ void store_partial(const f32x16 *acc, float factor, float *row, int dim) {
     const int half = __lane_id() >> 5;
 #pragma unroll
     for (int d = 0; d < DIM / 32; ++d)
@@ -155,8 +155,9 @@ __device__ __forceinline__ void store_partial(const f32x16 *acc, float *row, int
         for (int g = 0; g < 4; ++g) {
             const int column = 32 * d + result_row(4 * g, half);
             if (row && column < dim)
-                *(float4 *)(row + column) = make_float4(acc[d][4 * g], acc[d][4 * g + 1],
-                                                        acc[d][4 * g + 2], acc[d][4 * g + 3]);
+                *(float4 *)(row + column) =
+                    make_float4(acc[d][4 * g] * factor, acc[d][4 * g + 1] * factor,
+                                acc[d][4 * g + 2] * factor, acc[d][4 * g + 3] * factor);
         }
 }
 
@@ -370,8 +371,8 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
     if (partial.splits > 1) {
         const int64_t slot = (int64_t)split * a.rows_q * a.heads_q + at;
         if (real && half == 0) partial.max_sum[slot] = make_float2(top, sum);
-        store_partial<DIM>(acc, real && top != -INFINITY ? partial.sums + slot * a.dim : nullptr,
-                           a.dim);
+        store_partial<DIM>(acc, 1.0f,
+                           real && top != -INFINITY ? partial.sums + slot * a.dim : nullptr, a.dim);
         return;
     }
     // a row that saw nothing: zeros, whatever met them
@@ -435,6 +436,27 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
 // of two) and delta for the second; then the keys' and values', a workgroup a tile of
 // keys, over all the queries of all heads of the group.  Scores are computed again in
 // both: seven products in all where one launch with atomics needs five.
+//
+// Score gradients are rounded to the inputs' type for their products, which adds as much
+// again to the rounding of the result (1.41 times its error in all).  In float16 they are
+// first put into its range: weights times 2^10, so that those of long rows keep their
+// bits, and score gradients times 2^4 over the power of two of the row's largest
+// output gradient, so that neither small gradients vanish nor large ones overflow.  Where
+// rows are summed over, in the keys' launch, that power is the largest so far, and the
+// sums follow it.
+template <typename T>
+struct Range {
+    static constexpr bool kScaled = std::is_same<T, f16>::value;
+    static constexpr float kWeight = kScaled ? 10.0f : 0.0f;  // exponents of two
+    static constexpr float kGradient = 16.0f;
+};
+
+// The power of two at or below v's magnitude; 1 for zero, infinities and NaN.
+__device__ __forceinline__ float power_below(float v) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, v) & 0x7f800000u;
+    return bits == 0 || bits == 0x7f800000u ? 1.0f : __builtin_bit_cast(float, bits);
+}
+
 constexpr int kBackRows = 64;             // of a tile in LDS
 constexpr int kBackOwn = 32 * kWaves;     // rows or keys of a workgroup
 
@@ -443,7 +465,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
     GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
     const T *__restrict__ out, const T *__restrict__ out_rest, const float *__restrict__ log_sum,
     const T *__restrict__ go, int64_t go_row, int64_t go_head, T *__restrict__ dq, float *__restrict__ row_log,
-    float *__restrict__ row_delta, float *__restrict__ partial, int splits) {
+    float *__restrict__ row_delta, float *__restrict__ row_power, float *__restrict__ partial,
+    int splits) {
     using KTile = Tile<T, DIM, kBackRows, kWaves>;
     __shared__ __attribute__((aligned(1024))) char lds[4 * KTile::kBytes];
     lds_char *const tiles = (lds_char *)lds;
@@ -495,13 +518,27 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
                 delta = fmaf(to_float(gr.x[s][i]), to_float(o.x[s][i]), delta);
     }
     delta = half_sum(delta);
+    float power = 1.0f;  // of the row's output gradients
+    if constexpr (Range<T>::kScaled) {
+        float most = 0.0f;
+#pragma unroll
+        for (int s = 0; s < DIM / 16; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(to_float(gr.x[s][i])));
+        most = half_max(most);
+        power = power_below(most);
+        if (real && half == 0 && split == 0)  // (a row of zeros has no say in a tile's)
+            row_power[(int64_t)head * a.rows_q + p.q0 + query] = most > 0.0f ? power : 0.0f;
+    }
+    const float range = Range<T>::kScaled ? Range<T>::kGradient / power : 1.0f;
     // a row that saw nothing has no weights: exp2(x - infinity) = 0
     const float given = real ? log_sum[at] : -INFINITY;
     const float log2_sum = given == -INFINITY ? INFINITY : given * kLog2e;
-    if (real && half == 0 && split == 0) {
+    const float row_exponent = log2_sum - __builtin_amdgcn_logf(range);
+    if (real && half == 0 && split == 0) {  // as the keys' launch uses them
         const int64_t to = (int64_t)head * a.rows_q + p.q0 + query;
-        row_log[to] = log2_sum;
-        row_delta[to] = delta;
+        row_log[to] = log2_sum - Range<T>::kWeight;
+        row_delta[to] = -delta;
     }
 
     const float c = a.scale * kLog2e;
@@ -540,7 +577,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -log2_sum)) * (dp[r] - delta);
+                ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -row_exponent)) * (dp[r] - delta);
                 if (kMasks && key0 + 32 * n + result_row(r, half) > last) ds[r] = 0.0f;
             }
             const typename Vec<T>::x8 x[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
@@ -559,22 +596,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
         step(t, std::false_type{});
     for (; t < end_tile; ++t) step(t, std::true_type{});
     if (splits > 1)
-        store_partial<DIM>(acc, real ? partial + ((int64_t)split * a.rows_q * a.heads_q + at) * a.dim
-                                     : nullptr, a.dim);
+        store_partial<DIM>(acc, 1.0f / range,
+                           real ? partial + ((int64_t)split * a.rows_q * a.heads_q + at) * a.dim
+                                : nullptr,
+                           a.dim);
     else
-        store_columns<T, DIM>(acc, a.scale, real ? dq + at * a.dim : nullptr, a.dim);
+        store_columns<T, DIM>(acc, a.scale / range, real ? dq + at * a.dim : nullptr, a.dim);
 }
 
 template <typename T, int DIM>
 __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_kernel(
     GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
     const T *__restrict__ go, int64_t go_row, int64_t go_head, const float *__restrict__ row_log,
-    const float *__restrict__ row_delta, T *__restrict__ dk, T *__restrict__ dv,
-    float *__restrict__ partial, int splits) {
+    const float *__restrict__ row_delta, const float *__restrict__ row_power, T *__restrict__ dk,
+    T *__restrict__ dv, float *__restrict__ partial, int splits) {
     using QTile = Tile<T, DIM, kBackRows, kWaves>;
     constexpr int kFloats = kBackRows * 4;                         // bytes of one float a row
-    constexpr int kStage = 2 * QTile::kBytes + 1024;               // Q, dout, log-sums, deltas
-    static_assert(2 * kFloats <= 1024, "a tile's rows");
+    constexpr int kStage = 2 * QTile::kBytes + 1024;  // Q, dout, log-sums, deltas, powers
+    static_assert(3 * kFloats <= 1024, "a tile's rows");
     __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
     lds_char *const tiles = (lds_char *)lds;
 
@@ -609,6 +648,9 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
     const float c = a.scale * kLog2e;
     const auto copy_q = QTile::copy_of(wave, a.q_row, a.dim);
     const auto copy_g = QTile::copy_of(wave, go_row, a.dim);
+    // (chosen here: inside, the compiler would index what the function captures by it, and
+    // keep all of that in memory)
+    const float *row_floats = wave == 0 ? row_log : wave == 1 ? row_delta : row_power;
     const auto fetch = [&](int i) {
         lds_char *to = tiles + (i & 1) * kStage;
         const int t = end_tile - 1 - i / group, head = kh * group + i % group;
@@ -618,14 +660,14 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
         QTile::start(copy_g, wave, go + row * go_row + head * go_head, go_row, present, a.dim,
                      to + QTile::kBytes);
         const int64_t f = head * a.rows_q + row;
-        if (wave < 2)
-            QTile::start_floats((wave == 0 ? row_log : row_delta) + f, present,
-                                to + 2 * QTile::kBytes + wave * kFloats);
+        if (wave < (Range<T>::kScaled ? 3 : 2))
+            QTile::start_floats(row_floats + f, present, to + 2 * QTile::kBytes + wave * kFloats);
     };
 
     f32x16 gk[DIM / 32], gv[DIM / 32];
 #pragma unroll
     for (int d = 0; d < DIM / 32; ++d) gk[d] = gv[d] = f32x16{};
+    float power = 0.0f;  // the largest row's so far; gk is in units of it
 
     const auto step = [&](int i, auto masks) {
         constexpr bool kMasks = decltype(masks)::value;
@@ -633,6 +675,21 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
         const lds_char *qt = tiles + (i & 1) * kStage, *gt = qt + QTile::kBytes;
         const lds_char *logs = gt + QTile::kBytes, *deltas = logs + kFloats;
         const int query0 = (end_tile - 1 - i / group) * kBackRows;
+        float range = 1.0f;  // of a score gradient, its weight's 2^10 included
+        if constexpr (Range<T>::kScaled) {
+            const float now = __builtin_bit_cast(
+                float, uniform(__builtin_bit_cast(
+                           int, wave_max(*(const __attribute__((address_space(3))) float *)(
+                                    deltas + kFloats + lane * 4)))));
+            if (now > power) {
+                if (power > 0.0f) {
+#pragma unroll
+                    for (int d = 0; d < DIM / 32; ++d) gk[d] *= power / now;
+                }
+                power = now;
+            }
+            range = power > 0.0f ? Range<T>::kGradient / 1024.0f / power : 0.0f;
+        }
         uint64_t found_q = 0, found_g = 0;
         if constexpr (kMasks) {
             found_q = rows_not_finite<T, DIM, kBackRows>(qt, 0);
@@ -640,7 +697,14 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
         }
 #pragma unroll kUnroll
         for (int n = 0; n < kBackRows / 32; ++n) {
-            f32x16 s = {}, dp = {};
+            using lds_f4 = const __attribute__((address_space(3))) f32x4;
+            f32x16 s = {}, dp;  // dp - delta: the product's sum begins at -delta
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 e = *(lds_f4 *)(deltas + (32 * n + result_row(r, half)) * 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dp[r + j] = e[j];
+            }
 #pragma unroll
             for (int j = 0; j < DIM / 16; ++j) {
                 s = mfma(QTile::along(qt, 32 * n, j), kr.x[j], s);
@@ -649,14 +713,12 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
             float w[16], ds[16];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                using lds_f4 = const __attribute__((address_space(3))) f32x4;
                 const f32x4 l = *(lds_f4 *)(logs + (32 * n + result_row(4 * g, half)) * 4);
-                const f32x4 e = *(lds_f4 *)(deltas + (32 * n + result_row(4 * g, half)) * 4);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int r = 4 * g + j;
                     w[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -l[j]));
-                    ds[r] = w[r] * (dp[r] - e[j]);
+                    ds[r] = (Range<T>::kScaled ? w[r] * range : w[r]) * dp[r];
                     if (kMasks && query0 + 32 * n + result_row(r, half) < own_first)
                         w[r] = ds[r] = 0.0f;
                 }
@@ -684,18 +746,16 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
     const int share = (steps_all + splits - 1) / splits;  // this split's steps
     const int first_step = min(split * share, steps_all);
     const int steps = min(first_step + share, steps_all);
-    const auto begin = [&](int i) {
-        copies_done();  // tile i is in LDS, and tile i - 1 has been read
-        if (i + 1 < steps) fetch(i + 1);
-    };
     int i = first_step;
     if (i < steps) fetch(i);
     for (; i < min(whole_steps, steps); ++i) {
-        begin(i);
+        copies_done();  // tile i is in LDS, and tile i - 1 has been read
+        if (i + 1 < steps) fetch(i + 1);
         step(i, std::false_type{});
     }
     for (; i < steps; ++i) {
-        begin(i);
+        copies_done();
+        if (i + 1 < steps) fetch(i + 1);
         step(i, std::true_type{});
     }
     // keys past the length that counts have no gradient
@@ -709,15 +769,17 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
             }
     }
     const int64_t at = ((int64_t)(p.k0 + key) * a.heads_k + kh) * a.dim;
+    const float back_k = Range<T>::kScaled ? power / Range<T>::kGradient : 1.0f;
+    const float back_v = Range<T>::kScaled ? 1.0f / 1024.0f : 1.0f;
     if (splits > 1) {
         const int64_t size = a.rows_k * a.heads_k * a.dim;
         float *to = partial + split * size + at;
-        store_partial<DIM>(gk, real ? to : nullptr, a.dim);
-        store_partial<DIM>(gv, real ? to + splits * size : nullptr, a.dim);
+        store_partial<DIM>(gk, back_k, real ? to : nullptr, a.dim);
+        store_partial<DIM>(gv, back_v, real ? to + splits * size : nullptr, a.dim);
         return;
     }
-    store_columns<T, DIM>(gk, a.scale, real ? dk + at : nullptr, a.dim);
-    store_columns<T, DIM>(gv, 1.0f, real ? dv + at : nullptr, a.dim);
+    store_columns<T, DIM>(gk, a.scale * back_k, real ? dk + at : nullptr, a.dim);
+    store_columns<T, DIM>(gv, back_v, real ? dv + at : nullptr, a.dim);
 }
 
 // Sums of splits, rounded: the y-th of the launch's outputs, four elements a thread.
@@ -823,9 +885,9 @@ static size_t backward_partials(const GsAttention &a, const BackwardPlan &b) {
     return (q > k ? q : k) * sizeof(float);
 }
 
-// Bytes of the row log-sums and deltas, a multiple of 16.
+// Bytes of the rows' log-sums, deltas and powers, a multiple of 16.
 static size_t backward_rows(const GsAttention &a) {
-    return ((size_t)a.rows_q * a.heads_q * 2 * sizeof(float) + 15) / 16 * 16;
+    return ((size_t)a.rows_q * a.heads_q * 3 * sizeof(float) + 15) / 16 * 16;
 }
 
 static size_t partial_bytes(const GsAttention &a, int splits) {
@@ -934,6 +996,7 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
     const int64_t blocks_k = b.tiles_k * a->heads_k * b.splits_k;
     if (blocks_q > 0x7fffffffLL || blocks_k > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
     float *row_log = (float *)workspace, *row_delta = row_log + a->rows_q * a->heads_q;
+    float *row_power = row_delta + a->rows_q * a->heads_q;
     float *partial = (float *)((char *)workspace + backward_rows(*a));
     const auto launch = [&](auto t, auto d) {
         using T = decltype(t);
@@ -948,8 +1011,8 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
             hipLaunchKernelGGL((attention_dq_kernel<T, kDim>), dim3((unsigned)blocks_q),
                                block, 0, stream, *a, (const T *)q, (const T *)k, (const T *)v,
                                (const T *)out, (const T *)out_rest, log_sum, (const T *)grad_out,
-                               grad_out_row, grad_out_head, (T *)grad_q, row_log, row_delta, partial,
-                               b.splits_q);
+                               grad_out_row, grad_out_head, (T *)grad_q, row_log, row_delta,
+                               row_power, partial, b.splits_q);
             if (b.splits_q > 1)
                 join(a->rows_q * a->heads_q * a->dim, b.splits_q, 1, a->scale, (T *)grad_q,
                      (T *)nullptr);
@@ -960,7 +1023,7 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
             hipLaunchKernelGGL((attention_dkv_kernel<T, kDim>), dim3((unsigned)blocks_k),
                                block, 0, stream, *a, (const T *)q, (const T *)k, (const T *)v,
                                (const T *)grad_out, grad_out_row, grad_out_head, row_log, row_delta,
-                               (T *)grad_k, (T *)grad_v, partial, b.splits_k);
+                               row_power, (T *)grad_k, (T *)grad_v, partial, b.splits_k);
             if (b.splits_k > 1)
                 join(a->rows_k * a->heads_k * a->dim, b.splits_k, 2, a->scale, (T *)grad_k,
                      (T *)grad_v);

@@ -34,27 +34,34 @@ __device__ __forceinline__ float dpp(float v) {
                                          0, __builtin_bit_cast(int, v), PATTERN, 0xf, 0xf, true));
 }
 
-// The sum over LANES (16 or 64) neighbouring lanes, in each: quad permutations, the
+// f over LANES (16 or 64) neighbouring lanes' values, in each: quad permutations, the
 // mirrors of 8 and of 16 lanes, then exchanges of 16 and of 32 lanes.  No LDS.
-template <int LANES>
-__device__ __forceinline__ float lane_sum(float v) {
+template <int LANES, typename F>
+__device__ __forceinline__ float lane_reduce(float v, F f) {
     static_assert(LANES == 16 || LANES == 64, "a row of lanes or a wave");
-    v += dpp<0xb1>(v);
-    v += dpp<0x4e>(v);
-    v += dpp<0x141>(v);
-    v += dpp<0x140>(v);
+    v = f(v, dpp<0xb1>(v));
+    v = f(v, dpp<0x4e>(v));
+    v = f(v, dpp<0x141>(v));
+    v = f(v, dpp<0x140>(v));
     if constexpr (LANES == 64) {
         uint32_t u = __builtin_bit_cast(uint32_t, v);
         const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-        v = __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
+        v = f(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
         u = __builtin_bit_cast(uint32_t, v);
         const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-        v = __builtin_bit_cast(float, (uint32_t)b[0]) + __builtin_bit_cast(float, (uint32_t)b[1]);
+        v = f(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
     }
     return v;
 }
 
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float v) {
+    return lane_reduce<LANES>(v, [](float a, float b) { return a + b; });
+}
 __device__ __forceinline__ float wave_sum(float v) { return lane_sum<kWave>(v); }
+__device__ __forceinline__ float wave_max(float v) {
+    return lane_reduce<kWave>(v, [](float a, float b) { return fmaxf(a, b); });
+}
 
 // N neighbouring elements, read or written as one access.
 template <typename T, int N>

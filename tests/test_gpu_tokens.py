@@ -458,6 +458,24 @@ def test_attention_of_large_scores(gpu, dtype):
     check_attention(q, torch.ones_like(k), v, at, causal=True, go=go)
 
 
+@pytest.mark.parametrize("exponent", [-13, 8])
+def test_attention_of_small_and_large_gradients(gpu, exponent):
+    """float16 output gradients near the type's ends, and of very different rows: no score
+    gradient vanishes or overflows before its product.  Outputs below 2^-14 are rounded to
+    2^-24 units, no other absolute term."""
+    q, k, v, go = attention_inputs(gpu, 600, 600, 4, 2, 64, torch.float16)
+    go = (go * 2.0 ** exponent).half()
+    go[::7] = (go[::7] / 64).half()
+    go[3:9] = 0
+    at = offsets_of([250, 350], gpu)
+    for causal in (False, True):
+        ref = ot.attention(q, k, v, at, causal=causal, grad_out=go)
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = cr.packed_attention(*leaves, at, causal=causal)
+        for name, got in zip(("gq", "gk", "gv"), torch.autograd.grad(out, leaves, go)):
+            within(got, ref[name], 2.0 ** -11 * 1.1 * ref[name + "_slack"] + 2.0 ** -24, name)
+
+
 def test_attention_does_not_see_the_masked(gpu):
     """NaN and infinity in keys and values after a query change nothing before them."""
     for dtype in TYPES[1:]:
