@@ -458,7 +458,7 @@ __device__ __forceinline__ float power_below(float v) {
 }
 
 constexpr int kBackRows = 64;             // of a tile in LDS
-constexpr int kBackOwn = 32 * kWaves;     // rows or keys of a workgroup
+constexpr int kBackOwn = 32 * kWaves;     // rows of a workgroup
 
 template <typename T, int DIM>
 __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
@@ -604,34 +604,46 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
         store_columns<T, DIM>(acc, a.scale / range, real ? dq + at * a.dim : nullptr, a.dim);
 }
 
+// Above 64 dimensions the sums of two waves a SIMD leave no registers for V: it lies in LDS,
+// which then has room for one workgroup of eight waves.
+template <int DIM>
+struct KeysShape {
+    static constexpr bool kValuesInLds = DIM == 96;
+    static constexpr int kWaves = kValuesInLds ? 8 : 4;
+    static constexpr int kOwn = 32 * kWaves;  // keys of a workgroup
+};
+
 template <typename T, int DIM>
-__global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_kernel(
+__global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void attention_dkv_kernel(
     GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
     const T *__restrict__ go, int64_t go_row, int64_t go_head, const float *__restrict__ row_log,
     const float *__restrict__ row_delta, const float *__restrict__ row_power, T *__restrict__ dk,
     T *__restrict__ dv, float *__restrict__ partial, int splits) {
-    using QTile = Tile<T, DIM, kBackRows, kWaves>;
+    using Shape = KeysShape<DIM>;
+    constexpr int kOwn = Shape::kOwn;
+    using QTile = Tile<T, DIM, kBackRows, Shape::kWaves>;
+    using VTile = Tile<T, DIM, kOwn, Shape::kWaves>;
     constexpr int kFloats = kBackRows * 4;                         // bytes of one float a row
     constexpr int kStage = 2 * QTile::kBytes + 1024;  // Q, dout, log-sums, deltas, powers
     static_assert(3 * kFloats <= 1024, "a tile's rows");
-    __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
-    lds_char *const tiles = (lds_char *)lds;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * kStage + (Shape::kValuesInLds ? VTile::kBytes : 0)];
+    lds_char *const tiles = (lds_char *)lds, *const values = tiles + 2 * kStage;
 
     const Place at_grid = place_of(a.heads_k, splits);
     const int kh = at_grid.kh, split = at_grid.split, group = a.heads_q / a.heads_k;
     int sequence, number;
-    if (!find_tile(a.offsets_k, a.sequences, a.rows_k, 1, kBackOwn, at_grid.tile, false,
+    if (!find_tile(a.offsets_k, a.sequences, a.rows_k, 1, kOwn, at_grid.tile, false,
                    &sequence, &number))
         return;
     const Span p = span_of(a, sequence);
     const int lane = __lane_id(), half = lane >> 5, wave = uniform(threadIdx.x / kWave);
-    const int block_key = number * kBackOwn;
+    const int block_key = number * kOwn;
     const int key = block_key + 32 * wave + (lane & 31);  // in the sequence
     const bool real = key < p.k1 - p.k0, counts = key < p.lk;
 
     // queries from `first` on see some key of the workgroup, from `whole` on all of them
     const int shift = a.causal ? p.lk - p.lq : p.lk;
-    const int end_key = min(block_key + kBackOwn, p.lk);
+    const int end_key = min(block_key + kOwn, p.lk);
     const int first = a.causal ? max(block_key - shift, 0) : 0;
     const int whole = a.causal ? max(end_key - 1 - shift, 0) : 0;
     const int first_tile = first / kBackRows;
@@ -643,7 +655,7 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
     const T *value_row = counts ? v + (int64_t)(p.k0 + key) * a.v_row + (int64_t)kh * a.v_head : nullptr;
     RowOperand<T, DIM> kr, vr;
     kr.load(key_row, a.dim, false);
-    vr.load(value_row, a.dim, false);
+    if constexpr (!Shape::kValuesInLds) vr.load(value_row, a.dim, false);
 
     const float c = a.scale * kLog2e;
     const auto copy_q = QTile::copy_of(wave, a.q_row, a.dim);
@@ -668,10 +680,11 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
 #pragma unroll
     for (int d = 0; d < DIM / 32; ++d) gk[d] = gv[d] = f32x16{};
     float power = 0.0f;  // the largest row's so far; gk is in units of it
+    bool bad = false;    // the key is seen by a row with an infinity or NaN
 
     const auto step = [&](int i, auto masks) {
         constexpr bool kMasks = decltype(masks)::value;
-        constexpr int kUnroll = kMasks ? 1 : 2;
+        constexpr int kUnroll = kMasks || DIM > 64 ? 1 : 2;
         const lds_char *qt = tiles + (i & 1) * kStage, *gt = qt + QTile::kBytes;
         const lds_char *logs = gt + QTile::kBytes, *deltas = logs + kFloats;
         const int query0 = (end_tile - 1 - i / group) * kBackRows;
@@ -690,10 +703,23 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
             }
             range = power > 0.0f ? Range<T>::kGradient / 1024.0f / power : 0.0f;
         }
-        uint64_t found_q = 0, found_g = 0;
         if constexpr (kMasks) {
-            found_q = rows_not_finite<T, DIM, kBackRows>(qt, 0);
-            found_g = rows_not_finite<T, DIM, kBackRows>(gt, 0);
+            // rows with infinities or NaN become zeros, for they must not meet the weight 0 of a
+            // key that their query does not see; the gradients of keys that it sees are NaN
+            const uint64_t found = rows_not_finite<T, DIM, kBackRows>(qt, 0) |
+                                   rows_not_finite<T, DIM, kBackRows>(gt, 0);
+            if (found) {
+                const int from = max(own_first - query0, 0);
+                bad = bad || (from < 64 && found >> from != 0);
+                __syncthreads();  // all waves have looked
+                for (int at = threadIdx.x * 16; at < 2 * QTile::kBytes; at += 64 * Shape::kWaves * 16) {
+                    const int row = at % QTile::kBytes / (DIM * 2);
+                    if (found >> row & 1)
+                        *(__attribute__((address_space(3))) u32x4 *)(tiles + (i & 1) * kStage + at) =
+                            u32x4{0, 0, 0, 0};
+                }
+                __syncthreads();
+            }
         }
 #pragma unroll kUnroll
         for (int n = 0; n < kBackRows / 32; ++n) {
@@ -708,7 +734,10 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
 #pragma unroll
             for (int j = 0; j < DIM / 16; ++j) {
                 s = mfma(QTile::along(qt, 32 * n, j), kr.x[j], s);
-                dp = mfma(QTile::along(gt, 32 * n, j), vr.x[j], dp);
+                if constexpr (Shape::kValuesInLds)
+                    dp = mfma(QTile::along(gt, 32 * n, j), VTile::along(values, 32 * wave, j), dp);
+                else
+                    dp = mfma(QTile::along(gt, 32 * n, j), vr.x[j], dp);
             }
             float w[16], ds[16];
 #pragma unroll
@@ -725,17 +754,8 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
             }
             const typename Vec<T>::x8 pw[2] = {pack8<T>(w), pack8<T>(w + 8)};
             const typename Vec<T>::x8 pd[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
-            const auto sees = [&](int i) { return query0 + 32 * n + i >= own_first; };
-            const uint32_t part_q = (uint32_t)(found_q >> (32 * n));
-            const uint32_t part_g = (uint32_t)(found_g >> (32 * n));
-            if (kMasks && part_g)
-                add_product_seen<T, DIM, QTile>(gv, gt, 32 * n, pw, sees);
-            else
-                add_product<T, DIM, QTile>(gv, gt, 32 * n, pw);
-            if (kMasks && part_q)
-                add_product_seen<T, DIM, QTile>(gk, qt, 32 * n, pd, sees);
-            else
-                add_product<T, DIM, QTile>(gk, qt, 32 * n, pd);
+            add_product<T, DIM, QTile>(gv, gt, 32 * n, pw);
+            add_product<T, DIM, QTile>(gk, qt, 32 * n, pd);
         }
     };
     // from the last tile back, every head of the group in turn: workgroups that start together
@@ -747,7 +767,13 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
     const int first_step = min(split * share, steps_all);
     const int steps = min(first_step + share, steps_all);
     int i = first_step;
-    if (i < steps) fetch(i);
+    if (i < steps) {
+        if constexpr (Shape::kValuesInLds)
+            VTile::start(VTile::copy_of(wave, a.v_row, a.dim), wave,
+                         v + (int64_t)(p.k0 + block_key) * a.v_row + (int64_t)kh * a.v_head, a.v_row,
+                         p.lk - block_key, a.dim, values);
+        fetch(i);
+    }
     for (; i < min(whole_steps, steps); ++i) {
         copies_done();  // tile i is in LDS, and tile i - 1 has been read
         if (i + 1 < steps) fetch(i + 1);
@@ -759,17 +785,18 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 64 ? 1 : 2) void attention_dkv_k
         step(i, std::true_type{});
     }
     // keys past the length that counts have no gradient
-    if (__ballot(!counts)) {
+    if (__ballot(!counts || bad)) {
+        const float instead = counts ? NAN : 0.0f;
 #pragma unroll
         for (int d = 0; d < DIM / 32; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                gk[d][r] = counts ? gk[d][r] : 0.0f;
-                gv[d][r] = counts ? gv[d][r] : 0.0f;
+                gk[d][r] = counts && !bad ? gk[d][r] : instead;
+                gv[d][r] = counts && !bad ? gv[d][r] : instead;
             }
     }
     const int64_t at = ((int64_t)(p.k0 + key) * a.heads_k + kh) * a.dim;
-    const float back_k = Range<T>::kScaled ? power / Range<T>::kGradient : 1.0f;
+    const float back_k = Range<T>::kScaled && power > 0.0f ? power / Range<T>::kGradient : 1.0f;
     const float back_v = Range<T>::kScaled ? 1.0f / 1024.0f : 1.0f;
     if (splits > 1) {
         const int64_t size = a.rows_k * a.heads_k * a.dim;
@@ -870,11 +897,11 @@ static BackwardPlan plan_backward(const GsAttention &a) {
     const int64_t sequences = a.sequences > 0 ? a.sequences : 1, see = a.causal ? 2 : 1;
     BackwardPlan b;
     b.tiles_q = packed / kBackOwn + a.sequences + 2;
-    b.tiles_k = a.rows_k / kBackOwn + a.sequences + 2;
+    const int64_t own = a.dim > 96 ? KeysShape<128>::kOwn : a.dim > 64 ? KeysShape<96>::kOwn : KeysShape<64>::kOwn;
+    b.tiles_k = a.rows_k / own + a.sequences + 2;
     b.splits_q = backward_splits((packed + kBackOwn - 1) / kBackOwn * a.heads_k, 512,
                                  a.rows_k / sequences / kBackRows / see);
-    b.splits_k = backward_splits((a.rows_k + kBackOwn - 1) / kBackOwn * a.heads_k,
-                                 a.dim > 64 ? 768 : 1024,
+    b.splits_k = backward_splits((a.rows_k + own - 1) / own * a.heads_k, a.dim > 96 ? 768 : a.dim > 64 ? 384 : 1024,
                                  packed / sequences / kBackRows / see);
     return b;
 }
@@ -1021,8 +1048,8 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
         }
         if (a->rows_k > 0) {
             hipLaunchKernelGGL((attention_dkv_kernel<T, kDim>), dim3((unsigned)blocks_k),
-                               block, 0, stream, *a, (const T *)q, (const T *)k, (const T *)v,
-                               (const T *)grad_out, grad_out_row, grad_out_head, row_log, row_delta,
+                               dim3(64 * KeysShape<kDim>::kWaves), 0, stream, *a, (const T *)q,
+                               (const T *)k, (const T *)v, (const T *)grad_out, grad_out_row, grad_out_head, row_log, row_delta,
                                row_power, (T *)grad_k, (T *)grad_v, partial, b.splits_k);
             if (b.splits_k > 1)
                 join(a->rows_k * a->heads_k * a->dim, b.splits_k, 2, a->scale, (T *)grad_k,

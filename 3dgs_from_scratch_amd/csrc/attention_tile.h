@@ -179,8 +179,9 @@ template <typename T, int DIM, int ROWS, int WAVES>
 struct Tile {
     static constexpr int kChunks = DIM / 8;                      // of a row
     static constexpr int kBytes = ROWS * DIM * 2;
-    static constexpr int kCopies = ROWS * kChunks / (64 * WAVES);  // a wave's, 1 KiB each
-    static_assert(ROWS * kChunks % (64 * WAVES) == 0, "whole waves of chunks");
+    static constexpr int kPieces = ROWS * kChunks / 64;  // of 1 KiB, which a wave copies at once
+    static constexpr int kCopies = (kPieces + WAVES - 1) / WAVES;  // of a wave
+    static_assert(ROWS * kChunks % 64 == 0, "whole waves of chunks");
     using x8 = typename Vec<T>::x8;
 
     // Row r's chunk c lies at chunk c ^ swizzle(r); the same for row r + 8.
@@ -218,9 +219,10 @@ struct Tile {
         const auto from = __builtin_amdgcn_make_buffer_rsrc((void *)first, 0, bytes, 0x00027000);
 #pragma unroll
         for (int i = 0; i < kCopies; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                from, (__attribute__((address_space(3))) void *)(tile + (i * WAVES + wave) * 1024),
-                16, c.from[i], 0, 0, 0);
+            if (kPieces % WAVES == 0 || i * WAVES + wave < kPieces)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    from, (__attribute__((address_space(3))) void *)(tile + (i * WAVES + wave) * 1024),
+                    16, c.from[i], 0, 0, 0);
     }
 
     // Starts the copy of one float a row (64 rows, `present` of them in memory, the rest
