@@ -14,6 +14,7 @@ namespace gs {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kWaves = 4;
+constexpr int kKeysWaves = 2;  // where the waves share the rows
 
 // Factor of a raw score in the exponent of two.  A negative scale turns the queries'
 // sign instead, so that a row's maximum is that of its raw scores; 0 becomes the
@@ -182,37 +183,37 @@ __device__ __forceinline__ Place place_of(int heads_k, int splits) {
 
 template <typename T, int DIM, bool BY_KEYS>
 struct Forward {
+    // by keys: two waves, so that a CU's LDS holds two workgroups, and one's first tile and
+    // join pass beside the other's reads
+    static constexpr int kWaves = BY_KEYS ? kKeysWaves : gs::kWaves;
     static constexpr int kSub = BY_KEYS ? 1 : 2;                    // 32-key parts of a wave
     static constexpr int kKeys = BY_KEYS ? 32 * kWaves : 32 * kSub;  // of a tile
     static constexpr int kRows = BY_KEYS ? 32 : 32 * kWaves;
     using KTile = Tile<T, DIM, kKeys, kWaves>;
     static constexpr int kLds = 4 * KTile::kBytes;
-    static_assert(!BY_KEYS || kLds >= kWaves * 64 * DIM / 2 * 4 + kWaves * 64 * 8, "the join");
+    static_assert(!BY_KEYS || kLds >= kWaves * 64 * (DIM / 2 * 4 + 8), "the join");
 };
 
-// Rows of a split: un-normalised sums, and their maximum and sum of weights.
+// Parts of the keys of a row that other workgroups have: un-normalised sums, and their
+// maximum and sum of weights.
 struct Partial {
-    float *sums;        // (split, row, head, dim)
-    float2 *max_sum;    // (split, row, head)
-    int splits;
+    float *sums;      // (split, row, head, dim)
+    float2 *max_sum;  // (split, row, head)
+    int32_t *count;   // (row, head): splits that there are, where that depends on the keys
+    int splits;       // at most
 };
 
+// One tile of rows with one split of its keys; share: tiles of a split, or 0 for as many as
+// there are over the splits.
 template <typename T, int DIM, bool BY_KEYS>
-__global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel(
-    GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-    T *__restrict__ out, T *__restrict__ out_rest, float *__restrict__ log_sum, Partial partial) {
+__device__ __forceinline__ void forward_rows(
+    const GsAttention &a, const T *q, const T *k, const T *v, T *out, T *out_rest, float *log_sum,
+    const Partial &partial, lds_char *tiles, int kh, int sequence, int number, int split, int share) {
     using F = Forward<T, DIM, BY_KEYS>;
     using KTile = typename F::KTile;
-    __shared__ __attribute__((aligned(1024))) char lds[F::kLds];
-    lds_char *const tiles = (lds_char *)lds;
-
-    const Place at_grid = place_of(a.heads_k, partial.splits);
-    const int kh = at_grid.kh, split = at_grid.split, group = a.heads_q / a.heads_k;
-    int sequence, number;
-    if (!find_tile(a.offsets_q, a.sequences, a.rows_q, group, F::kRows, at_grid.tile,
-                   true, &sequence, &number))
-        return;
+    const int group = a.heads_q / a.heads_k;
     const Span p = span_of(a, sequence);
+    constexpr int kWaves = F::kWaves;
     const int lane = __lane_id(), half = lane >> 5, wave = uniform(threadIdx.x / kWave);
     const int rows = p.lq * group;
     const int row0 = number * F::kRows + (BY_KEYS ? 0 : 32 * wave);  // this wave's first
@@ -233,7 +234,8 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
 
     // this split's tiles
     const int tiles_all = seen > 0 ? (seen + F::kKeys - 1) / F::kKeys : 0;
-    const int share = (tiles_all + partial.splits - 1) / partial.splits;
+    const int tiles_keys = (p.lk + F::kKeys - 1) / F::kKeys;
+    if (!share) share = (tiles_all + partial.splits - 1) / partial.splits;
     const int first_tile = min(split * share, tiles_all);
     const int end_tile = min(first_tile + share, tiles_all);
 
@@ -333,26 +335,26 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
     sum = half_sum(sum);
 
     if constexpr (BY_KEYS) {
-        // the four waves' sums over their keys, in LDS: wave w adds up the w-th quarter
-        // of the registers
+        // the waves' sums over their keys, joined in LDS by the first
         __syncthreads();  // the tiles have been read
-        float *sums = (float *)lds;  // (wave, register, lane)
-        float2 *stats = (float2 *)(sums + kWaves * (DIM / 2) * 64);
+        auto *sums = (__attribute__((address_space(3))) float *)tiles;  // (wave, register, lane)
+        auto *stats = sums + kWaves * (DIM / 2) * 64;                  // (wave, lane) pairs
 #pragma unroll
         for (int d = 0; d < DIM / 32; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) sums[(wave * (DIM / 2) + 16 * d + r) * 64 + lane] = acc[d][r];
-        stats[wave * 64 + lane] = make_float2(top, sum);
+        stats[2 * (wave * 64 + lane)] = top;
+        stats[2 * (wave * 64 + lane) + 1] = sum;
         __syncthreads();
-        if (wave) return;
+        if (wave) return;  // (a wave of no rows of its own)
         float all = top, weight[kWaves], total = 0.0f;
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) all = fmaxf(all, stats[w * 64 + lane].x);
+        for (int w = 1; w < kWaves; ++w) all = fmaxf(all, stats[2 * (w * 64 + lane)]);
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const float2 o = stats[w * 64 + lane];
-            weight[w] = o.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(o.x - all);
-            total = fmaf(o.y, weight[w], total);
+            const float its = stats[2 * (w * 64 + lane)];
+            weight[w] = its == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(its - all);
+            total = fmaf(stats[2 * (w * 64 + lane) + 1], weight[w], total);
         }
 #pragma unroll
         for (int d = 0; d < DIM / 32; ++d)
@@ -370,7 +372,11 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
 
     if (partial.splits > 1) {
         const int64_t slot = (int64_t)split * a.rows_q * a.heads_q + at;
-        if (real && half == 0) partial.max_sum[slot] = make_float2(top, sum);
+        if (real && half == 0) {
+            partial.max_sum[slot] = make_float2(top, sum);
+            if (BY_KEYS && split == 0)
+                partial.count[at] = max((tiles_keys + share - 1) / share, 1);
+        }
         store_partial<DIM>(acc, 1.0f,
                            real && top != -INFINITY ? partial.sums + slot * a.dim : nullptr, a.dim);
         return;
@@ -389,45 +395,112 @@ __global__ __launch_bounds__(64 * kWaves, BY_KEYS ? 1 : 2) void attention_kernel
         log_sum[at] = none ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-// Joins the splits of a row: a wave a row, two elements a lane.
+template <typename T, int DIM>
+__global__ __launch_bounds__(64 * kWaves, 2) void attention_kernel(
+    GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+    T *__restrict__ out, T *__restrict__ out_rest, float *__restrict__ log_sum, Partial partial) {
+    using F = Forward<T, DIM, false>;
+    __shared__ __attribute__((aligned(1024))) char lds[F::kLds];
+    const Place at = place_of(a.heads_k, partial.splits);
+    int sequence, number;
+    if (!find_tile(a.offsets_q, a.sequences, a.rows_q, a.heads_q / a.heads_k, F::kRows, at.tile, true,
+                   &sequence, &number))
+        return;
+    forward_rows<T, DIM, false>(a, q, k, v, out, out_rest, log_sum, partial, (lds_char *)lds, at.kh, sequence,
+                                number, at.split, 0);
+}
+
+// Few rows a sequence.  Caches differ in length, and the host does not know them: a split is as
+// many tiles of any of them as make about kSplits splits in all, as far as a row may have
+// that many, and the workgroups take them in turn.  Bound by memory: a split costs a first
+// tile and a join of its own, so there are no more than run at a time on 256 CUs, two a CU
+// at 128 dimensions, less an eighth for the last splits of the sequences, which are shorter.
+// 16 sequences of 2500 to 32640 keys, 16 heads on 4, dim 128, with the join: 85 us, 4.7
+// TB/s; twice as many splits 99, four times 104; equal splits of each sequence 105.
+constexpr int kSplits = 448;
+
+template <typename T, int DIM>
+__global__ __launch_bounds__(64 * kKeysWaves, DIM > 96 ? 1 : 2) void attention_keys_kernel(
+    GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+    T *__restrict__ out, T *__restrict__ out_rest, float *__restrict__ log_sum, Partial partial) {
+    using F = Forward<T, DIM, true>;
+    __shared__ __attribute__((aligned(1024))) char lds[F::kLds];
+    const int group = a.heads_q / a.heads_k, all = a.sequences + 2;
+    const auto tiles_of = [&](int s) {  // of keys
+        const int n = keys_of(a, s, rows_of(a.offsets_k, a.sequences, a.rows_k, s));
+        return (n + F::kKeys - 1) / F::kKeys;
+    };
+    const auto rows_tiles_of = [&](int s) {
+        const int2 r = rows_of(a.offsets_q, a.sequences, a.rows_q, s);
+        return (int)(((int64_t)(r.y - r.x) * group + F::kRows - 1) / F::kRows);
+    };
+    float total = 0.0f;  // tiles of all (far below 2^24 where a split is more than one)
+    for (int first = 0; first < all; first += kWave) {
+        const int s = first + (int)__lane_id();
+        total += wave_sum(s < all ? (float)rows_tiles_of(s) * (float)tiles_of(s) : 0.0f);
+    }
+    const int least = uniform(max(4, (int)(total * (float)a.heads_k / (float)kSplits) + 1));
+    const auto share_of = [&](int t) { return max(least, (t + partial.splits - 1) / partial.splits); };
+    const auto splits_of = [&](int t) {
+        const int share = share_of(t);
+        return max((t + share - 1) / share, 1);
+    };
+    const auto count = [&](int s) { return rows_tiles_of(s) * splits_of(tiles_of(s)) * a.heads_k; };
+    int sequence, number;
+    for (int item = blockIdx.x; find_place(all, count, item, false, &sequence, &number);
+         item += gridDim.x) {
+        const int t = uniform(tiles_of(sequence)), splits = splits_of(t);
+        const int rest = number / a.heads_k;
+        forward_rows<T, DIM, true>(a, q, k, v, out, out_rest, log_sum, partial, (lds_char *)lds,
+                                   number % a.heads_k, sequence, rest / splits, rest % splits,
+                                   share_of(t));
+        __syncthreads();  // LDS has been read
+    }
+}
+
+// Joins the splits of a row: a workgroup a row, four elements a thread, every eighth split
+// in each of its eight parts.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int dim, Partial partial,
                                                              T *__restrict__ out,
                                                              T *__restrict__ out_rest,
                                                              float *__restrict__ log_sum) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
-    if (row >= rows) return;
-    const int lane = __lane_id();
-    const float2 mine = lane < partial.splits ? partial.max_sum[lane * rows + row]
-                                              : make_float2(-INFINITY, 0.0f);
-    float top = mine.x;
-#pragma unroll
-    for (int o = kWave / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
+    __shared__ f32x4 sums[8][32];
+    const int64_t row = blockIdx.x;
+    const int lane = __lane_id(), column = threadIdx.x % 32 * 4, part = threadIdx.x / 32;
+    const int splits = partial.count ? min(partial.count[row], partial.splits) : partial.splits;
+    const float2 mine = lane < splits ? partial.max_sum[lane * rows + row]
+                                      : make_float2(-INFINITY, 0.0f);
+    const float top = wave_max(mine.x);
     const float weight = mine.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine.x - top);
     const float sum = wave_sum(mine.x == -INFINITY ? 0.0f : mine.y * weight);
-    const bool in = 2 * lane < dim;
-    float x = 0.0f, y = 0.0f;
-    for (int s = 0; s < partial.splits; ++s) {
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+    for (int s = part; s < splits; s += 8) {
         const float w = __shfl(weight, s, kWave);
-        if (__shfl(mine.x, s, kWave) == -INFINITY) continue;
-        if (!in) continue;
-        const float2 o = *(const float2 *)(partial.sums + (s * rows + row) * dim + 2 * lane);
-        x = fmaf(o.x, w, x);
-        y = fmaf(o.y, w, y);
+        // (a split that saw nothing has written no sums)
+        const bool there = __shfl(mine.x, s, kWave) != -INFINITY && column < dim;
+        if (there) x += *(const f32x4 *)(partial.sums + (s * rows + row) * dim + column) * w;
     }
+    sums[part][threadIdx.x % 32] = x;
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+#pragma unroll
+    for (int p = 1; p < 8; ++p) x += sums[p][threadIdx.x];
     const bool none = top == -INFINITY;
     const float r = 1.0f / sum;
-    if (in) {
-        x = none ? 0.0f : x * r;
-        y = none ? 0.0f : y * r;
-        const typename Vec<T>::x2 o = {(T)x, (T)y};
-        *(typename Vec<T>::x2 *)(out + row * dim + 2 * lane) = o;
-        if (out_rest) {
-            const typename Vec<T>::x2 e = {(T)(x - to_float((T)o[0])), (T)(y - to_float((T)o[1]))};
-            *(typename Vec<T>::x2 *)(out_rest + row * dim + 2 * lane) = e;
+    if (column < dim) {
+        float o[4], e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o[i] = none ? 0.0f : x[i] * r;
+            e[i] = o[i] - to_float(from_float<T>(o[i]));
         }
+        store_floats<T, 4>(out + row * dim + column, o);
+        if (out_rest) store_floats<T, 4>(out_rest + row * dim + column, e);
     }
-    if (log_sum && lane == 0) log_sum[row] = none ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (log_sum && threadIdx.x == 0)
+        log_sum[row] = none ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 // ---------------------------------------------------------------- gradients
@@ -854,7 +927,7 @@ static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 // How a forward is launched.
 struct ForwardPlan {
     bool by_keys;
-    int64_t tiles;
+    int64_t groups;  // workgroups
     int splits;
 };
 
@@ -863,17 +936,25 @@ static ForwardPlan plan_forward(const GsAttention &a) {
     const int64_t sequences = a.sequences > 0 ? a.sequences : 1;
     ForwardPlan f;
     f.by_keys = packed <= 32 * sequences;
-    const int rows = f.by_keys ? 32 : 32 * kWaves;
-    f.tiles = packed / rows + a.sequences + 2;
+    if (f.by_keys) {
+        // a row may have up to 64 splits of at least 256 keys, as far as the rows' sums stay few
+        int64_t splits = 2048 / (sequences * a.heads_k);
+        const int64_t most = (a.rows_k + 255) / 256;
+        if (splits > most) splits = most;
+        f.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+        const int64_t items = (packed / 32 + a.sequences + 2) * f.splits * a.heads_k;
+        f.groups = items < 1024 ? items : 1024;
+        return f;
+    }
     // Workgroups that will find rows, at least, and how many splits of the keys fill the
     // card with them; a split of fewer than four tiles costs more than it hides.
-    int64_t busy = (packed + rows - 1) / rows;
-    if (busy < sequences) busy = sequences < a.rows_q ? sequences : a.rows_q;
-    busy = busy > 0 ? busy * a.heads_k : 1;
-    const int64_t want = (512 + busy - 1) / busy;
-    const int64_t most = a.rows_k / sequences / (f.by_keys ? 512 : 256);
-    int64_t splits = want < most ? want : most;
+    const int64_t rows = 32 * kWaves;
+    const int64_t busy = (packed + rows - 1) / rows * a.heads_k;
+    const int64_t want = busy > 0 ? (512 + busy - 1) / busy : 1;
+    const int64_t most = a.rows_k / sequences / 256;
+    const int64_t splits = want < most ? want : most;
     f.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+    f.groups = (packed / rows + a.sequences + 2) * a.heads_k * f.splits;
     return f;
 }
 
@@ -919,27 +1000,28 @@ static size_t backward_rows(const GsAttention &a) {
 
 static size_t partial_bytes(const GsAttention &a, int splits) {
     if (splits == 1) return 0;
-    return (size_t)splits * a.rows_q * a.heads_q * (a.dim * sizeof(float) + sizeof(float2));
+    const size_t rows = (size_t)a.rows_q * a.heads_q;
+    return splits * rows * (a.dim * sizeof(float) + sizeof(float2)) + rows * sizeof(int32_t);
 }
 
 template <typename T, int DIM>
 static int launch_forward(const GsAttention &a, const ForwardPlan &f, const void *q, const void *k,
                           const void *v, void *out, void *out_rest, float *log_sum,
                           const Partial &partial, hipStream_t stream) {
-    const dim3 grid((unsigned)(f.tiles * a.heads_k * f.splits));
+    const dim3 grid((unsigned)f.groups);
+    const T *tq = (const T *)q, *tk = (const T *)k, *tv = (const T *)v;
     if (f.by_keys)
-        hipLaunchKernelGGL((attention_kernel<T, DIM, true>), grid, dim3(64 * kWaves), 0, stream, a,
-                           (const T *)q, (const T *)k, (const T *)v, (T *)out, (T *)out_rest, log_sum,
-                           partial);
+        hipLaunchKernelGGL((attention_keys_kernel<T, DIM>), grid,
+                           dim3(64 * kKeysWaves), 0, stream, a, tq, tk, tv,
+                           (T *)out, (T *)out_rest, log_sum, partial);
     else
-        hipLaunchKernelGGL((attention_kernel<T, DIM, false>), grid, dim3(64 * kWaves), 0, stream, a,
-                           (const T *)q, (const T *)k, (const T *)v, (T *)out, (T *)out_rest, log_sum,
-                           partial);
+        hipLaunchKernelGGL((attention_kernel<T, DIM>), grid, dim3(64 * kWaves), 0, stream, a, tq, tk,
+                           tv, (T *)out, (T *)out_rest, log_sum, partial);
     int st = launch_status();
     if (st || f.splits == 1) return st;
     const int64_t rows = a.rows_q * a.heads_q;
-    hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0,
-                       stream, rows, a.dim, partial, (T *)out, (T *)out_rest, log_sum);
+    hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)rows), dim3(256), 0, stream,
+                       rows, a.dim, partial, (T *)out, (T *)out_rest, log_sum);
     return launch_status();
 }
 
@@ -973,14 +1055,16 @@ extern "C" int gs_attention_forward(const GsAttention *a, const void *q, const v
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(out_rest))
         return GS_ERR_UNSUPPORTED;
     const ForwardPlan f = plan_forward(*a);
-    if (f.tiles * a->heads_k * f.splits > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
+    if (f.groups > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
     const size_t need = partial_bytes(*a, f.splits);
     if (need && !workspace) return GS_ERR_INVALID_ARGUMENT;
     if (workspace_bytes < need) return GS_ERR_WORKSPACE_TOO_SMALL;
     Partial partial;
+    const size_t rows = (size_t)a->rows_q * a->heads_q;
     partial.splits = f.splits;
     partial.sums = (float *)workspace;
-    partial.max_sum = (float2 *)((float *)workspace + (size_t)f.splits * a->rows_q * a->heads_q * a->dim);
+    partial.max_sum = (float2 *)(partial.sums + f.splits * rows * a->dim);
+    partial.count = f.by_keys ? (int32_t *)(partial.max_sum + f.splits * rows) : nullptr;
     const auto launch = [&](auto t) {
         return with_tile(a->dim, [&](auto d) {
             return launch_forward<decltype(t), decltype(d)::value>(

@@ -82,6 +82,12 @@ __device__ __forceinline__ int2 rows_of(const int32_t *offsets, int sequences, i
     return r;
 }
 
+// The keys that count of sequence s, whose key rows are `k`.
+__device__ __forceinline__ int keys_of(const GsAttention &a, int s, int2 k) {
+    if (s == 0 || s > a.sequences) return 0;
+    return a.lengths_k ? clamp_row(a.lengths_k[s - 1], 0, k.y - k.x) : k.y - k.x;
+}
+
 struct Span {
     int q0, lq;  // first query row, number of queries
     int k0, lk;  // first key row, number of keys that count
@@ -96,65 +102,56 @@ __device__ __forceinline__ Span span_of(const GsAttention &a, int s) {
     p.lq = uniform(q.y - q.x);
     p.k0 = uniform(k.x);
     p.k1 = uniform(k.y);
-    int n = s == 0 || s > a.sequences ? 0 : k.y - k.x;
-    if (n > 0 && a.lengths_k) n = clamp_row(a.lengths_k[s - 1], 0, n);
-    p.lk = uniform(n);
+    p.lk = uniform(keys_of(a, s, k));
     return p;
 }
 
-// The sequence and the tile in it of a launch's tile number, tiles of `size` units,
-// `units` units a row.  Counted from the back on request: under a causal mask the last
-// queries see most, and should start first.  Every lane of a wave calls it.  False: no
-// such tile.
-__device__ __forceinline__ bool find_tile(const int32_t *offsets, int sequences, int64_t rows,
-                                          int units, int size, int number, bool from_back,
-                                          int *sequence, int *tile) {
-    const int lane = __lane_id(), all = sequences + 2;
+// The group (of `groups`) and the place in it of number `number`, where group g has count(g)
+// places; numbers count up from the first group's first place or down from the last one's
+// last.  Every lane of a wave calls it.  False: there are not so many places.
+template <typename Count>
+__device__ __forceinline__ bool find_place(int groups, Count count, int number, bool from_back,
+                                           int *group, int *place) {
+    const int lane = __lane_id();
     int total = 0, sum = 0;
-    for (int first = 0; first < all; first += kWave) {
-        const int s = first + lane;
-        int n = 0;
-        if (s < all) {
-            const int2 r = rows_of(offsets, sequences, rows, s);
-            n = (int)(((int64_t)(r.y - r.x) * units + size - 1) / size);
-        }
-        sum = n;
+    const auto running = [&](int first) {  // up to and with group first + lane
+        sum = first + lane < groups ? count(first + lane) : 0;
 #pragma unroll
         for (int o = 1; o < kWave; o <<= 1) {
             const int t = __shfl_up(sum, o, kWave);
             if (lane >= o) sum += t;
         }
-        total += __shfl(sum, kWave - 1, kWave);
-    }
+        // (uniform, also to the compiler: what is found here addresses whole waves' copies)
+        return uniform(__shfl(sum, kWave - 1, kWave));
+    };
+    for (int first = 0; first < groups; first += kWave) total += running(first);
     if (number >= total) return false;
     int want = from_back ? total - 1 - number : number;
-    // `sum` holds the last group's running count; the groups before it are counted again
-    for (int first = 0; first < all; first += kWave) {
-        if (all > kWave) {
-            const int s = first + lane;
-            int n = 0;
-            if (s < all) {
-                const int2 r = rows_of(offsets, sequences, rows, s);
-                n = (int)(((int64_t)(r.y - r.x) * units + size - 1) / size);
-            }
-            sum = n;
-#pragma unroll
-            for (int o = 1; o < kWave; o <<= 1) {
-                const int t = __shfl_up(sum, o, kWave);
-                if (lane >= o) sum += t;
-            }
-        }
-        const uint64_t after = __ballot(sum > want);
-        if (after) {
-            const int l = __ffsll((unsigned long long)after) - 1;
+    for (int first = 0; first < groups; first += kWave) {
+        const int here = groups > kWave ? running(first) : total;
+        if (want < here) {
+            const int l = __ffsll((unsigned long long)__ballot(sum > want)) - 1;
             const int before = l ? __shfl(sum, l - 1, kWave) : 0;
-            *sequence = uniform(first + l);
-            *tile = uniform(want - before);
+            *group = uniform(first + l);
+            *place = uniform(want - before);
             return true;
         }
-        want -= __shfl(sum, kWave - 1, kWave);
+        want -= here;
     }
     return false;
+}
+
+// The sequence and the tile in it of a launch's tile number, tiles of `size` units,
+// `units` units a row.  Counted from the back on request: under a causal mask the last
+// queries see most, and should start first.
+__device__ __forceinline__ bool find_tile(const int32_t *offsets, int sequences, int64_t rows,
+                                          int units, int size, int number, bool from_back,
+                                          int *sequence, int *tile) {
+    const auto count = [&](int s) {
+        const int2 r = rows_of(offsets, sequences, rows, s);
+        return (int)(((int64_t)(r.y - r.x) * units + size - 1) / size);
+    };
+    return find_place(sequences + 2, count, number, from_back, sequence, tile);
 }
 
 // -------------------------------------------------------------------- tiles
