@@ -476,9 +476,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
     const float sum = wave_sum(mine.x == -INFINITY ? 0.0f : mine.y * weight);
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 2
-    for (int s = part; s < splits; s += 8) {
+    for (int first = 0; first < splits; first += 8) {  // (the same rounds in every lane)
+        const int s = first + part;
         const float w = __shfl(weight, s, kWave);
-        // (a split that saw nothing has written no sums)
+        // (a split that saw nothing has written no sums, and those past the last are as it)
         const bool there = __shfl(mine.x, s, kWave) != -INFINITY && column < dim;
         if (there) x += *(const f32x4 *)(partial.sums + (s * rows + row) * dim + column) * w;
     }
