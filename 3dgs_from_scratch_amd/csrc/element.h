@@ -63,10 +63,12 @@ __device__ __forceinline__ float wave_max(float v) {
     return lane_reduce<kWave>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
-// N neighbouring elements, read or written as one access.
+// N neighbouring elements, read or written as one access, which on this target may begin at
+// any element.
 template <typename T, int N>
 struct Pack {
-    typedef T type __attribute__((ext_vector_type(N)));
+    typedef T aligned_type __attribute__((ext_vector_type(N)));
+    typedef aligned_type type __attribute__((aligned(sizeof(T))));
 };
 template <typename T>
 struct Pack<T, 1> {
@@ -90,6 +92,30 @@ __device__ __forceinline__ void store_floats(T *p, const float *v) {
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = from_float<T>(v[i]);
     *(typename Pack<T, N>::type *)p = x;
+}
+
+// The same of the first n, where there are not N.  WHOLE: there are N or none.
+template <bool WHOLE, typename T, int N>
+__device__ __forceinline__ void load_first(const T *p, float *v, int n, float rest) {
+    if (WHOLE ? n > 0 : n >= N) {
+        load_floats<T, N>(p, v);
+    } else if constexpr (WHOLE) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = rest;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i < n ? to_float(p[i]) : rest;
+    }
+}
+template <bool WHOLE, typename T, int N>
+__device__ __forceinline__ void store_first(T *p, const float *v, int n) {
+    if (WHOLE ? n > 0 : n >= N) {
+        store_floats<T, N>(p, v);
+    } else if constexpr (!WHOLE) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < n) p[i] = from_float<T>(v[i]);
+    }
 }
 
 }  // namespace gs

@@ -10,7 +10,6 @@
 // keeps the weight's sums of its rows in registers too, joins its waves in LDS, and a
 // second launch adds up the workgroups' sums in an order that the sizes alone give.
 
-#include <initializer_list>
 #include <type_traits>
 
 #include "element.h"
@@ -21,10 +20,11 @@ constexpr int kNormBlock = 256;
 constexpr int kNormGroups = 1024;  // most workgroups of a backward
 
 // How a row lies in registers: LANES lanes, SLOTS packs of VEC elements in each; pack i of
-// lane l is number i * LANES + l of the row.
-template <int LANES_, int SLOTS_, int VEC_>
+// lane l is number i * LANES + l of the row.  WHOLE: the row ends with a pack.
+template <int LANES_, int SLOTS_, int VEC_, bool WHOLE_>
 struct Shape {
     static constexpr int kLanes = LANES_, kSlots = SLOTS_, kVec = VEC_;
+    static constexpr bool kWhole = WHOLE_;
     static constexpr int kRows = kNormBlock / kLanes;  // of a workgroup at a time
     static constexpr int kHeld = kSlots * kVec;
 };
@@ -57,17 +57,17 @@ struct Weights {
     int32_t type;
 };
 
-template <int VEC>
-__device__ __forceinline__ void load_weights(const Weights &w, int at, float none, float *v) {
+template <bool WHOLE, int VEC>
+__device__ __forceinline__ void load_weights(const Weights &w, int at, int n, float none, float *v) {
     if (!w.p) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[i] = none;
     } else if (w.type == GS_F32) {
-        load_floats<float, VEC>((const float *)w.p + at, v);
+        load_first<WHOLE, float, VEC>((const float *)w.p + at, v, n, none);
     } else if (w.type == GS_F16) {
-        load_floats<f16, VEC>((const f16 *)w.p + at, v);
+        load_first<WHOLE, f16, VEC>((const f16 *)w.p + at, v, n, none);
     } else {
-        load_floats<bf16, VEC>((const bf16 *)w.p + at, v);
+        load_first<WHOLE, bf16, VEC>((const bf16 *)w.p + at, v, n, none);
     }
 }
 
@@ -77,12 +77,7 @@ __device__ __forceinline__ void load_row(const T *row, int lane, int channels, f
 #pragma unroll
     for (int i = 0; i < S::kSlots; ++i) {
         const int at = (i * S::kLanes + lane) * S::kVec;
-        if (at < channels) {
-            load_floats<T, S::kVec>(row + at, v + i * S::kVec);
-        } else {
-#pragma unroll
-            for (int j = 0; j < S::kVec; ++j) v[i * S::kVec + j] = 0.0f;
-        }
+        load_first<S::kWhole, T, S::kVec>(row + at, v + i * S::kVec, channels - at, 0.0f);
     }
 }
 
@@ -103,26 +98,28 @@ __global__ __launch_bounds__(kNormBlock) void layer_norm_kernel(
         const float mean = row_sum<S::kLanes>(s, 0.0f).x / n;
         float q = 0.0f;
 #pragma unroll
-        for (int i = 0; i < S::kSlots; ++i)
-            if ((i * S::kLanes + lane) * S::kVec < channels) {
+        for (int i = 0; i < S::kSlots; ++i) {
+            const int at = (i * S::kLanes + lane) * S::kVec;
+            if (at >= channels) continue;
 #pragma unroll
-                for (int j = 0; j < S::kVec; ++j) {
-                    float &d = v[i * S::kVec + j];
-                    d -= mean;
-                    q = fmaf(d, d, q);
-                }
+            for (int j = 0; j < S::kVec; ++j) {
+                float &d = v[i * S::kVec + j];
+                d = S::kWhole || at + j < channels ? d - mean : 0.0f;
+                q = fmaf(d, d, q);
             }
+        }
         const float r = 1.0f / sqrtf(row_sum<S::kLanes>(q, 0.0f).x / n + eps);
 #pragma unroll
         for (int i = 0; i < S::kSlots; ++i) {
             const int at = (i * S::kLanes + lane) * S::kVec;
             if (at >= channels) continue;
             float w[S::kVec], b[S::kVec];
-            load_weights<S::kVec>(weight, at, 1.0f, w);
-            load_weights<S::kVec>(bias, at, 0.0f, b);
+            const int held = S::kWhole ? S::kVec : channels - at;
+            load_weights<S::kWhole, S::kVec>(weight, at, held, 1.0f, w);
+            load_weights<S::kWhole, S::kVec>(bias, at, held, 0.0f, b);
 #pragma unroll
             for (int j = 0; j < S::kVec; ++j) w[j] = fmaf(v[i * S::kVec + j] * r, w[j], b[j]);
-            store_floats<T, S::kVec>(y + row * channels + at, w);
+            store_first<S::kWhole, T, S::kVec>(y + row * channels + at, w, held);
         }
         if (stats && lane == 0) stats[row] = make_float2(mean, r);
     }
@@ -140,8 +137,7 @@ __global__ __launch_bounds__(kNormBlock) void layer_norm_backward_kernel(
 #pragma unroll
     for (int i = 0; i < S::kSlots; ++i) {
         const int at = (i * S::kLanes + lane) * S::kVec;
-        load_weights<S::kVec>(at < channels ? weight : Weights{nullptr, GS_F32}, at, 1.0f,
-                              w + i * S::kVec);
+        load_weights<S::kWhole, S::kVec>(weight, at, channels - at, 1.0f, w + i * S::kVec);
     }
     if constexpr (SUMS)
 #pragma unroll
@@ -176,7 +172,8 @@ __global__ __launch_bounds__(kNormBlock) void layer_norm_backward_kernel(
                 const int e = i * S::kVec + j;
                 g[e] = st.y * (g[e] - ma - h[e] * mb);
             }
-            store_floats<T, S::kVec>(dx + row * channels + at, g + i * S::kVec);
+            store_first<S::kWhole, T, S::kVec>(dx + row * channels + at, g + i * S::kVec,
+                                               channels - at);
         }
     }
     if constexpr (SUMS) {
@@ -202,16 +199,19 @@ __global__ __launch_bounds__(kNormBlock) void layer_norm_backward_kernel(
                             a += joined[(2 * j) * kNormBlock + r * S::kLanes + lane];
                             b += joined[(2 * j + 1) * kNormBlock + r * S::kLanes + lane];
                         }
-                        to[at + j] = a;
-                        to[channels + at + j] = b;
+                        if (S::kWhole || at + j < channels) {
+                            to[at + j] = a;
+                            to[channels + at + j] = b;
+                        }
                     }
                 }
             } else if (at < channels) {
 #pragma unroll
-                for (int j = 0; j < S::kVec; ++j) {
-                    to[at + j] = sum_w[i * S::kVec + j];
-                    to[channels + at + j] = sum_b[i * S::kVec + j];
-                }
+                for (int j = 0; j < S::kVec; ++j)
+                    if (S::kWhole || at + j < channels) {
+                        to[at + j] = sum_w[i * S::kVec + j];
+                        to[channels + at + j] = sum_b[i * S::kVec + j];
+                    }
             }
         }
     }
@@ -236,8 +236,8 @@ __global__ __launch_bounds__(kNormBlock) void layer_norm_long_kernel(
         const float r = 1.0f / sqrtf(row_sum<kNormBlock>(q, 0.0f).x / (float)channels + eps);
         for (int c = threadIdx.x; c < channels; c += kNormBlock) {
             float w, b;
-            load_weights<1>(weight, c, 1.0f, &w);
-            load_weights<1>(bias, c, 0.0f, &b);
+            load_weights<true, 1>(weight, c, 1, 1.0f, &w);
+            load_weights<true, 1>(bias, c, 1, 0.0f, &b);
             y[row * channels + c] = from_float<T>(fmaf((to_float(xr[c]) - mean) * r, w, b));
         }
         if (stats && threadIdx.x == 0) stats[row] = make_float2(mean, r);
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(kNormBlock) void layer_norm_long_dx_kernel(
         const float2 st = stats[row];
         float a = 0.0f, b = 0.0f, w;
         for (int c = threadIdx.x; c < channels; c += kNormBlock) {
-            load_weights<1>(weight, c, 1.0f, &w);
+            load_weights<true, 1>(weight, c, 1, 1.0f, &w);
             const float g = to_float(gr[c]) * w;
             a += g;
             b = fmaf(g, (to_float(xr[c]) - st.x) * st.y, b);
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(kNormBlock) void layer_norm_long_dx_kernel(
         const float2 m = row_sum<kNormBlock>(a, b);
         const float ma = m.x / (float)channels, mb = m.y / (float)channels;
         for (int c = threadIdx.x; c < channels; c += kNormBlock) {
-            load_weights<1>(weight, c, 1.0f, &w);
+            load_weights<true, 1>(weight, c, 1, 1.0f, &w);
             const float g = to_float(gr[c]) * w;
             const float h = (to_float(xr[c]) - st.x) * st.y;
             dx[row * channels + c] = from_float<T>(st.y * (g - ma - h * mb));
@@ -317,44 +317,28 @@ __global__ __launch_bounds__(256) void layer_norm_join_kernel(const float *__res
         ((bf16 *)out)[at] = from_float<bf16>(s);
 }
 
-// Rows of lanes and packs for a number of channels.  VEC is 16 bytes where the channels,
-// the strides and the addresses allow it, else one element.  A row of 16 lanes where
-// that is enough, else a wave, else a workgroup; f gets the shape, or void if the row does
-// not fit in registers.
-template <int VEC, typename F>
+// Rows of lanes and packs of 16 bytes for a number of channels: a row of 16 lanes where that
+// is enough, else a wave, else a workgroup; f gets the shape, or 0 if the row does not fit in
+// registers.
+template <typename T, bool WHOLE, typename F>
 static int with_shape(int channels, F f) {
-    const int packs = (channels + VEC - 1) / VEC;
-    if (packs <= 16) return f(Shape<16, 1, VEC>{});
-    if (packs <= 32) return f(Shape<16, 2, VEC>{});
-    if (packs <= 64) return f(Shape<64, 1, VEC>{});
-    if (packs <= 128) return f(Shape<64, 2, VEC>{});
-    if (packs <= 192) return f(Shape<64, 3, VEC>{});
-    if (packs <= 256) return f(Shape<64, 4, VEC>{});
-    if constexpr (VEC == 1) {
-        if (packs <= 512) return f(Shape<64, 8, VEC>{});
-        if (packs <= 1024) return f(Shape<64, 16, VEC>{});
-        if (packs <= 4096) return f(Shape<256, 16, VEC>{});
-    } else {
-        if (packs <= 512) return f(Shape<256, 2, VEC>{});
-        if (packs <= 1024) return f(Shape<256, 4, VEC>{});
-    }
+    constexpr int kVec = 16 / sizeof(T);
+    const int packs = (channels + kVec - 1) / kVec;
+    if (packs <= 16) return f(Shape<16, 1, kVec, WHOLE>{});
+    if (packs <= 32) return f(Shape<16, 2, kVec, WHOLE>{});
+    if (packs <= 64) return f(Shape<64, 1, kVec, WHOLE>{});
+    if (packs <= 128) return f(Shape<64, 2, kVec, WHOLE>{});
+    if (packs <= 192) return f(Shape<64, 3, kVec, WHOLE>{});
+    if (packs <= 256) return f(Shape<64, 4, kVec, WHOLE>{});
+    if (packs <= 512) return f(Shape<256, 2, kVec, WHOLE>{});
+    if (packs <= 1024) return f(Shape<256, 4, kVec, WHOLE>{});
     return f(0);
 }
 
 template <typename T, typename F>
-static int with_shape(int channels, bool wide, F f) {
-    return wide ? with_shape<16 / sizeof(T)>(channels, f) : with_shape<1>(channels, f);
-}
-
-static bool wide_access(int size, int channels, std::initializer_list<int64_t> strides,
-                        std::initializer_list<const void *> pointers) {
-    const int vec = 16 / size;
-    if (channels % vec) return false;
-    for (int64_t s : strides)
-        if (s % vec) return false;
-    for (const void *p : pointers)
-        if ((uintptr_t)p % 16) return false;
-    return true;
+static int with_shape(int channels, F f) {
+    return channels % (16 / (int)sizeof(T)) == 0 ? with_shape<T, true>(channels, f)
+                                                 : with_shape<T, false>(channels, f);
 }
 
 // Workgroups of a backward: as many as the rows give, at most kNormGroups, and at least
@@ -382,10 +366,9 @@ extern "C" int gs_layer_norm_forward(const void *x, int64_t x_stride, const void
         return GS_ERR_INVALID_ARGUMENT;
     if (rows == 0) return GS_OK;
     if (!x || !y) return GS_ERR_INVALID_ARGUMENT;
-    const bool wide = wide_access(element_size(type), channels, {x_stride}, {x, y, weight, bias});
     return with_element(type, [&](auto t) {
         using T = decltype(t);
-        return with_shape<T>(channels, wide, [&](auto shape) {
+        return with_shape<T>(channels, [&](auto shape) {
             using S = decltype(shape);
             const Weights w = {weight, weight_type}, b = {bias, weight_type};
             if constexpr (std::is_same<S, int>::value)
@@ -426,11 +409,9 @@ extern "C" int gs_layer_norm_backward(const void *grad_y, int64_t grad_y_stride,
             return GS_ERR_WORKSPACE_TOO_SMALL;
     }
     if (rows > 0 && (sums || grad_x)) {
-        const bool wide = wide_access(element_size(type), channels, {x_stride, grad_y_stride},
-                                      {x, grad_y, grad_x, weight});
         const int st = with_element(type, [&](auto t) {
             using T = decltype(t);
-            return with_shape<T>(channels, wide, [&](auto shape) {
+            return with_shape<T>(channels, [&](auto shape) {
                 using S = decltype(shape);
                 const Weights w = {weight, weight_type};
                 const dim3 block(kNormBlock);
