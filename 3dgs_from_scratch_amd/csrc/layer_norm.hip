@@ -288,33 +288,40 @@ __global__ __launch_bounds__(kNormBlock) void layer_norm_long_sums_kernel(
     p[channels] = b;
 }
 
-// The sums of the workgroups' sums: 16 columns of the 2 * channels a workgroup, in 16
-// groups of workgroups each.
-__global__ __launch_bounds__(256) void layer_norm_join_kernel(const float *__restrict__ partial,
-                                                              int groups, int channels,
-                                                              int32_t type, void *__restrict__ dw,
-                                                              void *__restrict__ db) {
-    __shared__ float part[16][17];
-    const int across = threadIdx.x % 16, down = threadIdx.x / 16;
-    const int c = blockIdx.x * 16 + across;
+// The sums of the workgroups' sums: 16 columns of the 2 * channels a workgroup, in 64 groups
+// of workgroups each.
+constexpr int kJoinColumns = 16, kJoinRows = 64;
+
+__global__ __launch_bounds__(kJoinColumns *kJoinRows) void layer_norm_join_kernel(
+    const float *__restrict__ partial, int groups, int channels, int32_t type,
+    void *__restrict__ dw, void *__restrict__ db) {
+    __shared__ float part[kJoinRows][kJoinColumns + 1];
+    const int across = threadIdx.x % kJoinColumns, down = threadIdx.x / kJoinColumns;
+    const int c = blockIdx.x * kJoinColumns + across;
     float s = 0.0f;
     if (c < 2 * channels)
-        for (int g = down; g < groups; g += 16) s += partial[(int64_t)g * 2 * channels + c];
+#pragma unroll 8
+        for (int g = down; g < groups; g += kJoinRows) s += partial[(int64_t)g * 2 * channels + c];
     part[down][across] = s;
     __syncthreads();
-    if (down || c >= 2 * channels) return;
+    // a row of 16 lanes a column: 4 of its sums each, then across the lanes
+    const int column = threadIdx.x / 16, lane = threadIdx.x % 16;
+    if (column >= kJoinColumns) return;
     s = 0.0f;
 #pragma unroll
-    for (int g = 0; g < 16; ++g) s += part[g][across];
-    void *out = c < channels ? dw : db;
-    const int at = c < channels ? c : c - channels;
+    for (int g = 0; g < kJoinRows / 16; ++g) s += part[g * 16 + lane][column];
+    s = lane_sum<16>(s);
+    const int at = blockIdx.x * kJoinColumns + column;
+    if (lane || at >= 2 * channels) return;
+    void *out = at < channels ? dw : db;
+    const int to = at < channels ? at : at - channels;
     if (!out) return;
     if (type == GS_F32)
-        ((float *)out)[at] = s;
+        ((float *)out)[to] = s;
     else if (type == GS_F16)
-        ((f16 *)out)[at] = from_float<f16>(s);
+        ((f16 *)out)[to] = from_float<f16>(s);
     else
-        ((bf16 *)out)[at] = from_float<bf16>(s);
+        ((bf16 *)out)[to] = from_float<bf16>(s);
 }
 
 // Rows of lanes and packs of 16 bytes for a number of channels: a row of 16 lanes where that
@@ -445,8 +452,8 @@ extern "C" int gs_layer_norm_backward(const void *grad_y, int64_t grad_y_stride,
         if (st) return st;
     }
     if (!sums) return GS_OK;
-    hipLaunchKernelGGL(layer_norm_join_kernel, dim3(ceil_div(2 * (int64_t)channels, 16)), dim3(256),
-                       0, stream, (const float *)workspace, rows > 0 ? groups : 0, channels,
-                       weight_type, grad_weight, grad_bias);
+    hipLaunchKernelGGL(layer_norm_join_kernel, dim3(ceil_div(2 * (int64_t)channels, kJoinColumns)),
+                       dim3(kJoinColumns * kJoinRows), 0, stream, (const float *)workspace,
+                       rows > 0 ? groups : 0, channels, weight_type, grad_weight, grad_bias);
     return launch_status();
 }
