@@ -146,6 +146,26 @@ __device__ __forceinline__ void add_product_seen(f32x16 *acc, const lds_char *ti
     }
 }
 
+// sum + the 8 rounded weights.
+template <typename T>
+__device__ __forceinline__ float add_weights(const typename Vec<T>::x8 &w, float sum) {
+    const u32x4 pairs = __builtin_bit_cast(u32x4, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t pair = pairs[i];
+        if constexpr (std::is_same<T, f16>::value) {
+            using Two = __attribute__((ext_vector_type(2))) f16;
+            sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(Two, pair), Two{(f16)1.0f, (f16)1.0f},
+                                         sum, false);
+        } else {
+            using Two = __attribute__((ext_vector_type(2))) short;
+            sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(Two, pair),
+                                                  Two{0x3f80, 0x3f80}, sum, false);
+        }
+    }
+    return sum;
+}
+
 // The same, not rounded, for a sum that is joined later.
 template <int DIM>
 __device__ __forceinline__ void store_partial(const f32x16 *acc, float factor, float *row, int dim) {
@@ -204,8 +224,11 @@ struct Partial {
 };
 
 // One tile of rows with one split of its keys; share: tiles of a split, or 0 for as many as
-// there are over the splits.
-template <typename T, int DIM, bool BY_KEYS>
+// there are over the splits.  LOG_SUM: the weights' sum is kept as it is beside that of the
+// rounded weights, for the log-sum and for the shares of parts; it costs 16 of a step's
+// additions, 4% of the time at 128 dimensions (2.05 -> 2.13 ms for 16320 rows and keys, 16
+// heads on 4).
+template <typename T, int DIM, bool BY_KEYS, bool LOG_SUM>
 __device__ __forceinline__ void forward_rows(
     const GsAttention &a, const T *q, const T *k, const T *v, T *out, T *out_rest, float *log_sum,
     const Partial &partial, lds_char *tiles, int kh, int sequence, int number, int split, int share) {
@@ -259,7 +282,8 @@ __device__ __forceinline__ void forward_rows(
     f32x16 acc[DIM / 32];
 #pragma unroll
     for (int d = 0; d < DIM / 32; ++d) acc[d] = f32x16{};
-    float top = -INFINITY, sum = 0.0f;  // of c S; the sum of this half's keys
+    // the maximum of c S; the weights' sum over this half's keys, and that of the rounded ones
+    float top = -INFINITY, sum = 0.0f, rounded = 0.0f;
 
     const auto step = [&](int t, auto masks) {
         constexpr bool kMasks = decltype(masks)::value;
@@ -300,6 +324,7 @@ __device__ __forceinline__ void forward_rows(
             const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
             top = now;
             sum *= keep;
+            rounded *= keep;
 #pragma unroll
             for (int d = 0; d < DIM / 32; ++d) acc[d] *= keep;
         }
@@ -311,10 +336,11 @@ __device__ __forceinline__ void forward_rows(
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 w[r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, minus));
-                sum += w[r];
+                if (LOG_SUM) sum += w[r];
             }
             weights[2 * n] = pack8<T>(w);
             weights[2 * n + 1] = pack8<T>(w + 8);
+            rounded = add_weights<T>(weights[2 * n + 1], add_weights<T>(weights[2 * n], rounded));
         }
 #pragma unroll
         for (int n = 0; n < F::kSub; ++n) {
@@ -332,7 +358,18 @@ __device__ __forceinline__ void forward_rows(
     for (const int whole = min(end_tile, (all_see + 1) / F::kKeys); t < whole; ++t)
         step(t, std::false_type{});
     for (; t < end_tile; ++t) step(t, std::true_type{});
-    sum = half_sum(sum);
+    // The sums are over the rounded weights, and so is what they are divided by: a weight's error
+    // then counts by its value's distance from the output, which for a weight that outdoes the
+    // others is next to none.  The log-sum, and a part's share of the whole, are of the
+    // weights as they were.
+    rounded = half_sum(rounded);
+    sum = LOG_SUM ? half_sum(sum) : rounded;
+    if (LOG_SUM && (BY_KEYS || partial.splits > 1)) {
+        const float share_up = rounded > 0.0f ? sum / rounded : 1.0f;
+#pragma unroll
+        for (int d = 0; d < DIM / 32; ++d) acc[d] *= share_up;
+        rounded = sum;
+    }
 
     if constexpr (BY_KEYS) {
         // the waves' sums over their keys, joined in LDS by the first
@@ -367,7 +404,7 @@ __device__ __forceinline__ void forward_rows(
                 acc[d][r] = x;
             }
         top = all;
-        sum = total;
+        sum = rounded = total;
     }
 
     if (partial.splits > 1) {
@@ -389,13 +426,13 @@ __device__ __forceinline__ void forward_rows(
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[d][r] = none ? 0.0f : acc[d][r];
     }
-    store_columns<T, DIM>(acc, none ? 1.0f : 1.0f / sum, real ? out + at * a.dim : nullptr, a.dim,
+    store_columns<T, DIM>(acc, none ? 1.0f : 1.0f / rounded, real ? out + at * a.dim : nullptr, a.dim,
                           out_rest != nullptr, real && out_rest ? out_rest + at * a.dim : nullptr);
-    if (log_sum && real && half == 0)
+    if (LOG_SUM && log_sum && real && half == 0)
         log_sum[at] = none ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-template <typename T, int DIM>
+template <typename T, int DIM, bool LOG_SUM>
 __global__ __launch_bounds__(64 * kWaves, 2) void attention_kernel(
     GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
     T *__restrict__ out, T *__restrict__ out_rest, float *__restrict__ log_sum, Partial partial) {
@@ -406,8 +443,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kernel(
     if (!find_tile(a.offsets_q, a.sequences, a.rows_q, a.heads_q / a.heads_k, F::kRows, at.tile, true,
                    &sequence, &number))
         return;
-    forward_rows<T, DIM, false>(a, q, k, v, out, out_rest, log_sum, partial, (lds_char *)lds, at.kh, sequence,
-                                number, at.split, 0);
+    forward_rows<T, DIM, false, LOG_SUM>(a, q, k, v, out, out_rest, log_sum, partial, (lds_char *)lds,
+                                         at.kh, sequence, number, at.split, 0);
 }
 
 // Few rows a sequence.  Caches differ in length, and the host does not know them: a split is as
@@ -451,9 +488,9 @@ __global__ __launch_bounds__(64 * kKeysWaves, DIM > 96 ? 1 : 2) void attention_k
          item += gridDim.x) {
         const int t = uniform(tiles_of(sequence)), splits = splits_of(t);
         const int rest = number / a.heads_k;
-        forward_rows<T, DIM, true>(a, q, k, v, out, out_rest, log_sum, partial, (lds_char *)lds,
-                                   number % a.heads_k, sequence, rest / splits, rest % splits,
-                                   share_of(t));
+        forward_rows<T, DIM, true, true>(a, q, k, v, out, out_rest, log_sum, partial,
+                                         (lds_char *)lds, number % a.heads_k, sequence,
+                                         rest / splits, rest % splits, share_of(t));
         __syncthreads();  // LDS has been read
     }
 }
@@ -512,7 +549,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
 // both: seven products in all where one launch with atomics needs five.
 //
 // Score gradients are rounded to the inputs' type for their products, which adds as much
-// again to the rounding of the result (1.41 times its error in all).  In float16 they are
+// again to the rounding of the result (1.41 times its error in all, and up to 1.5 with what
+// delta has from the output's rounded weights).  In float16 they are
 // first put into its range: weights times 2^10, so that those of long rows keep their
 // bits, and score gradients times 2^4 over the power of two of the row's largest
 // output gradient, so that neither small gradients vanish nor large ones overflow.  Where
@@ -1015,9 +1053,12 @@ static int launch_forward(const GsAttention &a, const ForwardPlan &f, const void
         hipLaunchKernelGGL((attention_keys_kernel<T, DIM>), grid,
                            dim3(64 * kKeysWaves), 0, stream, a, tq, tk, tv,
                            (T *)out, (T *)out_rest, log_sum, partial);
+    else if (log_sum || f.splits > 1)
+        hipLaunchKernelGGL((attention_kernel<T, DIM, true>), grid, dim3(64 * kWaves), 0, stream, a,
+                           tq, tk, tv, (T *)out, (T *)out_rest, log_sum, partial);
     else
-        hipLaunchKernelGGL((attention_kernel<T, DIM>), grid, dim3(64 * kWaves), 0, stream, a, tq, tk,
-                           tv, (T *)out, (T *)out_rest, log_sum, partial);
+        hipLaunchKernelGGL((attention_kernel<T, DIM, false>), grid, dim3(64 * kWaves), 0, stream, a,
+                           tq, tk, tv, (T *)out, (T *)out_rest, log_sum, partial);
     int st = launch_status();
     if (st || f.splits == 1) return st;
     const int64_t rows = a.rows_q * a.heads_q;

@@ -476,6 +476,29 @@ def test_attention_of_small_and_large_gradients(gpu, exponent):
             within(got, ref[name], 2.0 ** -11 * 1.1 * ref[name + "_slack"] + 2.0 ** -24, name)
 
 
+@pytest.mark.parametrize("lq,heads,key_heads", [(64, 8, 8), (64, 256, 1), (4, 8, 8), (1, 16, 1)])
+def test_attention_of_one_great_weight(gpu, lq, heads, key_heads):
+    """A weight that outdoes all others leaves its value, whatever it was rounded to itself: with
+    the sum of the rounded weights below it, a weight's error e counts e (v - o), so the output
+    is off by its own rounding and 2 u (1 - p) 2 max|v| of the others' share 1 - p."""
+    g = rng(gpu, 11)
+    lk, dim, u = 300, 64, U[torch.float16]
+    q, k = (torch.zeros(n, h, dim, dtype=torch.float16, device=gpu)
+            for n, h in ((lq, heads), (lk, key_heads)))
+    q[:, :, 0] = 0.9 + 0.1 * torch.rand(lq, heads, generator=g, device=gpu)
+    k[:, :, 0] = -8.0
+    k[3], k[200] = 0.0, 0.0
+    k[200, :, 0] = 7.5  # in a later tile than the first reference, and less than 2^8 above it
+    v = randn(g, lk, key_heads, dim).half()
+    at_q, at_k = offsets_of([lq], gpu), offsets_of([lk], gpu)
+    out = cr.packed_attention(q, k, v, at_q, at_k, scale=math.log(2.0))
+    want = ot.attention(q, k, v, at_q, at_k, scale=math.log(2.0))["out"]
+    rest = 2.0 ** (7.5 * q[:, :, :1].double())
+    rest = 1 - rest / (rest + 1 + 298 * 2.0 ** (-8 * q[:, :, :1].double()))
+    assert float(rest.max()) < 0.05
+    within(out, want, u * want.abs() + 4 * u * rest * float(v.abs().max()) + 16 * E, "out")
+
+
 def test_attention_does_not_see_the_masked(gpu):
     """NaN and infinity in keys and values after a query change nothing before them."""
     for dtype in TYPES[1:]:
