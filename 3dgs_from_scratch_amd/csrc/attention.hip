@@ -108,24 +108,31 @@ __device__ __forceinline__ uint64_t rows_not_finite(const lds_char *tile, int ba
 // acc += X^T P over 32 rows of a tile X from `base`, P in two operands of 16 rows.
 template <typename T, int DIM, typename XTile>
 __device__ __forceinline__ void add_product(f32x16 *acc, const lds_char *tile, int base,
-                                            const typename Vec<T>::x8 *p) {
+                                            const typename Vec<T>::x8 *p,
+                                            const typename Vec<T>::x8 *rest = nullptr) {
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int d = 0; d < DIM / 32; ++d)
-            acc[d] = mfma(XTile::down(tile, base + 16 * g, d), p[g], acc[d]);
+        for (int d = 0; d < DIM / 32; ++d) {
+            const typename Vec<T>::x8 x = XTile::down(tile, base + 16 * g, d);
+            acc[d] = mfma(x, p[g], acc[d]);
+            if (rest) acc[d] = mfma(x, rest[g], acc[d]);
+        }
 }
 
 // The same where the rows hold infinities or NaN; sees(i): whether the lane's column sees row
 // base + i.
 template <typename T, int DIM, typename XTile, typename Sees>
 __device__ __forceinline__ void add_product_seen(f32x16 *acc, const lds_char *tile, int base,
-                                                 const typename Vec<T>::x8 *p, Sees sees) {
+                                                 const typename Vec<T>::x8 *p, Sees sees,
+                                                 const typename Vec<T>::x8 *rest = nullptr) {
     using x8 = typename Vec<T>::x8;
     const int half = __lane_id() >> 5;
 #pragma unroll 1
     for (int g = 0; g < 2; ++g) {
         const x8 weights = g ? p[1] : p[0];
+        x8 more = weights;
+        if (rest) more = g ? rest[1] : rest[0];
         x8 seen;
 #pragma unroll
         for (int j = 0; j < 8; ++j) seen[j] = (T)(sees(16 * g + result_row(j, half)) ? 1.0f : 0.0f);
@@ -139,6 +146,7 @@ __device__ __forceinline__ void add_product_seen(f32x16 *acc, const lds_char *ti
                 x[j] = b ? (T)0.0f : x[j];
             }
             acc[d] = mfma(x, weights, acc[d]);
+            if (rest) acc[d] = mfma(x, more, acc[d]);
             const f32x16 count = mfma(bad, seen, f32x16{});
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[d][r] = count[r] > 0.0f ? NAN : acc[d][r];
@@ -550,8 +558,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
 //
 // Score gradients are rounded to the inputs' type for their products, which adds as much
 // again to the rounding of the result (1.41 times its error in all, and up to 1.5 with what
-// delta has from the output's rounded weights).  In float16 they are
-// first put into its range: weights times 2^10, so that those of long rows keep their
+// delta has from the output's rounded weights).  In float16, which is chosen for its bits, the
+// queries' gradients add what was rounded off in a second product of the same tile of keys
+// (1.02 to 1.08 times the error); it costs the launch 28%, 171 -> 217 us for 4 sequences of
+// 2500, 12 heads of 72, and neither bfloat16 nor the keys' launch, longer by itself, pays it.
+// In float16 they are first put into its range: weights times 2^10, so that those of long rows keep their
 // bits, and score gradients times 2^4 over the power of two of the row's largest
 // output gradient, so that neither small gradients vanish nor large ones overflow.  Where
 // rows are summed over, in the keys' launch, that power is the largest so far, and the
@@ -693,13 +704,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
                 if (kMasks && key0 + 32 * n + result_row(r, half) > last) ds[r] = 0.0f;
             }
             const typename Vec<T>::x8 x[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
+            typename Vec<T>::x8 rests[2], *rest = nullptr;
+            if constexpr (Range<T>::kScaled) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) ds[r] -= to_float((T)x[r / 8][r % 8]);
+                rests[0] = pack8<T>(ds);
+                rests[1] = pack8<T>(ds + 8);
+                rest = rests;
+            }
             const uint32_t part = (uint32_t)(found >> (32 * n));
             if (kMasks && part)
-                add_product_seen<T, DIM, KTile>(acc, kt, 32 * n, x, [&](int i) {
-                    return key0 + 32 * n + i <= last;
-                });
+                add_product_seen<T, DIM, KTile>(
+                    acc, kt, 32 * n, x, [&](int i) { return key0 + 32 * n + i <= last; }, rest);
             else
-                add_product<T, DIM, KTile>(acc, kt, 32 * n, x);
+                add_product<T, DIM, KTile>(acc, kt, 32 * n, x, rest);
         }
     };
     if (first_tile < end_tile) fetch(first_tile);

@@ -499,6 +499,22 @@ def test_attention_of_one_great_weight(gpu, lq, heads, key_heads):
     within(out, want, u * want.abs() + 4 * u * rest * float(v.abs().max()) + 16 * E, "out")
 
 
+def test_attention_float16_query_gradients_keep_their_bits(gpu):
+    """Their error is about that of rounding them once; a second rounding of the same size, of
+    the score gradients, would make it sqrt(2) times as large."""
+    for lengths, heads, dim, causal in (([700], 4, 72, False), ([40] * 30, 4, 64, True)):
+        rows = sum(lengths)
+        q, k, v, go = attention_inputs(gpu, rows, rows, heads, heads, dim, torch.float16)
+        at = offsets_of(lengths, gpu)
+        leaves = [t.requires_grad_(True) for t in (q, k, v)]
+        out = cr.packed_attention(*leaves, at, causal=causal)
+        (gq,) = torch.autograd.grad(out, leaves[:1], go)
+        want = ot.attention(q.detach(), k.detach(), v.detach(), at, causal=causal,
+                                   grad_out=go)["gq"]
+        once = (want.half().double() - want).norm()
+        assert float((gq.double() - want).norm() / once) < 1.3
+
+
 def test_attention_does_not_see_the_masked(gpu):
     """NaN and infinity in keys and values after a query change nothing before them."""
     for dtype in TYPES[1:]:
