@@ -324,9 +324,12 @@ __global__ __launch_bounds__(kJoinColumns *kJoinRows) void layer_norm_join_kerne
         ((bf16 *)out)[to] = from_float<bf16>(s);
 }
 
-// Rows of lanes and packs of 16 bytes for a number of channels: a row of 16 lanes where that
-// is enough, else a wave, else a workgroup; f gets the shape, or 0 if the row does not fit in
-// registers.
+// Rows of lanes and packs of 16 bytes for a number of channels: a row of 16 lanes up to 2
+// packs a lane, else a wave up to 3, else a workgroup; f gets the shape, or 0 if the row does
+// not fit in registers.  Both sides, forward and backward of 65280 rows in bfloat16: 256
+// channels on 16 lanes 75 us, on a wave 137; 512 on a wave 73, on 16 lanes of 4 packs 144;
+// 1024 on a wave 138, on a workgroup 227; 1536 on a wave 267 (forward 83), on a workgroup 265
+// (98); 2048 on a wave of 4 packs 350, on a workgroup 297.
 template <typename T, bool WHOLE, typename F>
 static int with_shape(int channels, F f) {
     constexpr int kVec = 16 / sizeof(T);
@@ -336,7 +339,7 @@ static int with_shape(int channels, F f) {
     if (packs <= 64) return f(Shape<64, 1, kVec, WHOLE>{});
     if (packs <= 128) return f(Shape<64, 2, kVec, WHOLE>{});
     if (packs <= 192) return f(Shape<64, 3, kVec, WHOLE>{});
-    if (packs <= 256) return f(Shape<64, 4, kVec, WHOLE>{});
+    if (packs <= 256) return f(Shape<256, 1, kVec, WHOLE>{});
     if (packs <= 512) return f(Shape<256, 2, kVec, WHOLE>{});
     if (packs <= 1024) return f(Shape<256, 4, kVec, WHOLE>{});
     return f(0);
