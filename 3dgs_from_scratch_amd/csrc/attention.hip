@@ -1003,11 +1003,14 @@ static ForwardPlan plan_forward(const GsAttention &a) {
         f.groups = items < 1024 ? items : 1024;
         return f;
     }
-    // Workgroups that will find rows, at least, and how many splits of the keys fill the
-    // card with them; a split of fewer than four tiles costs more than it hides.
+    // Workgroups that will find rows, at least, and as many splits of the keys as run at a time
+    // with them, 512 workgroups in all, two a CU.  More wait for a second turn and pay a join:
+    // 2500 rows and keys, 16 heads on 4, dim 128, in 1 split of 316 workgroups 83 us, in 2 splits
+    // 113; 300 rows over 16320 keys, 48 workgroups, in 10 splits 82 us, in 1 split 301.  A split of
+    // fewer than four tiles costs more than it hides.
     const int64_t rows = 32 * kWaves;
     const int64_t busy = (packed + rows - 1) / rows * a.heads_k;
-    const int64_t want = busy > 0 ? (512 + busy - 1) / busy : 1;
+    const int64_t want = busy > 0 ? 512 / busy : 1;
     const int64_t most = a.rows_k / sequences / 256;
     const int64_t splits = want < most ? want : most;
     f.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
@@ -1015,9 +1018,10 @@ static ForwardPlan plan_forward(const GsAttention &a) {
     return f;
 }
 
-// How a backward is launched.  A launch of fewer workgroups than fill the card three times
-// (two of a SIMD's four waves fit at up to 64 dimensions in the keys' launch, one above)
-// splits its sums.
+// How a backward is launched: its sums in as many splits as run at a time, as the forward's,
+// 512 workgroups in all, or 256 of the eight waves that the keys' launch has for 65 to 96
+// dimensions.  Forward and gradients of 2500 rows and keys, 16 heads on 4, dim 128, 340 us,
+// with splits for 512 and 768 workgroups or more 396, with none 514.
 struct BackwardPlan {
     int64_t tiles_q, tiles_k;
     int splits_q, splits_k;
@@ -1025,7 +1029,7 @@ struct BackwardPlan {
 
 static int backward_splits(int64_t busy, int64_t slots, int64_t steps) {
     if (busy < 1 || busy >= slots) return 1;
-    const int64_t want = (slots + busy - 1) / busy, most = steps / 8;
+    const int64_t want = slots / busy, most = steps / 8;
     const int64_t splits = want < most ? want : most;
     return (int)(splits < 1 ? 1 : splits > 8 ? 8 : splits);
 }
@@ -1039,7 +1043,7 @@ static BackwardPlan plan_backward(const GsAttention &a) {
     b.tiles_k = a.rows_k / own + a.sequences + 2;
     b.splits_q = backward_splits((packed + kBackOwn - 1) / kBackOwn * a.heads_k, 512,
                                  a.rows_k / sequences / kBackRows / see);
-    b.splits_k = backward_splits((a.rows_k + own - 1) / own * a.heads_k, a.dim > 96 ? 768 : a.dim > 64 ? 384 : 1024,
+    b.splits_k = backward_splits((a.rows_k + own - 1) / own * a.heads_k, own > kBackOwn ? 256 : 512,
                                  packed / sequences / kBackRows / see);
     return b;
 }
