@@ -190,14 +190,6 @@ __device__ __forceinline__ void store_partial(const f32x16 *acc, float factor, f
         }
 }
 
-// Forward.  A workgroup takes a tile of packed rows of one key head (row r of a
-// sequence: query r / group, head r % group of the group) and walks the sequence's
-// keys, or a split's part of them, once:
-//   S^T = K Q^T,  P = exp2(c S - m),  O^T += V^T P^T
-// with a row in a lane pair, so that the softmax needs one exchange and the factors
-// that follow a new maximum none.  K and V go from memory into LDS beside the work on
-// the tile before.  BY_KEYS: a few rows only; the waves share the rows and split the
-// keys of a tile, and join at the end.
 // A workgroup's place in its launch: splits of a tile next to each other, so that the longest
 // tiles start first, and key heads innermost: workgroups go to the eight XCDs in turn, and
 // with 8 or a divisor of 8 key heads an XCD's L2 holds one of them.
@@ -209,6 +201,25 @@ __device__ __forceinline__ Place place_of(int heads_k, int splits) {
     return {(int)blockIdx.x % heads_k, rest % splits, rest / splits};
 }
 
+// Forward.  A workgroup takes a tile of packed rows of one key head (row r of a
+// sequence: query r / group, head r % group of the group) and walks the sequence's
+// keys, or a split's part of them, once:
+//   S^T = K Q^T,  P = exp2(c S - m),  O^T += V^T P^T
+// with a row in a lane pair, so that the softmax needs one exchange and the factors
+// that follow a new maximum none.  K and V go from memory into LDS beside the work on
+// the tile before.  BY_KEYS: a few rows only; the waves share the rows and split the
+// keys of a tile, and join at the end.
+//
+// Bound by the matrix units and by LDS at once: a wave's 32 rows read all of a tile of K and
+// V, so LDS is busy 80 to 93% of the time, and under that load the clock falls to 1.7 to 1.9
+// GHz.  128 rows a workgroup and two of them a CU are what 160 KB of LDS and 256 registers a
+// lane hold at 128 dimensions.  16320 rows and keys, 16 heads on 4, dim 128, bfloat16: 2.05
+// to 2.15 ms, 1.01 to 1.06 PFLOP/s; 7 causal sequences of 1 to 8160: 0.29 ms, 0.94.
+//
+// Weights are rounded to the inputs' type for their product with V: 2^-9 (2^-12 in float16)
+// of a weight, unbiased.  Infinities and NaN in rows that nothing sees change nothing; a
+// query that sees one in V gets NaN where its column holds it, a tile with both kinds of
+// query is told apart key by key; what a seen K holds goes into its score.
 template <typename T, int DIM, bool BY_KEYS>
 struct Forward {
     // by keys: two waves, so that a CU's LDS holds two workgroups, and one's first tile and
@@ -504,7 +515,7 @@ __global__ __launch_bounds__(64 * kKeysWaves, DIM > 96 ? 1 : 2) void attention_k
 }
 
 // Joins the splits of a row: a workgroup a row, four elements a thread, every eighth split
-// in each of its eight parts.
+// in each of its eight parts.  Bound by latency: 256 rows of 28 splits 4.8 us.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int dim, Partial partial,
                                                              T *__restrict__ out,
@@ -554,7 +565,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
 // packed rows as in the forward, which also leaves each row's log-sum (in the exponent
 // of two) and delta for the second; then the keys' and values', a workgroup a tile of
 // keys, over all the queries of all heads of the group.  Scores are computed again in
-// both: seven products in all where one launch with atomics needs five.
+// both: seven products in all where one launch with atomics needs five, whose sums' order
+// would change from run to run.
+//
+// Bound as the forward is, the keys' launch more by its registers: two sums of a tile of keys
+// and both operands leave one wave a SIMD above 96 dimensions.  16320 rows and keys, 16 heads
+// on 4, dim 128, bfloat16: queries 2.75 ms, 1.19 PFLOP/s of its three products; keys and
+// values 4.4 to 5.1 ms, 0.86 to 0.99 of its four.
 //
 // Score gradients are rounded to the inputs' type for their products, which adds as much
 // again to the rounding of the result (1.41 times its error in all, and up to 1.5 with what
@@ -657,7 +674,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
     // a row that saw nothing has no weights: exp2(x - infinity) = 0
     const float given = real ? log_sum[at] : -INFINITY;
     const float log2_sum = given == -INFINITY ? INFINITY : given * kLog2e;
-    const float row_exponent = log2_sum - __builtin_amdgcn_logf(range);
+    // a row that sees one key has no score gradient: its dout v^T and delta are the same sum in
+    // two orders, whose difference would be all there is of it
+    const float row_exponent = last == 0 ? INFINITY : log2_sum - __builtin_amdgcn_logf(range);
     if (real && half == 0 && split == 0) {  // as the keys' launch uses them
         const int64_t to = (int64_t)head * a.rows_q + p.q0 + query;
         row_log[to] = log2_sum - Range<T>::kWeight;
@@ -734,8 +753,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
         store_columns<T, DIM>(acc, a.scale / range, real ? dq + at * a.dim : nullptr, a.dim);
 }
 
-// Above 64 dimensions the sums of two waves a SIMD leave no registers for V: it lies in LDS,
-// which then has room for one workgroup of eight waves.
+// Up to 64 dimensions a wave holds its keys' K and V and both sums in half a SIMD's registers,
+// and four waves make a workgroup, two a CU.  At 65 to 96 two waves' sums leave no room for V,
+// which lies in LDS; that then has room for one workgroup of eight waves.  At 97 to 128 the
+// sums alone take half of a SIMD's registers: K and V stay in those of one wave, and four
+// waves make a workgroup.
 template <int DIM>
 struct KeysShape {
     static constexpr bool kValuesInLds = DIM == 96;
@@ -780,6 +802,9 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
     const int end_tile = block_key < p.lk ? (p.lq + kBackRows - 1) / kBackRows : 0;
     const int whole_tile = min((whole + kBackRows - 1) / kBackRows, end_tile);
     const int own_first = a.causal ? key - shift : 0;  // the first query that sees this key
+    // and the first that sees another one too, so that it has a score gradient (where the
+    // sequence has other keys: only with a causal mask)
+    const int own_shared = own_first + (a.causal && key == 0);
 
     const T *key_row = counts ? k + (int64_t)(p.k0 + key) * a.k_row + (int64_t)kh * a.k_head : nullptr;
     const T *value_row = counts ? v + (int64_t)(p.k0 + key) * a.v_row + (int64_t)kh * a.v_head : nullptr;
@@ -878,8 +903,11 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
                     const int r = 4 * g + j;
                     w[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -l[j]));
                     ds[r] = (Range<T>::kScaled ? w[r] * range : w[r]) * dp[r];
-                    if (kMasks && query0 + 32 * n + result_row(r, half) < own_first)
-                        w[r] = ds[r] = 0.0f;
+                    if (kMasks) {
+                        const int query = query0 + 32 * n + result_row(r, half);
+                        if (query < own_first) w[r] = 0.0f;
+                        if (query < own_shared) ds[r] = 0.0f;
+                    }
                 }
             }
             const typename Vec<T>::x8 pw[2] = {pack8<T>(w), pack8<T>(w + 8)};
@@ -914,6 +942,10 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
         if (i + 1 < steps) fetch(i + 1);
         step(i, std::true_type{});
     }
+    if (p.lk == 1) {  // no query sees another key
+#pragma unroll
+        for (int d = 0; d < DIM / 32; ++d) gk[d] *= 0.0f;
+    }
     // keys past the length that counts have no gradient
     if (__ballot(!counts || bad)) {
         const float instead = counts ? NAN : 0.0f;
@@ -939,7 +971,8 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
     store_columns<T, DIM>(gv, back_v, real ? dv + at : nullptr, a.dim);
 }
 
-// Sums of splits, rounded: the y-th of the launch's outputs, four elements a thread.
+// Sums of splits, rounded: the y-th of the launch's outputs, four elements a thread.  Bound by
+// memory: two splits of 16320 rows of 4 heads of 128, twice, 26 us.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_sum_kernel(const float *__restrict__ partial,
                                                             int64_t size, int splits, float scale0,
@@ -992,6 +1025,8 @@ static ForwardPlan plan_forward(const GsAttention &a) {
     const int64_t group = a.heads_q / a.heads_k, packed = a.rows_q * group;
     const int64_t sequences = a.sequences > 0 ? a.sequences : 1;
     ForwardPlan f;
+    // One tile of rows a sequence at most.  16 sequences over 16320 keys each, 16 heads on 4, dim
+    // 128: 1 query 113 us, otherwise 130; 8 queries (32 rows) 117 and 142; 12 (48) 143 and 133.
     f.by_keys = packed <= 32 * sequences;
     if (f.by_keys) {
         // a row may have up to 64 splits of at least 256 keys, as far as the rows' sums stay few

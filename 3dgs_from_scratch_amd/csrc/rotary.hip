@@ -194,7 +194,9 @@ extern "C" int gs_axial_rotary(const GsRotaryTensor *tensors, int32_t n_tensors,
             const int64_t units = Unit<kBetween, kVec>::count(dim, (int)pairs);
             const int64_t blocks = (tokens * units + kRotaryBlock - 1) / kRotaryBlock;
             if (blocks > 0x7fffffffLL) return (int)GS_ERR_UNSUPPORTED;
-            // as many heads a thread as leave the card 2048 workgroups
+            // as many heads a thread as leave the card 2048 workgroups, so that small calls
+            // spread and large ones compute an angle once: 65280 tokens of 20 heads of 128,
+            // there and back, 338 us, with one head a thread 342, with all 340
             RotaryBatch b = batch;
             int64_t at_once = blocks * heads / 2048;
             if (at_once < (heads + 65534) / 65535) at_once = (heads + 65534) / 65535;

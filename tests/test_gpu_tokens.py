@@ -499,6 +499,29 @@ def test_attention_of_one_great_weight(gpu, lq, heads, key_heads):
     within(out, want, u * want.abs() + 4 * u * rest * float(v.abs().max()) + 16 * E, "out")
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("dim", [32, 72, 128])
+def test_attention_of_one_key_has_no_score_gradient(gpu, dim, dtype):
+    """A query that sees one key: its weight is 1 whatever the score, so its gradient and what it
+    adds to the key's are zero, not the difference of two roundings of one sum."""
+    for lq, lk, causal in (([1] * 40, None, False), ([1] * 40, None, True), ([70, 3], [1, 1], False),
+                           ([70, 3], [1, 1], True), ([300], [1], False)):
+        at_q, at_k = offsets_of(lq, gpu), offsets_of(lk or lq, gpu)
+        q, k, v, go = attention_inputs(gpu, sum(lq), sum(lk or lq), 4, 2, dim, dtype)
+        _, _, gq, gk, gv = check_attention(q, k, v, at_q, at_k, causal=causal, go=go)
+        assert bool((gq == 0).all()) and bool((gk == 0).all()) and bool((gv != 0).any())
+    # the first query of a causal sequence, and the first that sees a key of fewer keys
+    for lq, lk, first in (([130, 65], [130, 65], [0, 130]), ([200], [140], [60])):
+        at_q, at_k = offsets_of(lq, gpu), offsets_of(lk, gpu)
+        q, k, v, go = attention_inputs(gpu, sum(lq), sum(lk), 4, 2, dim, dtype)
+        alone = torch.zeros_like(go)
+        alone[first] = go[first]
+        _, _, gq, gk, gv = check_attention(q, k, v, at_q, at_k, causal=True, go=alone)
+        assert bool((gq == 0).all()) and bool((gk == 0).all()) and bool((gv != 0).any())
+        _, _, gq, _, _ = check_attention(q, k, v, at_q, at_k, causal=True, go=go)
+        assert bool((gq[first] == 0).all()) and bool((gq != 0).any())
+
+
 def test_attention_float16_query_gradients_keep_their_bits(gpu):
     """Their error is about that of rounding them once; a second rounding of the same size, of
     the score gradients, would make it sqrt(2) times as large."""
