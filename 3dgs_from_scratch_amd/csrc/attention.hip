@@ -383,6 +383,8 @@ __device__ __forceinline__ void forward_rows(
     // weights as they were.
     rounded = half_sum(rounded);
     sum = LOG_SUM ? half_sum(sum) : rounded;
+    // a row whose scores are all NaN has no maximum, but is not one that saw nothing
+    if (sum != sum) top = fmaxf(top, 0.0f);
     if (LOG_SUM && (BY_KEYS || partial.splits > 1)) {
         const float share_up = rounded > 0.0f ? sum / rounded : 1.0f;
 #pragma unroll

@@ -553,6 +553,33 @@ def test_attention_does_not_see_the_masked(gpu):
             assert not bool(torch.isfinite(got[row:]).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("lq,lk", [(300, 300), (1, 1), (3, 5000), (300, 3000)])
+def test_attention_of_queries_that_are_nan(gpu, dtype, lq, lk):
+    """A NaN in a query makes its output, log-sum and gradient NaN, and no other's; so does one
+    in the only key of a sequence.  (Rows in tiles, few rows, and keys in splits.)"""
+    q, k, v, go = attention_inputs(gpu, lq, lk, 4, 2, 64, dtype)
+    oq, ok = offsets_of([lq], gpu), offsets_of([lk], gpu)
+    row = lq // 2
+    clean = cr.packed_attention(q, k, v, oq, ok, return_log_sum=True)
+    q2 = q.clone()
+    q2[row, :, 7] = math.nan
+    leaves = [t.clone().requires_grad_(True) for t in (q2, k, v)]
+    out, log_sum = cr.packed_attention(*leaves, oq, ok, return_log_sum=True)
+    gq, gk, gv = torch.autograd.grad(out, leaves, go)
+    alone = cr.packed_attention(q2, k, v, oq, ok)
+    others = torch.arange(lq, device=gpu) != row
+    for got, want in ((out, clean[0]), (log_sum, clean[1]), (alone, clean[0])):
+        assert bool(torch.isnan(got[row]).all())
+        assert torch.equal(got[others], want[others])
+    assert bool(torch.isnan(gq[row]).all()) and bool(torch.isfinite(gq[others]).all())
+    assert bool(torch.isnan(gk).all()) and bool(torch.isnan(gv).all())
+    k2 = k.clone()
+    k2[0, :, 7] = math.nan
+    one = cr.packed_attention(q, k2, v, oq, ok, torch.ones(1, device=gpu, dtype=torch.int32))
+    assert bool(torch.isnan(one).all())
+
+
 def test_attention_layouts(gpu):
     for dtype in TYPES[1:]:
         for dim in (64, 72):
