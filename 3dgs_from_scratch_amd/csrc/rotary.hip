@@ -2,7 +2,7 @@
 // the angle position[axis(p)] * frequency[p]; the gradient is the turn back.
 //
 // Bound by memory: every element is read and written once.  A thread takes the same
-// pairs of several heads of a token, so that an angle's sine and cosine are computed
+// pairs of up to five heads of a token, so that an angle's sine and cosine are computed
 // once for them, and reads and writes 16 (or 8) bytes at a time where the layout
 // allows it.
 
@@ -19,7 +19,7 @@ struct RotaryBatch {
     GsRotaryTensor t[kRotaryTensors];
     int32_t ends[GS_MAX_AXES];  // one past each axis's last pair
     int32_t axes, pairs, dim, n;
-    int32_t heads, heads_at_once;  // of all tensors; of a thread
+    int32_t heads, groups;  // of all tensors; a thread has every groups-th head
     const void *positions;
     int64_t position_stride;
     const float *frequencies;
@@ -69,9 +69,11 @@ __global__ __launch_bounds__(kRotaryBlock) void rotary_kernel(RotaryBatch b, int
     using U = Unit<INTERLEAVED, VEC>;
     const int units = (int)U::count(b.dim, b.pairs);
     const int64_t i = (int64_t)blockIdx.x * kRotaryBlock + threadIdx.x;
-    const int64_t token = i / units;
+    const int64_t token = i / ((int64_t)units * b.groups);
     if (token >= tokens) return;
-    const int unit = (int)(i - token * units), pair = unit * U::kPairs;
+    const int64_t place = i - token * units * b.groups;
+    const int head0 = (int)(place / units);
+    const int unit = (int)(place - (int64_t)head0 * units), pair = unit * U::kPairs;
     const bool turned = pair < b.pairs;
     float s[U::kPairs], c[U::kPairs];
     if (turned) {
@@ -86,10 +88,8 @@ __global__ __launch_bounds__(kRotaryBlock) void rotary_kernel(RotaryBatch b, int
     }
     const int first = INTERLEAVED ? unit * U::kElements : turned ? pair : pair + b.pairs;
     const bool odd_end = U::kElements > VEC && first + 1 >= b.dim;  // one element is left
-    const int head0 = blockIdx.y * b.heads_at_once;
-    const int end = min(head0 + b.heads_at_once, b.heads);
 #pragma unroll 2
-    for (int head = head0; head < end; ++head) {
+    for (int head = head0; head < b.heads; head += b.groups) {
         const bool second = head >= b.t[0].heads;
         const GsRotaryTensor &t = b.t[second];
         const int h = second ? head - b.t[0].heads : head;
@@ -192,17 +192,19 @@ extern "C" int gs_axial_rotary(const GsRotaryTensor *tensors, int32_t n_tensors,
             constexpr int kVec = decltype(vec)::value;
             constexpr bool kBetween = decltype(between)::value;
             const int64_t units = Unit<kBetween, kVec>::count(dim, (int)pairs);
-            const int64_t blocks = (tokens * units + kRotaryBlock - 1) / kRotaryBlock;
-            if (blocks > 0x7fffffffLL) return (int)GS_ERR_UNSUPPORTED;
-            // as many heads a thread as leave the card 2048 workgroups, so that small calls
-            // spread and large ones compute an angle once: 65280 tokens of 20 heads of 128,
-            // there and back, 338 us, with one head a thread 342, with all 340
+            // Five heads a thread, so that an angle is computed a fifth as often, or fewer where
+            // the card would have less than 512 workgroups; a token's threads lie next to each
+            // other and take every groups-th head, so that a wave's accesses do too.  65280
+            // tokens of 20 heads of 128, bfloat16, one way: 5 heads a thread 136 us (4.9 TB/s),
+            // 10 151, 20 168, 1 173; 2500 tokens: 3 heads 9 us, 20 25; 12 tokens: 1 head 4, 20 13.
+            int64_t each = 5;
+            const auto threads = [&] { return tokens * units * ((heads + each - 1) / each); };
+            while (each > 1 && threads() < 512 * kRotaryBlock) each = (each + 1) / 2;
             RotaryBatch b = batch;
-            int64_t at_once = blocks * heads / 2048;
-            if (at_once < (heads + 65534) / 65535) at_once = (heads + 65534) / 65535;
-            b.heads_at_once = (int32_t)(at_once < 1 ? 1 : at_once > heads ? heads : at_once);
-            hipLaunchKernelGGL((rotary_kernel<T, P, kVec, kBetween>),
-                               dim3((unsigned)blocks, ceil_div(heads, b.heads_at_once)),
+            b.groups = (int32_t)((heads + each - 1) / each);
+            const int64_t blocks = (threads() + kRotaryBlock - 1) / kRotaryBlock;
+            if (blocks > 0x7fffffffLL) return (int)GS_ERR_UNSUPPORTED;
+            hipLaunchKernelGGL((rotary_kernel<T, P, kVec, kBetween>), dim3((unsigned)blocks),
                                dim3(kRotaryBlock), 0, stream, b, tokens);
             return launch_status();
         };
