@@ -576,11 +576,15 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
 // values 4.4 to 5.1 ms, 0.86 to 0.99 of its four.
 //
 // Score gradients are rounded to the inputs' type for their products, which adds as much
-// again to the rounding of the result (1.41 times its error in all, and up to 1.5 with what
-// delta has from the output's rounded weights).  In float16, which is chosen for its bits, the
-// queries' gradients add what was rounded off in a second product of the same tile of keys
-// (1.02 to 1.08 times the error); it costs the launch 28%, 171 -> 217 us for 4 sequences of
-// 2500, 12 heads of 72, and neither bfloat16 nor the keys' launch, longer by itself, pays it.
+// again to the rounding of the result (1.41 times its error in all, and more with what delta
+// has from the output's rounded weights: 1.55 for rows of a few keys).  A second product of the
+// same tile with what was rounded off takes it back.  In tiles with a mask, and so for
+// sequences of up to 64 rows, where delta's part is largest, both launches have it (1.3 times
+// the error for rows of 1 to 7 keys in bfloat16; the training pass over scenes of 12566 and
+// 16320 tokens 8.53 -> 8.65 ms).  In float16, which is chosen for its bits, the queries'
+// gradients have it in every tile (1.02 to 1.08 times the error); that costs the launch 28%,
+// 171 -> 217 us for 4 sequences of 2500, 12 heads of 72, and neither bfloat16 nor the keys'
+// launch, longer by itself, pays it.
 // In float16 they are first put into its range: weights times 2^10, so that those of long rows keep their
 // bits, and score gradients times 2^4 over the power of two of the row's largest
 // output gradient, so that neither small gradients vanish nor large ones overflow.  Where
@@ -726,7 +730,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
             }
             const typename Vec<T>::x8 x[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
             typename Vec<T>::x8 rests[2], *rest = nullptr;
-            if constexpr (Range<T>::kScaled) {
+            if constexpr (Range<T>::kScaled || kMasks) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) ds[r] -= to_float((T)x[r / 8][r % 8]);
                 rests[0] = pack8<T>(ds);
@@ -802,7 +806,8 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
     const int whole = a.causal ? max(end_key - 1 - shift, 0) : 0;
     const int first_tile = first / kBackRows;
     const int end_tile = block_key < p.lk ? (p.lq + kBackRows - 1) / kBackRows : 0;
-    const int whole_tile = min((whole + kBackRows - 1) / kBackRows, end_tile);
+    // (one tile of queries goes the way of masked ones, which keeps what rounding takes off)
+    const int whole_tile = end_tile == 1 ? 1 : min((whole + kBackRows - 1) / kBackRows, end_tile);
     const int own_first = a.causal ? key - shift : 0;  // the first query that sees this key
     // and the first that sees another one too, so that it has a score gradient (where the
     // sequence has other keys: only with a causal mask)
@@ -915,7 +920,14 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
             const typename Vec<T>::x8 pw[2] = {pack8<T>(w), pack8<T>(w + 8)};
             const typename Vec<T>::x8 pd[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
             add_product<T, DIM, QTile>(gv, gt, 32 * n, pw);
-            add_product<T, DIM, QTile>(gk, qt, 32 * n, pd);
+            if constexpr (kMasks) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) ds[r] -= to_float((T)pd[r / 8][r % 8]);
+                const typename Vec<T>::x8 rest[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
+                add_product<T, DIM, QTile>(gk, qt, 32 * n, pd, rest);
+            } else {
+                add_product<T, DIM, QTile>(gk, qt, 32 * n, pd);
+            }
         }
     };
     // from the last tile back, every head of the group in turn: workgroups that start together

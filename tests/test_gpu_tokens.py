@@ -538,6 +538,23 @@ def test_attention_float16_query_gradients_keep_their_bits(gpu):
         assert float((gq.double() - want).norm() / once) < 1.3
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [64, 72, 128])
+def test_attention_gradients_of_short_rows_keep_their_bits(gpu, dim, causal):
+    """Score gradients of one tile are not rounded a second time: that would make the error
+    sqrt(2) times that of rounding the gradients once, and more with what delta has of its own."""
+    lengths = torch.randint(2, 8, (300,), generator=torch.Generator().manual_seed(dim)).tolist()
+    rows = sum(lengths)
+    q, k, v, go = attention_inputs(gpu, rows, rows, 2, 2, dim, torch.bfloat16)
+    at = offsets_of(lengths, gpu)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(cr.packed_attention(*leaves, at, causal=causal), leaves[:2], go)
+    ref = ot.attention(q.detach(), k.detach(), v.detach(), at, causal=causal, grad_out=go)
+    for grad, name in zip(got, ("gq", "gk")):
+        once = (ref[name].bfloat16().double() - ref[name]).norm()
+        assert float((grad.double() - ref[name]).norm() / once) < 2 ** 0.5, name
+
+
 def test_attention_does_not_see_the_masked(gpu):
     """NaN and infinity in keys and values after a query change nothing before them."""
     for dtype in TYPES[1:]:
