@@ -586,10 +586,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
 // 171 -> 217 us for 4 sequences of 2500, 12 heads of 72, and neither bfloat16 nor the keys'
 // launch, longer by itself, pays it.
 // In float16 they are first put into its range: weights times 2^10, so that those of long rows keep their
-// bits, and score gradients times 2^4 over the power of two of the row's largest
-// output gradient, so that neither small gradients vanish nor large ones overflow.  Where
-// rows are summed over, in the keys' launch, that power is the largest so far, and the
-// sums follow it.
+// bits, and score gradients times a power of two: in the queries' launch one that brings the
+// largest that the query has met so far to 2^9 and more (Fit), in the keys' launch
+// 2^4 over that of the rows' largest output gradient so far.  The sums follow the powers.
 template <typename T>
 struct Range {
     static constexpr bool kScaled = std::is_same<T, f16>::value;
@@ -602,6 +601,34 @@ __device__ __forceinline__ float power_below(float v) {
     const uint32_t bits = __builtin_bit_cast(uint32_t, v) & 0x7f800000u;
     return bits == 0 || bits == 0x7f800000u ? 1.0f : __builtin_bit_cast(float, bits);
 }
+
+// A column's score gradients in float16: `scale` times themselves, at most 2^15.  The bound is
+// on what is rounded, whatever sizes of queries, values and output gradients made it: a
+// column's largest so far is brought to between 2^9 and 2^10 when it is first met and whenever
+// a greater one passes 2^15, so that what is 2^23 times smaller still has all its bits, and
+// what falls below float16's smallest number is 2^-33 of the largest.  Greater than 2^60 the
+// scale does not become, so that no product with it overflows; what that leaves too small is
+// below any gradient's last bit.
+struct Fit {
+    float scale = 1.0f, limit = 0.0f;
+    template <int SUMS>
+    __device__ __forceinline__ void follow(float *ds, f32x16 *acc) {
+        float most = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(ds[r]));
+        most = half_max(most);  // (an infinity or NaN leaves the scale: its sums are lost)
+        if (__ballot(most > limit)) {
+            const bool passes = most > limit && most < INFINITY;
+            const float ratio = passes ? fminf(512.0f / power_below(most), 0x1p60f / scale) : 1.0f;
+            limit = passes ? 32768.0f : limit;
+            scale *= ratio;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] *= ratio;
+#pragma unroll
+            for (int d = 0; d < SUMS; ++d) acc[d] *= ratio;
+        }
+    }
+};
 
 constexpr int kBackRows = 64;             // of a tile in LDS
 constexpr int kBackOwn = 32 * kWaves;     // rows of a workgroup
@@ -664,7 +691,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
                 delta = fmaf(to_float(gr.x[s][i]), to_float(o.x[s][i]), delta);
     }
     delta = half_sum(delta);
-    float power = 1.0f;  // of the row's output gradients
     if constexpr (Range<T>::kScaled) {
         float most = 0.0f;
 #pragma unroll
@@ -672,17 +698,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
 #pragma unroll
             for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(to_float(gr.x[s][i])));
         most = half_max(most);
-        power = power_below(most);
         if (real && half == 0 && split == 0)  // (a row of zeros has no say in a tile's)
-            row_power[(int64_t)head * a.rows_q + p.q0 + query] = most > 0.0f ? power : 0.0f;
+            row_power[(int64_t)head * a.rows_q + p.q0 + query] =
+                most > 0.0f ? power_below(most) : 0.0f;
     }
-    const float range = Range<T>::kScaled ? Range<T>::kGradient / power : 1.0f;
     // a row that saw nothing has no weights: exp2(x - infinity) = 0
     const float given = real ? log_sum[at] : -INFINITY;
     const float log2_sum = given == -INFINITY ? INFINITY : given * kLog2e;
     // a row that sees one key has no score gradient: its dout v^T and delta are the same sum in
     // two orders, whose difference would be all there is of it
-    const float row_exponent = last == 0 ? INFINITY : log2_sum - __builtin_amdgcn_logf(range);
+    const float row_exponent = last == 0 ? INFINITY : log2_sum;
     if (real && half == 0 && split == 0) {  // as the keys' launch uses them
         const int64_t to = (int64_t)head * a.rows_q + p.q0 + query;
         row_log[to] = log2_sum - Range<T>::kWeight;
@@ -704,6 +729,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
     f32x16 acc[DIM / 32];
 #pragma unroll
     for (int d = 0; d < DIM / 32; ++d) acc[d] = f32x16{};
+    Fit fit;
 
     const auto step = [&](int t, auto masks) {
         constexpr bool kMasks = decltype(masks)::value;
@@ -725,9 +751,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -row_exponent)) * (dp[r] - delta);
+                const float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, -row_exponent));
+                // (the scale is a power of two: the same as scaling the difference)
+                ds[r] = w * (Range<T>::kScaled ? fmaf(dp[r], fit.scale, -delta * fit.scale)
+                                               : dp[r] - delta);
                 if (kMasks && key0 + 32 * n + result_row(r, half) > last) ds[r] = 0.0f;
             }
+            if constexpr (Range<T>::kScaled) fit.follow<DIM / 32>(ds, acc);
             const typename Vec<T>::x8 x[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
             typename Vec<T>::x8 rests[2], *rest = nullptr;
             if constexpr (Range<T>::kScaled || kMasks) {
@@ -751,12 +781,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
         step(t, std::false_type{});
     for (; t < end_tile; ++t) step(t, std::true_type{});
     if (splits > 1)
-        store_partial<DIM>(acc, 1.0f / range,
+        store_partial<DIM>(acc, 1.0f / fit.scale,
                            real ? partial + ((int64_t)split * a.rows_q * a.heads_q + at) * a.dim
                                 : nullptr,
                            a.dim);
     else
-        store_columns<T, DIM>(acc, a.scale / range, real ? dq + at * a.dim : nullptr, a.dim);
+        store_columns<T, DIM>(acc, a.scale / fit.scale, real ? dq + at * a.dim : nullptr, a.dim);
 }
 
 // Up to 64 dimensions a wave holds its keys' K and V and both sums in half a SIMD's registers,

@@ -1,0 +1,95 @@
+"""GPU parity of the patch-network operators where types, lengths and layouts end: float16's
+range, infinities, tiles that a sequence just fills, rows far apart, callers that want part of
+the work.
+
+Gradients of attention are held to oracle/tokens.py::attention_gradients, which derives a bound
+for every element, and as a whole to 3 u of their length: each element has three roundings of at
+most u that matter (its own, its score gradients', delta's), which are independent, so that
+their root mean square together is no more than u."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import helpers  # noqa: F401
+import cuda_rasterizer as cr
+from oracle import tokens as ot
+
+pytestmark = pytest.mark.gpu
+
+HALVES = [torch.float16, torch.bfloat16]
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+def randn(g, *shape):
+    return torch.randn(shape, generator=g, device=g.device)
+
+
+def offsets_of(lengths, gpu):
+    return torch.tensor([0] + lengths, device=gpu).cumsum(0).to(torch.int32)
+
+
+def inputs(gpu, tq, tk, heads, key_heads, dim, dtype, seed=0):
+    g = torch.Generator(device=gpu).manual_seed(11 * tq + tk + dim + seed)
+    return ((1.5 * randn(g, tq, heads, dim)).to(dtype), (1.5 * randn(g, tk, key_heads, dim)).to(dtype),
+            randn(g, tk, key_heads, dim).to(dtype), randn(g, tq, heads, dim).to(dtype))
+
+
+def gradients(q, k, v, go, oq, ok=None, lk=None, causal=False, scale=None):
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = cr.packed_attention(*leaves, oq, ok, lk, causal=causal, scale=scale)
+    return out.detach(), torch.autograd.grad(out, leaves, go)
+
+
+def check_gradients(q, k, v, go, oq, ok=None, lk=None, causal=False, scale=None, names="qkv"):
+    """Against the oracle, element by element and as a whole; gradients of zeros would fail."""
+    ref = ot.attention_gradients(q, k, v, oq, go, ok, lk, causal, scale)
+    _, grads = gradients(q, k, v, go, oq, ok, lk, causal, scale)
+    for name, grad in zip("qkv", grads):
+        if name not in names:
+            continue
+        want, bound = ref["g" + name], ref[f"g{name}_bound"]
+        assert bool(torch.isfinite(grad).all()), name
+        off = (grad.double() - want).abs()
+        assert float((off - bound).max()) <= 0.0, (name, float(off.max()), float((off - bound).max()))
+        length = float(want.norm())
+        assert float(off.norm()) <= 3 * U[q.dtype] * length and length > 0.0, (
+            name, float(off.norm()) / length)
+    return grads
+
+
+# --------------------------------------------------------------- float16's range
+def ranged(gpu, kind, dim):
+    """float16 inputs (q, k, v, go, lengths) whose score gradients, or what leads to them, lie near
+    the ends of float16, though the gradients do not."""
+    g = torch.Generator(device=gpu).manual_seed(dim)
+    lengths = [2] * 20 if kind == "two equal weights" else [64, 250, 350]
+    n = sum(lengths)
+    q, k, v, go = (randn(g, n, 2, dim) for _ in range(4))
+    sign = torch.sign(randn(g, n, 2, 1))
+    if kind == "two equal weights":  # the difference to the output is as large as the values
+        q, k, go = 0.01 * q, 0.25 * k, 1.9 + 0.0 * go
+        v = 34.0 * torch.tensor([1.0, -1.0], device=gpu).repeat(n // 2)[:, None, None] + 0.0 * v
+    elif kind == "values equal along a row":
+        q, k, v, go = 0.3 * q, 0.3 * k, 100.0 * sign + 0.0 * v, 1e-3 * torch.sign(go[..., :1]) + 0.0 * go
+    elif kind == "large values":
+        q, k, v = 0.3 * q, 0.3 * k, 1000.0 * v
+    elif kind == "largest values":
+        q, k, v, go = 0.1 * q, 0.1 * k, 30000.0 * sign + 0.0 * v, 0.5 * go
+    elif kind == "small values":
+        q, k, v = 3.0 * q, 3.0 * k, v / 1024.0
+    else:  # "first queries large"
+        go = go * torch.where(torch.arange(n, device=gpu) % 64 < 40, 2.0 ** 10, 2.0 ** -7)[:, None, None]
+    return *(t.half() for t in (q, k, v, go)), lengths
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [64, 72, 128])
+@pytest.mark.parametrize("kind", ["two equal weights", "values equal along a row", "large values",
+                                  "largest values", "small values", "first queries large"])
+def test_attention_query_gradients_stay_in_float16(gpu, kind, dim, causal):
+    q, k, v, go, lengths = ranged(gpu, kind, dim)
+    check_gradients(q, k, v, go, offsets_of(lengths, gpu), causal=causal, names="q")
