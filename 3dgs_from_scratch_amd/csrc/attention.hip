@@ -586,14 +586,12 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
 // 171 -> 217 us for 4 sequences of 2500, 12 heads of 72, and neither bfloat16 nor the keys'
 // launch, longer by itself, pays it.
 // In float16 they are first put into its range: weights times 2^10, so that those of long rows keep their
-// bits, and score gradients times a power of two: in the queries' launch one that brings the
-// largest that the query has met so far to 2^9 and more (Fit), in the keys' launch
-// 2^4 over that of the rows' largest output gradient so far.  The sums follow the powers.
+// bits, and score gradients times a power of two that follows the largest that the query, or
+// the key, has met so far (Fit), and that the sums follow.
 template <typename T>
 struct Range {
     static constexpr bool kScaled = std::is_same<T, f16>::value;
     static constexpr float kWeight = kScaled ? 10.0f : 0.0f;  // exponents of two
-    static constexpr float kGradient = 16.0f;
 };
 
 // The power of two at or below v's magnitude; 1 for zero, infinities and NaN.
@@ -608,7 +606,10 @@ __device__ __forceinline__ float power_below(float v) {
 // a greater one passes 2^15, so that what is 2^23 times smaller still has all its bits, and
 // what falls below float16's smallest number is 2^-33 of the largest.  Greater than 2^60 the
 // scale does not become, so that no product with it overflows; what that leaves too small is
-// below any gradient's last bit.
+// below any gradient's last bit.  Forward and gradients with it, and with a factor from the
+// output gradients alone, which values of 34 overflow: 8160 rows and keys, 16 heads on 4, dim
+// 128, 2.80 ms and 2.85; 4 sequences of 2500, 12 heads of 72, 638 us and 646; of 64, causal,
+// 357 and 346.
 struct Fit {
     float scale = 1.0f, limit = 0.0f;
     template <int SUMS>
@@ -638,8 +639,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
     GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
     const T *__restrict__ out, const T *__restrict__ out_rest, const float *__restrict__ log_sum,
     const T *__restrict__ go, int64_t go_row, int64_t go_head, T *__restrict__ dq, float *__restrict__ row_log,
-    float *__restrict__ row_delta, float *__restrict__ row_power, float *__restrict__ partial,
-    int splits) {
+    float *__restrict__ row_delta, float *__restrict__ partial, int splits) {
     using KTile = Tile<T, DIM, kBackRows, kWaves>;
     __shared__ __attribute__((aligned(1024))) char lds[4 * KTile::kBytes];
     lds_char *const tiles = (lds_char *)lds;
@@ -691,17 +691,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
                 delta = fmaf(to_float(gr.x[s][i]), to_float(o.x[s][i]), delta);
     }
     delta = half_sum(delta);
-    if constexpr (Range<T>::kScaled) {
-        float most = 0.0f;
-#pragma unroll
-        for (int s = 0; s < DIM / 16; ++s)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(to_float(gr.x[s][i])));
-        most = half_max(most);
-        if (real && half == 0 && split == 0)  // (a row of zeros has no say in a tile's)
-            row_power[(int64_t)head * a.rows_q + p.q0 + query] =
-                most > 0.0f ? power_below(most) : 0.0f;
-    }
     // a row that saw nothing has no weights: exp2(x - infinity) = 0
     const float given = real ? log_sum[at] : -INFINITY;
     const float log2_sum = given == -INFINITY ? INFINITY : given * kLog2e;
@@ -805,15 +794,13 @@ template <typename T, int DIM>
 __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void attention_dkv_kernel(
     GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
     const T *__restrict__ go, int64_t go_row, int64_t go_head, const float *__restrict__ row_log,
-    const float *__restrict__ row_delta, const float *__restrict__ row_power, T *__restrict__ dk,
-    T *__restrict__ dv, float *__restrict__ partial, int splits) {
+    const float *__restrict__ row_delta, T *__restrict__ dk, T *__restrict__ dv, float *__restrict__ partial, int splits) {
     using Shape = KeysShape<DIM>;
     constexpr int kOwn = Shape::kOwn;
     using QTile = Tile<T, DIM, kBackRows, Shape::kWaves>;
     using VTile = Tile<T, DIM, kOwn, Shape::kWaves>;
     constexpr int kFloats = kBackRows * 4;                         // bytes of one float a row
-    constexpr int kStage = 2 * QTile::kBytes + 1024;  // Q, dout, log-sums, deltas, powers
-    static_assert(3 * kFloats <= 1024, "a tile's rows");
+    constexpr int kStage = 2 * QTile::kBytes + 2 * kFloats;  // Q, dout, log-sums, deltas
     __shared__ __attribute__((aligned(1024))) char lds[2 * kStage + (Shape::kValuesInLds ? VTile::kBytes : 0)];
     lds_char *const tiles = (lds_char *)lds, *const values = tiles + 2 * kStage;
 
@@ -854,7 +841,7 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
     const auto copy_g = QTile::copy_of(wave, go_row, a.dim);
     // (chosen here: inside, the compiler would index what the function captures by it, and
     // keep all of that in memory)
-    const float *row_floats = wave == 0 ? row_log : wave == 1 ? row_delta : row_power;
+    const float *row_floats = wave == 0 ? row_log : row_delta;
     const auto fetch = [&](int i) {
         lds_char *to = tiles + (i & 1) * kStage;
         const int t = end_tile - 1 - i / group, head = kh * group + i % group;
@@ -864,14 +851,14 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
         QTile::start(copy_g, wave, go + row * go_row + head * go_head, go_row, present, a.dim,
                      to + QTile::kBytes);
         const int64_t f = head * a.rows_q + row;
-        if (wave < (Range<T>::kScaled ? 3 : 2))
+        if (wave < 2)
             QTile::start_floats(row_floats + f, present, to + 2 * QTile::kBytes + wave * kFloats);
     };
 
     f32x16 gk[DIM / 32], gv[DIM / 32];
 #pragma unroll
     for (int d = 0; d < DIM / 32; ++d) gk[d] = gv[d] = f32x16{};
-    float power = 0.0f;  // the largest row's so far; gk is in units of it
+    Fit fit;             // of the key's score gradients, their weights' 2^10 included
     bool bad = false;    // the key is seen by a row with an infinity or NaN
 
     const auto step = [&](int i, auto masks) {
@@ -880,21 +867,6 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
         const lds_char *qt = tiles + (i & 1) * kStage, *gt = qt + QTile::kBytes;
         const lds_char *logs = gt + QTile::kBytes, *deltas = logs + kFloats;
         const int query0 = (end_tile - 1 - i / group) * kBackRows;
-        float range = 1.0f;  // of a score gradient, its weight's 2^10 included
-        if constexpr (Range<T>::kScaled) {
-            const float now = __builtin_bit_cast(
-                float, uniform(__builtin_bit_cast(
-                           int, wave_max(*(const __attribute__((address_space(3))) float *)(
-                                    deltas + kFloats + lane * 4)))));
-            if (now > power) {
-                if (power > 0.0f) {
-#pragma unroll
-                    for (int d = 0; d < DIM / 32; ++d) gk[d] *= power / now;
-                }
-                power = now;
-            }
-            range = power > 0.0f ? Range<T>::kGradient / 1024.0f / power : 0.0f;
-        }
         if constexpr (kMasks) {
             // rows with infinities or NaN become zeros, for they must not meet the weight 0 of a
             // key that their query does not see; the gradients of keys that it sees are NaN
@@ -939,7 +911,7 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
                 for (int j = 0; j < 4; ++j) {
                     const int r = 4 * g + j;
                     w[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -l[j]));
-                    ds[r] = (Range<T>::kScaled ? w[r] * range : w[r]) * dp[r];
+                    ds[r] = (Range<T>::kScaled ? w[r] * fit.scale : w[r]) * dp[r];
                     if (kMasks) {
                         const int query = query0 + 32 * n + result_row(r, half);
                         if (query < own_first) w[r] = 0.0f;
@@ -948,8 +920,9 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
                 }
             }
             const typename Vec<T>::x8 pw[2] = {pack8<T>(w), pack8<T>(w + 8)};
-            const typename Vec<T>::x8 pd[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
             add_product<T, DIM, QTile>(gv, gt, 32 * n, pw);
+            if constexpr (Range<T>::kScaled) fit.follow<DIM / 32>(ds, gk);
+            const typename Vec<T>::x8 pd[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
             if constexpr (kMasks) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) ds[r] -= to_float((T)pd[r / 8][r % 8]);
@@ -1002,8 +975,7 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
             }
     }
     const int64_t at = ((int64_t)(p.k0 + key) * a.heads_k + kh) * a.dim;
-    const float back_k = Range<T>::kScaled && power > 0.0f ? power / Range<T>::kGradient : 1.0f;
-    const float back_v = Range<T>::kScaled ? 1.0f / 1024.0f : 1.0f;
+    const float back_v = Range<T>::kScaled ? 1.0f / 1024.0f : 1.0f, back_k = back_v / fit.scale;
     if (splits > 1) {
         const int64_t size = a.rows_k * a.heads_k * a.dim;
         float *to = partial + split * size + at;
@@ -1133,9 +1105,9 @@ static size_t backward_partials(const GsAttention &a, const BackwardPlan &b) {
     return (q > k ? q : k) * sizeof(float);
 }
 
-// Bytes of the rows' log-sums, deltas and powers, a multiple of 16.
+// Bytes of the rows' log-sums and deltas, a multiple of 16.
 static size_t backward_rows(const GsAttention &a) {
-    return ((size_t)a.rows_q * a.heads_q * 3 * sizeof(float) + 15) / 16 * 16;
+    return ((size_t)a.rows_q * a.heads_q * 2 * sizeof(float) + 15) / 16 * 16;
 }
 
 static size_t partial_bytes(const GsAttention &a, int splits) {
@@ -1250,7 +1222,6 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
     const int64_t blocks_k = b.tiles_k * a->heads_k * b.splits_k;
     if (blocks_q > 0x7fffffffLL || blocks_k > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
     float *row_log = (float *)workspace, *row_delta = row_log + a->rows_q * a->heads_q;
-    float *row_power = row_delta + a->rows_q * a->heads_q;
     float *partial = (float *)((char *)workspace + backward_rows(*a));
     const auto launch = [&](auto t, auto d) {
         using T = decltype(t);
@@ -1266,7 +1237,7 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
                                block, 0, stream, *a, (const T *)q, (const T *)k, (const T *)v,
                                (const T *)out, (const T *)out_rest, log_sum, (const T *)grad_out,
                                grad_out_row, grad_out_head, (T *)grad_q, row_log, row_delta,
-                               row_power, partial, b.splits_q);
+                               partial, b.splits_q);
             if (b.splits_q > 1)
                 join(a->rows_q * a->heads_q * a->dim, b.splits_q, 1, a->scale, (T *)grad_q,
                      (T *)nullptr);
@@ -1277,7 +1248,7 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
             hipLaunchKernelGGL((attention_dkv_kernel<T, kDim>), dim3((unsigned)blocks_k),
                                dim3(64 * KeysShape<kDim>::kWaves), 0, stream, *a, (const T *)q,
                                (const T *)k, (const T *)v, (const T *)grad_out, grad_out_row, grad_out_head, row_log, row_delta,
-                               row_power, (T *)grad_k, (T *)grad_v, partial, b.splits_k);
+                               (T *)grad_k, (T *)grad_v, partial, b.splits_k);
             if (b.splits_k > 1)
                 join(a->rows_k * a->heads_k * a->dim, b.splits_k, 2, a->scale, (T *)grad_k,
                      (T *)grad_v);

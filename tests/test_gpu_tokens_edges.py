@@ -93,3 +93,14 @@ def ranged(gpu, kind, dim):
 def test_attention_query_gradients_stay_in_float16(gpu, kind, dim, causal):
     q, k, v, go, lengths = ranged(gpu, kind, dim)
     check_gradients(q, k, v, go, offsets_of(lengths, gpu), causal=causal, names="q")
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [64, 72, 128])
+@pytest.mark.parametrize("kind", ["two equal weights", "values equal along a row", "large values",
+                                  "largest values", "small values", "first queries large"])
+def test_attention_key_gradients_stay_in_float16(gpu, kind, dim, causal):
+    """Under a causal mask a key's gradient keeps its bits beside rows, however large, that do not
+    see it."""
+    q, k, v, go, lengths = ranged(gpu, kind, dim)
+    check_gradients(q, k, v, go, offsets_of(lengths, gpu), causal=causal, names="kv")
