@@ -76,8 +76,10 @@ __device__ __forceinline__ void store_columns(const f32x16 *acc, float factor, T
 
 // Infinities and NaN in rows of a tile that some columns do not see: their weights there are
 // 0, but 0 times them is no 0.  Tiles at a causal edge are looked through for such rows; where
-// there are any, the product takes zeros for these values, and a second one finds the sums
-// that such a value belongs to, which become NaN.
+// there are any, the product takes zeros for these values, and a second one counts which of
+// them each sum has: 1 an infinity, 64 a negative one, 2048 a NaN, and 2048 times that where the
+// weight is 0, among 16 rows.  The sum becomes what the product itself gives in other tiles: an
+// infinity, or NaN for a NaN, a weight of 0 and infinities of both signs.
 template <typename T>
 __device__ __forceinline__ bool not_finite(uint32_t bits) {
     constexpr uint32_t kInfinity = std::is_same<T, bf16>::value ? 0x7f80 : 0x7c00;
@@ -92,6 +94,9 @@ __device__ __forceinline__ uint64_t rows_not_finite(const lds_char *tile, int ba
     const int row = __lane_id() % ROWS;
     const lds_char *p = tile + (base + row) * DIM * 2;
     int chunk = row % kChunks;  // each lane begins elsewhere: other banks
+    // (or the compiler would keep all the chunks' addresses from tile to tile, and registers that
+    // the products need would lie in memory)
+    asm volatile("" : "+v"(chunk));
     u16x8 most = {};
     for (int i = 0; i < kChunks; ++i) {
         const u16x8 x = *(const __attribute__((address_space(3))) u16x8 *)(p + chunk * 16);
@@ -121,12 +126,18 @@ __device__ __forceinline__ void add_product(f32x16 *acc, const lds_char *tile, i
 }
 
 // The same where the rows hold infinities or NaN; sees(i): whether the lane's column sees row
-// base + i.
-template <typename T, int DIM, typename XTile, typename Sees>
+// base + i.  SCORES: the rows made the weights' scores, so that a value that is not finite has
+// made its weight 0 or NaN, and the sum NaN.
+template <typename T, int DIM, typename XTile, bool SCORES, typename Sees>
 __device__ __forceinline__ void add_product_seen(f32x16 *acc, const lds_char *tile, int base,
                                                  const typename Vec<T>::x8 *p, Sees sees,
                                                  const typename Vec<T>::x8 *rest = nullptr) {
     using x8 = typename Vec<T>::x8;
+    using u16x8 = __attribute__((ext_vector_type(8))) uint16_t;
+    constexpr bool kBf16 = std::is_same<T, bf16>::value;
+    constexpr uint16_t kExponent = kBf16 ? 0x80 : 0x400;  // the last bit of an exponent
+    constexpr uint16_t kOne = (kBf16 ? 127 : 15) * kExponent;  // 1.0
+    const u16x8 one = 1, before = (kBf16 ? 255 : 31) * kExponent - 1;  // the largest finite number
     const int half = __lane_id() >> 5;
 #pragma unroll 1
     for (int g = 0; g < 2; ++g) {
@@ -135,21 +146,41 @@ __device__ __forceinline__ void add_product_seen(f32x16 *acc, const lds_char *ti
         if (rest) more = g ? rest[1] : rest[0];
         x8 seen;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) seen[j] = (T)(sees(16 * g + result_row(j, half)) ? 1.0f : 0.0f);
+        for (int j = 0; j < 8; ++j)
+            seen[j] = (T)(!sees(16 * g + result_row(j, half))  ? 0.0f
+                          : (T)weights[j] == (T)0.0f ? 2048.0f
+                                                     : 1.0f);
 #pragma unroll
         for (int d = 0; d < DIM / 32; ++d) {
-            x8 x = XTile::down(tile, base + 16 * g, d), bad;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const bool b = not_finite<T>(__builtin_bit_cast(uint16_t, (T)x[j]));
-                bad[j] = (T)(b ? 1.0f : 0.0f);
-                x[j] = b ? (T)0.0f : x[j];
-            }
+            const u16x8 bits = __builtin_bit_cast(u16x8, (x8)XTile::down(tile, base + 16 * g, d));
+            // 0 finite, 1 an infinity, more NaN
+            const u16x8 what = __builtin_elementwise_max(bits & (uint16_t)0x7fff, before) - before;
+            const u16x8 bad = __builtin_elementwise_min(what, one);
+            const x8 x = __builtin_bit_cast(x8, bits & (bad - one));
             acc[d] = mfma(x, weights, acc[d]);
             if (rest) acc[d] = mfma(x, more, acc[d]);
-            const f32x16 count = mfma(bad, seen, f32x16{});
+            const u32x4 any = __builtin_bit_cast(u32x4, bad);
+            if (!__ballot((any[0] | any[1] | any[2] | any[3]) != 0)) continue;
+            if constexpr (SCORES) {
+                const f32x16 count = mfma(__builtin_bit_cast(x8, bad * kOne), seen, f32x16{});
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[d][r] = count[r] > 0.0f ? NAN : acc[d][r];
+                for (int r = 0; r < 16; ++r) acc[d][r] = count[r] > 0.0f ? NAN : acc[d][r];
+                continue;
+            }
+            const u16x8 nan = __builtin_elementwise_min(what - bad, one);
+            const x8 kind = __builtin_bit_cast(
+                x8, bad * kOne + (bits >> 15 & (bad - nan)) * (uint16_t)(6 * kExponent) +
+                        nan * (uint16_t)(11 * kExponent));
+            const f32x16 count = mfma(kind, seen, f32x16{});
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float c = count[r];
+                // what is left of c without its multiple of 64: the infinities that are positive
+                const float up = c - 64.0f * floorf(c * (1.0f / 64.0f));
+                acc[d][r] += up > 0.0f ? INFINITY : 0.0f;
+                acc[d][r] -= c - up > 0.0f ? INFINITY : 0.0f;
+                acc[d][r] = c < 2048.0f ? acc[d][r] : NAN;
+            }
         }
     }
 }
@@ -218,8 +249,9 @@ __device__ __forceinline__ Place place_of(int heads_k, int splits) {
 //
 // Weights are rounded to the inputs' type for their product with V: 2^-9 (2^-12 in float16)
 // of a weight, unbiased.  Infinities and NaN in rows that nothing sees change nothing; a
-// query that sees one in V gets NaN where its column holds it, a tile with both kinds of
-// query is told apart key by key; what a seen K holds goes into its score.
+// query that sees one in V gets it where its column holds it (NaN where the weight was rounded
+// to 0 or infinities of both signs meet), a tile with both kinds of query is told apart key by
+// key; what a seen K holds goes into its score.
 template <typename T, int DIM, bool BY_KEYS>
 struct Forward {
     // by keys: two waves, so that a CU's LDS holds two workgroups, and one's first tile and
@@ -365,8 +397,9 @@ __device__ __forceinline__ void forward_rows(
         for (int n = 0; n < F::kSub; ++n) {
             const uint32_t part = (uint32_t)(found >> (32 * n));
             if (kMasks && part)
-                add_product_seen<T, DIM, KTile>(acc, vt, base + 32 * n, weights + 2 * n,
-                                                [&](int i) { return key0 + 32 * n + i <= last; });
+                add_product_seen<T, DIM, KTile, false>(
+                    acc, vt, base + 32 * n, weights + 2 * n,
+                    [&](int i) { return key0 + 32 * n + i <= last; });
             else
                 add_product<T, DIM, KTile>(acc, vt, base + 32 * n, weights + 2 * n);
         }
@@ -758,7 +791,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
             }
             const uint32_t part = (uint32_t)(found >> (32 * n));
             if (kMasks && part)
-                add_product_seen<T, DIM, KTile>(
+                add_product_seen<T, DIM, KTile, true>(
                     acc, kt, 32 * n, x, [&](int i) { return key0 + 32 * n + i <= last; }, rest);
             else
                 add_product<T, DIM, KTile>(acc, kt, 32 * n, x, rest);

@@ -104,3 +104,38 @@ def test_attention_key_gradients_stay_in_float16(gpu, kind, dim, causal):
     see it."""
     q, k, v, go, lengths = ranged(gpu, kind, dim)
     check_gradients(q, k, v, go, offsets_of(lengths, gpu), causal=causal, names="kv")
+
+
+# ------------------------------------------------------------- infinities and NaN
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dim", [64, 72, 128])
+@pytest.mark.parametrize("lq,lk", [(300, 300), (40, 40), (3, 5000), (300, 3000)])
+def test_attention_gives_infinities_that_a_query_sees(gpu, lq, lk, dim, dtype):
+    """In tiles that all rows see and at a causal edge alike, in rows, few rows and splits: an
+    infinity in a value comes out as one, infinities of both signs and NaN as NaN, in the columns
+    that hold them and in the rows that see them."""
+    q, k, v, _ = inputs(gpu, lq, lk, 4, 2, dim, dtype)
+    q, k = q / 5, k / 5  # no weight is rounded to 0
+    oq, ok = offsets_of([lq], gpu), offsets_of([lk], gpu)
+    first, second = lk - lq // 2 - 1, lk - lq // 4 - 1
+    w = v.clone()
+    w[first, :, 3], w[second, :, 3] = math.inf, -math.inf
+    w[first, :, 20] = -math.inf
+    w[second, :, 41] = math.nan
+    w[second, 1, 50] = math.inf  # one of two key heads
+    for causal in (False, True):
+        ref = ot.attention(q, k, v, oq, ok, causal=causal)
+        got = cr.packed_attention(q, k, w, oq, ok, causal=causal)
+        at = torch.arange(lq, device=gpu) + (lk - lq if causal else lk)
+        one, two = (at >= first)[:, None], (at >= second)[:, None]
+        want = ref["out"].clone()
+        want[..., 3] = torch.where(two, math.nan, torch.where(one, math.inf, want[..., 3]))
+        want[..., 20] = torch.where(one, -math.inf, want[..., 20])
+        want[..., 41] = torch.where(two, math.nan, want[..., 41])
+        want[:, 2:, 50] = torch.where(two, math.inf, want[:, 2:, 50])
+        got = got.double()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(torch.isinf(got) * got.sign(), torch.isinf(want) * want.sign())
+        there = torch.isfinite(want)
+        off = (got - want)[there].abs() - 1.1 * U[dtype] * ref["out_slack"][there]
+        assert float(off.max()) <= 2.0 ** -24
