@@ -5,6 +5,7 @@
 // with dk and dv summed over the query heads of a group.  Scores, softmax
 // statistics and sums are in float.
 
+#include <cfloat>
 #include <initializer_list>
 #include <type_traits>
 
@@ -460,6 +461,9 @@ __device__ __forceinline__ void forward_rows(
         top = all;
         sum = rounded = total;
     }
+    // a row whose scores are all minus infinity has seen keys: its weights are 0 / 0.  (Not so
+    // low as a part that saw none, so that it counts where all of a row's parts are such.)
+    if (top == -INFINITY && last >= first_tile * F::kKeys) top = -FLT_MAX;
 
     if (partial.splits > 1) {
         const int64_t slot = (int64_t)split * a.rows_q * a.heads_q + at;
@@ -724,9 +728,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
                 delta = fmaf(to_float(gr.x[s][i]), to_float(o.x[s][i]), delta);
     }
     delta = half_sum(delta);
-    // a row that saw nothing has no weights: exp2(x - infinity) = 0
+    // a row that saw nothing has no weights: exp2(x - infinity) = 0; one that saw keys, with scores
+    // of minus infinity, has none that are numbers
     const float given = real ? log_sum[at] : -INFINITY;
-    const float log2_sum = given == -INFINITY ? INFINITY : given * kLog2e;
+    const float log2_sum =
+        given == -INFINITY ? (real && last >= 0 ? NAN : INFINITY) : given * kLog2e;
     // a row that sees one key has no score gradient: its dout v^T and delta are the same sum in
     // two orders, whose difference would be all there is of it
     const float row_exponent = last == 0 ? INFINITY : log2_sum;

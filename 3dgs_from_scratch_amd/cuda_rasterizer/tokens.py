@@ -363,7 +363,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets_
 
     What a query does not see, whatever it is, changes nothing.  An infinity in a value
     that it sees gives that infinity, or NaN where its probability was rounded to 0 or
-    both signs meet.
+    both signs meet; keys that all score minus infinity, though it sees them, give NaN.
     """
     _check("packed_attention", "q", q, 3, (torch.float16, torch.bfloat16))
     dev = q.device

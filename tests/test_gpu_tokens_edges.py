@@ -139,3 +139,32 @@ def test_attention_gives_infinities_that_a_query_sees(gpu, lq, lk, dim, dtype):
         there = torch.isfinite(want)
         off = (got - want)[there].abs() - 1.1 * U[dtype] * ref["out_slack"][there]
         assert float(off.max()) <= 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lq,lk", [([30, 200], [30, 200]), ([2, 3], [700, 5000]), ([40, 300], [600, 3000]),
+                                   ([30, 200], [30, 150])])
+def test_attention_of_keys_that_all_score_minus_infinity(gpu, lq, lk, causal, dtype):
+    """They are seen: weights of 0 / 0 give NaN, with its gradients, where a query that sees no key
+    gives 0.  The other sequence does not change."""
+    q, k, v, go = inputs(gpu, sum(lq), sum(lk), 4, 2, 64, dtype)
+    q[lq[0]:, :, 0] = 1.0
+    k[lk[0]:, :, 0] = -math.inf
+    oq, ok = offsets_of(lq, gpu), offsets_of(lk, gpu)
+    sees = torch.arange(lq[1], device=gpu) + lk[1] - lq[1] >= 0 if causal else torch.ones(
+        lq[1], device=gpu, dtype=torch.bool)
+    with torch.no_grad():
+        alone = cr.packed_attention(q, k, v, oq, ok, causal=causal)
+    out, log_sum = cr.packed_attention(q, k, v, oq, ok, causal=causal, return_log_sum=True)
+    first = gradients(q[:lq[0]], k[:lk[0]], v[:lk[0]], go[:lq[0]], oq[:2], ok[:2], causal=causal)
+    whole = gradients(q, k, v, go, oq, ok, causal=causal)
+    for got in (alone, out, whole[0], whole[1][0]):
+        second = got[lq[0]:]
+        assert bool(torch.isnan(second[sees]).all()) and bool((second[~sees] == 0).all())
+    assert bool((log_sum[lq[0]:] == -math.inf).all())
+    for grad, one in zip(whole[1], first[1]):
+        assert bool(torch.isfinite(grad[:one.shape[0]]).all())
+        assert float((grad[:one.shape[0]] - one).float().norm()) <= 4 * U[dtype] * float(one.float().norm())
+    for grad in whole[1][1:]:
+        assert bool(torch.isnan(grad[lk[0]:]).all())
