@@ -81,6 +81,8 @@ __device__ __forceinline__ void store_columns(const f32x16 *acc, float factor, T
 // them each sum has: 1 an infinity, 64 a negative one, 2048 a NaN, and 2048 times that where the
 // weight is 0, among 16 rows.  The sum becomes what the product itself gives in other tiles: an
 // infinity, or NaN for a NaN, a weight of 0 and infinities of both signs.
+using u16x8 = __attribute__((ext_vector_type(8))) uint16_t;
+
 template <typename T>
 __device__ __forceinline__ bool not_finite(uint32_t bits) {
     constexpr uint32_t kInfinity = std::is_same<T, bf16>::value ? 0x7f80 : 0x7c00;
@@ -90,7 +92,6 @@ __device__ __forceinline__ bool not_finite(uint32_t bits) {
 // The rows from `base` on, ROWS of them, that hold such a value: a bit each, in every lane.
 template <typename T, int DIM, int ROWS>
 __device__ __forceinline__ uint64_t rows_not_finite(const lds_char *tile, int base) {
-    using u16x8 = __attribute__((ext_vector_type(8))) uint16_t;
     constexpr int kChunks = DIM / 8;
     const int row = __lane_id() % ROWS;
     const lds_char *p = tile + (base + row) * DIM * 2;
@@ -126,7 +127,49 @@ __device__ __forceinline__ void add_product(f32x16 *acc, const lds_char *tile, i
         }
 }
 
-// The same where the rows hold infinities or NaN; sees(i): whether the lane's column sees row
+// Eight elements, told apart; what: 0 finite, 1 an infinity, more NaN.
+template <typename T>
+struct Told {
+    using x8 = typename Vec<T>::x8;
+    static constexpr bool kBf16 = std::is_same<T, bf16>::value;
+    static constexpr uint16_t kExponent = kBf16 ? 0x80 : 0x400;  // the last bit of an exponent
+    static constexpr uint16_t kOne = (kBf16 ? 127 : 15) * kExponent;          // 1.0
+    static constexpr uint16_t kLast = (kBf16 ? 255 : 31) * kExponent - 1;  // the largest number
+    u16x8 bits, what, bad;
+    __device__ __forceinline__ Told(x8 x) {
+        bits = __builtin_bit_cast(u16x8, x);
+        const u16x8 last = kLast;
+        what = __builtin_elementwise_max(bits & (uint16_t)0x7fff, last) - last;
+        bad = __builtin_elementwise_min(what, (u16x8)(uint16_t)1);
+    }
+    __device__ __forceinline__ x8 finite() const {  // zeros for the others
+        return __builtin_bit_cast(x8, bits & (bad - (uint16_t)1));
+    }
+    __device__ __forceinline__ bool any() const {  // of all lanes'
+        const u32x4 b = __builtin_bit_cast(u32x4, bad);
+        return __ballot((b[0] | b[1] | b[2] | b[3]) != 0) != 0;
+    }
+    __device__ __forceinline__ x8 ones() const { return __builtin_bit_cast(x8, bad * kOne); }
+    __device__ __forceinline__ x8 kinds() const {  // 0, 1, 64 or 2048 each
+        const u16x8 nan = __builtin_elementwise_min(what - bad, (u16x8)(uint16_t)1);
+        return __builtin_bit_cast(x8, bad * kOne + (bits >> 15 & (bad - nan)) * (uint16_t)(6 * kExponent) +
+                                          nan * (uint16_t)(11 * kExponent));
+    }
+};
+
+__device__ __forceinline__ void add_infinities(f32x16 &acc, const f32x16 &count) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const float c = count[r];
+        // what is left of c without its multiple of 64: the infinities that are positive
+        const float up = c - 64.0f * floorf(c * (1.0f / 64.0f));
+        acc[r] += up > 0.0f ? INFINITY : 0.0f;
+        acc[r] -= c - up > 0.0f ? INFINITY : 0.0f;
+        acc[r] = c < 2048.0f ? acc[r] : NAN;
+    }
+}
+
+// add_product where the rows hold infinities or NaN; sees(i): whether the lane's column sees row
 // base + i.  SCORES: the rows made the weights' scores, so that a value that is not finite has
 // made its weight 0 or NaN, and the sum NaN.
 template <typename T, int DIM, typename XTile, bool SCORES, typename Sees>
@@ -134,11 +177,6 @@ __device__ __forceinline__ void add_product_seen(f32x16 *acc, const lds_char *ti
                                                  const typename Vec<T>::x8 *p, Sees sees,
                                                  const typename Vec<T>::x8 *rest = nullptr) {
     using x8 = typename Vec<T>::x8;
-    using u16x8 = __attribute__((ext_vector_type(8))) uint16_t;
-    constexpr bool kBf16 = std::is_same<T, bf16>::value;
-    constexpr uint16_t kExponent = kBf16 ? 0x80 : 0x400;  // the last bit of an exponent
-    constexpr uint16_t kOne = (kBf16 ? 127 : 15) * kExponent;  // 1.0
-    const u16x8 one = 1, before = (kBf16 ? 255 : 31) * kExponent - 1;  // the largest finite number
     const int half = __lane_id() >> 5;
 #pragma unroll 1
     for (int g = 0; g < 2; ++g) {
@@ -153,35 +191,36 @@ __device__ __forceinline__ void add_product_seen(f32x16 *acc, const lds_char *ti
                                                      : 1.0f);
 #pragma unroll
         for (int d = 0; d < DIM / 32; ++d) {
-            const u16x8 bits = __builtin_bit_cast(u16x8, (x8)XTile::down(tile, base + 16 * g, d));
-            // 0 finite, 1 an infinity, more NaN
-            const u16x8 what = __builtin_elementwise_max(bits & (uint16_t)0x7fff, before) - before;
-            const u16x8 bad = __builtin_elementwise_min(what, one);
-            const x8 x = __builtin_bit_cast(x8, bits & (bad - one));
-            acc[d] = mfma(x, weights, acc[d]);
-            if (rest) acc[d] = mfma(x, more, acc[d]);
-            const u32x4 any = __builtin_bit_cast(u32x4, bad);
-            if (!__ballot((any[0] | any[1] | any[2] | any[3]) != 0)) continue;
+            const Told<T> x(XTile::down(tile, base + 16 * g, d));
+            acc[d] = mfma(x.finite(), weights, acc[d]);
+            if (rest) acc[d] = mfma(x.finite(), more, acc[d]);
+            if (!x.any()) continue;
             if constexpr (SCORES) {
-                const f32x16 count = mfma(__builtin_bit_cast(x8, bad * kOne), seen, f32x16{});
+                const f32x16 count = mfma(x.ones(), seen, f32x16{});
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[d][r] = count[r] > 0.0f ? NAN : acc[d][r];
-                continue;
+            } else {
+                add_infinities(acc[d], mfma(x.kinds(), seen, f32x16{}));
             }
-            const u16x8 nan = __builtin_elementwise_min(what - bad, one);
-            const x8 kind = __builtin_bit_cast(
-                x8, bad * kOne + (bits >> 15 & (bad - nan)) * (uint16_t)(6 * kExponent) +
-                        nan * (uint16_t)(11 * kExponent));
-            const f32x16 count = mfma(kind, seen, f32x16{});
+        }
+    }
+}
+
+// What the infinities and NaN of ROWS rows of a tile add to a product, by itself; no weight is
+// taken for 0.
+template <typename T, int DIM, typename XTile, int ROWS, typename Sees>
+__device__ __forceinline__ void add_infinities_seen(f32x16 *acc, const lds_char *tile, Sees sees) {
+    const int half = __lane_id() >> 5;
+#pragma unroll 1
+    for (int base = 0; base < ROWS; base += 16) {
+        typename Vec<T>::x8 seen;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float c = count[r];
-                // what is left of c without its multiple of 64: the infinities that are positive
-                const float up = c - 64.0f * floorf(c * (1.0f / 64.0f));
-                acc[d][r] += up > 0.0f ? INFINITY : 0.0f;
-                acc[d][r] -= c - up > 0.0f ? INFINITY : 0.0f;
-                acc[d][r] = c < 2048.0f ? acc[d][r] : NAN;
-            }
+        for (int j = 0; j < 8; ++j)
+            seen[j] = (T)(sees(base + result_row(j, half)) ? 1.0f : 0.0f);
+#pragma unroll
+        for (int d = 0; d < DIM / 32; ++d) {
+            const Told<T> x(XTile::down(tile, base, d));
+            if (x.any()) add_infinities(acc[d], mfma(x.kinds(), seen, f32x16{}));
         }
     }
 }
@@ -898,7 +937,6 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
 #pragma unroll
     for (int d = 0; d < DIM / 32; ++d) gk[d] = gv[d] = f32x16{};
     Fit fit;             // of the key's score gradients, their weights' 2^10 included
-    bool bad = false;    // the key is seen by a row with an infinity or NaN
 
     const auto step = [&](int i, auto masks) {
         constexpr bool kMasks = decltype(masks)::value;
@@ -907,19 +945,20 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
         const lds_char *logs = gt + QTile::kBytes, *deltas = logs + kFloats;
         const int query0 = (end_tile - 1 - i / group) * kBackRows;
         if constexpr (kMasks) {
-            // rows with infinities or NaN become zeros, for they must not meet the weight 0 of a
-            // key that their query does not see; the gradients of keys that it sees are NaN
-            const uint64_t found = rows_not_finite<T, DIM, kBackRows>(qt, 0) |
-                                   rows_not_finite<T, DIM, kBackRows>(gt, 0);
-            if (found) {
-                const int from = max(own_first - query0, 0);
-                bad = bad || (from < 64 && found >> from != 0);
+            // infinities and NaN become zeros, for they must not meet the weight 0 of a key that
+            // their query does not see.  Those of an output gradient reach the value gradients, in
+            // their columns, of the keys that it sees; its query's delta, or the log-sum of a
+            // query that holds such a value, is no number either, and makes the rest of it.
+            const uint64_t found_g = rows_not_finite<T, DIM, kBackRows>(gt, 0);
+            if (found_g | rows_not_finite<T, DIM, kBackRows>(qt, 0)) {
+                if (found_g)
+                    add_infinities_seen<T, DIM, QTile, kBackRows>(
+                        gv, gt, [&](int j) { return query0 + j >= own_first; });
                 __syncthreads();  // all waves have looked
                 for (int at = threadIdx.x * 16; at < 2 * QTile::kBytes; at += 64 * Shape::kWaves * 16) {
-                    const int row = at % QTile::kBytes / (DIM * 2);
-                    if (found >> row & 1)
-                        *(__attribute__((address_space(3))) u32x4 *)(tiles + (i & 1) * kStage + at) =
-                            u32x4{0, 0, 0, 0};
+                    auto *x = (__attribute__((address_space(3))) typename Vec<T>::x8 *)(
+                        tiles + (i & 1) * kStage + at);
+                    *x = Told<T>(*x).finite();
                 }
                 __syncthreads();
             }
@@ -1003,14 +1042,13 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
         for (int d = 0; d < DIM / 32; ++d) gk[d] *= 0.0f;
     }
     // keys past the length that counts have no gradient
-    if (__ballot(!counts || bad)) {
-        const float instead = counts ? NAN : 0.0f;
+    if (__ballot(!counts)) {
 #pragma unroll
         for (int d = 0; d < DIM / 32; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                gk[d][r] = counts && !bad ? gk[d][r] : instead;
-                gv[d][r] = counts && !bad ? gv[d][r] : instead;
+                gk[d][r] = counts ? gk[d][r] : 0.0f;
+                gv[d][r] = counts ? gv[d][r] : 0.0f;
             }
     }
     const int64_t at = ((int64_t)(p.k0 + key) * a.heads_k + kh) * a.dim;

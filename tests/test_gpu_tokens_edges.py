@@ -168,3 +168,38 @@ def test_attention_of_keys_that_all_score_minus_infinity(gpu, lq, lk, causal, dt
         assert float((grad[:one.shape[0]] - one).float().norm()) <= 4 * U[dtype] * float(one.float().norm())
     for grad in whole[1][1:]:
         assert bool(torch.isnan(grad[lk[0]:]).all())
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dim", [64, 72, 128])
+@pytest.mark.parametrize("row,value", [(40, math.inf), (100, -math.inf), (299, math.inf), (60, math.nan)])
+def test_attention_gradients_of_one_infinite_output_gradient(gpu, row, value, dim, dtype):
+    """It reaches the value gradients of the keys that its query sees, in its own column only, and
+    their key gradients; in tiles that see the query whole and at a causal edge."""
+    q, k, v, go = inputs(gpu, 300, 300, 4, 2, dim, dtype)
+    q, k = q / 5, k / 5
+    at = offsets_of([300], gpu)
+    bad, none = go.clone(), go.clone()
+    bad[row, 1, 7], none[row, 1, 7] = value, 0.0
+    for causal in (False, True):
+        ref = ot.attention_gradients(q, k, v, at, none, causal=causal)
+        _, (gq, gk, gv) = gradients(q, k, v, bad, at, causal=causal)
+        seen = torch.arange(300, device=gpu) <= (row if causal else 299)
+        want, bound = ref["gv"].clone(), ref["gv_bound"]
+        want[seen, 0, 7] = value
+        assert torch.equal(torch.isfinite(gv), torch.isfinite(want))
+        assert bool(torch.isnan(gv[seen, 0, 7]).all()) or bool((gv[seen, 0, 7] == value).all())
+        assert (value != value) == bool(torch.isnan(gv).any())
+        there = torch.isfinite(want)
+        assert float(((gv.double() - want)[there].abs() - bound[there]).max()) <= 0.0
+        # keys that the query does not see, and the other key head
+        assert not bool(torch.isfinite(gk[seen, 0]).any())
+        for got, name, rows in ((gk[~seen, 0], "gk", (~seen, 0)), (gk[:, 1], "gk", (slice(None), 1))):
+            if got.numel():
+                off = (got.double() - ref[name][rows]).abs() - ref[name + "_bound"][rows]
+                assert float(off.max()) <= 0.0
+        others = torch.ones(300, 4, device=gpu, dtype=torch.bool)
+        others[row, 1] = False
+        assert not bool(torch.isfinite(gq[row, 1]).any())
+        off = (gq.double() - ref["gq"]).abs() - ref["gq_bound"]
+        assert float(off[others].max()) <= 0.0
