@@ -693,8 +693,8 @@ struct Fit {
         float most = 0.0f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(ds[r]));
-        most = half_max(most);  // (an infinity or NaN leaves the scale: its sums are lost)
         if (__ballot(most > limit)) {
+            most = half_max(most);  // (an infinity or NaN leaves the scale: its sums are lost)
             const bool passes = most > limit && most < INFINITY;
             const float ratio = passes ? fminf(512.0f / power_below(most), 0x1p60f / scale) : 1.0f;
             limit = passes ? 32768.0f : limit;
