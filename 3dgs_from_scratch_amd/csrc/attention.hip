@@ -654,10 +654,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
 // Score gradients are rounded to the inputs' type for their products, which adds as much
 // again to the rounding of the result (1.41 times its error in all, and more with what delta
 // has from the output's rounded weights: 1.55 for rows of a few keys).  A second product of the
-// same tile with what was rounded off takes it back.  In tiles with a mask, and so for
-// sequences of up to 64 rows, where delta's part is largest, both launches have it (1.3 times
-// the error for rows of 1 to 7 keys in bfloat16; the training pass over scenes of 12566 and
-// 16320 tokens 8.53 -> 8.65 ms).  In float16, which is chosen for its bits, the queries'
+// same tile with what was rounded off takes it back.  In tiles with a mask, and where a sequence
+// has only one, of up to 64 keys (or queries, in the keys' launch), where delta's part is
+// largest, both launches have it (1.3 times the error for rows of 1 to 7 keys in bfloat16; the
+// training pass over scenes of 12566 and 16320 tokens 8.53 -> 8.65 ms).  In float16, which is chosen for its bits, the queries'
 // gradients have it in every tile (1.02 to 1.08 times the error); that costs the launch 28%,
 // 171 -> 217 us for 4 sequences of 2500, 12 heads of 72, and neither bfloat16 nor the keys'
 // launch, longer by itself, pays it.
@@ -844,8 +844,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
     };
     if (first_tile < end_tile) fetch(first_tile);
     int t = first_tile;
-    for (const int whole = min(end_tile, (all_see + 1) / kBackRows); t < whole; ++t)
-        step(t, std::false_type{});
+    // (one tile of keys goes the way of masked ones, which keeps what rounding takes off)
+    const int whole = p.lk <= kBackRows ? 0 : min(end_tile, (all_see + 1) / kBackRows);
+    for (; t < whole; ++t) step(t, std::false_type{});
     for (; t < end_tile; ++t) step(t, std::true_type{});
     if (splits > 1)
         store_partial<DIM>(acc, 1.0f / fit.scale,

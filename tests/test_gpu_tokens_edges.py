@@ -203,3 +203,20 @@ def test_attention_gradients_of_one_infinite_output_gradient(gpu, row, value, di
         assert not bool(torch.isfinite(gq[row, 1]).any())
         off = (gq.double() - ref["gq"]).abs() - ref["gq_bound"]
         assert float(off[others].max()) <= 0.0
+
+
+# ------------------------------------------------------ tiles that are just filled
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [64, 72, 128])
+@pytest.mark.parametrize("lq,lk", [(64, 64), (63, 64), (64, 60), (7, 64)])
+def test_attention_gradients_of_one_full_tile_keep_their_bits(gpu, lq, lk, dim, causal):
+    """Score gradients of up to 64 keys and queries are not rounded a second time, the full tile's
+    among them: that would make the error sqrt(2) times that of rounding the gradients once."""
+    n = 40
+    q, k, v, go = inputs(gpu, n * lq, n * lk, 2, 2, dim, torch.bfloat16)
+    oq, ok = offsets_of([lq] * n, gpu), offsets_of([lk] * n, gpu)
+    ref = ot.attention_gradients(q, k, v, oq, go, ok, causal=causal)
+    _, grads = gradients(q, k, v, go, oq, ok, causal=causal)
+    for grad, name in zip(grads[:2], ("gq", "gk")):
+        once = (ref[name].bfloat16().double() - ref[name]).norm()
+        assert float((grad.double() - ref[name]).norm() / once) < 1.3, name
