@@ -15,8 +15,8 @@ the matrix products, its blocks need
   not, or new queries over a cache of earlier keys and values.
 
 All run on the library's gfx950 kernels on the current HIP stream, without host
-synchronisation, and are differentiable once (packed_attention in q, k and v;
-axial_rotary in q and k; layer_norm in all three).  Inputs are float32, float16 or
+synchronisation, and are differentiable once, backwards (packed_attention in q, k and
+v; axial_rotary in q and k; layer_norm in all three); forward-mode tangents are refused.  Inputs are float32, float16 or
 bfloat16 (packed_attention: float16 or bfloat16); sums and statistics are held in
 float32 and each output is rounded once.  Nothing here has a counterpart in the
 reference.
@@ -28,6 +28,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -67,9 +68,16 @@ def _workspace(query, *args, device):
     return torch.empty(size.value, dtype=torch.uint8, device=device), size.value
 
 
-def _differentiable(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
-                                           for t in tensors)
+def _differentiable(what: str, *tensors) -> bool:
+    """Whether autograd has to record the call.  A tangent of forward-mode differentiation is
+    refused: the operators have no such rule, and their outputs would drop it."""
+    grad, found = torch.is_grad_enabled(), False
+    for t in tensors:
+        if isinstance(t, torch.Tensor):
+            found = found or (grad and t.requires_grad)
+            if unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode derivative")
+    return found
 
 
 # ------------------------------------------------------------------ layer norm
@@ -163,7 +171,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
                bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over x's last dimension, in x's
     type; weight and bias may have another (float32 weights for bfloat16 x)."""
-    if _differentiable(x, weight, bias):
+    if _differentiable("layer_norm", x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps)
     return layer_norm_forward(x, weight, bias, eps, with_stats=False)[0]
 
@@ -252,7 +260,7 @@ def axial_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
                            f"{frequencies.shape[0]}")
     positions = positions if positions.stride(1) == 1 else positions.contiguous()
     frequencies = frequencies.contiguous()
-    if _differentiable(q, k):
+    if _differentiable("axial_rotary", q, k):
         return _AxialRotary.apply(q, k, positions, frequencies, sections, bool(interleaved))
     out = _rotate([t for t in (q, k) if t is not None], positions, frequencies, sections,
                   bool(interleaved), False)
@@ -400,7 +408,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets_
     if not math.isfinite(scale):
         raise ValueError(f"packed_attention: scale must be finite, got {scale}")
     args = (q, k, v, offsets_q, offsets_k, lengths_k, bool(causal), scale)
-    if _differentiable(q, k, v):
+    if _differentiable("packed_attention", q, k, v):
         out, log_sum = _PackedAttention.apply(*args)
     else:
         out, _, log_sum = attention_forward(*args, with_log_sum=return_log_sum, with_rest=False)

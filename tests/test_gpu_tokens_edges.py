@@ -220,3 +220,30 @@ def test_attention_gradients_of_one_full_tile_keep_their_bits(gpu, lq, lk, dim, 
     for grad, name in zip(grads[:2], ("gq", "gk")):
         once = (ref[name].bfloat16().double() - ref[name]).norm()
         assert float((grad.double() - ref[name]).norm() / once) < 1.3, name
+
+
+# ------------------------------------------------------------ how callers call them
+def operators(gpu):
+    """(name, function of its differentiable inputs, these inputs) of each operator."""
+    g = torch.Generator(device=gpu).manual_seed(9)
+    x, w, b = randn(g, 20, 64), randn(g, 64), randn(g, 64)
+    pos = torch.arange(40, device=gpu, dtype=torch.int32).view(20, 2)
+    f, at = cr.axial_frequencies((8, 24), 100.0, gpu), offsets_of([12, 8], gpu)
+    q, k, v = (randn(g, 20, h, 64) for h in (4, 2, 2))
+    return [("layer_norm", lambda x, w, b: cr.layer_norm(x, w, b), (x, w, b)),
+            ("axial_rotary", lambda q, k: cr.axial_rotary(q, k, pos, f, (8, 24)), (q, k)),
+            ("packed_attention", lambda q, k, v: cr.packed_attention(q, k, v, at, causal=True),
+             tuple(t.half() for t in (q, k, v)))]
+
+
+def test_forward_mode_tangents_are_refused(gpu):
+    """In every differentiable input, with and without gradients enabled: no output silently
+    without its tangent."""
+    with torch.autograd.forward_ad.dual_level():
+        for name, run, args in operators(gpu):
+            run(*args)
+            for i, t in enumerate(args):
+                dual = torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match=name):
+                        run(*args[:i], dual, *args[i + 1:])
