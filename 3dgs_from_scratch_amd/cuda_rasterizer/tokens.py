@@ -69,9 +69,11 @@ def _workspace(query, *args, device):
 
 
 def _differentiable(what: str, *tensors) -> bool:
-    """Whether autograd has to record the call.  A tangent of forward-mode differentiation is
-    refused: the operators have no such rule, and their outputs would drop it."""
-    grad, found = torch.is_grad_enabled(), False
+    """Whether the call has to be an autograd function's: where gradients are recorded, and where
+    torch.jit.trace records, which would find only the allocation of the outputs otherwise.  A
+    tangent of forward-mode differentiation is refused: the operators have no such rule, and
+    their outputs would drop it."""
+    grad, found = torch.is_grad_enabled(), torch.jit.is_tracing()
     for t in tensors:
         if isinstance(t, torch.Tensor):
             found = found or (grad and t.requires_grad)

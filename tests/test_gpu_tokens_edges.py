@@ -247,3 +247,21 @@ def test_forward_mode_tangents_are_refused(gpu):
                 for grad in (True, False):
                     with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match=name):
                         run(*args[:i], dual, *args[i + 1:])
+
+
+def test_traced_calls_compute(gpu):
+    """A traced function runs the operator on its new inputs, with gradients enabled or not; it
+    does not return what memory holds."""
+    for name, run, args in operators(gpu):
+        new = tuple(t.flip(0).contiguous() for t in args)
+        want = run(*new)
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                traced = torch.jit.trace(run, args, check_trace=False)
+            for _ in range(2):
+                spoil = [torch.full_like(t, math.nan) for t in args for _ in range(4)]
+                del spoil  # an output that is only allocated would hold these
+                got = traced(*new)
+                for a, b in zip(got if isinstance(got, tuple) else (got,),
+                                want if isinstance(want, tuple) else (want,)):
+                    assert torch.equal(a, b), (name, grad)
