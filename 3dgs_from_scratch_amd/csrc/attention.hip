@@ -877,10 +877,10 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
     using Shape = KeysShape<DIM>;
     constexpr int kOwn = Shape::kOwn;
     using QTile = Tile<T, DIM, kBackRows, Shape::kWaves>;
-    using VTile = Tile<T, DIM, kOwn, Shape::kWaves>;
+    using VTile = Tile<T, DIM, kOwn / 2, Shape::kWaves>;  // two, one behind the other
     constexpr int kFloats = kBackRows * 4;                         // bytes of one float a row
     constexpr int kStage = 2 * QTile::kBytes + 2 * kFloats;  // Q, dout, log-sums, deltas
-    __shared__ __attribute__((aligned(1024))) char lds[2 * kStage + (Shape::kValuesInLds ? VTile::kBytes : 0)];
+    __shared__ __attribute__((aligned(1024))) char lds[2 * kStage + (Shape::kValuesInLds ? 2 * VTile::kBytes : 0)];
     lds_char *const tiles = (lds_char *)lds, *const values = tiles + 2 * kStage;
 
     const Place at_grid = place_of(a.heads_k, splits);
@@ -1022,10 +1022,13 @@ __global__ __launch_bounds__(64 * KeysShape<DIM>::kWaves, DIM > 96 ? 1 : 2) void
     const int steps = min(first_step + share, steps_all);
     int i = first_step;
     if (i < steps) {
-        if constexpr (Shape::kValuesInLds)
-            VTile::start(VTile::copy_of(wave, a.v_row, a.dim), wave,
-                         v + (int64_t)(p.k0 + block_key) * a.v_row + (int64_t)kh * a.v_head, a.v_row,
-                         p.lk - block_key, a.dim, values);
+        if constexpr (Shape::kValuesInLds) {
+            const auto copy_v = VTile::copy_of(wave, a.v_row, a.dim);
+            for (int at = 0; at < kOwn; at += kOwn / 2)
+                VTile::start(copy_v, wave,
+                             v + (int64_t)(p.k0 + block_key + at) * a.v_row + (int64_t)kh * a.v_head,
+                             a.v_row, p.lk - block_key - at, a.dim, values + at * DIM * 2);
+        }
         fetch(i);
     }
     for (; i < min(whole_steps, steps); ++i) {
@@ -1083,7 +1086,6 @@ __global__ __launch_bounds__(256) void attention_sum_kernel(const float *__restr
 }
 
 constexpr int64_t kMaxRows = 0x7fffffffLL - 65536;  // row numbers stay in 32 bits
-constexpr int64_t kMaxStride = 1 << 23;             // and a tile's byte offsets in 31
 
 // Rows that a tile can be copied from: byte offsets fit, and a row past the last one lies
 // wholly behind the copy's bound.

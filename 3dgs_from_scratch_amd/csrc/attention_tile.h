@@ -172,8 +172,12 @@ __device__ __forceinline__ i16x4 transposed(const lds_x4 *__restrict__ p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_x4 *)p);
 }
 
+constexpr int64_t kMaxStride = 1 << 23;  // of rows, elements
+
 template <typename T, int DIM, int ROWS, int WAVES>
 struct Tile {
+    // byte offsets and the bound in start() stay in 31 bits, below copy_of()'s mark
+    static_assert(((ROWS - 1) * kMaxStride + DIM) * 2 < (1LL << 31), "offsets of a copy");
     static constexpr int kChunks = DIM / 8;                      // of a row
     static constexpr int kBytes = ROWS * DIM * 2;
     static constexpr int kPieces = ROWS * kChunks / 64;  // of 1 KiB, which a wave copies at once

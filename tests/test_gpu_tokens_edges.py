@@ -265,3 +265,21 @@ def test_traced_calls_compute(gpu):
                 for a, b in zip(got if isinstance(got, tuple) else (got,),
                                 want if isinstance(want, tuple) else (want,)):
                     assert torch.equal(a, b), (name, grad)
+
+
+# --------------------------------------------------------------------- layouts
+@pytest.mark.parametrize("dim", [64, 72, 88, 128])
+def test_attention_of_rows_megabytes_apart(gpu, dim):
+    """Values whose rows lie 12 MB apart, so that a tile of keys spans more than 2^31 bytes: what
+    lies between them, also at that distance, is not read."""
+    stride, rows = 6_000_000, 200
+    q, k, v, go = inputs(gpu, rows, rows, 4, 1, dim, torch.bfloat16)
+    wide = torch.full((rows * stride,), math.nan, dtype=torch.bfloat16, device=gpu)
+    far = wide.as_strided((rows, 1, dim), (stride, dim, 1))
+    far.copy_(v)
+    at = offsets_of([rows], gpu)
+    for causal in (False, True):
+        want = gradients(q, k, v, go, at, causal=causal)
+        got = gradients(q, k, far, go, at, causal=causal)
+        for a, b in zip((want[0], *want[1]), (got[0], *got[1])):
+            assert torch.equal(a, b)
