@@ -641,7 +641,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
 // ---------------------------------------------------------------- gradients
 // Two launches, neither with atomics: the queries' gradients, a workgroup a tile of
 // packed rows as in the forward, which also leaves each row's log-sum (in the exponent
-// of two) and delta for the second; then the keys' and values', a workgroup a tile of
+// of two) and delta for the second (and only these where queries have no gradient); then the keys' and values', a workgroup a tile of
 // keys, over all the queries of all heads of the group.  Scores are computed again in
 // both: seven products in all where one launch with atomics needs five, whose sums' order
 // would change from run to run.
@@ -745,7 +745,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
     const int tiles_all = seen > 0 ? (seen + kBackRows - 1) / kBackRows : 0;
     const int share = (tiles_all + splits - 1) / splits;  // this split's tiles
     const int first_tile = min(split * share, tiles_all);
-    const int end_tile = min(first_tile + share, tiles_all);
+    const int end_tile = dq ? min(first_tile + share, tiles_all) : first_tile;
 
     RowOperand<T, DIM> qr, gr;
     qr.load(real ? q + (int64_t)(p.q0 + query) * a.q_row + (int64_t)head * a.q_head : nullptr,
@@ -854,7 +854,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
                                 : nullptr,
                            a.dim);
     else
-        store_columns<T, DIM>(acc, a.scale / fit.scale, real ? dq + at * a.dim : nullptr, a.dim);
+        store_columns<T, DIM>(acc, a.scale / fit.scale, real && dq ? dq + at * a.dim : nullptr, a.dim);
 }
 
 // Up to 64 dimensions a wave holds its keys' K and V and both sums in half a SIMD's registers,
@@ -1288,16 +1288,17 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
     int st = gs_attention_backward_workspace_size(a, &need);
     if (st) return st;
     if (grad_out_row < 0 || grad_out_head < 0) return GS_ERR_INVALID_ARGUMENT;
-    if (a->rows_q > 0 && (!q || !out || !out_rest || !log_sum || !grad_out || !grad_q || !workspace))
+    if (a->rows_q > 0 && (!q || !out || !out_rest || !log_sum || !grad_out || !workspace))
         return GS_ERR_INVALID_ARGUMENT;
-    if (a->rows_k > 0 && (!k || !v || !grad_k || !grad_v)) return GS_ERR_INVALID_ARGUMENT;
+    if (!grad_k != !grad_v || (a->rows_k > 0 && (!k || !v))) return GS_ERR_INVALID_ARGUMENT;
     for (const void *x : {q, k, v, out, out_rest, grad_out, (const void *)grad_q, (const void *)grad_k,
                           (const void *)grad_v})
         if (!aligned16(x)) return GS_ERR_UNSUPPORTED;
     if ((grad_out_row | grad_out_head) % 8 != 0 || !tile_stride(grad_out_row, a->dim))
         return GS_ERR_UNSUPPORTED;
     if (workspace_bytes < need) return GS_ERR_WORKSPACE_TOO_SMALL;
-    const BackwardPlan b = plan_backward(*a);
+    BackwardPlan b = plan_backward(*a);
+    if (!grad_q) b.splits_q = 1;
     const int64_t blocks_q = b.tiles_q * a->heads_k * b.splits_q;
     const int64_t blocks_k = b.tiles_k * a->heads_k * b.splits_k;
     if (blocks_q > 0x7fffffffLL || blocks_k > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
@@ -1312,7 +1313,7 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
                                dim3(256), 0, stream, (const float *)partial, size, splits, scale0,
                                1.0f, out0, out1);
         };
-        if (a->rows_q > 0) {
+        if (a->rows_q > 0 && (grad_q || grad_k)) {
             hipLaunchKernelGGL((attention_dq_kernel<T, kDim>), dim3((unsigned)blocks_q),
                                block, 0, stream, *a, (const T *)q, (const T *)k, (const T *)v,
                                (const T *)out, (const T *)out_rest, log_sum, (const T *)grad_out,
@@ -1324,7 +1325,7 @@ extern "C" int gs_attention_backward(const GsAttention *a, const void *q, const 
             const int s = launch_status();
             if (s) return s;
         }
-        if (a->rows_k > 0) {
+        if (a->rows_k > 0 && grad_k) {
             hipLaunchKernelGGL((attention_dkv_kernel<T, kDim>), dim3((unsigned)blocks_k),
                                dim3(64 * KeysShape<kDim>::kWaves), 0, stream, *a, (const T *)q,
                                (const T *)k, (const T *)v, (const T *)grad_out, grad_out_row, grad_out_head, row_log, row_delta,

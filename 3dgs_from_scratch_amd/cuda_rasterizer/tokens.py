@@ -309,15 +309,18 @@ def attention_forward(q, k, v, offsets_q, offsets_k, lengths_k, causal: bool, sc
 
 
 def attention_backward(grad_out, q, k, v, out, out_rest, log_sum, offsets_q, offsets_k, lengths_k,
-                       causal: bool, scale: float):
-    """(grad_q, grad_k, grad_v), contiguous, of attention_forward's out."""
+                       causal: bool, scale: float, needs=(True, True, True)):
+    """(grad_q, grad_k, grad_v), contiguous, of attention_forward's out, None where needs is
+    False; those of k and v are computed together."""
     _check("packed_attention", "grad_out", grad_out, 3, (q.dtype,), q.device)
     if grad_out.shape != q.shape:
         raise RuntimeError(f"packed_attention: grad_out must be {tuple(q.shape)}, got "
                            f"{tuple(grad_out.shape)}")
     q, k, v, go = _laid_out(q), _laid_out(k), _laid_out(v), _laid_out(grad_out)
     dev = q.device
-    gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+    wanted = needs[0], needs[1] or needs[2], needs[1] or needs[2]
+    gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=dev) if want else None
+                  for t, want in zip((q, k, v), wanted))
     a = _problem(q, k, v, offsets_q, offsets_k, lengths_k, causal, scale)
     lib = _lib.load()
     with _lib.on_device(dev):
@@ -326,10 +329,10 @@ def attention_backward(grad_out, q, k, v, out, out_rest, log_sum, offsets_q, off
         _lib.check(lib.gs_attention_backward(
             ctypes.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
             out_rest.data_ptr(), log_sum.data_ptr(), go.data_ptr(), go.stride(0), go.stride(1),
-            gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _ptr(ws), size, _lib.stream_of(dev)),
+            _ptr(gq), _ptr(gk), _ptr(gv), _ptr(ws), size, _lib.stream_of(dev)),
             "attention_backward")
         _lib.timer.stop(ev, dev)
-    return gq, gk, gv
+    return gq, gk if needs[1] else None, gv if needs[2] else None
 
 
 class _PackedAttention(torch.autograd.Function):
@@ -345,7 +348,8 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out, _):
-        return (*attention_backward(grad_out, *ctx.saved_tensors, *ctx.how),
+        return (*attention_backward(grad_out, *ctx.saved_tensors, *ctx.how,
+                                    ctx.needs_input_grad[:3]),
                 None, None, None, None, None)
 
 

@@ -758,7 +758,9 @@ typedef struct {
  *   the natural logarithm of each softmax's denominator, (rows_q, heads_q), and
  *   out_rest, laid out as out, what rounding took from out.
  * gs_attention_backward: gradients of q, k and v from out, out_rest, log_sum and
- *   grad_out; every row is written.  Deterministic: no atomics.
+ *   grad_out; every row is written.  grad_q may be NULL, and so may grad_k and
+ *   grad_v together: what is not asked for is not computed.  Deterministic: no
+ *   atomics.
  */
 int gs_attention_forward_workspace_size(const GsAttention *a, size_t *bytes);
 int gs_attention_forward(const GsAttention *a, const void *q, const void *k, const void *v,

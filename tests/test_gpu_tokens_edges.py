@@ -283,3 +283,25 @@ def test_attention_of_rows_megabytes_apart(gpu, dim):
         got = gradients(q, k, far, go, at, causal=causal)
         for a, b in zip((want[0], *want[1]), (got[0], *got[1])):
             assert torch.equal(a, b)
+
+
+# --------------------------------------------------------- part of the gradients
+@pytest.mark.parametrize("lq,lk", [([30, 200], [30, 200]), ([3], [20_000]), ([40], [0])])
+def test_attention_gradients_that_are_asked_for(gpu, lq, lk):
+    """The same values as all together, for every choice of inputs that have one; keys and values
+    without a gradient get no memory for it."""
+    q, k, v, go = inputs(gpu, sum(lq), sum(lk), 8, 8, 128, torch.bfloat16)
+    oq, ok = offsets_of(lq, gpu), offsets_of(lk, gpu)
+    whole = gradients(q, k, v, go, oq, ok, causal=True)[1]
+    for choice in range(1, 8):
+        leaves = [t.clone().requires_grad_(bool(choice >> i & 1)) for i, t in enumerate((q, k, v))]
+        out = cr.packed_attention(*leaves, oq, ok, causal=True)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = torch.autograd.grad(out, [t for t in leaves if t.requires_grad], go)
+        peak = torch.cuda.max_memory_allocated() - before
+        for a, b in zip(got, [w for i, w in enumerate(whole) if choice >> i & 1]):
+            assert torch.equal(a, b)
+        if choice == 1 and sum(lk) > 10_000:
+            assert peak < k.numel() * k.element_size()
