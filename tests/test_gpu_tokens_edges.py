@@ -305,3 +305,25 @@ def test_attention_gradients_that_are_asked_for(gpu, lq, lk):
             assert torch.equal(a, b)
         if choice == 1 and sum(lk) > 10_000:
             assert peak < k.numel() * k.element_size()
+
+
+# ---------------------------------------------- gradients within their derived bounds
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [40, 64, 72, 88, 96, 128])
+@pytest.mark.parametrize("lq,lk", [([700, 5, 100], None), ([257], None), ([128, 129, 64, 65], None),
+                                   ([40, 256, 1], [300, 513, 256])])
+def test_attention_gradients_within_bounds(gpu, lq, lk, dim, causal, dtype):
+    """Blocks of 128 and 256 keys, their remainders and their places among the values."""
+    q, k, v, go = inputs(gpu, sum(lq), sum(lk or lq), 4, 2, dim, dtype)
+    check_gradients(q, k, v, go, offsets_of(lq, gpu), offsets_of(lk or lq, gpu), causal=causal)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("lq,lk,heads", [([1], [20_001], 4), ([70], [3000], 4), ([1500], [700], 4),
+                                         ([3000, 100], [300, 300], 8), ([700], [5000], 2)])
+@pytest.mark.parametrize("dim", [64, 72, 96, 128])
+def test_attention_gradients_in_splits_within_bounds(gpu, lq, lk, heads, dim, dtype):
+    """Few queries over many keys and many queries over few, whose sums are split."""
+    q, k, v, go = inputs(gpu, sum(lq), sum(lk), heads, 1, dim, dtype)
+    check_gradients(q, k, v, go, offsets_of(lq, gpu), offsets_of(lk, gpu))
