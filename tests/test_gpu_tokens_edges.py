@@ -327,3 +327,28 @@ def test_attention_gradients_in_splits_within_bounds(gpu, lq, lk, heads, dim, dt
     """Few queries over many keys and many queries over few, whose sums are split."""
     q, k, v, go = inputs(gpu, sum(lq), sum(lk), heads, 1, dim, dtype)
     check_gradients(q, k, v, go, offsets_of(lq, gpu), offsets_of(lk, gpu))
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("slab,longs,sequences", [(700, 290, 300), (6400, 5, 127)])
+def test_attention_over_more_caches_than_workgroups(gpu, slab, longs, sequences, dtype):
+    """More parts of caches than the launch has workgroups, so that one takes several in turn: 2400
+    whole caches, and 1056 parts of which some are halves."""
+    g = torch.Generator().manual_seed(slab)
+    few = torch.randint(1, 64, (sequences,), generator=g)
+    many = torch.randint(slab - 100, slab + 1, (sequences,), generator=g)
+    lengths = torch.where(torch.randperm(sequences, generator=g) < longs, many, few)
+    q, k, v, _ = inputs(gpu, sequences, sequences * slab, 8, 8, 64, dtype)
+    oq, ok = offsets_of([1] * sequences, gpu), offsets_of([slab] * sequences, gpu)
+    lk = lengths.to(device=gpu, dtype=torch.int32)
+    for causal in (False, True):
+        out, log_sum = cr.packed_attention(q, k, v, oq, ok, lk, causal=causal, return_log_sum=True)
+        ref = ot.attention(q, k, v, oq, ok, lk, causal)
+        off = (out.double() - ref["out"]).abs()
+        least = 2.0 ** -25 * slab * float(v.abs().max()) if dtype == torch.float16 else 0.0
+        assert float((off - 1.1 * U[dtype] * ref["out_slack"]).max()) <= least
+        assert float(off.norm()) <= 3 * U[dtype] * float(ref["out"].norm())
+        # scores off by (dim + 16) 2^-24 of their largest, and the sum's logarithm rounded
+        reach = 64 ** -0.5 * float(q.double().norm(dim=2).max() * k.double().norm(dim=2).max())
+        bound = (64 + 16) * 2.0 ** -24 * (reach + ref["log_sum"].abs() + 1)
+        assert float(((log_sum - ref["log_sum"]).abs() - bound).max()) <= 0.0
