@@ -15,7 +15,6 @@ template <typename T>
 __device__ __forceinline__ T from_float(float v) { return (T)v; }
 
 inline bool element_type(int32_t t) { return t == GS_F32 || t == GS_F16 || t == GS_BF16; }
-inline int element_size(int32_t t) { return t == GS_F32 ? 4 : 2; }
 
 // Calls f with a value of the element type that `type` names.
 template <typename F>

@@ -356,8 +356,8 @@ static int with_shape(int channels, F f) {
                                                  : with_shape<T, false>(channels, f);
 }
 
-// Workgroups of a backward: as many as the rows give, at most kNormGroups, and at least
-// four rows a row of lanes where there are more.
+// Workgroups of a backward: one for every 16 rows (four a wave, or one a row of 16 lanes), at
+// most kNormGroups.
 static int norm_groups(int64_t rows) {
     const int64_t g = (rows + 15) / 16;
     return (int)(g < kNormGroups ? g : kNormGroups);
