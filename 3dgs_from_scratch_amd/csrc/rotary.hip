@@ -29,12 +29,20 @@ struct RotaryBatch {
 // sin and cos of position * frequency.  The product is reduced to an eighth of a turn
 // to either side in double: a float product of a position in the thousands is off by
 // 1e-4 of a radian before any sine is taken.  On what is left, at most pi / 4, Taylor's
-// sums to x^9 and x^10 are within 2e-9.
-__device__ __forceinline__ void turn_of(double position, float frequency, float *s, float *c) {
-    const double angle = position * (double)frequency;
+// sums to x^9 and x^10 are within 2e-9.  FAR: also where the number of quarter turns is rounded,
+// from 2^53 on by whole ones (a position may be a time in nanoseconds): what it is off by is
+// reduced again.
+template <bool FAR>
+__device__ __forceinline__ void turn_of(double angle, float *s, float *c) {
     const double quarters = rint(angle * 0.63661977236758134308);
     // pi / 2 in two parts: quarters * the first is exact to 2^-53 of the angle
-    const double rest = fma(quarters, -6.123233995736766e-17, fma(quarters, -1.5707963267948966, angle));
+    double rest = fma(quarters, -6.123233995736766e-17, fma(quarters, -1.5707963267948966, angle));
+    int quarter = (int)((int64_t)quarters & 3);
+    if constexpr (FAR) {
+        const double more = rint(rest * 0.63661977236758134308);
+        rest = fma(more, -6.123233995736766e-17, fma(more, -1.5707963267948966, rest));
+        quarter = (int)(quarters - 4.0 * floor(quarters * 0.25)) + (int)more;
+    }
     const float x = (float)rest, x2 = x * x;
     float sine = fmaf(x2, 2.7557319e-6f, -1.9841270e-4f);
     sine = fmaf(x2, sine, 8.3333333e-3f);
@@ -45,7 +53,6 @@ __device__ __forceinline__ void turn_of(double position, float frequency, float 
     cosine = fmaf(x2, cosine, 4.1666667e-2f);
     cosine = fmaf(x2, cosine, -0.5f);
     cosine = fmaf(x2, cosine, 1.0f);
-    const int quarter = (int)((int64_t)quarters & 3);
     const float a = quarter & 1 ? cosine : sine, b = quarter & 1 ? sine : cosine;
     *s = quarter & 2 ? -a : a;
     *c = (quarter + 1) & 2 ? -b : b;
@@ -78,13 +85,20 @@ __global__ __launch_bounds__(kRotaryBlock) void rotary_kernel(RotaryBatch b, int
     float s[U::kPairs], c[U::kPairs];
     if (turned) {
         const P *at = (const P *)b.positions + token * b.position_stride;
+        const auto turns = [&](auto far) {
+            bool near = true;
 #pragma unroll
-        for (int j = 0; j < U::kPairs; ++j) {
-            int axis = 0;
-            for (int a = 0; a + 1 < b.axes; ++a) axis += pair + j >= b.ends[a];
-            turn_of((double)at[axis], b.frequencies[pair + j], &s[j], &c[j]);
-            s[j] *= b.sign;
-        }
+            for (int j = 0; j < U::kPairs; ++j) {
+                int axis = 0;
+                for (int a = 0; a + 1 < b.axes; ++a) axis += pair + j >= b.ends[a];
+                const double angle = (double)at[axis] * (double)b.frequencies[pair + j];
+                near = near && !(fabs(angle) > 0x1p40);
+                turn_of<decltype(far)::value>(angle, &s[j], &c[j]);
+                s[j] *= b.sign;
+            }
+            return near;
+        };
+        if (!turns(std::false_type{})) turns(std::true_type{});
     }
     const int first = INTERLEAVED ? unit * U::kElements : turned ? pair : pair + b.pairs;
     const bool odd_end = U::kElements > VEC && first + 1 >= b.dim;  // one element is left

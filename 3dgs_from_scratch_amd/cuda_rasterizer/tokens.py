@@ -236,7 +236,8 @@ def axial_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     pairs go to each axis, in order, and frequencies (float32) has one entry a
     pair.  With P pairs in all, pair p is elements (p, p + P) of a head, or
     (2 p, 2 p + 1) when interleaved; elements from 2 P on stay as they are.  Angles
-    are reduced in float64, so large positions keep their accuracy.  No gradient
+    are products in float64, off by 2^-53 of themselves, and are reduced there, so
+    large positions keep their accuracy.  No gradient
     goes to positions or frequencies."""
     _check("axial_rotary", "q", q, 3)
     dev = q.device

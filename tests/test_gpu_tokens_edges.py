@@ -352,3 +352,26 @@ def test_attention_over_more_caches_than_workgroups(gpu, slab, longs, sequences,
         reach = 64 ** -0.5 * float(q.double().norm(dim=2).max() * k.double().norm(dim=2).max())
         bound = (64 + 16) * 2.0 ** -24 * (reach + ref["log_sum"].abs() + 1)
         assert float(((log_sum - ref["log_sum"]).abs() - bound).max()) <= 0.0
+
+
+# -------------------------------------------------------------------- positions
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("ptype,sizes", [(torch.int64, (10 ** 12, 10 ** 15, 10 ** 17, 17 * 10 ** 17)),
+                                         (torch.float32, (1e12, 1e16, 1e19, 1e22))])
+def test_axial_rotary_of_times_in_nanoseconds(gpu, ptype, sizes, interleaved):
+    """Positions up to the types' large numbers turn pairs by the angle that float64 holds, to a
+    float's accuracy, and keep their length."""
+    g = torch.Generator(device=gpu).manual_seed(12)
+    rows = 64
+    q = randn(g, rows, 2, 32)
+    scale = torch.tensor(sizes, dtype=torch.float64).repeat(rows // 4)[:, None]
+    part = 1 + torch.rand(rows, 2, generator=torch.Generator().manual_seed(1), dtype=torch.float64)
+    positions = (scale * part * torch.tensor([1.0, -1.0])).to(ptype)
+    f = cr.axial_frequencies((7, 9), 100.0, "cpu")
+    got = cr.axial_rotary(q, None, positions.to(gpu), f.to(gpu), (7, 9), interleaved=interleaved)[0]
+    want = ot.rotary(q.cpu(), positions, f, (7, 9), interleaved)
+    lo, hi = (slice(0, 32, 2), slice(1, 32, 2)) if interleaved else (slice(0, 16), slice(16, 32))
+    length = torch.hypot(q.cpu().double()[..., lo], q.cpu().double()[..., hi])
+    for part in (lo, hi):
+        off = (got.cpu().double()[..., part] - want[..., part]).abs()
+        assert float((off - 9 * 2.0 ** -24 * length).max()) <= 0.0
