@@ -379,6 +379,7 @@ extern "C" int gs_layer_norm_forward(const void *x, int64_t x_stride, const void
     if (rows < 0 || channels <= 0 || x_stride < 0 || !(eps >= 0.0f) || !element_type(type) ||
         !element_type(weight_type))
         return GS_ERR_INVALID_ARGUMENT;
+    if (channels > GS_MAX_CHANNELS) return GS_ERR_UNSUPPORTED;
     if (rows == 0) return GS_OK;
     if (!x || !y) return GS_ERR_INVALID_ARGUMENT;
     return with_element(type, [&](auto t) {
@@ -402,6 +403,7 @@ extern "C" int gs_layer_norm_forward(const void *x, int64_t x_stride, const void
 extern "C" int gs_layer_norm_backward_workspace_size(int64_t rows, int32_t channels,
                                                      size_t *bytes) {
     if (rows < 0 || channels <= 0 || !bytes) return GS_ERR_INVALID_ARGUMENT;
+    if (channels > GS_MAX_CHANNELS) return GS_ERR_UNSUPPORTED;
     *bytes = (size_t)norm_groups(rows) * 2 * channels * sizeof(float);
     return GS_OK;
 }
@@ -415,6 +417,7 @@ extern "C" int gs_layer_norm_backward(const void *grad_y, int64_t grad_y_stride,
     if (rows < 0 || channels <= 0 || x_stride < 0 || grad_y_stride < 0 || !element_type(type) ||
         !element_type(weight_type))
         return GS_ERR_INVALID_ARGUMENT;
+    if (channels > GS_MAX_CHANNELS) return GS_ERR_UNSUPPORTED;
     if (rows > 0 && (!grad_y || !x || !stats)) return GS_ERR_INVALID_ARGUMENT;
     const bool sums = grad_weight || grad_bias;
     const int groups = norm_groups(rows);

@@ -36,6 +36,7 @@ from ._lib import GsAttention, GsRotaryTensor
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+MAX_CHANNELS = 1 << 30
 MAX_AXES = 4
 MAX_HEAD_DIM = 128
 _MAX_STRIDE = 1 << 23  # elements from a row to the next
@@ -97,6 +98,8 @@ def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5, with_stats:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f"layer_norm: x needs channels in its last dimension, got {tuple(x.shape)}")
     channels = x.shape[-1]
+    if channels > MAX_CHANNELS:
+        raise RuntimeError(f"layer_norm: at most {MAX_CHANNELS} channels are supported, got {channels}")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue

@@ -687,13 +687,14 @@ int gs_rasterize_work(const int32_t *indexing_offset, const int32_t *gaussian_id
  */
 enum { GS_F32 = 0, GS_F16 = 1, GS_BF16 = 2 };
 enum { GS_POS_I32 = 0, GS_POS_I64 = 1, GS_POS_F32 = 2 };
-enum { GS_MAX_AXES = 4, GS_MAX_HEAD_DIM = 128 };
+enum { GS_MAX_AXES = 4, GS_MAX_HEAD_DIM = 128, GS_MAX_CHANNELS = 1 << 30 };
 
 /*
  * gs_layer_norm_forward: y = (x - mean) / sqrt(var + eps) * weight + bias over
  *   each row of `channels` elements; rows x_stride apart, y contiguous.  weight
  *   and bias (weight_type) may be NULL.  stats, when set, receives (mean,
  *   1 / sqrt(var + eps)) a row for the backward.
+ *   More than GS_MAX_CHANNELS channels are GS_ERR_UNSUPPORTED.
  * gs_layer_norm_backward: any of grad_x, grad_weight, grad_bias may be NULL;
  *   what is set is overwritten.  The weight's gradients are summed over the rows
  *   in an order that depends on the sizes alone.

@@ -375,3 +375,12 @@ def test_axial_rotary_of_times_in_nanoseconds(gpu, ptype, sizes, interleaved):
     for part in (lo, hi):
         off = (got.cpu().double()[..., part] - want[..., part]).abs()
         assert float((off - 9 * 2.0 ** -24 * length).max()) <= 0.0
+
+
+# --------------------------------------------------------------------- refusals
+def test_layer_norm_refuses_channels_past_its_numbers(gpu):
+    """More channels than 32-bit numbers hold, which would be taken for their lowest bits."""
+    x = torch.zeros(1, 1, device=gpu)
+    for channels in (2 ** 30 + 1, 2 ** 31 + 8, 2 ** 32 + 8):
+        with pytest.raises(RuntimeError, match="channels"):
+            cr.layer_norm(x.expand(1, channels))

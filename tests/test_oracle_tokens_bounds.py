@@ -1,13 +1,16 @@
 """The bounds that gradients of attention are held to (oracle/tokens.py::attention_gradients):
 the same gradients as the formulas', bounds that a rounding implementation keeps, and that zeros
-do not."""
+do not; and a host check of layer norm's entry points (no GPU)."""
 
 from __future__ import annotations
+
+import ctypes
 
 import pytest
 import torch
 
 import helpers  # noqa: F401
+from cuda_rasterizer import _lib
 from oracle import tokens as ot
 
 U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
@@ -61,3 +64,12 @@ def test_bounds_let_roundings_pass_and_zeros_fail(lq, lk, causal, dtype):
         assert float(want.norm()) > 0.0  # so that zeros are not within 3 u of it
         if dtype == torch.float16:  # and element by element, where the type has the bits
             assert float((want.abs() > bound).double().mean()) > 0.6, name
+
+
+def test_layer_norm_entry_points_refuse_too_many_channels():
+    lib, size = _lib.load(), ctypes.c_size_t(0)
+    some, many = ctypes.c_void_p(4096), 2 ** 30 + 1  # rejected before anything is read
+    assert lib.gs_layer_norm_forward(some, many, None, None, 1, many, 1e-5, 0, 0, some, None, None) == -4
+    assert lib.gs_layer_norm_backward_workspace_size(1, many, ctypes.byref(size)) == -4
+    assert lib.gs_layer_norm_backward(some, many, some, many, None, some, 1, many, 0, 0, some, None,
+                                      None, None, 0, None) == -4
