@@ -640,10 +640,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
 // ---------------------------------------------------------------- gradients
 // Two launches, neither with atomics: the queries' gradients, a workgroup a tile of
 // packed rows as in the forward, which also leaves each row's log-sum (in the exponent
-// of two) and delta for the second (and only these where queries have no gradient); then the keys' and values', a workgroup a tile of
-// keys, over all the queries of all heads of the group.  Scores are computed again in
-// both: seven products in all where one launch with atomics needs five, whose sums' order
-// would change from run to run.
+// of two) and delta for the second (and only these where queries have no gradient); then
+// the keys' and values', a workgroup a tile of keys, over all the queries of all heads of
+// the group.  Scores are computed again in both: seven products in all where one launch
+// with atomics needs five, whose sums' order would change from run to run.
 //
 // Bound as the forward is, the keys' launch more by its registers: two sums of a tile of keys
 // and both operands leave one wave a SIMD above 96 dimensions.  16320 rows and keys, 16 heads
@@ -658,8 +658,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
 // largest, both launches have it (1.3 times the error for rows of 1 to 7 keys in bfloat16; the
 // training pass over scenes of 12566 and 16320 tokens 8.53 -> 8.65 ms).  In float16, which is chosen for its bits, the queries'
 // gradients have it in every tile (1.02 to 1.08 times the error); that costs the launch 28%,
-// 171 -> 217 us for 4 sequences of 2500, 12 heads of 72, and neither bfloat16 nor the keys'
-// launch, longer by itself, pays it.
+// 171 -> 217 us for 4 sequences of 2500, 12 heads of 72 (249 with the range below), and neither
+// bfloat16 nor the keys' launch, longer by itself, pays it.
 // In float16 they are first put into its range: weights times 2^10, so that those of long rows keep their
 // bits, and score gradients times a power of two that follows the largest that the query, or
 // the key, has met so far (Fit), and that the sums follow.
@@ -683,8 +683,8 @@ __device__ __forceinline__ float power_below(float v) {
 // scale does not become, so that no product with it overflows; what that leaves too small is
 // below any gradient's last bit.  Forward and gradients with it, and with a factor from the
 // output gradients alone, which values of 34 overflow: 8160 rows and keys, 16 heads on 4, dim
-// 128, 2.80 ms and 2.85; 4 sequences of 2500, 12 heads of 72, 638 us and 646; of 64, causal,
-// 357 and 346.
+// 128, 2.80 ms and 2.78; 4 sequences of 2500, 12 heads of 72, 611 us and 624; of 64, causal,
+// 354 and 341.
 struct Fit {
     float scale = 1.0f, limit = 0.0f;
     template <int SUMS>
@@ -859,8 +859,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(
 // Up to 64 dimensions a wave holds its keys' K and V and both sums in half a SIMD's registers,
 // and four waves make a workgroup, two a CU.  At 65 to 96 two waves' sums leave no room for V,
 // which lies in LDS; that then has room for one workgroup of eight waves.  At 97 to 128 the
-// sums alone take half of a SIMD's registers: K and V stay in those of one wave, and four
-// waves make a workgroup.
+// sums alone would take half of what two waves a SIMD have: one wave has K, V and both sums
+// in 369 of 512, and four waves make a workgroup.
 template <int DIM>
 struct KeysShape {
     static constexpr bool kValuesInLds = DIM == 96;

@@ -7,7 +7,7 @@
 // a lane, by the LDS's transposed read, as one that contracts over the rows.  The
 // chunks of a row are permuted by an exclusive or with a function of the row, so that
 // eight lanes at a time meet different banks either way, no more than half of the 64.  Of
-// sixteen some meet the same: conflicts are 0.21 to 0.32 of the large launches' cycles.
+// sixteen some meet the same: conflicts are 0.21 to 0.29 of the large launches' cycles.
 //
 // Products are v_mfma_f32_32x32x16: lane l gives column l % 32 of an operand and 8 of
 // its 16 contracted places (half l / 32); of the 32x32 result it holds column l % 32

@@ -377,7 +377,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets_
 
     scale defaults to dim ** -0.5.  With return_log_sum also the float32 (queries,
     heads) natural logarithm of each softmax's denominator (no gradient).  Scores
-    and sums are float32; probabilities are rounded to q's type before they meet v.
+    and sums are float32; probabilities are rounded to q's type before they meet v, and in
+    the backward they and the score gradients before they meet grad_out, q and k.
 
     What a query does not see, whatever it is, changes nothing.  An infinity in a value
     that it sees gives that infinity, or NaN where its probability was rounded to 0 or
