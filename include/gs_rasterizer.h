@@ -740,7 +740,7 @@ int gs_axial_rotary(const GsRotaryTensor *tensors, int32_t n_tensors, const void
  * query head h reads key head h / (heads_q / heads_k).  causal: query i of a
  * sequence's Lq sees keys j <= i + Lk - Lq, else every key.  A query that sees
  * no key, and a row of no sequence, has output 0 and log-sum -infinity, and
- * sends no gradient.
+ * sends no gradient; one that sees keys which all score -infinity has output NaN.
  * dim is a multiple of 8 and at most GS_MAX_HEAD_DIM, type GS_F16 or GS_BF16;
  * q, k, v and grad_out are 16-byte aligned with strides that are multiples of 8,
  * row strides from dim to 2^23 (GS_ERR_UNSUPPORTED otherwise).  Outputs are 16-byte
