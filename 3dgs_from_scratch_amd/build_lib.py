@@ -18,7 +18,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "cuda_rasterizer", "libgsraster.so")
 SOURCES = ["capi.hip", "preprocess.hip", "binning.hip", "blend.hip", "train.hip", "ssim.hip",
-           "layer_norm.hip", "rotary.hip", "attention.hip"]
+           "layer_norm.hip", "rotary.hip", "attention.hip", "paged.hip", "paged_attention.hip"]
 ARCH = "gfx950"
 
 # -ffp-contract=off: the preprocess and blend decisions are bit-exact against

@@ -31,6 +31,7 @@ import torch
 
 from . import _lib
 from ._lib import RasterizerError, on_device as _on, stream_of as _stream
+from .paged import paged_append, paged_attention, paged_evict
 from .ssim import fused_ssim
 from .tokens import axial_frequencies, axial_rotary, layer_norm, packed_attention
 
@@ -72,6 +73,9 @@ __all__ = [
     "axial_rotary",
     "axial_frequencies",
     "packed_attention",
+    "paged_append",
+    "paged_attention",
+    "paged_evict",
     "RasterizerError",
 ]
 

@@ -103,6 +103,23 @@ class GsAttention(ctypes.Structure):
                 ("causal", _I32), ("scale", _F)]
 
 
+class GsPages(ctypes.Structure):
+    """include/gs_rasterizer.h GsPages."""
+
+    _fields_ = [("pages", _I64), ("page_stride", _I64), ("slot_stride", _I64),
+                ("head_stride", _I64), ("sum_page", _I64), ("sum_slot", _I64), ("sum_head", _I64),
+                ("tables", _P), ("lengths", _P), ("table_stride", _I64), ("table_width", _I32),
+                ("sequences", _I32), ("page_size", _I32), ("heads", _I32), ("dim", _I32),
+                ("type", _I32)]
+
+
+class GsPagedQueries(ctypes.Structure):
+    """include/gs_rasterizer.h GsPagedQueries."""
+
+    _fields_ = [("rows_q", _I64), ("row_stride", _I64), ("head_stride", _I64), ("offsets", _P),
+                ("heads_q", _I32), ("causal", _I32), ("scale", _F)]
+
+
 SIGNATURES.update({
     "gs_adam_step": [ctypes.POINTER(GsAdamTensor), _I32, ctypes.c_double, ctypes.c_double,
                      ctypes.c_double, _P],
@@ -124,6 +141,14 @@ SIGNATURES.update({
     "gs_attention_backward_workspace_size": [ctypes.POINTER(GsAttention), _PSZ],
     "gs_attention_backward": [ctypes.POINTER(GsAttention)] + [_P] * 7 + [_I64, _I64]
     + [_P] * 4 + [_SZ, _P],
+    "gs_paged_append": [ctypes.POINTER(GsPages), _P, _I64, _I64, _P, _I64, _I64, _I64]
+    + [_P] * 4 + [_P],
+    "gs_paged_attention_workspace_size": [ctypes.POINTER(GsPages), ctypes.POINTER(GsPagedQueries),
+                                          _I32, _PSZ],
+    "gs_paged_attention": [ctypes.POINTER(GsPages), ctypes.POINTER(GsPagedQueries)] + [_P] * 7
+    + [_SZ, _P],
+    "gs_paged_evict": [ctypes.POINTER(GsPages)] + [_P] * 4 + [_I64, _I32, _I32, _I32] + [_P] * 2
+    + [_P],
 })
 
 _lib = None

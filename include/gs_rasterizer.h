@@ -774,6 +774,81 @@ int gs_attention_backward(const GsAttention *a, const void *q, const void *k, co
                           void *grad_q, void *grad_k, void *grad_v, void *workspace,
                           size_t workspace_bytes, hipStream_t stream);
 
+/* ------------------------------------------------------------ a paged cache
+ *
+ * Keys and values of sequences in pages of a pool, for attention of new tokens over
+ * all before them, where sequences grow by unknown lengths.  No counterpart in the
+ * reference.  Slot i of sequence b lies in page tables[b * table_stride +
+ * i / page_size] at place i % page_size; its key and value of head h begin at element
+ * page * page_stride + place * slot_stride + h * head_stride of k_pages and v_pages
+ * (pages by tokens or by heads, or a part of a larger pool), and its weight, a float,
+ * at page * sum_page + place * sum_slot + h * sum_head of weights.  A page number
+ * outside 0 .. pages - 1 stands for slots that are not there: nothing is read or
+ * written, no query sees them.  lengths[b] slots are filled, clamped to the table's
+ * page_size * table_width.  tables, lengths and offsets are device memory.
+ * dim is a multiple of 8 and at most GS_MAX_HEAD_DIM, type GS_F16 or GS_BF16; pools
+ * are 16-byte aligned with strides that are multiples of 8, slot_stride from dim to
+ * 2^23; a table covers less than 2^31 - 65536 slots (GS_ERR_UNSUPPORTED otherwise).
+ */
+typedef struct {
+    int64_t pages;
+    int64_t page_stride, slot_stride, head_stride; /* elements */
+    int64_t sum_page, sum_slot, sum_head;          /* elements */
+    const int32_t *tables, *lengths;
+    int64_t table_stride;
+    int32_t table_width, sequences, page_size, heads, dim, type;
+} GsPages;
+
+/*
+ * gs_paged_append: row offsets[b] + t of k and v (rows k_row and v_row apart, heads
+ *   k_head and v_head, 16-byte aligned, multiples of 8) goes to slot lengths[b] -
+ *   (offsets[b + 1] - offsets[b]) + t of sequence b, so lengths count the new slots;
+ *   their weights become 0 where weights is set.  Rows of no sequence, and rows whose
+ *   slot is below 0, past the table or on no page, go nowhere.
+ */
+int gs_paged_append(const GsPages *p, const void *k, int64_t k_row, int64_t k_head, const void *v,
+                    int64_t v_row, int64_t v_head, int64_t rows, const int32_t *offsets,
+                    void *k_pages, void *v_pages, float *weights, hipStream_t stream);
+
+/* Queries over a paged cache: sequence b has the rows offsets[b] to offsets[b + 1] of
+ * rows_q, heads_q heads each (a multiple of the cache's), row_stride and head_stride
+ * apart (multiples of 8, the first 16-byte aligned).  causal: query i of Lq sees slots
+ * j <= i + lengths[b] - Lq, else every filled slot. */
+typedef struct {
+    int64_t rows_q, row_stride, head_stride;
+    const int32_t *offsets;
+    int32_t heads_q, causal;
+    float scale;
+} GsPagedQueries;
+
+/*
+ * gs_paged_attention: out = softmax(scale q k^T) v, contiguous (rows_q, heads_q, dim);
+ *   log_sum as gs_attention_forward's.  When weights is set, every slot's weight of
+ *   head h grows by exp(scale q k^T - log_sum) summed over the sequence's queries that
+ *   see it and the query heads that read head h; then log_sum has to be set.  Queries
+ *   with a log-sum of -infinity add nothing.  Deterministic: no atomics.
+ */
+int gs_paged_attention_workspace_size(const GsPages *p, const GsPagedQueries *q, int32_t weights,
+                                      size_t *bytes);
+int gs_paged_attention(const GsPages *p, const GsPagedQueries *a, const void *q,
+                       const void *k_pages, const void *v_pages, void *out, float *log_sum,
+                       float *weights, void *workspace, size_t workspace_bytes,
+                       hipStream_t stream);
+
+/*
+ * gs_paged_evict: for every sequence and head, of the slots below lengths[b] that are
+ *   there, the last `recent` slots and those with the largest weights among the others,
+ *   `keep` in all or as many as there are (equal weights: the lower slot; NaN counts as
+ *   the largest), move in their order to slots 0, 1, ... of the pages in new_tables
+ *   (new_width >= keep / page_size entries a sequence), keys, values and weights.
+ *   kept (sequences, heads, keep) receives their slots, -1 behind the last, and
+ *   new_lengths their number.  0 <= recent <= keep.  The old pages stay as they are; a page
+ *   that the call moves to must be no sequence's old one, and one sequence's only.
+ */
+int gs_paged_evict(const GsPages *p, void *k_pages, void *v_pages, float *weights,
+                   const int32_t *new_tables, int64_t new_stride, int32_t new_width, int32_t keep,
+                   int32_t recent, int32_t *new_lengths, int32_t *kept, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
