@@ -179,7 +179,7 @@ struct Tile {
     // byte offsets and the bound in start() stay in 31 bits, below copy_of()'s mark
     static_assert(((ROWS - 1) * kMaxStride + DIM) * 2 < (1LL << 31), "offsets of a copy");
     static constexpr int kChunks = DIM / 8;                      // of a row
-    static constexpr int kBytes = ROWS * DIM * 2;
+    static constexpr int kRows = ROWS, kCopyWaves = WAVES, kBytes = ROWS * DIM * 2;
     static constexpr int kPieces = ROWS * kChunks / 64;  // of 1 KiB, which a wave copies at once
     static constexpr int kCopies = (kPieces + WAVES - 1) / WAVES;  // of a wave
     static_assert(ROWS * kChunks % 64 == 0, "whole waves of chunks");

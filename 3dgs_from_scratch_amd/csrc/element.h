@@ -16,6 +16,8 @@ __device__ __forceinline__ T from_float(float v) { return (T)v; }
 
 inline bool element_type(int32_t t) { return t == GS_F32 || t == GS_F16 || t == GS_BF16; }
 
+inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
 // Calls f with a value of the element type that `type` names.
 template <typename F>
 inline int with_element(int32_t type, F f) {

@@ -30,6 +30,4 @@ __device__ __forceinline__ int64_t sum_at(const GsPages &p, int page, int place,
 // Status of a cache's description; nothing is launched where it is not GS_OK.
 int check_pages(const GsPages *p, bool weights);
 
-inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
-
 }  // namespace gs
