@@ -135,38 +135,179 @@ __global__ __launch_bounds__(256) void paged_join_kernel(int64_t rows, int dim, 
     join_row<T>(rows, dim, partial, out, (T *)nullptr, log_sum, sums);
 }
 
-// A wave a slot and head; a lane takes every 64th of the rows that see it.
-template <typename T>
-__global__ __launch_bounds__(64) void paged_weights_kernel(GsPages p, GsPagedQueries a,
-                                                           const T *__restrict__ q,
-                                                           const T *__restrict__ k_pages,
-                                                           const float *__restrict__ log_sum,
-                                                           float *__restrict__ weights) {
-    __shared__ float key[GS_MAX_HEAD_DIM];
-    const int slot = blockIdx.x, b = blockIdx.y / p.heads, kh = blockIdx.y % p.heads;
-    const int filled = filled_slots(p, b), lane = threadIdx.x, group = a.heads_q / p.heads;
-    if (slot >= filled) return;
-    const int page = page_of(p, b, slot / p.page_size), place = slot % p.page_size;
-    if (page < 0) return;
-    const int64_t from = row_at(p, page, place) + kh * p.head_stride;
-    for (int d = lane; d < p.dim; d += 64) key[d] = to_float(k_pages[from + d]);
-    __syncthreads();
-    const int64_t first = a.offsets[b] < 0 ? 0 : a.offsets[b];
-    const int64_t end = a.offsets[b + 1] < a.rows_q ? a.offsets[b + 1] : a.rows_q;
-    // query i sees slots up to i + filled - Lq
-    const int64_t least = a.causal ? slot - filled + (end - first) : 0;
-    float sum = 0.0f;
-    for (int64_t i = (least > 0 ? least : 0) * group + lane; i < (end - first) * group; i += 64) {
-        const int64_t r = first + i / group;
-        const int head = kh * group + (int)(i % group);
-        const float l = log_sum[r * a.heads_q + head];
-        float s = 0.0f;
-        for (int d = 0; d < p.dim; ++d)
-            s = fmaf(key[d], to_float(q[r * a.row_stride + head * a.head_stride + d]), s);
-        if (l != -INFINITY) sum += expf(s * a.scale - l);
+// ---------------------------------------------------------------- slots' weights
+// S = Q K^T once more, now that a row's log-sum L is known: a lane has a slot, and adds up
+// exp2(c S - L) over the rows in its registers.  No atomics: a slot and head is one wave's.
+
+// Sum over the 16 rows of a 32x32 result that a lane holds; minus: -L of each, minus infinity for
+// rows that add nothing; sees(i): whether row i of the 32 counts for the lane's slot.
+template <bool MASKS, typename Sees>
+__device__ __forceinline__ float sum_of_weights(const f32x16 &s, float c, const float *minus, Sees sees) {
+    const int half = __lane_id() >> 5;
+    float w[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        w[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, minus[r]));
+        if (MASKS) w[r] = sees(result_row(r, half)) ? w[r] : 0.0f;
     }
-    sum = wave_sum(sum);
-    if (lane == 0) weights[sum_at(p, page, place, kh)] += sum;
+#pragma unroll
+    for (int n = 8; n > 0; n >>= 1)
+#pragma unroll
+        for (int r = 0; r < n; ++r) w[r] += w[r + n];
+    return w[0];
+}
+
+// -L in the exponent of two; a row that saw nothing adds nothing.
+__device__ __forceinline__ float minus_log(float log_sum) {
+    return log_sum == -INFINITY ? -INFINITY : -log_sum * kLog2e;
+}
+
+constexpr int kWeightSlots = 32 * kWaves;  // of a workgroup
+
+// The slots of a workgroup, and what its lanes have of them.
+template <typename T, int DIM>
+struct SlotOperand {
+    RowOperand<T, DIM> k;
+    float *weight;  // null: no such slot
+    __device__ __forceinline__ SlotOperand(const GsPages &p, const T *keys, float *weights, int sequence,
+                                           int slot, int filled, int kh, bool negate)
+        : weight(nullptr) {
+        const T *row = nullptr;
+        if (slot < filled) {
+            const int index = slot / p.page_size, place = slot - index * p.page_size;
+            const int page = page_of(p, sequence - 1, index);
+            if (page >= 0) {
+                row = keys + row_at(p, page, place) + kh * p.head_stride;
+                weight = weights + sum_at(p, page, place, kh);
+            }
+        }
+        k.load(row, p.dim, negate);
+    }
+};
+
+// f(sequence, tile, key head) for the tiles of slots of all sequences that have queries.
+template <typename F>
+__device__ __forceinline__ void for_slot_tiles(const GsAttention &a, const GsPages &p, F f) {
+    const auto count = [&](int s) {
+        const int2 q = rows_of(a.offsets_q, a.sequences, a.rows_q, s);
+        return q.x == q.y ? 0 : (slots_of(p, s) + kWeightSlots - 1) / kWeightSlots * a.heads_k;
+    };
+    int sequence, place;
+    for (int item = blockIdx.x; find_place(a.sequences + 2, count, item, false, &sequence, &place);
+         item += gridDim.x)
+        f(sequence, place / a.heads_k, place % a.heads_k);
+}
+
+// Many rows: tiles of a head's queries go through LDS, which the workgroup's waves share.
+template <typename T, int DIM>
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
+    GsAttention a, GsPages p, const T *__restrict__ q, const T *__restrict__ k,
+    const float *__restrict__ log_sum, float *__restrict__ weights) {
+    constexpr int kRows = 64;
+    using QTile = Tile<T, DIM, kRows, kWaves>;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * QTile::kBytes];
+    __shared__ __attribute__((aligned(16))) float minus[2][kRows];
+    const int group = a.heads_q / a.heads_k, lane = __lane_id(), half = lane >> 5;
+    const int wave = uniform(threadIdx.x / kWave);
+    const float c = exponent_factor(a.scale);
+    const auto copy = QTile::copy_of(wave, a.q_row, a.dim);
+    for_slot_tiles(a, p, [&](int sequence, int tile, int kh) {
+        const int2 rows = rows_of(a.offsets_q, a.sequences, a.rows_q, sequence);
+        const int q0 = uniform(rows.x), lq = uniform(rows.y - rows.x);
+        const int filled = uniform(slots_of(p, sequence));
+        const int slot0 = tile * kWeightSlots + 32 * wave, slot = slot0 + (lane & 31);
+        const SlotOperand<T, DIM> mine(p, k, weights, sequence, slot, filled, kh, a.scale < 0.0f);
+        // query i sees slots up to i + shift
+        const int shift = a.causal ? filled - lq : filled;
+        const int first = max(tile * kWeightSlots - shift, 0) / kRows;
+        const int tiles = (lq + kRows - 1) / kRows - first, steps = tiles * group;
+        int head = kh * group, at = first;  // of the tile that is fetched next
+        float next = 0.0f;                  // its rows' -L, a lane each
+        const auto fetch = [&](int buffer) {
+            const int rows = lq - at * kRows;
+            const int64_t row = q0 + at * kRows;
+            QTile::start(copy, wave, q + row * a.q_row + head * a.q_head, a.q_row, rows, a.dim,
+                         (lds_char *)lds + buffer * QTile::kBytes);
+            if (wave == 0)
+                next = lane < rows ? minus_log(log_sum[(row + lane) * a.heads_q + head]) : -INFINITY;
+            if (++at == first + tiles) at = first, ++head;
+        };
+        float sum = 0.0f;
+        int now = first;
+        if (steps > 0) {
+            fetch(0);
+            if (wave == 0) minus[0][lane] = next;
+        }
+        for (int t = 0; t < steps; ++t) {
+            copies_done();
+            if (t + 1 < steps) fetch((t + 1) & 1);
+            const lds_char *qt = (const lds_char *)lds + (t & 1) * QTile::kBytes;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int row0 = now * kRows + 32 * n;
+                f32x16 s = {};
+#pragma unroll
+                for (int i = 0; i < DIM / 16; ++i) s = mfma(QTile::along(qt, 32 * n, i), mine.k.x[i], s);
+                float m[16];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 x = *(const f32x4 *)&minus[t & 1][32 * n + result_row(4 * g, half)];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m[4 * g + i] = x[i];
+                }
+                if (row0 + shift >= slot0 + 31 && row0 + 32 <= lq)
+                    sum += sum_of_weights<false>(s, c, m, [](int) { return true; });
+                else
+                    sum += sum_of_weights<true>(
+                        s, c, m, [&](int i) { return row0 + i < lq && row0 + i + shift >= slot; });
+            }
+            if (++now == first + tiles) now = first;
+            if (wave == 0 && t + 1 < steps) minus[(t + 1) & 1][lane] = next;
+        }
+        sum = half_sum(sum);
+        if (half == 0 && mine.weight) *mine.weight += sum;
+        __syncthreads();  // LDS has been read
+    });
+}
+
+// Few rows: a wave takes them from memory.
+template <typename T, int DIM>
+__global__ __launch_bounds__(64 * kWaves) void paged_few_weights_kernel(
+    GsAttention a, GsPages p, const T *__restrict__ q, const T *__restrict__ k,
+    const float *__restrict__ log_sum, float *__restrict__ weights) {
+    const int group = a.heads_q / a.heads_k, lane = __lane_id(), half = lane >> 5;
+    const int wave = uniform(threadIdx.x / kWave);
+    const float c = exponent_factor(a.scale);
+    for_slot_tiles(a, p, [&](int sequence, int tile, int kh) {
+        const int2 range = rows_of(a.offsets_q, a.sequences, a.rows_q, sequence);
+        const int q0 = uniform(range.x), lq = uniform(range.y - range.x), rows = lq * group;
+        const int filled = uniform(slots_of(p, sequence));
+        const int slot0 = tile * kWeightSlots + 32 * wave, slot = slot0 + (lane & 31);
+        if (slot0 >= filled) return;
+        const SlotOperand<T, DIM> mine(p, k, weights, sequence, slot, filled, kh, a.scale < 0.0f);
+        const int shift = a.causal ? filled - lq : filled;
+        float sum = 0.0f;
+        for (int row0 = max(slot0 - shift, 0) * group / 32 * 32; row0 < rows; row0 += 32) {
+            const int row = row0 + (lane & 31);
+            const bool real = row < rows;
+            const int query = row / group, head = kh * group + row - query * group;
+            RowOperand<T, DIM> x;
+            x.load(real ? q + (int64_t)(q0 + query) * a.q_row + (int64_t)head * a.q_head : nullptr, a.dim,
+                   false);
+            const float l = real ? minus_log(log_sum[(int64_t)(q0 + query) * a.heads_q + head]) : -INFINITY;
+            f32x16 s = {};
+#pragma unroll
+            for (int i = 0; i < DIM / 16; ++i) s = mfma(x.x[i], mine.k.x[i], s);
+            float m[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) m[r] = __shfl(l, result_row(r, half), kWave);
+            // the first row that sees the lane's slot
+            const int least = max(slot - shift, 0) * group - row0;
+            sum += sum_of_weights<true>(s, c, m, [&](int i) { return i >= least && row0 + i < rows; });
+        }
+        sum = half_sum(sum);
+        if (half == 0 && mine.weight) *mine.weight += sum;
+    });
 }
 
 static int check_queries(const GsPages *p, const GsPagedQueries *a) {
@@ -264,10 +405,16 @@ extern "C" int gs_paged_attention(const GsPages *p, const GsPagedQueries *querie
                           : launch<T, kDim, false>(*p, a, f, tq, tk, tv, (T *)out, log_sum, partial, stream);
         if (s) return s;
         const int64_t slots = (int64_t)p->page_size * p->table_width;
-        if (weights && slots > 0 && p->sequences > 0)
-            hipLaunchKernelGGL((paged_weights_kernel<T>),
-                               dim3((unsigned)slots, (unsigned)(p->sequences * p->heads)), dim3(64),
-                               0, stream, *p, *queries, tq, tk, (const float *)log_sum, weights);
+        int64_t groups = (slots + kWeightSlots - 1) / kWeightSlots * p->sequences * p->heads;
+        if (!weights || groups == 0) return s;
+        // (a workgroup takes every 8192nd tile: tables may be much wider than what is filled)
+        if (groups > 8192) groups = 8192;
+        if (f.by_keys)
+            hipLaunchKernelGGL((paged_few_weights_kernel<T, kDim>), dim3((unsigned)groups),
+                               dim3(64 * kWaves), 0, stream, a, *p, tq, tk, (const float *)log_sum, weights);
+        else
+            hipLaunchKernelGGL((paged_weights_kernel<T, kDim>), dim3((unsigned)groups), dim3(64 * kWaves),
+                               0, stream, a, *p, tq, tk, (const float *)log_sum, weights);
         return launch_status();
     };
     return p->type == GS_F16 ? with_tile(p->dim, [&](auto d) { return all(f16{}, d); })
