@@ -65,7 +65,6 @@ __device__ __forceinline__ constexpr int result_row(int r, int h) {
     return (r & 3) + 8 * (r >> 2) + 4 * h;
 }
 
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // ---------------------------------------------------------------- sequences
 // Sequence s = 1 .. sequences; 0 and sequences + 1 hold the rows before the first

@@ -28,6 +28,9 @@ inline int with_element(int32_t type, F f) {
     }
 }
 
+// A value that is the same in every lane, known to the compiler as such.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // v of the lane that differs in the bits of a pattern, within 16 lanes.
 template <int PATTERN>
 __device__ __forceinline__ float dpp(float v) {

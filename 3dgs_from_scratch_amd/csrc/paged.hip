@@ -54,80 +54,173 @@ __device__ __forceinline__ uint32_t order_of(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kPick = 1024;  // threads
+constexpr int kPick = 1024, kPickWaves = kPick / kWave;
+constexpr int kDigit = 11, kBins = 1 << kDigit;
+constexpr int kHeld = 32 * kPick;  // slots whose orders fit in LDS
 
-// Which slots stay: a workgroup a sequence and head.  The smallest order that stays is found
-// by its bytes, from the highest, with a histogram of the slots that agree so far; then the
-// slots are walked in order.
+struct PickShared {
+    uint32_t histogram[kBins];
+    uint32_t waves[2][kPickWaves];  // counts of each wave
+    uint32_t found[3];
+};
+
+// Sums over the waves before this one, or all, of a count that each wave has left.
+__device__ __forceinline__ uint32_t sum_of_waves(const uint32_t *counts, int before) {
+    uint32_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < kPickWaves; ++w) sum += w < before ? counts[w] : 0;
+    return sum;
+}
+
+// Which slots of a sequence and head stay: a workgroup, each wave a stretch of slots that follow
+// one another, 64 at a time.  HELD: the slots' orders stay in LDS, else they are read again for
+// every pass.  The smallest order that stays is found by its digits from the highest, with a
+// histogram of the slots that agree so far; then each wave counts what it keeps, and writes it
+// behind what the waves before it keep.
+template <bool HELD>
+__device__ __forceinline__ void pick(const GsPages &p, const float *weights, int b, int head, int filled,
+                                     int32_t keep, int32_t recent, int32_t *new_lengths, int32_t *out,
+                                     PickShared &shared, uint32_t *orders) {
+    const int t = threadIdx.x, lane = t % kWave, wave = uniform(t / kWave);
+    const int old = max(filled - recent, 0);
+    const int rounds = (filled + kPick - 1) / kPick;   // of a wave
+    const int first = wave * rounds * kWave + lane;    // the lane's first slot
+    const int more_pages = kWave / p.page_size, more_places = kWave - more_pages * p.page_size;
+    // f(slot, order) for the lane's slots in turn; the order of a slot that is not there is 0, which
+    // no weight has.  Pages and weights of BATCH slots are on their way at a time.
+    const auto from_memory = [&](auto f) {
+        constexpr int BATCH = 16;
+        int index = first / p.page_size, place = first - index * p.page_size;
+        for (int i0 = 0; i0 < rounds; i0 += BATCH) {
+            int pages[BATCH], places[BATCH];
+            float w[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const bool is = i0 + i < rounds && first + (i0 + i) * kWave < filled;
+                pages[i] = is ? page_of(p, b, index) : -1;
+                places[i] = place;
+                index += more_pages;
+                place += more_places;
+                if (place >= p.page_size) place -= p.page_size, ++index;
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i)
+                w[i] = pages[i] >= 0 ? weights[sum_at(p, pages[i], places[i], head)] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i)
+                if (i0 + i < rounds)
+                    f(first + (i0 + i) * kWave, pages[i] >= 0 ? order_of(w[i]) : 0u);
+        }
+    };
+    const auto each = [&](auto f) {
+        if constexpr (HELD) {
+            for (int slot = first, i = 0; i < rounds; ++i, slot += kWave) f(slot, orders[slot]);
+        } else {
+            from_memory(f);
+        }
+    };
+    const auto add_to_bin = [&](bool counts, uint32_t bin) {
+        // (many weights are alike, such as zeros: one addition for a wave of them)
+        const uint64_t some = __ballot(counts);
+        if (!some) return;
+        const int leader = __builtin_ctzll(some);
+        const uint64_t alike = __ballot(counts && bin == (uint32_t)__builtin_amdgcn_readlane((int)bin, leader));
+        if (lane == leader) atomicAdd(&shared.histogram[bin], (uint32_t)__popcll(alike));
+        if (counts && !(alike >> lane & 1)) atomicAdd(&shared.histogram[bin], 1u);
+    };
+    // orders, how many there are, and the histogram of the highest digit
+    for (int i = t; i < kBins; i += kPick) shared.histogram[i] = 0;
+    __syncthreads();
+    uint32_t there = 0, there_old = 0;
+    from_memory([&](int slot, uint32_t order) {
+        if (HELD) orders[slot] = order;
+        const bool counts = order && slot < old;
+        there += __popcll(__ballot(order != 0));
+        there_old += __popcll(__ballot(counts));
+        add_to_bin(counts, order >> (32 - kDigit));
+    });
+    if (lane == 0) shared.waves[0][wave] = there, shared.waves[1][wave] = there_old;
+    __syncthreads();
+    const uint32_t all = sum_of_waves(shared.waves[0], kPickWaves);
+    const uint32_t all_old = sum_of_waves(shared.waves[1], kPickWaves);
+    __syncthreads();
+    // `want` of the old slots stay: those whose digits under the mask are above the threshold's, and
+    // the first `need` with the threshold's
+    const uint32_t want = min((uint32_t)keep - (all - all_old), all_old);
+    uint32_t threshold = 0, mask = 0, need = want;
+    if (want > 0 && want < all_old) {
+        for (int shift = 32 - kDigit, digit = kDigit;;) {
+            // bins from the largest down, two a thread: the one in which the count passes need
+            const int bin = kBins - 1 - 2 * t;
+            const uint32_t one = shared.histogram[bin], two = shared.histogram[bin - 1];
+            shared.histogram[bin] = shared.histogram[bin - 1] = 0;
+            const uint32_t upto = wave_inclusive_scan(one + two);
+            if (lane == kWave - 1) shared.waves[0][wave] = upto;
+            __syncthreads();
+            const uint32_t before = upto - one - two + sum_of_waves(shared.waves[0], wave);
+            if (before < need && need <= before + one + two) {
+                const bool second = need > before + one;
+                shared.found[0] = second ? bin - 1 : bin;
+                shared.found[1] = need - before - (second ? one : 0);
+                shared.found[2] = second ? two : one;
+            }
+            __syncthreads();
+            threshold |= shared.found[0] << shift;
+            mask |= ((1u << digit) - 1) << shift;
+            need = shared.found[1];
+            // (done too where all with these digits stay)
+            if (shift == 0 || need == shared.found[2]) break;
+            digit = min(shift, kDigit);
+            shift -= digit;
+            each([&](int slot, uint32_t order) {
+                add_to_bin(order && slot < old && (order & mask) == threshold,
+                           order >> shift & ((1u << digit) - 1));
+            });
+            __syncthreads();
+        }
+    }
+    const auto certain = [&](int slot, uint32_t order) {
+        return order && (slot >= old || (order & mask) > threshold);
+    };
+    const auto same = [&](int slot, uint32_t order) {
+        return order && slot < old && (order & mask) == threshold;
+    };
+    uint32_t sure = 0, equal = 0;
+    each([&](int slot, uint32_t order) {
+        sure += __popcll(__ballot(certain(slot, order)));
+        equal += __popcll(__ballot(same(slot, order)));
+    });
+    __syncthreads();
+    if (lane == 0) shared.waves[0][wave] = sure, shared.waves[1][wave] = equal;
+    __syncthreads();
+    uint32_t equals = sum_of_waves(shared.waves[1], wave);
+    uint32_t written = sum_of_waves(shared.waves[0], wave) + min(equals, need);
+    each([&](int slot, uint32_t order) {
+        const uint64_t alike = __ballot(same(slot, order));
+        const bool stays = certain(slot, order) ||
+                           ((alike >> lane & 1) && equals + __popcll(alike & lanemask_lt()) < need);
+        const uint64_t stay = __ballot(stays);
+        const uint32_t to = written + __popcll(stay & lanemask_lt());
+        if (stays && to < (uint32_t)keep) out[to] = slot;
+        equals += __popcll(alike);
+        written += __popcll(stay);
+    });
+    const uint32_t stayed = all - all_old + want;
+    for (int j = stayed + t; j < keep; j += kPick) out[j] = -1;
+    if (head == 0 && t == 0) new_lengths[b] = (int32_t)stayed;
+}
+
+template <bool HELD>
 __global__ __launch_bounds__(kPick) void paged_pick_kernel(GsPages p,
                                                            const float *__restrict__ weights,
                                                            int32_t keep, int32_t recent,
                                                            int32_t *__restrict__ new_lengths,
                                                            int32_t *__restrict__ kept) {
-    __shared__ uint32_t histogram[256];
-    __shared__ uint32_t scan[kPick / kWave + 1];
-    __shared__ uint32_t found[2];
-    const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads, t = threadIdx.x;
-    const int filled = filled_slots(p, b), old = max(filled - recent, 0);
-    int32_t *out = kept + (int64_t)blockIdx.x * keep;
-    const auto sum_of = [&](int slot, uint32_t *order) {  // false: the slot is not there
-        const int index = slot / p.page_size, page = page_of(p, b, index);
-        if (page < 0) return false;
-        *order = order_of(weights[sum_at(p, page, slot - index * p.page_size, head)]);
-        return true;
-    };
-    // slots that are there: recent ones and others
-    uint32_t there = 0, there_old = 0, order;
-    for (int slot = t; slot < filled; slot += kPick)
-        if (sum_of(slot, &order)) {
-            ++there;
-            there_old += slot < old;
-        }
-    uint32_t all, all_old;
-    block_exclusive_scan<uint32_t, kPick>(there, scan, all);
-    block_exclusive_scan<uint32_t, kPick>(there_old, scan, all_old);
-    // the old slots that stay: `want` of all_old
-    const uint32_t want = min((uint32_t)keep - (all - all_old), all_old);
-    uint32_t threshold = 0, need = want;  // those above it stay, and the first `need` equal to it
-    if (want > 0 && want < all_old) {
-        uint32_t mask = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (t < 256) histogram[t] = 0;
-            __syncthreads();
-            for (int slot = t; slot < old; slot += kPick)
-                if (sum_of(slot, &order) && (order & mask) == threshold)
-                    atomicAdd(&histogram[order >> shift & 255], 1u);
-            __syncthreads();
-            if (t == 0) {
-                uint32_t above = 0;
-                int byte = 255;
-                while (above + histogram[byte] < need) above += histogram[byte--];
-                found[0] = byte;
-                found[1] = need - above;
-            }
-            __syncthreads();
-            threshold |= found[0] << shift;
-            need = found[1];
-            mask |= 255u << shift;
-            __syncthreads();
-        }
-    }
-    const bool none = want == 0, every = want == all_old;
-    uint32_t written = 0, equal = 0;
-    for (int first = 0; first < filled; first += kPick) {
-        const int slot = first + t;
-        const bool is = slot < filled && sum_of(slot, &order), late = slot >= old;
-        const bool same = is && !late && !none && !every && order == threshold;
-        uint32_t total;
-        const uint32_t before = equal + block_exclusive_scan<uint32_t, kPick>(same, scan, total);
-        equal += total;
-        const bool stays = is && (late || every || (!none && (order > threshold || (same && before < need))));
-        const uint32_t to = written + block_exclusive_scan<uint32_t, kPick>(stays, scan, total);
-        written += total;
-        if (stays && to < (uint32_t)keep) out[to] = slot;
-    }
-    for (int j = written + t; j < keep; j += kPick) out[j] = -1;
-    if (head == 0 && t == 0) new_lengths[b] = (int32_t)written;
+    __shared__ PickShared shared;
+    extern __shared__ uint32_t orders[];
+    const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
+    pick<HELD>(p, weights, b, head, filled_slots(p, b), keep, recent, new_lengths,
+               kept + (int64_t)blockIdx.x * keep, shared, orders);
 }
 
 // The picked slots to the new pages: a thread moves 8 elements of a key and a value.
@@ -210,12 +303,21 @@ extern "C" int gs_paged_evict(const GsPages *p, void *k_pages, void *v_pages, fl
     if (!new_tables || !new_lengths || !kept || (p->pages > 0 && (!k_pages || !v_pages || !weights)))
         return GS_ERR_INVALID_ARGUMENT;
     if (!aligned16(k_pages) || !aligned16(v_pages)) return GS_ERR_UNSUPPORTED;
-    const int64_t pick = (int64_t)p->sequences * p->heads;
+    const int64_t picks = (int64_t)p->sequences * p->heads;
     const int64_t groups = ((int64_t)keep * (p->dim / 8) * p->heads + 255) / 256;
-    if (pick > 0x7fffffffLL || groups > 0x7fffffffLL || p->sequences > 65535)
+    if (picks > 0x7fffffffLL || groups > 0x7fffffffLL || p->sequences > 65535)
         return GS_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL(paged_pick_kernel, dim3((unsigned)pick), dim3(kPick), 0, stream, *p,
-                       (const float *)weights, keep, recent, new_lengths, kept);
+    // (by the slots that a table could hold: what is filled is not known here)
+    const int64_t slots = (int64_t)p->page_size * p->table_width;
+    if (slots <= kHeld) {
+        // every wave's stretch is whole
+        const unsigned lds = (unsigned)((slots + kPick - 1) / kPick * kPick * sizeof(uint32_t));
+        hipLaunchKernelGGL(paged_pick_kernel<true>, dim3((unsigned)picks), dim3(kPick), lds, stream, *p,
+                           (const float *)weights, keep, recent, new_lengths, kept);
+    } else {
+        hipLaunchKernelGGL(paged_pick_kernel<false>, dim3((unsigned)picks), dim3(kPick), 0, stream, *p,
+                           (const float *)weights, keep, recent, new_lengths, kept);
+    }
     hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)groups, (unsigned)p->sequences), dim3(256),
                        0, stream, *p, (uint16_t *)k_pages, (uint16_t *)v_pages, weights, new_tables,
                        new_stride, keep, (const int32_t *)kept);

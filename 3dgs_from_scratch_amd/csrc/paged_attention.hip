@@ -405,9 +405,12 @@ extern "C" int gs_paged_attention(const GsPages *p, const GsPagedQueries *querie
                           : launch<T, kDim, false>(*p, a, f, tq, tk, tv, (T *)out, log_sum, partial, stream);
         if (s) return s;
         const int64_t slots = (int64_t)p->page_size * p->table_width;
-        int64_t groups = (slots + kWeightSlots - 1) / kWeightSlots * p->sequences * p->heads;
+        // as many workgroups as there are tiles if no page is in two tables; the workgroups go on
+        // while there are more
+        const int64_t tiles = (slots + kWeightSlots - 1) / kWeightSlots * p->sequences;
+        const int64_t pool = p->pages * p->page_size / kWeightSlots + p->sequences;
+        int64_t groups = (tiles < pool ? tiles : pool) * p->heads;
         if (!weights || groups == 0) return s;
-        // (a workgroup takes every 8192nd tile: tables may be much wider than what is filled)
         if (groups > 8192) groups = 8192;
         if (f.by_keys)
             hipLaunchKernelGGL((paged_few_weights_kernel<T, kDim>), dim3((unsigned)groups),
