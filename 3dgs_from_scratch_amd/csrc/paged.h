@@ -19,12 +19,17 @@ __device__ __forceinline__ int filled_slots(const GsPages &p, int sequence) {
     return n < 0 ? 0 : n < most ? n : (int)most;
 }
 
+// a b in 64 bits, by one multiplication: the strides of a pool fit in 31 bits.
+__device__ __forceinline__ int64_t times(int a, int64_t b) {
+    return (int64_t)((uint64_t)(uint32_t)a * (uint32_t)b);
+}
+
 // First element of a slot's key or value of head 0, and its weight's.
 __device__ __forceinline__ int64_t row_at(const GsPages &p, int page, int place) {
-    return page * p.page_stride + place * p.slot_stride;
+    return times(page, p.page_stride) + times(place, p.slot_stride);
 }
 __device__ __forceinline__ int64_t sum_at(const GsPages &p, int page, int place, int head) {
-    return page * p.sum_page + place * p.sum_slot + head * p.sum_head;
+    return times(page, p.sum_page) + times(place, p.sum_slot) + times(head, p.sum_head);
 }
 
 // Status of a cache's description; nothing is launched where it is not GS_OK.

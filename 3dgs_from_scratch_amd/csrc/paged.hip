@@ -57,6 +57,24 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 constexpr int kPick = 1024, kPickWaves = kPick / kWave;
 constexpr int kDigit = 11, kBins = 1 << kDigit;
 constexpr int kHeld = 32 * kPick;  // slots whose orders fit in LDS
+constexpr int kUnroll = 4;
+
+// Of 64 slots, for each of the waves, to cover so many.
+__host__ __device__ __forceinline__ int rounds_of(int64_t slots) {
+    return (int)((slots + kUnroll * kPick - 1) / (kUnroll * kPick)) * kUnroll;
+}
+
+// Sum over the lanes up to this one.
+__device__ __forceinline__ uint32_t lanes_sum_upto(uint32_t v) {
+    int x = (int)v;
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // a lane to the right within 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // 16 to the next 16, 32 to the rest
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return (uint32_t)x;
+}
 
 struct PickShared {
     uint32_t histogram[kBins];
@@ -72,61 +90,88 @@ __device__ __forceinline__ uint32_t sum_of_waves(const uint32_t *counts, int bef
     return sum;
 }
 
+// How many of the lanes before this one are in a mask.
+__device__ __forceinline__ uint32_t lanes_before(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
 // Which slots of a sequence and head stay: a workgroup, each wave a stretch of slots that follow
 // one another, 64 at a time.  HELD: the slots' orders stay in LDS, else they are read again for
 // every pass.  The smallest order that stays is found by its digits from the highest, with a
 // histogram of the slots that agree so far; then each wave counts what it keeps, and writes it
 // behind what the waves before it keep.
-template <bool HELD>
+template <bool HELD, bool WHOLE>
 __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int b, int head, int filled,
                                      int32_t keep, int32_t recent, int32_t *new_lengths, int32_t *out,
                                      PickShared &shared, uint32_t *orders) {
     const int t = threadIdx.x, lane = t % kWave, wave = uniform(t / kWave);
     const int old = max(filled - recent, 0);
-    const int rounds = (filled + kPick - 1) / kPick;   // of a wave
-    const int first = wave * rounds * kWave + lane;    // the lane's first slot
+    const int rounds = rounds_of(filled);            // of a wave
+    const int first = wave * rounds * kWave + lane;  // the lane's first slot
     const int more_pages = kWave / p.page_size, more_places = kWave - more_pages * p.page_size;
     // f(slot, order) for the lane's slots in turn; the order of a slot that is not there is 0, which
     // no weight has.  Pages and weights of BATCH slots are on their way at a time.
     const auto from_memory = [&](auto f) {
         constexpr int BATCH = 16;
-        int index = first / p.page_size, place = first - index * p.page_size;
-        for (int i0 = 0; i0 < rounds; i0 += BATCH) {
-            int pages[BATCH], places[BATCH];
-            float w[BATCH];
+        if constexpr (WHOLE) {
+            // a lane looks for the page of a round's 64 slots
+            for (int i0 = 0; i0 < rounds; i0 += kWave) {
+                const int begin = (wave * rounds + i0 + lane) * kWave, index = begin / p.page_size;
+                const bool is = i0 + lane < rounds && begin < filled;
+                const int mine = is ? page_of(p, b, index) : -1, place = begin - index * p.page_size;
+                const float *line = weights + lane * p.sum_slot;
+                for (int j0 = 0; j0 < kWave && i0 + j0 < rounds; j0 += BATCH) {
+                    float w[BATCH];
+                    bool has[BATCH];
 #pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-                const bool is = i0 + i < rounds && first + (i0 + i) * kWave < filled;
-                pages[i] = is ? page_of(p, b, index) : -1;
-                places[i] = place;
-                index += more_pages;
-                place += more_places;
-                if (place >= p.page_size) place -= p.page_size, ++index;
+                    for (int j = 0; j < BATCH; ++j) {
+                        const int page = __builtin_amdgcn_readlane(mine, j0 + j);
+                        has[j] = page >= 0 && first + (i0 + j0 + j) * kWave < filled;
+                        const int64_t at = sum_at(p, page, __builtin_amdgcn_readlane(place, j0 + j), head);
+                        w[j] = has[j] ? line[at] : 0.0f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < BATCH; ++j)
+                        if (i0 + j0 + j < rounds)
+                            f(first + (i0 + j0 + j) * kWave, has[j] ? order_of(w[j]) : 0u);
+                }
             }
+        } else {
+            int index = first / p.page_size, place = first - index * p.page_size;
+            for (int i0 = 0; i0 < rounds; i0 += BATCH) {
+                int pages[BATCH], places[BATCH];
+                float w[BATCH];
 #pragma unroll
-            for (int i = 0; i < BATCH; ++i)
-                w[i] = pages[i] >= 0 ? weights[sum_at(p, pages[i], places[i], head)] : 0.0f;
+                for (int i = 0; i < BATCH; ++i) {
+                    const bool is = i0 + i < rounds && first + (i0 + i) * kWave < filled;
+                    pages[i] = is ? page_of(p, b, index) : -1;
+                    places[i] = place;
+                    index += more_pages;
+                    place += more_places;
+                    if (place >= p.page_size) place -= p.page_size, ++index;
+                }
 #pragma unroll
-            for (int i = 0; i < BATCH; ++i)
-                if (i0 + i < rounds)
-                    f(first + (i0 + i) * kWave, pages[i] >= 0 ? order_of(w[i]) : 0u);
+                for (int i = 0; i < BATCH; ++i)
+                    w[i] = pages[i] >= 0 ? weights[sum_at(p, pages[i], places[i], head)] : 0.0f;
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i)
+                    if (i0 + i < rounds)
+                        f(first + (i0 + i) * kWave, pages[i] >= 0 ? order_of(w[i]) : 0u);
+            }
         }
     };
     const auto each = [&](auto f) {
         if constexpr (HELD) {
-            for (int slot = first, i = 0; i < rounds; ++i, slot += kWave) f(slot, orders[slot]);
+            for (int slot = first, i = 0; i < rounds; i += kUnroll, slot += kUnroll * kWave) {
+                uint32_t some[kUnroll];
+#pragma unroll
+                for (int n = 0; n < kUnroll; ++n) some[n] = orders[slot + n * kWave];
+#pragma unroll
+                for (int n = 0; n < kUnroll; ++n) f(slot + n * kWave, some[n]);
+            }
         } else {
             from_memory(f);
         }
-    };
-    const auto add_to_bin = [&](bool counts, uint32_t bin) {
-        // (many weights are alike, such as zeros: one addition for a wave of them)
-        const uint64_t some = __ballot(counts);
-        if (!some) return;
-        const int leader = __builtin_ctzll(some);
-        const uint64_t alike = __ballot(counts && bin == (uint32_t)__builtin_amdgcn_readlane((int)bin, leader));
-        if (lane == leader) atomicAdd(&shared.histogram[bin], (uint32_t)__popcll(alike));
-        if (counts && !(alike >> lane & 1)) atomicAdd(&shared.histogram[bin], 1u);
     };
     // orders, how many there are, and the histogram of the highest digit
     for (int i = t; i < kBins; i += kPick) shared.histogram[i] = 0;
@@ -137,7 +182,7 @@ __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int
         const bool counts = order && slot < old;
         there += __popcll(__ballot(order != 0));
         there_old += __popcll(__ballot(counts));
-        add_to_bin(counts, order >> (32 - kDigit));
+        if (counts) atomicAdd(&shared.histogram[order >> (32 - kDigit)], 1u);
     });
     if (lane == 0) shared.waves[0][wave] = there, shared.waves[1][wave] = there_old;
     __syncthreads();
@@ -154,7 +199,7 @@ __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int
             const int bin = kBins - 1 - 2 * t;
             const uint32_t one = shared.histogram[bin], two = shared.histogram[bin - 1];
             shared.histogram[bin] = shared.histogram[bin - 1] = 0;
-            const uint32_t upto = wave_inclusive_scan(one + two);
+            const uint32_t upto = lanes_sum_upto(one + two);
             if (lane == kWave - 1) shared.waves[0][wave] = upto;
             __syncthreads();
             const uint32_t before = upto - one - two + sum_of_waves(shared.waves[0], wave);
@@ -173,8 +218,8 @@ __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int
             digit = min(shift, kDigit);
             shift -= digit;
             each([&](int slot, uint32_t order) {
-                add_to_bin(order && slot < old && (order & mask) == threshold,
-                           order >> shift & ((1u << digit) - 1));
+                if (order && slot < old && (order & mask) == threshold)
+                    atomicAdd(&shared.histogram[order >> shift & ((1u << digit) - 1)], 1u);
             });
             __syncthreads();
         }
@@ -196,13 +241,15 @@ __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int
     uint32_t equals = sum_of_waves(shared.waves[1], wave);
     uint32_t written = sum_of_waves(shared.waves[0], wave) + min(equals, need);
     each([&](int slot, uint32_t order) {
+        bool stays = certain(slot, order);
         const uint64_t alike = __ballot(same(slot, order));
-        const bool stays = certain(slot, order) ||
-                           ((alike >> lane & 1) && equals + __popcll(alike & lanemask_lt()) < need);
+        if (alike) {
+            stays = stays || ((alike >> lane & 1) && equals + lanes_before(alike) < need);
+            equals += __popcll(alike);
+        }
         const uint64_t stay = __ballot(stays);
-        const uint32_t to = written + __popcll(stay & lanemask_lt());
+        const uint32_t to = written + lanes_before(stay);
         if (stays && to < (uint32_t)keep) out[to] = slot;
-        equals += __popcll(alike);
         written += __popcll(stay);
     });
     const uint32_t stayed = all - all_old + want;
@@ -210,7 +257,7 @@ __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int
     if (head == 0 && t == 0) new_lengths[b] = (int32_t)stayed;
 }
 
-template <bool HELD>
+template <bool HELD, bool WHOLE>
 __global__ __launch_bounds__(kPick) void paged_pick_kernel(GsPages p,
                                                            const float *__restrict__ weights,
                                                            int32_t keep, int32_t recent,
@@ -219,7 +266,7 @@ __global__ __launch_bounds__(kPick) void paged_pick_kernel(GsPages p,
     __shared__ PickShared shared;
     extern __shared__ uint32_t orders[];
     const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
-    pick<HELD>(p, weights, b, head, filled_slots(p, b), keep, recent, new_lengths,
+    pick<HELD, WHOLE>(p, weights, b, head, filled_slots(p, b), keep, recent, new_lengths,
                kept + (int64_t)blockIdx.x * keep, shared, orders);
 }
 
@@ -257,6 +304,10 @@ int check_pages(const GsPages *p, bool weights) {
         return GS_ERR_INVALID_ARGUMENT;
     if (p->sequences > 0 && (!p->lengths || (p->table_width > 0 && !p->tables)))
         return GS_ERR_INVALID_ARGUMENT;
+    constexpr int64_t most = 0x7fffffff;
+    if (p->page_stride > most || p->head_stride > most ||
+        (weights && (p->sum_page > most || p->sum_slot > most || p->sum_head > most)))
+        return GS_ERR_UNSUPPORTED;
     if (p->type == GS_F32 || p->dim % 8 != 0 || p->dim > GS_MAX_HEAD_DIM ||
         p->pages > 0x7fffffffLL || (int64_t)p->page_size * p->table_width > kMaxSlots ||
         p->slot_stride < p->dim || p->slot_stride > (1 << 23) ||
@@ -309,15 +360,12 @@ extern "C" int gs_paged_evict(const GsPages *p, void *k_pages, void *v_pages, fl
         return GS_ERR_UNSUPPORTED;
     // (by the slots that a table could hold: what is filled is not known here)
     const int64_t slots = (int64_t)p->page_size * p->table_width;
-    if (slots <= kHeld) {
-        // every wave's stretch is whole
-        const unsigned lds = (unsigned)((slots + kPick - 1) / kPick * kPick * sizeof(uint32_t));
-        hipLaunchKernelGGL(paged_pick_kernel<true>, dim3((unsigned)picks), dim3(kPick), lds, stream, *p,
-                           (const float *)weights, keep, recent, new_lengths, kept);
-    } else {
-        hipLaunchKernelGGL(paged_pick_kernel<false>, dim3((unsigned)picks), dim3(kPick), 0, stream, *p,
-                           (const float *)weights, keep, recent, new_lengths, kept);
-    }
+    const bool held = slots <= kHeld, whole = p->page_size % kWave == 0;
+    const unsigned lds = held ? (unsigned)(rounds_of(slots) * kPick * sizeof(uint32_t)) : 0;
+    const auto kernel = held ? whole ? paged_pick_kernel<true, true> : paged_pick_kernel<true, false>
+                             : whole ? paged_pick_kernel<false, true> : paged_pick_kernel<false, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)picks), dim3(kPick), lds, stream, *p,
+                       (const float *)weights, keep, recent, new_lengths, kept);
     hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)groups, (unsigned)p->sequences), dim3(256),
                        0, stream, *p, (uint16_t *)k_pages, (uint16_t *)v_pages, weights, new_tables,
                        new_stride, keep, (const int32_t *)kept);

@@ -97,11 +97,11 @@ def _pages(what: str, k_pages, v_pages, weights, tables, lengths) -> GsPages:
     if page_size == 1:
         slot_stride = dim
     if (k_pages.stride(3) != 1 or page_stride % 8 or slot_stride % 8 or head_stride % 8
-            or slot_stride > _MAX_STRIDE or k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16
+            or slot_stride > _MAX_STRIDE or max(strides) >= 1 << 31 or k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16
             or not _apart(k_pages, 3)):
         raise RuntimeError(f"{what}: k_pages and v_pages must begin on 16 bytes, with neighbouring "
                            "elements in the last dimension, other strides that are multiples of 8, "
-                           "that of a page's slots at most 2^23, and rows that do not overlap; "
+                           "below 2^31, that of a page's slots at most 2^23, and rows that do not overlap; "
                            f"got strides {k_pages.stride()}")
     sums = (0, 0, 0)
     if weights is not None:
@@ -109,9 +109,10 @@ def _pages(what: str, k_pages, v_pages, weights, tables, lengths) -> GsPages:
         if weights.shape != k_pages.shape[:3]:
             raise RuntimeError(f"{what}: weights must be {tuple(k_pages.shape[:3])}, got "
                                f"{tuple(weights.shape)}")
-        if not _apart(weights, 3):
-            raise RuntimeError(f"{what}: weights overlap in memory, with strides {weights.stride()}")
-        sums = weights.stride()
+        sums = [s if n > 1 else 0 for n, s in zip(weights.shape, weights.stride())]
+        if max(sums) >= 1 << 31 or not _apart(weights, 3):
+            raise RuntimeError(f"{what}: weights overlap in memory or have strides of 2^31 or more, "
+                               f"got {weights.stride()}")
     _check(what, "tables", tables, 2, (torch.int32,), dev)
     _check(what, "lengths", lengths, 1, (torch.int32,), dev)
     sequences, width = tables.shape

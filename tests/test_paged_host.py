@@ -41,6 +41,7 @@ BAD_PAGES = [
     (dict(dim=60), UNSUPPORTED), (dict(dim=136, slot_stride=136), UNSUPPORTED),
     (dict(pages=1 << 31), UNSUPPORTED), (dict(page_size=1 << 20, table_width=1 << 11), UNSUPPORTED),
     (dict(slot_stride=56), UNSUPPORTED), (dict(slot_stride=(1 << 23) + 8), UNSUPPORTED),
+    (dict(page_stride=1 << 31), UNSUPPORTED), (dict(head_stride=1 << 31), UNSUPPORTED),
     (dict(page_stride=1028), UNSUPPORTED), (dict(head_stride=4), UNSUPPORTED)]
 
 
@@ -98,6 +99,8 @@ def test_refused_arguments(lib):
         assert evict(lib, p, **change) == INVALID
     assert evict(lib, p, pool=FAKE + 2) == UNSUPPORTED
     assert evict(lib, pages(sum_page=-1)) == INVALID
+    for stride in ("sum_page", "sum_slot", "sum_head"):
+        assert evict(lib, pages(**{stride: 1 << 31})) == UNSUPPORTED
 
 
 def test_nothing_to_do(lib):
