@@ -18,8 +18,9 @@ __device__ __forceinline__ int slots_of(const GsPages &p, int s) {
 __device__ const __attribute__((aligned(16))) uint32_t kZeros[4] = {0, 0, 0, 0};
 
 // Keys and values in pages.  WHOLE: pages of a multiple of a tile's rows, so that a tile lies in
-// one; else each row of a tile finds its own.  A tile's pages are read from the table while the
-// tile before it is copied, and its rows that are there are told by bits.
+// one; else each row of a tile finds its own, and a wave copies the rows of its 64 chunks as they
+// follow one another in a page, or chunk by chunk where a page ends between them.  A tile's pages
+// are read from the table while the tile before it is copied; a bit tells each row that is there.
 template <typename T, bool WHOLE>
 struct PagedKeys {
     static constexpr bool kHoles = true;
@@ -42,7 +43,9 @@ struct PagedKeys {
         // WHOLE: of the tile that is fetched next; else of the lane's row of it
         int index, place, page;
         int more_pages, more_places;  // of a tile's rows: whole pages, and places
-        typename KTile::Copy copy;    // WHOLE: a tile's chunks
+        // byte offsets of the lane's chunks from the tile's (WHOLE) or the copy's first row; past
+        // every bound where the chunk lies behind the dimension
+        typename KTile::Copy copy;
 
         __device__ __forceinline__ Reader(const PagedKeys &s, const GsAttention &, const Span &span,
                                           int sequence, int kh, int wave, int first, int end)
@@ -54,8 +57,17 @@ struct PagedKeys {
             place = slot - index * p.page_size;
             more_pages = KTile::kRows / p.page_size;
             more_places = KTile::kRows - more_pages * p.page_size;
-            if (WHOLE) copy = KTile::copy_of(wave, p.slot_stride, p.dim);
+            copy = KTile::copy_of(wave, p.slot_stride, p.dim);
+            if constexpr (!WHOLE) {
+#pragma unroll
+                for (int i = 0; i < KTile::kCopies; ++i)
+                    copy.from[i] -= copy.from[i] >> 31 ? 0u : first_row(i) * (uint32_t)p.slot_stride * 2u;
+            }
             look(first);
+        }
+        // The first row that the wave's copy i has chunks of.
+        __device__ __forceinline__ int first_row(int i) const {
+            return (i * KTile::kCopyWaves + wave) * 64 / KTile::kChunks;
         }
         __device__ __forceinline__ void look(int t) {
             const bool is = WHOLE ? t < end : t * KTile::kRows + (int)__lane_id() < lk;
@@ -76,6 +88,7 @@ struct PagedKeys {
             } else {
                 const bool is = (uint32_t)page < (uint64_t)p.pages;
                 there = __ballot(is);
+                const uint64_t begins = __ballot(place == 0);  // rows that begin a page
                 // bytes from the first element; below 0 where the row is not there
                 const int64_t from = is ? row_at(p, page, place) * 2 : -1;
                 const int low = (int)from, high = (int)(from >> 32);
@@ -83,15 +96,27 @@ struct PagedKeys {
                 for (int i = 0; i < KTile::kCopies; ++i) {
                     const int piece = i * KTile::kCopyWaves + wave;
                     if (KTile::kPieces % KTile::kCopyWaves != 0 && piece >= KTile::kPieces) break;
-                    const int at = piece * 64 + (int)__lane_id(), row = at / KTile::kChunks;
-                    const int chunk = (at % KTile::kChunks) ^ KTile::swizzle(row);
+                    const int row0 = first_row(i), rows = (piece * 64 + 63) / KTile::kChunks - row0 + 1;
+                    lds_char *const key_to = to + piece * 1024, *const value_to = key_to + KTile::kBytes;
+                    if (!((begins >> row0 >> 1) & ((1ull << (rows - 1)) - 1))) {
+                        // in one page, those that are there come first
+                        const int n = __popcll((there >> row0) & ((1ull << rows) - 1));
+                        const int bytes = n ? ((n - 1) * (int)p.slot_stride + p.dim) * 2 : 0;
+                        const int64_t at =
+                            (int64_t)(uint32_t)__builtin_amdgcn_readlane(low, row0) |
+                            (int64_t)__builtin_amdgcn_readlane(high, row0) << 32;
+                        copy_rows((const char *)k + at, bytes, copy.from[i], key_to);
+                        copy_rows((const char *)v + at, bytes, copy.from[i], value_to);
+                        continue;
+                    }
+                    const int chunk_at = piece * 64 + (int)__lane_id(), row = chunk_at / KTile::kChunks;
+                    const int chunk = (chunk_at % KTile::kChunks) ^ KTile::swizzle(row);
                     const int64_t mine = (int64_t)(uint32_t)__builtin_amdgcn_ds_bpermute(row * 4, low) |
                                          (int64_t)__builtin_amdgcn_ds_bpermute(row * 4, high) << 32;
                     const bool has = mine >= 0 && chunk * 8 < p.dim;
                     const int64_t byte = mine + chunk * 16;
-                    copy_chunk(has ? (const char *)k + byte : (const char *)kZeros, to + piece * 1024);
-                    copy_chunk(has ? (const char *)v + byte : (const char *)kZeros,
-                               to + KTile::kBytes + piece * 1024);
+                    copy_chunk(has ? (const char *)k + byte : (const char *)kZeros, key_to);
+                    copy_chunk(has ? (const char *)v + byte : (const char *)kZeros, value_to);
                 }
                 // the lane's row of the next tile
                 place += more_places;
@@ -100,7 +125,14 @@ struct PagedKeys {
             }
             look(t + 1);
         }
-        // 16 bytes a lane, from the lane's address to the wave's piece of LDS.
+        // 16 bytes a lane to the wave's piece of LDS: from an offset, or zeros past the bound, or from
+        // the lane's own address.
+        static __device__ __forceinline__ void copy_rows(const char *first, int bytes, uint32_t from,
+                                                         lds_char *to) {
+            const auto all = __builtin_amdgcn_make_buffer_rsrc((void *)first, 0, bytes, 0x00027000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                all, (__attribute__((address_space(3))) void *)to, 16, from, 0, 0, 0);
+        }
         static __device__ __forceinline__ void copy_chunk(const char *from, lds_char *to) {
             __builtin_amdgcn_global_load_lds(
                 (const __attribute__((address_space(1))) void *)from,
