@@ -14,7 +14,7 @@ namespace gs {
 // Keys and values in packed rows.
 template <typename T>
 struct PackedKeys {
-    static constexpr bool kHoles = false;
+    static constexpr bool kHoles = false, kScores = false;
     const T *k, *v;
     __device__ __forceinline__ Span span(const GsAttention &a, int s) const { return span_of(a, s); }
     __device__ __forceinline__ int keys(const GsAttention &a, int s) const {

@@ -410,6 +410,9 @@ __device__ __forceinline__ void forward_rows(
                 }
             }
         }
+        if constexpr (Source::kScores) {
+            if (real) source.keep(at, key0 + 4 * half, s[0]);
+        }
         float m = s[0][0];
 #pragma unroll
         for (int n = 0; n < F::kSub; ++n)

@@ -21,11 +21,21 @@ __device__ const __attribute__((aligned(16))) uint32_t kZeros[4] = {0, 0, 0, 0};
 // one; else each row of a tile finds its own, and a wave copies the rows of its 64 chunks as they
 // follow one another in a page, or chunk by chunk where a page ends between them.  A tile's pages
 // are read from the table while the tile before it is copied; a bit tells each row that is there.
-template <typename T, bool WHOLE>
+// SCORES: the scores of few rows are kept, for the slots' weights.
+template <typename T, bool WHOLE, bool SCORES = false>
 struct PagedKeys {
-    static constexpr bool kHoles = true;
+    static constexpr bool kHoles = true, kScores = SCORES;
     GsPages p;
     const T *k, *v;
+    float *scores;        // (row and head, slot)
+    int64_t score_slots;  // of a row, a multiple of 64
+    // Scores of a row and head in a lane's registers, its first slot: four slots in every eight.
+    __device__ __forceinline__ void keep(int64_t row, int slot, const f32x16 &s) const {
+        float *to = scores + row * score_slots + slot;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *(float4 *)(to + 8 * g) = make_float4(s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]);
+    }
     __device__ __forceinline__ Span span(const GsAttention &a, int s) const {
         const int2 q = rows_of(a.offsets_q, a.sequences, a.rows_q, s);
         return {uniform(q.x), uniform(q.y - q.x), 0, uniform(slots_of(p, s)), 0};
@@ -40,12 +50,18 @@ struct PagedKeys {
         const int32_t *table;
         int wave, lk, end;
         uint64_t there;  // of the tile that was fetched last
-        // WHOLE: of the tile that is fetched next; else of the lane's row of it
+        // WHOLE: of the tile that is looked for next; else of the lane's row of it
         int index, place, page;
         int more_pages, more_places;  // of a tile's rows: whole pages, and places
         // byte offsets of the lane's chunks from the tile's (WHOLE) or the copy's first row; past
         // every bound where the chunk lies behind the dimension
         typename KTile::Copy copy;
+        // the tile that is fetched next.  WHOLE: its first element; else of the lane's row: bytes from
+        // the first element, below 0 where it is not there, and how many may be copied from it, -1
+        // where a page ends among the rows of the copy that it begins
+        uint64_t ready;
+        int64_t from;
+        int bytes;
 
         __device__ __forceinline__ Reader(const PagedKeys &s, const GsAttention &, const Span &span,
                                           int sequence, int kh, int wave, int first, int end)
@@ -73,40 +89,54 @@ struct PagedKeys {
             const bool is = WHOLE ? t < end : t * KTile::kRows + (int)__lane_id() < lk;
             page = is ? table[index] : -1;
         }
-        // Starts the copies of a tile of keys and, behind it, of values.  Tiles come in order.
-        __device__ __forceinline__ void fetch(int t, lds_char *to) {
+        // Finds the tile that was looked for.
+        __device__ __forceinline__ void prepare() {
             if constexpr (WHOLE) {
                 const int32_t number = uniform(page);
                 const bool is = (uint32_t)number < (uint64_t)p.pages;
-                const int rows = is ? lk - t * KTile::kRows : 0;
-                const int64_t from = is ? row_at(p, number, place) : 0;
-                there = is ? ~0ull : 0;
-                KTile::start(copy, wave, k + from, p.slot_stride, rows, p.dim, to);
-                KTile::start(copy, wave, v + from, p.slot_stride, rows, p.dim, to + KTile::kBytes);
+                from = is ? row_at(p, number, place) : 0;
+                ready = is ? ~0ull : 0;
                 place += KTile::kRows;
                 if (place == p.page_size) place = 0, ++index;
             } else {
                 const bool is = (uint32_t)page < (uint64_t)p.pages;
-                there = __ballot(is);
+                ready = __ballot(is);
                 const uint64_t begins = __ballot(place == 0);  // rows that begin a page
-                // bytes from the first element; below 0 where the row is not there
-                const int64_t from = is ? row_at(p, page, place) * 2 : -1;
+                from = is ? row_at(p, page, place) * 2 : -1;
+                // a copy that begins here: rows in one page, of which those that are there come first
+                constexpr int rows = (64 + KTile::kChunks - 1) / KTile::kChunks;
+                const int row = __lane_id();
+                const int n = __popcll((ready >> row) & ((1ull << rows) - 1));
+                const bool breaks = (begins >> row >> 1) & ((1ull << (rows - 1)) - 1);
+                bytes = breaks ? -1 : n ? ((n - 1) * (int)p.slot_stride + p.dim) * 2 : 0;
+                place += more_places;
+                index += more_pages;
+                if (place >= p.page_size) place -= p.page_size, ++index;
+            }
+        }
+        // Starts the copies of a tile of keys and, behind it, of values.  Tiles come in order.
+        __device__ __forceinline__ void fetch(int t, lds_char *to) {
+            prepare();
+            there = ready;
+            look(t + 1);  // (before the copies, so that it is there before them)
+            if constexpr (WHOLE) {
+                const int rows = ready ? lk - t * KTile::kRows : 0;
+                KTile::start(copy, wave, k + from, p.slot_stride, rows, p.dim, to);
+                KTile::start(copy, wave, v + from, p.slot_stride, rows, p.dim, to + KTile::kBytes);
+            } else {
                 const int low = (int)from, high = (int)(from >> 32);
 #pragma unroll
                 for (int i = 0; i < KTile::kCopies; ++i) {
                     const int piece = i * KTile::kCopyWaves + wave;
                     if (KTile::kPieces % KTile::kCopyWaves != 0 && piece >= KTile::kPieces) break;
-                    const int row0 = first_row(i), rows = (piece * 64 + 63) / KTile::kChunks - row0 + 1;
                     lds_char *const key_to = to + piece * 1024, *const value_to = key_to + KTile::kBytes;
-                    if (!((begins >> row0 >> 1) & ((1ull << (rows - 1)) - 1))) {
-                        // in one page, those that are there come first
-                        const int n = __popcll((there >> row0) & ((1ull << rows) - 1));
-                        const int bytes = n ? ((n - 1) * (int)p.slot_stride + p.dim) * 2 : 0;
+                    const int row0 = first_row(i), many = __builtin_amdgcn_readlane(bytes, row0);
+                    if (many >= 0) {
                         const int64_t at =
                             (int64_t)(uint32_t)__builtin_amdgcn_readlane(low, row0) |
                             (int64_t)__builtin_amdgcn_readlane(high, row0) << 32;
-                        copy_rows((const char *)k + at, bytes, copy.from[i], key_to);
-                        copy_rows((const char *)v + at, bytes, copy.from[i], value_to);
+                        copy_rows((const char *)k + at, many, copy.from[i], key_to);
+                        copy_rows((const char *)v + at, many, copy.from[i], value_to);
                         continue;
                     }
                     const int chunk_at = piece * 64 + (int)__lane_id(), row = chunk_at / KTile::kChunks;
@@ -118,12 +148,7 @@ struct PagedKeys {
                     copy_chunk(has ? (const char *)k + byte : (const char *)kZeros, key_to);
                     copy_chunk(has ? (const char *)v + byte : (const char *)kZeros, value_to);
                 }
-                // the lane's row of the next tile
-                place += more_places;
-                index += more_pages;
-                if (place >= p.page_size) place -= p.page_size, ++index;
             }
-            look(t + 1);
         }
         // 16 bytes a lane to the wave's piece of LDS: from an offset, or zeros past the bound, or from
         // the lane's own address.
@@ -146,17 +171,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_kernel(
     GsAttention a, GsPages p, const T *__restrict__ q, const T *__restrict__ k,
     const T *__restrict__ v, T *__restrict__ out, float *__restrict__ log_sum, Partial partial) {
     __shared__ __attribute__((aligned(1024))) char lds[Forward<T, DIM, false>::kLds];
-    forward_tile<T, DIM, LOG_SUM>(a, PagedKeys<T, WHOLE>{p, k, v}, q, out, (T *)nullptr, log_sum, partial,
-                                  (lds_char *)lds);
+    forward_tile<T, DIM, LOG_SUM>(a, PagedKeys<T, WHOLE>{p, k, v, nullptr, 0}, q, out, (T *)nullptr, log_sum,
+                                  partial, (lds_char *)lds);
 }
 
-template <typename T, int DIM, bool WHOLE>
+template <typename T, int DIM, bool WHOLE, bool SCORES>
 __global__ __launch_bounds__(64 * kKeysWaves, DIM > 96 ? 1 : 2) void paged_attention_keys_kernel(
     GsAttention a, GsPages p, const T *__restrict__ q, const T *__restrict__ k,
-    const T *__restrict__ v, T *__restrict__ out, float *__restrict__ log_sum, Partial partial) {
+    const T *__restrict__ v, T *__restrict__ out, float *__restrict__ log_sum, Partial partial,
+    float *__restrict__ scores, int64_t score_slots) {
     __shared__ __attribute__((aligned(1024))) char lds[Forward<T, DIM, true>::kLds];
-    forward_by_keys<T, DIM>(a, PagedKeys<T, WHOLE>{p, k, v}, q, out, (T *)nullptr, log_sum, partial,
-                            (lds_char *)lds);
+    forward_by_keys<T, DIM>(a, PagedKeys<T, WHOLE, SCORES>{p, k, v, scores, score_slots}, q, out,
+                            (T *)nullptr, log_sum, partial, (lds_char *)lds);
 }
 
 template <typename T>
@@ -195,6 +221,7 @@ __device__ __forceinline__ float minus_log(float log_sum) {
 }
 
 constexpr int kWeightSlots = 32 * kWaves;  // of a workgroup
+constexpr int kScoreSlots = 256;           // of one where the scores are there
 
 // The slots of a workgroup, and what its lanes have of them.
 template <typename T, int DIM>
@@ -217,12 +244,12 @@ struct SlotOperand {
     }
 };
 
-// f(sequence, tile, key head) for the tiles of slots of all sequences that have queries.
-template <typename F>
+// f(sequence, tile, key head) for the tiles of SLOTS slots of all sequences that have queries.
+template <int SLOTS, typename F>
 __device__ __forceinline__ void for_slot_tiles(const GsAttention &a, const GsPages &p, F f) {
     const auto count = [&](int s) {
         const int2 q = rows_of(a.offsets_q, a.sequences, a.rows_q, s);
-        return q.x == q.y ? 0 : (slots_of(p, s) + kWeightSlots - 1) / kWeightSlots * a.heads_k;
+        return q.x == q.y ? 0 : (slots_of(p, s) + SLOTS - 1) / SLOTS * a.heads_k;
     };
     int sequence, place;
     for (int item = blockIdx.x; find_place(a.sequences + 2, count, item, false, &sequence, &place);
@@ -243,7 +270,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
     const int wave = uniform(threadIdx.x / kWave);
     const float c = exponent_factor(a.scale);
     const auto copy = QTile::copy_of(wave, a.q_row, a.dim);
-    for_slot_tiles(a, p, [&](int sequence, int tile, int kh) {
+    for_slot_tiles<kWeightSlots>(a, p, [&](int sequence, int tile, int kh) {
         const int2 rows = rows_of(a.offsets_q, a.sequences, a.rows_q, sequence);
         const int q0 = uniform(rows.x), lq = uniform(rows.y - rows.x);
         const int filled = uniform(slots_of(p, sequence));
@@ -310,7 +337,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_few_weights_kernel(
     const int group = a.heads_q / a.heads_k, lane = __lane_id(), half = lane >> 5;
     const int wave = uniform(threadIdx.x / kWave);
     const float c = exponent_factor(a.scale);
-    for_slot_tiles(a, p, [&](int sequence, int tile, int kh) {
+    for_slot_tiles<kWeightSlots>(a, p, [&](int sequence, int tile, int kh) {
         const int2 range = rows_of(a.offsets_q, a.sequences, a.rows_q, sequence);
         const int q0 = uniform(range.x), lq = uniform(range.y - range.x), rows = lq * group;
         const int filled = uniform(slots_of(p, sequence));
@@ -339,6 +366,32 @@ __global__ __launch_bounds__(64 * kWaves) void paged_few_weights_kernel(
         }
         sum = half_sum(sum);
         if (half == 0 && mine.weight) *mine.weight += sum;
+    });
+}
+
+// Few rows whose scores the attention has kept: a thread a slot.
+__global__ __launch_bounds__(kScoreSlots) void paged_score_weights_kernel(
+    GsAttention a, GsPages p, const float *__restrict__ scores, int64_t score_slots,
+    const float *__restrict__ log_sum, float *__restrict__ weights) {
+    const int group = a.heads_q / a.heads_k;
+    const float c = exponent_factor(a.scale);
+    for_slot_tiles<kScoreSlots>(a, p, [&](int sequence, int tile, int kh) {
+        const int2 range = rows_of(a.offsets_q, a.sequences, a.rows_q, sequence);
+        const int q0 = uniform(range.x), lq = uniform(range.y - range.x);
+        const int filled = uniform(slots_of(p, sequence)), slot = tile * kScoreSlots + (int)threadIdx.x;
+        if (slot >= filled) return;
+        const int index = slot / p.page_size, page = page_of(p, sequence - 1, index);
+        if (page < 0) return;
+        float sum = 0.0f;
+        for (int i = a.causal ? max(slot - (filled - lq), 0) : 0; i < lq; ++i) {
+            const int64_t row = (int64_t)(q0 + i) * a.heads_q + kh * group;
+            float part = 0.0f;
+            for (int h = 0; h < group; ++h)
+                part += __builtin_amdgcn_exp2f(fmaf(scores[(row + h) * score_slots + slot], c,
+                                                    minus_log(log_sum[row + h])));
+            sum += part;
+        }
+        weights[sum_at(p, page, slot - index * p.page_size, kh)] += sum;
     });
 }
 
@@ -374,13 +427,25 @@ static ForwardPlan plan_of(const GsPages &p, const GsAttention &a) {
     return plan_forward(a, slots, slots);
 }
 
+// Floats a row and head where the scores of few rows are kept for the slots' weights, 0 where they
+// are not: where they would take more than 256 MB (a table may be much wider than what is filled),
+// the keys are read a second time.
+static int64_t score_slots_of(const GsPages &p, const GsAttention &a, const ForwardPlan &f) {
+    const int64_t slots = ((int64_t)p.page_size * p.table_width + 63) / 64 * 64;
+    return f.by_keys && slots * a.rows_q * a.heads_q <= (64 << 20) ? slots : 0;
+}
+
 template <typename T, int DIM, bool WHOLE>
 static int launch(const GsPages &p, const GsAttention &a, const ForwardPlan &f, const T *q, const T *k,
-                  const T *v, T *out, float *log_sum, const Partial &partial, hipStream_t stream) {
+                  const T *v, T *out, float *log_sum, const Partial &partial, float *scores,
+                  int64_t score_slots, hipStream_t stream) {
     const dim3 grid((unsigned)f.groups);
-    if (f.by_keys)
-        hipLaunchKernelGGL((paged_attention_keys_kernel<T, DIM, WHOLE>), grid, dim3(64 * kKeysWaves), 0,
-                           stream, a, p, q, k, v, out, log_sum, partial);
+    if (f.by_keys && scores)
+        hipLaunchKernelGGL((paged_attention_keys_kernel<T, DIM, WHOLE, true>), grid, dim3(64 * kKeysWaves),
+                           0, stream, a, p, q, k, v, out, log_sum, partial, scores, score_slots);
+    else if (f.by_keys)
+        hipLaunchKernelGGL((paged_attention_keys_kernel<T, DIM, WHOLE, false>), grid, dim3(64 * kKeysWaves),
+                           0, stream, a, p, q, k, v, out, log_sum, partial, scores, score_slots);
     else if (log_sum || f.splits > 1)
         hipLaunchKernelGGL((paged_attention_kernel<T, DIM, true, WHOLE>), grid, dim3(64 * kWaves), 0,
                            stream, a, p, q, k, v, out, log_sum, partial);
@@ -406,7 +471,9 @@ extern "C" int gs_paged_attention_workspace_size(const GsPages *p, const GsPaged
     if (st) return st;
     if (!bytes) return GS_ERR_INVALID_ARGUMENT;
     const GsAttention a = problem_of(*p, *q);
-    *bytes = partial_bytes(a, plan_of(*p, a).splits);
+    const ForwardPlan f = plan_of(*p, a);
+    const size_t scores = weights ? score_slots_of(*p, a, f) * a.rows_q * a.heads_q * sizeof(float) : 0;
+    *bytes = scores + partial_bytes(a, f.splits);
     return GS_OK;
 }
 
@@ -427,29 +494,39 @@ extern "C" int gs_paged_attention(const GsPages *p, const GsPagedQueries *querie
     if (f.groups > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
     if (need && !workspace) return GS_ERR_INVALID_ARGUMENT;
     if (workspace_bytes < need) return GS_ERR_WORKSPACE_TOO_SMALL;
-    const Partial partial = partial_of(a, f, workspace);
+    // the scores, whole lines, then the parts
+    const int64_t score_slots = weights ? score_slots_of(*p, a, f) : 0;
+    float *const scores = score_slots ? (float *)workspace : nullptr;
+    const Partial partial = partial_of(a, f, (float *)workspace + score_slots * a.rows_q * a.heads_q);
     const auto all = [&](auto t, auto d) {
         using T = decltype(t);
         constexpr int kDim = decltype(d)::value;
         const T *tq = (const T *)q, *tk = (const T *)k_pages, *tv = (const T *)v_pages;
         const int s = p->page_size % 64 == 0
-                          ? launch<T, kDim, true>(*p, a, f, tq, tk, tv, (T *)out, log_sum, partial, stream)
-                          : launch<T, kDim, false>(*p, a, f, tq, tk, tv, (T *)out, log_sum, partial, stream);
-        if (s) return s;
-        const int64_t slots = (int64_t)p->page_size * p->table_width;
+                          ? launch<T, kDim, true>(*p, a, f, tq, tk, tv, (T *)out, log_sum, partial,
+                                                   scores, score_slots, stream)
+                          : launch<T, kDim, false>(*p, a, f, tq, tk, tv, (T *)out, log_sum, partial,
+                                                    scores, score_slots, stream);
+        if (s || !weights || p->sequences == 0 || p->table_width == 0) return s;
         // as many workgroups as there are tiles if no page is in two tables; the workgroups go on
         // while there are more
-        const int64_t tiles = (slots + kWeightSlots - 1) / kWeightSlots * p->sequences;
-        const int64_t pool = p->pages * p->page_size / kWeightSlots + p->sequences;
-        int64_t groups = (tiles < pool ? tiles : pool) * p->heads;
-        if (!weights || groups == 0) return s;
-        if (groups > 8192) groups = 8192;
-        if (f.by_keys)
-            hipLaunchKernelGGL((paged_few_weights_kernel<T, kDim>), dim3((unsigned)groups),
-                               dim3(64 * kWaves), 0, stream, a, *p, tq, tk, (const float *)log_sum, weights);
+        const auto grid = [&](int64_t size) {
+            const int64_t slots = (int64_t)p->page_size * p->table_width;
+            const int64_t tables = (slots + size - 1) / size * p->sequences;
+            const int64_t pool = p->pages * p->page_size / size + p->sequences;
+            const int64_t groups = (tables < pool ? tables : pool) * p->heads;
+            return dim3((unsigned)(groups < 8192 ? groups : 8192));
+        };
+        const float *log = log_sum;
+        if (scores)
+            hipLaunchKernelGGL(paged_score_weights_kernel, grid(kScoreSlots), dim3(kScoreSlots), 0, stream, a,
+                               *p, (const float *)scores, score_slots, log, weights);
+        else if (f.by_keys)
+            hipLaunchKernelGGL((paged_few_weights_kernel<T, kDim>), grid(kWeightSlots), dim3(64 * kWaves), 0,
+                               stream, a, *p, tq, tk, log, weights);
         else
-            hipLaunchKernelGGL((paged_weights_kernel<T, kDim>), dim3((unsigned)groups), dim3(64 * kWaves),
-                               0, stream, a, *p, tq, tk, (const float *)log_sum, weights);
+            hipLaunchKernelGGL((paged_weights_kernel<T, kDim>), grid(kWeightSlots), dim3(64 * kWaves), 0,
+                               stream, a, *p, tq, tk, log, weights);
         return launch_status();
     };
     return p->type == GS_F16 ? with_tile(p->dim, [&](auto d) { return all(f16{}, d); })

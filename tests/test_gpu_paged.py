@@ -270,6 +270,17 @@ def test_attention_without_some_pages(gpu, causal, page):
             check_attention(queries(gpu, sum(new), 4, 64, dtype), c, offsets_of(new, gpu), causal)
 
 
+@pytest.mark.parametrize("page", [24, 64])
+def test_attention_over_wide_tables(gpu, page):
+    """Tables far wider than what is filled: few rows whose scores would take too much room."""
+    for dtype, dim in zip(TYPES, (64, 128)):
+        for new in ([1] * 4, [3, 0, 1, 2]):
+            c = Cache(gpu, [700, 64, 0, 129], page, 2, dim, dtype, width=(1 << 22) // page)
+            q = queries(gpu, sum(new), 8, dim, dtype)
+            check_attention(q, c, offsets_of(new, gpu))
+            check_attention(q, c, offsets_of(new, gpu), causal=False, scale=-0.2)
+
+
 def test_attention_of_rows_of_no_sequence(gpu):
     c = Cache(gpu, [60, 70], 16, 2, 64, torch.float16)
     q = queries(gpu, 150, 4, 64, torch.float16)
