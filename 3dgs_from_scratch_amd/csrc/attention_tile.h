@@ -114,14 +114,9 @@ __device__ __forceinline__ bool find_place(int groups, Count count, int number, 
     const int lane = __lane_id();
     int total = 0, sum = 0;
     const auto running = [&](int first) {  // up to and with group first + lane
-        sum = first + lane < groups ? count(first + lane) : 0;
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const int t = __shfl_up(sum, o, kWave);
-            if (lane >= o) sum += t;
-        }
+        sum = (int)lanes_sum_upto(first + lane < groups ? (uint32_t)count(first + lane) : 0u);
         // (uniform, also to the compiler: what is found here addresses whole waves' copies)
-        return uniform(__shfl(sum, kWave - 1, kWave));
+        return __builtin_amdgcn_readlane(sum, kWave - 1);
     };
     for (int first = 0; first < groups; first += kWave) total += running(first);
     if (number >= total) return false;

@@ -67,6 +67,18 @@ __device__ __forceinline__ float wave_max(float v) {
     return lane_reduce<kWave>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
+// Sum over the lanes up to this one.
+__device__ __forceinline__ uint32_t lanes_sum_upto(uint32_t v) {
+    int x = (int)v;
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // a lane to the right within 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // 16 to the next 16, 32 to the rest
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return (uint32_t)x;
+}
+
 // N neighbouring elements, read or written as one access, which on this target may begin at
 // any element.
 template <typename T, int N>

@@ -64,18 +64,6 @@ __host__ __device__ __forceinline__ int rounds_of(int64_t slots) {
     return (int)((slots + kUnroll * kPick - 1) / (kUnroll * kPick)) * kUnroll;
 }
 
-// Sum over the lanes up to this one.
-__device__ __forceinline__ uint32_t lanes_sum_upto(uint32_t v) {
-    int x = (int)v;
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // a lane to the right within 16
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // 16 to the next 16, 32 to the rest
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
-    return (uint32_t)x;
-}
-
 struct PickShared {
     uint32_t histogram[kBins];
     uint32_t waves[2][kPickWaves];  // counts of each wave

@@ -244,17 +244,35 @@ struct SlotOperand {
     }
 };
 
-// f(sequence, tile, key head) for the tiles of SLOTS slots of all sequences that have queries.
+// f(sequence, tile, key head) for the tiles of SLOTS slots of all sequences that have queries.  The
+// workgroups take them in turn; most have one, and find it in one look through the sequences.
 template <int SLOTS, typename F>
 __device__ __forceinline__ void for_slot_tiles(const GsAttention &a, const GsPages &p, F f) {
-    const auto count = [&](int s) {
-        const int2 q = rows_of(a.offsets_q, a.sequences, a.rows_q, s);
-        return q.x == q.y ? 0 : (slots_of(p, s) + SLOTS - 1) / SLOTS * a.heads_k;
+    const int lane = __lane_id();
+    int upto = 0;  // places of 64 sequences up to and with the lane's
+    const auto look = [&](int first) {  // all of them
+        const int s = first + lane + 1;
+        int n = 0;
+        if (s <= a.sequences) {
+            const int2 q = rows_of(a.offsets_q, a.sequences, a.rows_q, s);
+            n = q.x == q.y ? 0 : (slots_of(p, s) + SLOTS - 1) / SLOTS * a.heads_k;
+        }
+        upto = (int)lanes_sum_upto((uint32_t)n);
+        return __builtin_amdgcn_readlane(upto, kWave - 1);
     };
-    int sequence, place;
-    for (int item = blockIdx.x; find_place(a.sequences + 2, count, item, false, &sequence, &place);
-         item += gridDim.x)
-        f(sequence, place / a.heads_k, place % a.heads_k);
+    int item = blockIdx.x, first = 0, before = 0, here = look(0);
+    for (;;) {
+        while (item - before >= here) {
+            before += here;
+            first += kWave;
+            if (first >= a.sequences) return;
+            here = look(first);
+        }
+        const int l = __builtin_ctzll(__ballot(before + upto > item));
+        const int place = item - before - (l ? __builtin_amdgcn_readlane(upto, l - 1) : 0);
+        f(first + l + 1, place / a.heads_k, place % a.heads_k);
+        item += gridDim.x;
+    }
 }
 
 // Many rows: tiles of a head's queries go through LDS, which the workgroup's waves share.
@@ -301,24 +319,29 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
             copies_done();
             if (t + 1 < steps) fetch((t + 1) & 1);
             const lds_char *qt = (const lds_char *)lds + (t & 1) * QTile::kBytes;
+            f32x16 s[2] = {};
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int row0 = now * kRows + 32 * n;
-                f32x16 s = {};
+            for (int i = 0; i < DIM / 16; ++i)
 #pragma unroll
-                for (int i = 0; i < DIM / 16; ++i) s = mfma(QTile::along(qt, 32 * n, i), mine.k.x[i], s);
-                float m[16];
+                for (int n = 0; n < 2; ++n) s[n] = mfma(QTile::along(qt, 32 * n, i), mine.k.x[i], s[n]);
+            float m[2][16];
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 x = *(const f32x4 *)&minus[t & 1][32 * n + result_row(4 * g, half)];
+            for (int g = 0; g < 8; ++g) {
+                const f32x4 x = *(const f32x4 *)&minus[t & 1][32 * (g / 4) + result_row(4 * (g % 4), half)];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) m[4 * g + i] = x[i];
-                }
-                if (row0 + shift >= slot0 + 31 && row0 + 32 <= lq)
-                    sum += sum_of_weights<false>(s, c, m, [](int) { return true; });
-                else
+                for (int i = 0; i < 4; ++i) m[g / 4][4 * (g % 4) + i] = x[i];
+            }
+            const int row0 = now * kRows;
+            if (row0 + shift >= slot0 + 31 && row0 + kRows <= lq) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n) sum += sum_of_weights<false>(s[n], c, m[n], [](int) { return true; });
+            } else {
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int row = row0 + 32 * n;
                     sum += sum_of_weights<true>(
-                        s, c, m, [&](int i) { return row0 + i < lq && row0 + i + shift >= slot; });
+                        s[n], c, m[n], [&](int i) { return row + i < lq && row + i + shift >= slot; });
+                }
             }
             if (++now == first + tiles) now = first;
             if (wave == 0 && t + 1 < steps) minus[(t + 1) & 1][lane] = next;
@@ -381,17 +404,24 @@ __global__ __launch_bounds__(kScoreSlots) void paged_score_weights_kernel(
         const int filled = uniform(slots_of(p, sequence)), slot = tile * kScoreSlots + (int)threadIdx.x;
         if (slot >= filled) return;
         const int index = slot / p.page_size, page = page_of(p, sequence - 1, index);
-        if (page < 0) return;
         float sum = 0.0f;
         for (int i = a.causal ? max(slot - (filled - lq), 0) : 0; i < lq; ++i) {
             const int64_t row = (int64_t)(q0 + i) * a.heads_q + kh * group;
-            float part = 0.0f;
-            for (int h = 0; h < group; ++h)
-                part += __builtin_amdgcn_exp2f(fmaf(scores[(row + h) * score_slots + slot], c,
-                                                    minus_log(log_sum[row + h])));
-            sum += part;
+            const float *line = scores + row * score_slots + slot;
+            for (int h0 = 0; h0 < group; h0 += 4) {
+                float s[4], l[4];
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    s[h] = h0 + h < group ? line[(h0 + h) * score_slots] : 0.0f;
+                    l[h] = h0 + h < group ? minus_log(log_sum[row + h0 + h]) : -INFINITY;
+                }
+                float w[4];
+#pragma unroll
+                for (int h = 0; h < 4; ++h) w[h] = __builtin_amdgcn_exp2f(fmaf(s[h], c, l[h]));
+                sum += (w[0] + w[1]) + (w[2] + w[3]);
+            }
         }
-        weights[sum_at(p, page, slot - index * p.page_size, kh)] += sum;
+        if (page >= 0) weights[sum_at(p, page, slot - index * p.page_size, kh)] += sum;
     });
 }
 
