@@ -56,8 +56,8 @@ __global__ __launch_bounds__(64 * kKeysWaves, DIM > 96 ? 1 : 2) void attention_k
     GsAttention a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
     T *__restrict__ out, T *__restrict__ out_rest, float *__restrict__ log_sum, Partial partial) {
     __shared__ __attribute__((aligned(1024))) char lds[Forward<T, DIM, true>::kLds];
-    forward_by_keys<T, DIM>(a, PackedKeys<T>{k, v}, q, out, out_rest, log_sum, partial,
-                            (lds_char *)lds);
+    forward_shared<T, DIM, true>(a, PackedKeys<T>{k, v}, q, out, out_rest, log_sum, partial,
+                                 (lds_char *)lds);
 }
 
 template <typename T>
@@ -628,7 +628,7 @@ extern "C" int gs_attention_forward(const GsAttention *a, const void *q, const v
     const size_t need = partial_bytes(*a, f.splits);
     if (need && !workspace) return GS_ERR_INVALID_ARGUMENT;
     if (workspace_bytes < need) return GS_ERR_WORKSPACE_TOO_SMALL;
-    const Partial partial = partial_of(*a, f, workspace);
+    const Partial partial = partial_of(*a, f, f.by_keys, workspace);
     const auto launch = [&](auto t) {
         return with_tile(a->dim, [&](auto d) {
             return launch_forward<decltype(t), decltype(d)::value>(

@@ -526,7 +526,7 @@ __device__ __forceinline__ void forward_rows(
         const int64_t slot = (int64_t)split * a.rows_q * a.heads_q + at;
         if (real && half == 0) {
             partial.max_sum[slot] = make_float2(top, sum);
-            if (BY_KEYS && split == 0)
+            if (partial.count && split == 0)
                 partial.count[at] = max((tiles_keys + share - 1) / share, 1);
         }
         store_partial<DIM>(acc, 1.0f,
@@ -571,11 +571,11 @@ __device__ __forceinline__ void forward_tile(const GsAttention &a, const Source 
 // TB/s; twice as many splits 99, four times 104; equal splits of each sequence 105.
 constexpr int kSplits = 448;
 
-template <typename T, int DIM, typename Source>
-__device__ __forceinline__ void forward_by_keys(const GsAttention &a, const Source &source,
-                                                const T *q, T *out, T *out_rest, float *log_sum,
-                                                const Partial &partial, lds_char *lds) {
-    using F = Forward<T, DIM, true>;
+template <typename T, int DIM, bool BY_KEYS, typename Source>
+__device__ __forceinline__ void forward_shared(const GsAttention &a, const Source &source,
+                                               const T *q, T *out, T *out_rest, float *log_sum,
+                                               const Partial &partial, lds_char *lds) {
+    using F = Forward<T, DIM, BY_KEYS>;
     const int group = a.heads_q / a.heads_k, all = a.sequences + 2;
     const auto tiles_of = [&](int s) {  // of keys
         return (source.keys(a, s) + F::kKeys - 1) / F::kKeys;
@@ -601,8 +601,8 @@ __device__ __forceinline__ void forward_by_keys(const GsAttention &a, const Sour
          item += gridDim.x) {
         const int t = uniform(tiles_of(sequence)), splits = splits_of(t);
         const int rest = number / a.heads_k;
-        forward_rows<T, DIM, true, true>(a, source, q, out, out_rest, log_sum, partial, lds,
-                                         number % a.heads_k, sequence, rest / splits, rest % splits,
+        forward_rows<T, DIM, BY_KEYS, true>(a, source, q, out, out_rest, log_sum, partial, lds,
+                                            number % a.heads_k, sequence, rest / splits, rest % splits,
                                          share_of(t));
         __syncthreads();  // LDS has been read
     }
@@ -708,14 +708,14 @@ inline size_t partial_bytes(const GsAttention &a, int splits) {
     return splits * rows * (a.dim * sizeof(float) + sizeof(float2)) + rows * sizeof(int32_t);
 }
 
-// The parts in a workspace of that size.
-inline Partial partial_of(const GsAttention &a, const ForwardPlan &f, void *workspace) {
+// The parts in a workspace of that size; counted: rows may have fewer of them.
+inline Partial partial_of(const GsAttention &a, const ForwardPlan &f, bool counted, void *workspace) {
     Partial partial;
     const size_t rows = (size_t)a.rows_q * a.heads_q;
     partial.splits = f.splits;
     partial.sums = (float *)workspace;
     partial.max_sum = (float2 *)(partial.sums + f.splits * rows * a.dim);
-    partial.count = f.by_keys ? (int32_t *)(partial.max_sum + f.splits * rows) : nullptr;
+    partial.count = counted ? (int32_t *)(partial.max_sum + f.splits * rows) : nullptr;
     return partial;
 }
 

@@ -181,8 +181,18 @@ __global__ __launch_bounds__(64 * kKeysWaves, DIM > 96 ? 1 : 2) void paged_atten
     const T *__restrict__ v, T *__restrict__ out, float *__restrict__ log_sum, Partial partial,
     float *__restrict__ scores, int64_t score_slots) {
     __shared__ __attribute__((aligned(1024))) char lds[Forward<T, DIM, true>::kLds];
-    forward_by_keys<T, DIM>(a, PagedKeys<T, WHOLE, SCORES>{p, k, v, scores, score_slots}, q, out,
-                            (T *)nullptr, log_sum, partial, (lds_char *)lds);
+    forward_shared<T, DIM, true>(a, PagedKeys<T, WHOLE, SCORES>{p, k, v, scores, score_slots}, q, out,
+                                 (T *)nullptr, log_sum, partial, (lds_char *)lds);
+}
+
+// Tiles of rows too few for the GPU: their keys in splits of equal length across sequences.
+template <typename T, int DIM, bool WHOLE>
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_split_kernel(
+    GsAttention a, GsPages p, const T *__restrict__ q, const T *__restrict__ k,
+    const T *__restrict__ v, T *__restrict__ out, float *__restrict__ log_sum, Partial partial) {
+    __shared__ __attribute__((aligned(1024))) char lds[Forward<T, DIM, false>::kLds];
+    forward_shared<T, DIM, false>(a, PagedKeys<T, WHOLE>{p, k, v, nullptr, 0}, q, out, (T *)nullptr, log_sum,
+                                  partial, (lds_char *)lds);
 }
 
 template <typename T>
@@ -454,7 +464,16 @@ static GsAttention problem_of(const GsPages &p, const GsPagedQueries &q) {
 
 static ForwardPlan plan_of(const GsPages &p, const GsAttention &a) {
     const int64_t slots = (int64_t)p.page_size * p.table_width;
-    return plan_forward(a, slots, slots);
+    ForwardPlan f = plan_forward(a, slots, slots);
+    // Few tiles of rows: as many splits as make kSplits items in all, which the workgroups find from
+    // the lengths.  A sequence longer than the others may have twice as many as the average.
+    if (!f.by_keys && f.splits > 1) {
+        const int64_t most = (slots + 255) / 256;
+        f.splits = (int)(2 * f.splits < most ? 2 * f.splits : most);
+        if (f.splits > 64) f.splits = 64;
+        if (f.groups > 1024) f.groups = 1024;
+    }
+    return f;
 }
 
 // Floats a row and head where the scores of few rows are kept for the slots' weights, 0 where they
@@ -476,7 +495,10 @@ static int launch(const GsPages &p, const GsAttention &a, const ForwardPlan &f, 
     else if (f.by_keys)
         hipLaunchKernelGGL((paged_attention_keys_kernel<T, DIM, WHOLE, false>), grid, dim3(64 * kKeysWaves),
                            0, stream, a, p, q, k, v, out, log_sum, partial, scores, score_slots);
-    else if (log_sum || f.splits > 1)
+    else if (f.splits > 1)
+        hipLaunchKernelGGL((paged_attention_split_kernel<T, DIM, WHOLE>), grid, dim3(64 * kWaves), 0,
+                           stream, a, p, q, k, v, out, log_sum, partial);
+    else if (log_sum)
         hipLaunchKernelGGL((paged_attention_kernel<T, DIM, true, WHOLE>), grid, dim3(64 * kWaves), 0,
                            stream, a, p, q, k, v, out, log_sum, partial);
     else
@@ -527,7 +549,8 @@ extern "C" int gs_paged_attention(const GsPages *p, const GsPagedQueries *querie
     // the scores, whole lines, then the parts
     const int64_t score_slots = weights ? score_slots_of(*p, a, f) : 0;
     float *const scores = score_slots ? (float *)workspace : nullptr;
-    const Partial partial = partial_of(a, f, (float *)workspace + score_slots * a.rows_q * a.heads_q);
+    const Partial partial =
+        partial_of(a, f, true, (float *)workspace + score_slots * a.rows_q * a.heads_q);
     const auto all = [&](auto t, auto d) {
         using T = decltype(t);
         constexpr int kDim = decltype(d)::value;
