@@ -30,6 +30,7 @@ sees them, nothing is written to them.  Nothing here has a counterpart in the re
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -49,12 +50,11 @@ def _no_gradient(what: str, *tensors) -> None:
         raise RuntimeError(f"{what} cannot be traced")
     grad = torch.is_grad_enabled()
     for t in tensors:
-        if not isinstance(t, torch.Tensor):
-            continue
-        if grad and t.requires_grad:
-            raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad()")
-        if unpack_dual(t).tangent is not None:
-            raise NotImplementedError(f"{what} has no forward-mode derivative")
+        if isinstance(t, torch.Tensor):
+            if grad and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad()")
+            if unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def _written(*tensors) -> None:
@@ -63,12 +63,17 @@ def _written(*tensors) -> None:
                                             if t is not None and not t.is_inference()])
 
 
-def _apart(t: torch.Tensor, dims: int) -> bool:
-    """Whether no two of the blocks that the first dims dimensions number overlap in memory."""
-    extent = 1
-    for size, stride in sorted(zip(t.shape[dims:], t.stride()[dims:]), key=lambda x: x[1]):
-        extent += (size - 1) * stride
-    for stride, size in sorted(zip(t.stride()[:dims], t.shape[:dims])):
+def _is(what: str, name: str, t, dims: int, types, device=None) -> None:
+    """_check, where it finds nothing at less of the host's time."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in types and t.dim() == dims
+            and (device is None or t.device == device)):
+        _check(what, name, t, dims, types, device)
+
+
+def _apart(shape, strides, inner: int) -> bool:
+    """Whether no two of the blocks of `inner` elements that the dimensions number overlap."""
+    extent = inner
+    for stride, size in sorted(zip(strides, shape)):
         if size > 1:
             if stride < extent:
                 return False
@@ -76,68 +81,76 @@ def _apart(t: torch.Tensor, dims: int) -> bool:
     return True
 
 
+# What follows from sizes alone is remembered by them.
+@functools.lru_cache(maxsize=256)
+def _pool_strides(shape, strides):
+    """Strides of pages, slots and heads, 0 where there is but one (and of slots dim); None where
+    the kernels cannot read or write such a pool."""
+    *shape, dim = shape
+    strides, last = [s if n > 1 else 0 for n, s in zip(shape, strides)], strides[3]
+    apart = _apart(shape, strides, dim)
+    if shape[1] == 1:
+        strides[1] = dim
+    if (last != 1 or any(s % 8 or s >= 1 << 31 for s in strides) or strides[1] > _MAX_STRIDE
+            or not apart):
+        return None
+    return strides
+
+
+@functools.lru_cache(maxsize=256)
+def _weight_strides(shape, strides):
+    strides = [s if n > 1 else 0 for n, s in zip(shape, strides)]
+    return strides if max(strides) < 1 << 31 and _apart(shape, strides, 1) else None
+
+
 def _pages(what: str, k_pages, v_pages, weights, tables, lengths) -> GsPages:
     """The checked description of a cache."""
-    _check(what, "k_pages", k_pages, 4, _HALVES)
-    dev = k_pages.device
-    _check(what, "v_pages", v_pages, 4, (k_pages.dtype,), dev)
-    # (a dimension of one page, place or head may have any stride)
-    strides, others = ([s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
-                       for t in (k_pages, v_pages))
-    if v_pages.shape != k_pages.shape or strides != others:
-        raise RuntimeError(f"{what}: k_pages {tuple(k_pages.shape)} and v_pages "
-                           f"{tuple(v_pages.shape)} must have the same shape and strides, got "
-                           f"{k_pages.stride()} and {v_pages.stride()}")
-    pages, page_size, heads, dim = k_pages.shape
-    page_stride, slot_stride, head_stride, _ = strides
+    _is(what, "k_pages", k_pages, 4, _HALVES)
+    dev, dtype, shape = k_pages.device, k_pages.dtype, k_pages.shape
+    _is(what, "v_pages", v_pages, 4, (dtype,), dev)
+    pages, page_size, heads, dim = shape
+    if v_pages.shape != shape:
+        raise RuntimeError(f"{what}: k_pages {tuple(shape)} and v_pages {tuple(v_pages.shape)} must have "
+                           "the same shape")
     if page_size < 1 or heads < 1:
-        raise RuntimeError(f"{what}: k_pages {tuple(k_pages.shape)} has pages of nothing")
+        raise RuntimeError(f"{what}: k_pages {tuple(shape)} has pages of nothing")
     if dim % 8 or not 8 <= dim <= MAX_HEAD_DIM:
         raise RuntimeError(f"{what}: dimension must be a multiple of 8 up to {MAX_HEAD_DIM}, got {dim}")
-    if page_size == 1:
-        slot_stride = dim
-    if (k_pages.stride(3) != 1 or page_stride % 8 or slot_stride % 8 or head_stride % 8
-            or slot_stride > _MAX_STRIDE or max(strides) >= 1 << 31 or k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16
-            or not _apart(k_pages, 3)):
-        raise RuntimeError(f"{what}: k_pages and v_pages must begin on 16 bytes, with neighbouring "
-                           "elements in the last dimension, other strides that are multiples of 8, "
-                           "below 2^31, that of a page's slots at most 2^23, and rows that do not overlap; "
-                           f"got strides {k_pages.stride()}")
+    strides = _pool_strides(shape, k_pages.stride())
+    if (strides is None or k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16
+            or strides != _pool_strides(shape, v_pages.stride())):
+        raise RuntimeError(f"{what}: k_pages and v_pages must have the same strides, begin on 16 bytes, "
+                           "with neighbouring elements in the last dimension, other strides that are "
+                           "multiples of 8 below 2^31, that of a page's slots at most 2^23, and rows that "
+                           f"do not overlap; got {k_pages.stride()} and {v_pages.stride()}")
     sums = (0, 0, 0)
     if weights is not None:
-        _check(what, "weights", weights, 3, (torch.float32,), dev)
-        if weights.shape != k_pages.shape[:3]:
-            raise RuntimeError(f"{what}: weights must be {tuple(k_pages.shape[:3])}, got "
-                               f"{tuple(weights.shape)}")
-        sums = [s if n > 1 else 0 for n, s in zip(weights.shape, weights.stride())]
-        if max(sums) >= 1 << 31 or not _apart(weights, 3):
+        _is(what, "weights", weights, 3, (torch.float32,), dev)
+        if weights.shape != shape[:3]:
+            raise RuntimeError(f"{what}: weights must be {tuple(shape[:3])}, got {tuple(weights.shape)}")
+        sums = _weight_strides(weights.shape, weights.stride())
+        if sums is None:
             raise RuntimeError(f"{what}: weights overlap in memory or have strides of 2^31 or more, "
                                f"got {weights.stride()}")
-    _check(what, "tables", tables, 2, (torch.int32,), dev)
-    _check(what, "lengths", lengths, 1, (torch.int32,), dev)
+    _is(what, "tables", tables, 2, (torch.int32,), dev)
+    _is(what, "lengths", lengths, 1, (torch.int32,), dev)
     sequences, width = tables.shape
     if lengths.shape[0] != sequences:
         raise RuntimeError(f"{what}: lengths must have {sequences} entries, got {lengths.shape[0]}")
     if width * page_size > MAX_SLOTS:
         raise RuntimeError(f"{what}: at most {MAX_SLOTS} slots a sequence are supported, got "
                            f"{width} pages of {page_size}")
-    return GsPages(pages, page_stride, slot_stride, head_stride, *sums, tables.data_ptr(),
-                   lengths.data_ptr(), tables.stride(0), width, sequences, page_size, heads, dim,
-                   _TYPES[k_pages.dtype])
+    return GsPages(pages, *strides, *sums, tables.data_ptr(), lengths.data_ptr(), tables.stride(0),
+                   width, sequences, page_size, heads, dim, _TYPES[dtype])
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t with neighbouring entries in its last dimension."""
-    return t if t.stride(-1) == 1 else t.contiguous()
-
-
-def _tables(what, *tensors):
-    """Tables, lengths and offsets with neighbouring entries (what is no tensor is refused later)."""
-    return (_rows(t) if isinstance(t, torch.Tensor) and t.dim() else t for t in tensors)
+def _rows(t):
+    """t with neighbouring entries in its last dimension (what is no tensor is refused later)."""
+    return t.contiguous() if isinstance(t, torch.Tensor) and t.dim() and t.stride(-1) != 1 else t
 
 
 def _offsets(what: str, offsets, tables) -> None:
-    _check(what, "offsets", offsets, 1, (torch.int32,), tables.device)
+    _is(what, "offsets", offsets, 1, (torch.int32,), tables.device)
     if offsets.shape[0] != tables.shape[0] + 1:
         raise RuntimeError(f"{what}: offsets must have {tables.shape[0] + 1} entries, got "
                            f"{offsets.shape[0]}")
@@ -156,12 +169,12 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     tables, offsets to the tokens.  Two tokens on one place of a page (a page that two tables have) leave either."""
     what = "paged_append"
     _no_gradient(what, k, v, k_pages, v_pages, weights)
-    tables, lengths, offsets = _tables(what, tables, lengths, offsets)
+    tables, lengths, offsets = _rows(tables), _rows(lengths), _rows(offsets)
     p = _pages(what, k_pages, v_pages, weights, tables, lengths)
     dev = k_pages.device
     for name, t in (("k", k), ("v", v)):
-        _check(what, name, t, 3, (k_pages.dtype,), dev)
-        if tuple(t.shape[1:]) != (p.heads, p.dim):
+        _is(what, name, t, 3, (k_pages.dtype,), dev)
+        if t.shape[1] != p.heads or t.shape[2] != p.dim:
             raise RuntimeError(f"{what}: {name} must have {p.heads} heads of {p.dim}, got "
                                f"{tuple(t.shape)}")
     if k.shape != v.shape:
@@ -202,10 +215,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     are as packed_attention's; queries with a log-sum of -infinity add no weights."""
     what = "paged_attention"
     _no_gradient(what, q, k_pages, v_pages, weights)
-    tables, lengths, offsets = _tables(what, tables, lengths, offsets)
+    tables, lengths, offsets = _rows(tables), _rows(lengths), _rows(offsets)
     p = _pages(what, k_pages, v_pages, weights, tables, lengths)
     dev = k_pages.device
-    _check(what, "q", q, 3, (k_pages.dtype,), dev)
+    _is(what, "q", q, 3, (k_pages.dtype,), dev)
     heads = q.shape[1]
     if q.shape[2] != p.dim:
         raise RuntimeError(f"{what}: q must have dimension {p.dim}, got {tuple(q.shape)}")
@@ -253,12 +266,12 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     (sequences, key_heads, keep)) which, rising, -1 behind the last."""
     what = "paged_evict"
     _no_gradient(what, k_pages, v_pages, weights)
-    tables, lengths, new_tables = _tables(what, tables, lengths, new_tables)
+    tables, lengths, new_tables = _rows(tables), _rows(lengths), _rows(new_tables)
     if weights is None:
         raise RuntimeError(f"{what}: weights must be a torch.Tensor, got NoneType")
     p = _pages(what, k_pages, v_pages, weights, tables, lengths)
     dev = k_pages.device
-    _check(what, "new_tables", new_tables, 2, (torch.int32,), dev)
+    _is(what, "new_tables", new_tables, 2, (torch.int32,), dev)
     keep, recent = int(keep), int(recent)
     if keep < 1 or not 0 <= recent <= keep:
         raise ValueError(f"{what}: keep must be at least 1 and recent from 0 to keep, got {keep} "

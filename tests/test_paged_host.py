@@ -13,7 +13,7 @@ import helpers  # noqa: F401
 import cuda_rasterizer as cr
 from cuda_rasterizer import _lib
 from cuda_rasterizer._lib import GsPagedQueries, GsPages
-from cuda_rasterizer.paged import _apart
+from cuda_rasterizer.paged import _pool_strides, _weight_strides
 from oracle import paged as op
 from oracle import tokens as ot
 
@@ -126,13 +126,23 @@ def test_refuses_cpu_tensors():
 
 
 def test_rows_that_overlap_are_found():
+    def apart(t):
+        return _pool_strides(t.shape, t.stride()) is not None
+
     t = torch.zeros(6, 5, 4, 8)
-    assert _apart(t, 3) and _apart(t.transpose(1, 2), 3) and _apart(t[::2, 1:, :2], 3)
-    assert _apart(t[..., 0], 3) and _apart(t[:0], 3)
-    assert not _apart(t[:1].expand(6, 5, 4, 8), 3) and not _apart(t[:, :, :1].expand(6, 5, 4, 8), 3)
-    assert not _apart(t.as_strided((6, 5, 4, 8), (160, 32, 4, 1)), 3)
-    assert not _apart(t.as_strided((6, 5, 4, 8), (160, 24, 8, 1)), 3)
-    assert _apart(t.as_strided((1, 5, 1, 8), (0, 8, 3, 1)), 3)
+    assert apart(t) and apart(t.transpose(1, 2)) and apart(t[::2, 1:, :2]) and apart(t[:0])
+    assert not apart(t[:1].expand(6, 5, 4, 8)) and not apart(t[:, :, :1].expand(6, 5, 4, 8))
+    assert not apart(t.as_strided((6, 5, 4, 8), (160, 32, 4, 1)))
+    assert not apart(t.as_strided((6, 5, 4, 8), (160, 24, 8, 1)))
+    assert not apart(t.as_strided((2, 2, 2, 8), (64, 32, 12, 1))) and not apart(t[..., ::2])
+    assert _pool_strides((1, 5, 1, 8), (0, 8, 3, 1)) == [0, 8, 0]
+    assert _pool_strides((6, 1, 4, 8), (32, 3, 8, 1)) == [32, 8, 8]
+    assert _pool_strides((6, 5, 1, 8), (1 << 31, 8, 8, 1)) is None
+    assert _pool_strides((6, 5, 1, 8), (1 << 30, 1 << 24, 8, 1)) is None
+    w = t[..., 0]
+    assert _weight_strides(w.shape, w.stride()) == [160, 32, 8]
+    assert _weight_strides((6, 5, 4), (20, 4, 0)) is None and _weight_strides((6, 5, 4), (1, 6, 30))
+    assert _weight_strides((6, 5, 4), (1 << 31, 4, 1)) is None
 
 
 # ----------------------------------------------------------------- the oracle
