@@ -603,7 +603,7 @@ __device__ __forceinline__ void forward_shared(const GsAttention &a, const Sourc
         const int rest = number / a.heads_k;
         forward_rows<T, DIM, BY_KEYS, true>(a, source, q, out, out_rest, log_sum, partial, lds,
                                             number % a.heads_k, sequence, rest / splits, rest % splits,
-                                         share_of(t));
+                                            share_of(t));
         __syncthreads();  // LDS has been read
     }
 }

@@ -195,12 +195,75 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_split_kernel(
                                   partial, (lds_char *)lds);
 }
 
+// Few rows with many splits: a workgroup a row.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_join_kernel(int64_t rows, int dim, Partial partial,
                                                          T *__restrict__ out,
                                                          float *__restrict__ log_sum) {
     __shared__ f32x4 sums[8][32];
     join_row<T>(rows, dim, partial, out, (T *)nullptr, log_sum, sums);
+}
+
+// Many rows with few splits: 32 threads a row, four elements each; a lane has the maximum and the
+// sum of two splits.  6864 rows of up to 16 splits, dim 72: 5.9 us, and 9.0 in workgroups a row; 256
+// rows of 28, dim 128: 6.9 and 4.8.
+constexpr int kJoinRows = 8;  // of a workgroup
+
+template <typename T>
+__global__ __launch_bounds__(32 * kJoinRows) void paged_join_rows_kernel(
+    int64_t rows, int dim, Partial partial, T *__restrict__ out, float *__restrict__ log_sum) {
+    const int lane = threadIdx.x % 32, column = 4 * lane, half = __lane_id() & 32;
+    const int64_t at = (int64_t)blockIdx.x * kJoinRows + threadIdx.x / 32;
+    const int64_t row = at < rows ? at : rows - 1;  // (every lane takes part in the exchanges)
+    const int splits = min(partial.count[row], partial.splits);
+    float most[2], weight[2], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int s = lane + 32 * n;
+        const float2 x = s < splits ? partial.max_sum[s * rows + row] : make_float2(-INFINITY, 0.0f);
+        most[n] = x.x;
+        weight[n] = x.y;
+        top = fmaxf(top, x.x);
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const float share = most[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(most[n] - top);
+        sum += most[n] == -INFINITY ? 0.0f : weight[n] * share;
+        weight[n] = share;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor(sum, o, kWave);
+    const int all = max(splits, __shfl_xor(splits, 32, kWave));  // (the same rounds in every lane)
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kAhead = 4;
+    for (int first = 0; first < all; first += kAhead) {
+        f32x4 part[kAhead];
+        float w[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int s = first + i, from = half + (s & 31);
+            w[i] = s < 32 ? __shfl(weight[0], from, kWave) : __shfl(weight[1], from, kWave);
+            // (a split that saw nothing has written no sums, and those past the last are as it)
+            const float m = s < 32 ? __shfl(most[0], from, kWave) : __shfl(most[1], from, kWave);
+            part[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (m != -INFINITY && s < splits && column < dim)
+                part[i] = *(const f32x4 *)(partial.sums + (s * rows + row) * dim + column);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) x += part[i] * w[i];
+    }
+    if (at >= rows) return;
+    const bool none = top == -INFINITY;
+    const float r = 1.0f / sum;
+    if (column < dim) {
+        float o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = none ? 0.0f : x[i] * r;
+        store_floats<T, 4>(out + row * dim + column, o);
+    }
+    if (log_sum && lane == 0) log_sum[row] = none ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 // ---------------------------------------------------------------- slots' weights
@@ -462,17 +525,26 @@ static GsAttention problem_of(const GsPages &p, const GsPagedQueries &q) {
     return a;
 }
 
+// As the packed kernels', but that a call's few tiles of rows take splits of equal length across
+// sequences, as many as make kSplits items in all; a sequence longer than the others may have twice
+// as many as the average.  5 sequences of up to 300 over 8044 to 16320 slots, 12 heads on 4, dim 72:
+// 85 us in equal splits of each sequence, 77 in equal splits of all; 1200 rows over 20000, 16 heads
+// on 4, dim 128: 393 in 1, 243.  Not over short tables (600 over 1000: 34 in 1, 44), and not where the
+// tiles fill the GPU once (2500 over 10000: 260 in 1, 434): a second workgroup on a CU adds little.
 static ForwardPlan plan_of(const GsPages &p, const GsAttention &a) {
     const int64_t slots = (int64_t)p.page_size * p.table_width;
     ForwardPlan f = plan_forward(a, slots, slots);
-    // Few tiles of rows: as many splits as make kSplits items in all, which the workgroups find from
-    // the lengths.  A sequence longer than the others may have twice as many as the average.
-    if (!f.by_keys && f.splits > 1) {
-        const int64_t most = (slots + 255) / 256;
-        f.splits = (int)(2 * f.splits < most ? 2 * f.splits : most);
-        if (f.splits > 64) f.splits = 64;
-        if (f.groups > 1024) f.groups = 1024;
-    }
+    if (f.by_keys) return f;
+    const int64_t packed = a.rows_q * (a.heads_q / a.heads_k), rows = 32 * kWaves;
+    const int64_t busy = (packed + rows - 1) / rows * a.heads_k;
+    f.splits = 1;
+    f.groups = (packed / rows + a.sequences + 2) * a.heads_k;
+    if (busy < 1 || busy > 256 || slots < 2048) return f;
+    const int64_t want = 2 * ((kSplits + busy - 1) / busy), most = slots / 256;
+    f.splits = (int)(want < most ? want : most);
+    if (f.splits > 64) f.splits = 64;
+    f.groups *= f.splits;
+    if (f.groups > 1024) f.groups = 1024;
     return f;
 }
 
@@ -507,8 +579,13 @@ static int launch(const GsPages &p, const GsAttention &a, const ForwardPlan &f, 
     const int st = launch_status();
     if (st || f.splits == 1) return st;
     const int64_t rows = a.rows_q * a.heads_q;
-    hipLaunchKernelGGL((paged_join_kernel<T>), dim3((unsigned)rows), dim3(256), 0, stream, rows, a.dim,
-                       partial, out, log_sum);
+    if (f.by_keys)
+        hipLaunchKernelGGL((paged_join_kernel<T>), dim3((unsigned)rows), dim3(256), 0, stream, rows, a.dim,
+                           partial, out, log_sum);
+    else
+        hipLaunchKernelGGL((paged_join_rows_kernel<T>),
+                           dim3((unsigned)((rows + kJoinRows - 1) / kJoinRows)), dim3(32 * kJoinRows), 0,
+                           stream, rows, a.dim, partial, out, log_sum);
     return launch_status();
 }
 
