@@ -4,12 +4,15 @@ Every 16x16 tile of a view is a token: its pixels and the rays through them.  To
 scene's views follow one another, scenes of different numbers of views are packed, and each
 token sees its scene's views up to its own place (causal), so that views may arrive one by one:
 `predict_next` gives a new view's Gaussians from its tokens and a cache of the earlier views'
-keys and values, without looking at those again.
+keys and values, without looking at those again: `Cache`, a slab of rows a scene, or `PagedCache`,
+pages of one pool, which scenes take as they grow and leave when the keys that got the least
+attention are evicted.
 
 A block is  x += attention(layer_norm(x));  x += mlp(layer_norm(x))  with
   layer_norm        normalisation (bfloat16 tokens, float32 weights)
   axial_rotary      rotary positions by view, tile row and tile column
   packed_attention  grouped heads over the packed scenes, or over the cache
+  paged_append, paged_attention, paged_evict   the same over pages
 and the last layer gives each token a grid of Gaussians along its rays, which render_l1 draws and
 compares with a view; the loss goes back through all of it into float32 weights.
 
@@ -23,7 +26,8 @@ import math
 
 import torch
 
-from cuda_rasterizer import axial_frequencies, axial_rotary, layer_norm, packed_attention
+from cuda_rasterizer import (axial_frequencies, axial_rotary, layer_norm, packed_attention,
+                             paged_append, paged_attention, paged_evict)
 from cuda_rasterizer.fused import render_l1
 from cuda_rasterizer.train import FusedAdam
 from cuda_rasterizer.wrapper import render
@@ -99,6 +103,9 @@ class Cache:
         self.lengths = torch.zeros(scenes, dtype=torch.int32, device=device)
         self.offsets = torch.arange(scenes + 1, dtype=torch.int32, device=device) * slab
 
+    def grow(self, new):
+        """Room for `new` tokens of each scene: the slab has it."""
+
     def attend(self, layer, q, k, v, offsets):
         new = offsets.diff()
         scene = torch.repeat_interleave(torch.arange(new.shape[0], device=q.device), new,
@@ -108,6 +115,65 @@ class Cache:
         self.k[layer, at], self.v[layer, at] = k, v
         return packed_attention(q, self.k[layer], self.v[layer], offsets, self.offsets,
                                 self.lengths + new, causal=True)
+
+
+class PagedCache:
+    """Keys and values of the views so far in pages that all scenes share; a page's number is the same
+    in every layer's pool.  The host knows how many tokens come, and deals out the pages."""
+
+    def __init__(self, network, scenes, pages, page=64, width=None, device="cuda"):
+        shape = (network.layers, pages, page, network.key_heads, network.dim)
+        self.k = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        self.v = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        self.weights = torch.zeros(shape[:4], device=device)
+        self.page, self.free = page, list(range(pages))
+        self.tables = torch.full((scenes, width or pages), -1, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(scenes, dtype=torch.int32, device=device)
+        self.owned, self.filled = [[] for _ in range(scenes)], [0] * scenes
+
+    def _take(self, tokens):
+        count = -(-tokens // self.page)
+        if count > len(self.free):
+            raise RuntimeError(f"{count} pages are wanted and {len(self.free)} are free")
+        taken, self.free = self.free[:count], self.free[count:]
+        return taken
+
+    def _deal(self):
+        table = torch.full(self.tables.shape, -1, dtype=torch.int32)
+        for b, pages in enumerate(self.owned):
+            table[b, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+        self.tables.copy_(table)
+
+    def grow(self, new):
+        """Room for `new` tokens of each scene."""
+        for b, n in enumerate(new):
+            self.filled[b] += n
+            self.owned[b] += self._take(self.filled[b] - len(self.owned[b]) * self.page)
+        self._deal()
+
+    def attend(self, layer, q, k, v, offsets):
+        lengths = self.lengths + offsets.diff()
+        pools = self.k[layer], self.v[layer], self.tables, lengths, offsets
+        paged_append(k, v, *pools, weights=self.weights[layer])
+        return paged_attention(q, *pools, causal=True, weights=self.weights[layer])
+
+    def evict(self, keep, recent):
+        """Scenes of more than `keep` tokens keep so many: the last `recent`, and those that got the
+        most attention so far, each layer and key head its own."""
+        full = [b for b, n in enumerate(self.filled) if n > keep]
+        if not full:
+            return
+        fresh = [self._take(keep) for _ in full]
+        rows = torch.tensor(full, device=self.tables.device)
+        new_tables = torch.tensor(fresh, dtype=torch.int32).to(self.tables.device)
+        for layer in range(self.k.shape[0]):
+            lengths, _ = paged_evict(self.k[layer], self.v[layer], self.weights[layer], self.tables[rows],
+                                     self.lengths[rows], new_tables, keep, recent)
+        self.lengths[rows] = lengths
+        for b, pages in zip(full, fresh):
+            self.free += self.owned[b]
+            self.owned[b], self.filled[b] = pages, keep
+        self._deal()
 
 
 # --------------------------------------------------------------- views and tokens
@@ -231,6 +297,7 @@ def predict_next(network, cache, views, number):
     parts = [tokens_of(v, number) for v in views if v is not None]
     lengths = [0 if v is None else v[0].shape[0] * v[0].shape[1] // TILE ** 2 for v in views]
     offsets = torch.tensor([0] + lengths, device=cache.lengths.device).cumsum(0).to(torch.int32)
+    cache.grow(lengths)
     return network(torch.cat([t for t, _ in parts]), torch.cat([p for _, p in parts]), offsets, cache)
 
 
@@ -247,14 +314,25 @@ def main():
         whole = network(*batch)
     per_view = a.width * a.height // TILE ** 2
     most = max(len(s) for s in scenes)
-    cache = Cache(network, len(scenes), most * per_view)
-    worst, starts = 0.0, batch[2][:-1].tolist()
-    for i in range(most):
-        there = [b for b, s in enumerate(scenes) if i < len(s)]
-        got = predict_next(network, cache, [s[i] if i < len(s) else None for s in scenes], i)
-        want = torch.cat([whole[starts[b] + i * per_view:starts[b] + (i + 1) * per_view] for b in there])
-        worst = max(worst, float((got - want).norm() / want.norm()))
-    print(f"a view at a time against all at once: {worst:.4f} apart")
+    starts = batch[2][:-1].tolist()
+
+    def apart(cache, after=lambda: None):
+        worst = 0.0
+        for i in range(most):
+            there = [b for b, s in enumerate(scenes) if i < len(s)]
+            got = predict_next(network, cache, [s[i] if i < len(s) else None for s in scenes], i)
+            want = torch.cat([whole[starts[b] + i * per_view:starts[b] + (i + 1) * per_view] for b in there])
+            worst = max(worst, float((got - want).norm() / want.norm()))
+            after()
+        return worst
+
+    slabs = Cache(network, len(scenes), most * per_view)
+    print(f"a view at a time against all at once: {apart(slabs):.4f} apart")
+    room = len(scenes) * (most * per_view // 16 + 1)
+    print(f"  over pages of 16 tokens: {apart(PagedCache(network, len(scenes), room, 16)):.4f}")
+    pages = PagedCache(network, len(scenes), room, 16)
+    few = apart(pages, lambda: pages.evict(2 * per_view, per_view))
+    print(f"  and no more than two views' tokens kept: {few:.4f}")
 
 
 if __name__ == "__main__":
