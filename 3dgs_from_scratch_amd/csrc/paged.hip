@@ -264,23 +264,24 @@ __global__ __launch_bounds__(256) void paged_move_kernel(GsPages p, uint16_t *k_
                                                          const int32_t *__restrict__ new_tables,
                                                          int64_t new_stride, int32_t keep,
                                                          const int32_t *__restrict__ kept) {
-    const int chunks = p.dim / 8, a_row = chunks * p.heads, b = blockIdx.y;
+    const int chunks = p.dim / 8, a_row = chunks * p.heads;
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t row = at / a_row;
     if (row >= keep) return;
     const int rest = (int)(at - row * a_row), head = rest / chunks, chunk = rest - head * chunks;
-    const int j = (int)row;
-    const int slot = kept[((int64_t)b * p.heads + head) * keep + j];
-    if (slot < 0) return;
-    const int to_page = new_tables[b * new_stride + j / p.page_size], to_place = j % p.page_size;
-    if ((uint32_t)to_page >= (uint64_t)p.pages) return;
-    const int page = page_of(p, b, slot / p.page_size), place = slot % p.page_size;
-    const int64_t from = row_at(p, page, place) + head * p.head_stride + chunk * 8;
-    const int64_t to = row_at(p, to_page, to_place) + head * p.head_stride + chunk * 8;
-    *(Chunk *)(k_pages + to) = *(const Chunk *)(k_pages + from);
-    *(Chunk *)(v_pages + to) = *(const Chunk *)(v_pages + from);
-    if (chunk == 0)
-        weights[sum_at(p, to_page, to_place, head)] = weights[sum_at(p, page, place, head)];
+    const int j = (int)row, index = j / p.page_size, to_place = j - index * p.page_size;
+    for (int b = blockIdx.y; b < p.sequences; b += gridDim.y) {
+        const int slot = kept[((int64_t)b * p.heads + head) * keep + j];
+        const int to_page = new_tables[b * new_stride + index];
+        if (slot < 0 || (uint32_t)to_page >= (uint64_t)p.pages) continue;
+        const int page = page_of(p, b, slot / p.page_size), place = slot % p.page_size;
+        const int64_t from = row_at(p, page, place) + head * p.head_stride + chunk * 8;
+        const int64_t to = row_at(p, to_page, to_place) + head * p.head_stride + chunk * 8;
+        *(Chunk *)(k_pages + to) = *(const Chunk *)(k_pages + from);
+        *(Chunk *)(v_pages + to) = *(const Chunk *)(v_pages + from);
+        if (chunk == 0)
+            weights[sum_at(p, to_page, to_place, head)] = weights[sum_at(p, page, place, head)];
+    }
 }
 
 int check_pages(const GsPages *p, bool weights) {
@@ -344,8 +345,7 @@ extern "C" int gs_paged_evict(const GsPages *p, void *k_pages, void *v_pages, fl
     if (!aligned16(k_pages) || !aligned16(v_pages)) return GS_ERR_UNSUPPORTED;
     const int64_t picks = (int64_t)p->sequences * p->heads;
     const int64_t groups = ((int64_t)keep * (p->dim / 8) * p->heads + 255) / 256;
-    if (picks > 0x7fffffffLL || groups > 0x7fffffffLL || p->sequences > 65535)
-        return GS_ERR_UNSUPPORTED;
+    if (picks > 0x7fffffffLL || groups > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
     // (by the slots that a table could hold: what is filled is not known here)
     const int64_t slots = (int64_t)p->page_size * p->table_width;
     const bool held = slots <= kHeld, whole = p->page_size % kWave == 0;
@@ -354,8 +354,8 @@ extern "C" int gs_paged_evict(const GsPages *p, void *k_pages, void *v_pages, fl
                              : whole ? paged_pick_kernel<false, true> : paged_pick_kernel<false, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)picks), dim3(kPick), lds, stream, *p,
                        (const float *)weights, keep, recent, new_lengths, kept);
-    hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)groups, (unsigned)p->sequences), dim3(256),
-                       0, stream, *p, (uint16_t *)k_pages, (uint16_t *)v_pages, weights, new_tables,
+    hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)groups, (unsigned)(p->sequences < 65535 ? p->sequences : 65535)),
+                       dim3(256), 0, stream, *p, (uint16_t *)k_pages, (uint16_t *)v_pages, weights, new_tables,
                        new_stride, keep, (const int32_t *)kept);
     return launch_status();
 }

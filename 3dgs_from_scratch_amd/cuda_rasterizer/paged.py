@@ -207,8 +207,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     With weights also adds to each slot's weight the probabilities that it gets, summed over
     the sequence's queries and the heads that share its key head, in float32 and in an order
-    that depends on the sizes and tables alone.  A page that two sequences share gets its
-    weights from one of them, whichever.
+    that depends on the sizes and tables alone.  A page that the tables hold twice gets its
+    weights from one of its places there, whichever.
 
     scale defaults to dim ** -0.5.  With return_log_sum also the float32 (queries, heads)
     natural logarithm of each softmax's denominator.  Types, rounding and what is not finite
@@ -279,6 +279,8 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     if new_tables.shape[0] != p.sequences or new_tables.shape[1] * p.page_size < keep:
         raise RuntimeError(f"{what}: new_tables must have {p.sequences} rows of "
                            f"{-(-keep // p.page_size)} pages at least, got {tuple(new_tables.shape)}")
+    if new_tables.data_ptr() == tables.data_ptr() and tables.numel():
+        raise ValueError(f"{what}: new_tables are the tables that are read; slots move to other pages")
     new_lengths = torch.empty(p.sequences, dtype=torch.int32, device=dev)
     kept = torch.empty((p.sequences, p.heads, keep), dtype=torch.int32, device=dev)
     with _lib.on_device(dev):

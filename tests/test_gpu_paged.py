@@ -364,6 +364,33 @@ def test_attention_of_what_is_not_finite(gpu):
                 c.v[there] = was
 
 
+@pytest.mark.parametrize("page", [24, 64])
+def test_attention_of_skewed_chunks(gpu, page):
+    """One long chunk among single tokens, and one long cache among short ones."""
+    for dtype in TYPES:
+        for lengths, new in (([2000] + [30] * 40, [300] + [1] * 40), ([20, 9000, 1] + [5] * 70, [1] * 73),
+                             ([6000, 300, 2500], [130, 1, 0])):
+            c = Cache(gpu, lengths, page, 2, 64, dtype)
+            check_attention(queries(gpu, sum(new), 4, 64, dtype), c, offsets_of(new, gpu))
+
+
+@pytest.mark.parametrize("page", [24, 64])
+@pytest.mark.parametrize("lengths,new", [([300], [300]), ([5000], [1]), ([3000], [100])])
+def test_attention_of_keys_that_all_score_minus_infinity(gpu, lengths, new, page):
+    """Seen, they give NaN and no weight; on pages that are not there, zeros."""
+    for dtype in TYPES:
+        c = Cache(gpu, lengths, page, 1, 64, dtype)
+        slots = torch.arange(lengths[0], device=gpu)
+        at = c.tables[0, slots // page].long(), slots % page
+        c.k[at], c.v[at], c.w[at] = -math.inf, 1.0, 0.5
+        q, offsets = torch.ones(new[0], 2, 64, dtype=dtype, device=gpu), offsets_of(new, gpu)
+        out = cr.paged_attention(q, *c.args(), offsets, weights=c.w)
+        assert bool(torch.isnan(out).all()) and bool((c.w[at] == 0.5).all())
+        c.tables.fill_(-1)
+        out = cr.paged_attention(q, *c.args(), offsets, weights=c.w)
+        assert bool((out == 0).all()) and bool((c.w[at] == 0.5).all())
+
+
 # ------------------------------------------------------------------- eviction
 def check_evict(c, new_tables, keep, recent=0):
     want = op.evict(c.k, c.v, c.w, c.tables, c.lengths, new_tables, keep, recent)
@@ -428,7 +455,8 @@ def test_evict_without_some_pages(gpu):
         check_evict(c, new_tables, keep, 30)
 
 
-@pytest.mark.parametrize("length,keep", [(70_000, 30_000), (140_001, 3), (40_000, 39_999)])
+@pytest.mark.parametrize("length,keep", [(20_000, 9000), (32_768, 20_000), (32_769, 100), (70_000, 30_000),
+                                         (140_001, 3), (40_000, 39_999)])
 def test_evict_of_long_sequences(gpu, length, keep):
     fresh = -(-keep // 64)
     c = Cache(gpu, [length, 500], 64, 2, 8, torch.float16, spare=2 * fresh)
@@ -598,6 +626,8 @@ def test_refusals(gpu):
         if what == "paged_evict":
             bad += [dict(new_tables=fresh.long()), dict(new_tables=fresh[:1]), dict(new_tables=fresh[0]),
                     dict(keep=17), dict(weights=None)]
+            with pytest.raises(ValueError, match="other pages"):
+                call(**{**good, "new_tables": c.tables})
             for keep, recent in ((0, 0), (16, 17), (16, -1), (-3, 0)):
                 with pytest.raises(ValueError, match=what):
                     call(**{**good, "keep": keep, "recent": recent})
