@@ -300,7 +300,8 @@ constexpr int kScoreSlots = 256;           // of one where the scores are there
 template <typename T, int DIM>
 struct SlotOperand {
     RowOperand<T, DIM> k;
-    float *weight;  // null: no such slot
+    float *weight;        // null: no such slot
+    float before = 0.0f;  // what it is, read beside the key
     __device__ __forceinline__ SlotOperand(const GsPages &p, const T *keys, float *weights, int sequence,
                                            int slot, int filled, int kh, bool negate)
         : weight(nullptr) {
@@ -314,6 +315,12 @@ struct SlotOperand {
             }
         }
         k.load(row, p.dim, negate);
+        if (weight) before = *weight;
+    }
+    // sum: of the lane's rows, half of all
+    __device__ __forceinline__ void add(float sum) const {
+        sum = half_sum(sum);
+        if (__lane_id() < 32 && weight) *weight = before + sum;
     }
 };
 
@@ -366,7 +373,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
         const int q0 = uniform(rows.x), lq = uniform(rows.y - rows.x);
         const int filled = uniform(slots_of(p, sequence));
         const int slot0 = tile * kWeightSlots + 32 * wave, slot = slot0 + (lane & 31);
-        const SlotOperand<T, DIM> mine(p, k, weights, sequence, slot, filled, kh, a.scale < 0.0f);
         // query i sees slots up to i + shift
         const int shift = a.causal ? filled - lq : filled;
         const int first = max(tile * kWeightSlots - shift, 0) / kRows;
@@ -384,10 +390,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
         };
         float sum = 0.0f;
         int now = first;
-        if (steps > 0) {
-            fetch(0);
-            if (wave == 0) minus[0][lane] = next;
-        }
+        if (steps > 0) fetch(0);
+        // (beside the first copy)
+        const SlotOperand<T, DIM> mine(p, k, weights, sequence, slot, filled, kh, a.scale < 0.0f);
+        if (steps > 0 && wave == 0) minus[0][lane] = next;
         for (int t = 0; t < steps; ++t) {
             copies_done();
             if (t + 1 < steps) fetch((t + 1) & 1);
@@ -419,8 +425,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
             if (++now == first + tiles) now = first;
             if (wave == 0 && t + 1 < steps) minus[(t + 1) & 1][lane] = next;
         }
-        sum = half_sum(sum);
-        if (half == 0 && mine.weight) *mine.weight += sum;
+        mine.add(sum);
         __syncthreads();  // LDS has been read
     });
 }
@@ -460,8 +465,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_few_weights_kernel(
             const int least = max(slot - shift, 0) * group - row0;
             sum += sum_of_weights<true>(s, c, m, [&](int i) { return i >= least && row0 + i < rows; });
         }
-        sum = half_sum(sum);
-        if (half == 0 && mine.weight) *mine.weight += sum;
+        mine.add(sum);
     });
 }
 
