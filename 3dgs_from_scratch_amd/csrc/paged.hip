@@ -270,18 +270,18 @@ __global__ __launch_bounds__(256) void paged_move_kernel(GsPages p, uint16_t *k_
     if (row >= keep) return;
     const int rest = (int)(at - row * a_row), head = rest / chunks, chunk = rest - head * chunks;
     const int j = (int)row, index = j / p.page_size, to_place = j - index * p.page_size;
-    for (int b = blockIdx.y; b < p.sequences; b += gridDim.y) {
-        const int slot = kept[((int64_t)b * p.heads + head) * keep + j];
-        const int to_page = new_tables[b * new_stride + index];
-        if (slot < 0 || (uint32_t)to_page >= (uint64_t)p.pages) continue;
-        const int page = page_of(p, b, slot / p.page_size), place = slot % p.page_size;
-        const int64_t from = row_at(p, page, place) + head * p.head_stride + chunk * 8;
-        const int64_t to = row_at(p, to_page, to_place) + head * p.head_stride + chunk * 8;
-        *(Chunk *)(k_pages + to) = *(const Chunk *)(k_pages + from);
-        *(Chunk *)(v_pages + to) = *(const Chunk *)(v_pages + from);
-        if (chunk == 0)
-            weights[sum_at(p, to_page, to_place, head)] = weights[sum_at(p, page, place, head)];
-    }
+    const int64_t b = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+    if (b >= p.sequences) return;
+    const int slot = kept[(b * p.heads + head) * keep + j];
+    const int to_page = new_tables[b * new_stride + index];
+    if (slot < 0 || (uint32_t)to_page >= (uint64_t)p.pages) return;
+    const int page = page_of(p, (int)b, slot / p.page_size), place = slot % p.page_size;
+    const int64_t from = row_at(p, page, place) + head * p.head_stride + chunk * 8;
+    const int64_t to = row_at(p, to_page, to_place) + head * p.head_stride + chunk * 8;
+    *(Chunk *)(k_pages + to) = *(const Chunk *)(k_pages + from);
+    *(Chunk *)(v_pages + to) = *(const Chunk *)(v_pages + from);
+    if (chunk == 0)
+        weights[sum_at(p, to_page, to_place, head)] = weights[sum_at(p, page, place, head)];
 }
 
 int check_pages(const GsPages *p, bool weights) {
@@ -354,7 +354,9 @@ extern "C" int gs_paged_evict(const GsPages *p, void *k_pages, void *v_pages, fl
                              : whole ? paged_pick_kernel<false, true> : paged_pick_kernel<false, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)picks), dim3(kPick), lds, stream, *p,
                        (const float *)weights, keep, recent, new_lengths, kept);
-    hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)groups, (unsigned)(p->sequences < 65535 ? p->sequences : 65535)),
+    const int32_t rows = p->sequences < 65535 ? p->sequences : 65535;  // of the grid's second dimension
+    hipLaunchKernelGGL(paged_move_kernel,
+                       dim3((unsigned)groups, (unsigned)rows, (unsigned)((p->sequences + rows - 1) / rows)),
                        dim3(256), 0, stream, *p, (uint16_t *)k_pages, (uint16_t *)v_pages, weights, new_tables,
                        new_stride, keep, (const int32_t *)kept);
     return launch_status();

@@ -398,28 +398,39 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
             copies_done();
             if (t + 1 < steps) fetch((t + 1) & 1);
             const lds_char *qt = (const lds_char *)lds + (t & 1) * QTile::kBytes;
-            f32x16 s[2] = {};
+            const auto minus_of = [&](int n, float *m) {
 #pragma unroll
-            for (int i = 0; i < DIM / 16; ++i)
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 x = *(const f32x4 *)&minus[t & 1][32 * n + result_row(4 * g, half)];
 #pragma unroll
-                for (int n = 0; n < 2; ++n) s[n] = mfma(QTile::along(qt, 32 * n, i), mine.k.x[i], s[n]);
-            float m[2][16];
-#pragma unroll
-            for (int g = 0; g < 8; ++g) {
-                const f32x4 x = *(const f32x4 *)&minus[t & 1][32 * (g / 4) + result_row(4 * (g % 4), half)];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) m[g / 4][4 * (g % 4) + i] = x[i];
-            }
+                    for (int i = 0; i < 4; ++i) m[4 * g + i] = x[i];
+                }
+            };
             const int row0 = now * kRows;
             if (row0 + shift >= slot0 + 31 && row0 + kRows <= lq) {
+                f32x16 s[2] = {};
 #pragma unroll
-                for (int n = 0; n < 2; ++n) sum += sum_of_weights<false>(s[n], c, m[n], [](int) { return true; });
+                for (int i = 0; i < DIM / 16; ++i)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) s[n] = mfma(QTile::along(qt, 32 * n, i), mine.k.x[i], s[n]);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    float m[16];
+                    minus_of(n, m);
+                    sum += sum_of_weights<false>(s[n], c, m, [](int) { return true; });
+                }
             } else {
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const int row = row0 + 32 * n;
+                    if (row >= lq || row + 31 + shift < slot0) continue;
+                    f32x16 s = {};
+#pragma unroll
+                    for (int i = 0; i < DIM / 16; ++i) s = mfma(QTile::along(qt, 32 * n, i), mine.k.x[i], s);
+                    float m[16];
+                    minus_of(n, m);
                     sum += sum_of_weights<true>(
-                        s[n], c, m[n], [&](int i) { return row + i < lq && row + i + shift >= slot; });
+                        s, c, m, [&](int i) { return row + i < lq && row + i + shift >= slot; });
                 }
             }
             if (++now == first + tiles) now = first;
