@@ -12,7 +12,7 @@ the matrix products, its blocks need
   usual frequencies;
 - packed_attention(q, k, v, offsets_q, ...): softmax attention over scenes of any
   sizes packed one after another, grouped heads, causal (a stream of views) or
-  not, or new queries over a cache of earlier keys and values.
+  not, or new queries over a cache of earlier keys and values (paged.py: a cache in pages).
 
 All run on the library's gfx950 kernels on the current HIP stream, without host
 synchronisation, and are differentiable once, backwards (packed_attention in q, k and
