@@ -34,7 +34,7 @@ import functools
 import math
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import GsPagedQueries, GsPages
@@ -49,11 +49,15 @@ def _no_gradient(what: str, *tensors) -> None:
     if torch.jit.is_tracing():
         raise RuntimeError(f"{what} cannot be traced")
     grad = torch.is_grad_enabled()
+    # (outside of every dual level, -1, there are no tangents)
+    dual = getattr(forward_ad, "_current_level", 0) >= 0
+    if not grad and not dual:
+        return
     for t in tensors:
         if isinstance(t, torch.Tensor):
             if grad and t.requires_grad:
                 raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad()")
-            if unpack_dual(t).tangent is not None:
+            if dual and forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
@@ -61,13 +65,6 @@ def _written(*tensors) -> None:
     """Tells autograd that the tensors' values have changed."""
     torch.autograd.graph.increment_version([t for t in tensors
                                             if t is not None and not t.is_inference()])
-
-
-def _is(what: str, name: str, t, dims: int, types, device=None) -> None:
-    """_check, where it finds nothing at less of the host's time."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in types and t.dim() == dims
-            and (device is None or t.device == device)):
-        _check(what, name, t, dims, types, device)
 
 
 def _apart(shape, strides, inner: int) -> bool:
@@ -94,54 +91,85 @@ def _pool_strides(shape, strides):
     if (last != 1 or any(s % 8 or s >= 1 << 31 for s in strides) or strides[1] > _MAX_STRIDE
             or not apart):
         return None
-    return strides
+    return tuple(strides)
 
 
 @functools.lru_cache(maxsize=256)
 def _weight_strides(shape, strides):
-    strides = [s if n > 1 else 0 for n, s in zip(shape, strides)]
+    strides = tuple(s if n > 1 else 0 for n, s in zip(shape, strides))
     return strides if max(strides) < 1 << 31 and _apart(shape, strides, 1) else None
 
 
-def _pages(what: str, k_pages, v_pages, weights, tables, lengths) -> GsPages:
-    """The checked description of a cache."""
-    _is(what, "k_pages", k_pages, 4, _HALVES)
-    dev, dtype, shape = k_pages.device, k_pages.dtype, k_pages.shape
-    _is(what, "v_pages", v_pages, 4, (dtype,), dev)
+@functools.lru_cache(maxsize=256)
+def _layout(what: str, shape, k_strides, v_shape, v_strides, w_shape, w_strides, tables, lengths):
+    """The numbers of a cache's description between its pointers, for sizes that go together."""
     pages, page_size, heads, dim = shape
-    if v_pages.shape != shape:
-        raise RuntimeError(f"{what}: k_pages {tuple(shape)} and v_pages {tuple(v_pages.shape)} must have "
+    if v_shape != shape:
+        raise RuntimeError(f"{what}: k_pages {tuple(shape)} and v_pages {tuple(v_shape)} must have "
                            "the same shape")
     if page_size < 1 or heads < 1:
         raise RuntimeError(f"{what}: k_pages {tuple(shape)} has pages of nothing")
     if dim % 8 or not 8 <= dim <= MAX_HEAD_DIM:
         raise RuntimeError(f"{what}: dimension must be a multiple of 8 up to {MAX_HEAD_DIM}, got {dim}")
-    strides = _pool_strides(shape, k_pages.stride())
-    if (strides is None or k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16
-            or strides != _pool_strides(shape, v_pages.stride())):
-        raise RuntimeError(f"{what}: k_pages and v_pages must have the same strides, begin on 16 bytes, "
+    strides = _pool_strides(shape, k_strides)
+    if strides is None or strides != _pool_strides(shape, v_strides):
+        raise RuntimeError(f"{what}: k_pages and v_pages must have the same strides, "
                            "with neighbouring elements in the last dimension, other strides that are "
                            "multiples of 8 below 2^31, that of a page's slots at most 2^23, and rows that "
-                           f"do not overlap; got {k_pages.stride()} and {v_pages.stride()}")
+                           f"do not overlap; got {k_strides} and {v_strides}")
     sums = (0, 0, 0)
-    if weights is not None:
-        _is(what, "weights", weights, 3, (torch.float32,), dev)
-        if weights.shape != shape[:3]:
-            raise RuntimeError(f"{what}: weights must be {tuple(shape[:3])}, got {tuple(weights.shape)}")
-        sums = _weight_strides(weights.shape, weights.stride())
+    if w_shape is not None:
+        if w_shape != shape[:3]:
+            raise RuntimeError(f"{what}: weights must be {tuple(shape[:3])}, got {tuple(w_shape)}")
+        sums = _weight_strides(w_shape, w_strides)
         if sums is None:
             raise RuntimeError(f"{what}: weights overlap in memory or have strides of 2^31 or more, "
-                               f"got {weights.stride()}")
-    _is(what, "tables", tables, 2, (torch.int32,), dev)
-    _is(what, "lengths", lengths, 1, (torch.int32,), dev)
-    sequences, width = tables.shape
-    if lengths.shape[0] != sequences:
-        raise RuntimeError(f"{what}: lengths must have {sequences} entries, got {lengths.shape[0]}")
+                               f"got {w_strides}")
+    sequences, width = tables
+    if lengths[0] != sequences:
+        raise RuntimeError(f"{what}: lengths must have {sequences} entries, got {lengths[0]}")
     if width * page_size > MAX_SLOTS:
         raise RuntimeError(f"{what}: at most {MAX_SLOTS} slots a sequence are supported, got "
                            f"{width} pages of {page_size}")
-    return GsPages(pages, *strides, *sums, tables.data_ptr(), lengths.data_ptr(), tables.stride(0),
-                   width, sequences, page_size, heads, dim, _TYPES[dtype])
+    return (pages, *strides, *sums), (width, sequences, page_size, heads, dim)
+
+
+def _pages(what: str, k_pages, v_pages, weights, tables, lengths) -> GsPages:
+    """The checked description of a cache."""
+    if not (_on(k_pages, v_pages, tables, lengths) and (weights is None or (
+            isinstance(weights, torch.Tensor) and weights.dtype is torch.float32
+            and weights.get_device() == k_pages.get_device() and weights.dim() == 3))):
+        _check(what, "k_pages", k_pages, 4, _HALVES)
+        dev = k_pages.device
+        _check(what, "v_pages", v_pages, 4, (k_pages.dtype,), dev)
+        if weights is not None:
+            _check(what, "weights", weights, 3, (torch.float32,), dev)
+        _check(what, "tables", tables, 2, (torch.int32,), dev)
+        _check(what, "lengths", lengths, 1, (torch.int32,), dev)
+    w = (None, None) if weights is None else (weights.shape, weights.stride())
+    first, last = _layout(what, k_pages.shape, k_pages.stride(), v_pages.shape, v_pages.stride(), *w,
+                          tables.shape, lengths.shape)
+    if (k_pages.data_ptr() | v_pages.data_ptr()) % 16:
+        raise RuntimeError(f"{what}: k_pages and v_pages must begin on 16 bytes")
+    return GsPages(*first, tables.data_ptr(), lengths.data_ptr(), tables.stride(0), *last,
+                   _TYPES[k_pages.dtype])
+
+
+# The checks find nothing where these are true, at less of the host's time.
+def _on(k_pages, v_pages, tables, lengths) -> bool:
+    try:
+        device, dtype = k_pages.get_device(), k_pages.dtype
+        return (device >= 0 and dtype in _HALVES and v_pages.dtype is dtype
+                and tables.dtype is torch.int32 and lengths.dtype is torch.int32
+                and device == v_pages.get_device() == tables.get_device() == lengths.get_device()
+                and k_pages.dim() == v_pages.dim() == 4 and tables.dim() == 2 and lengths.dim() == 1)
+    except AttributeError:  # no tensor
+        return False
+
+
+def _heads_on(t, k_pages) -> bool:
+    return (isinstance(t, torch.Tensor) and t.dtype is k_pages.dtype and t.dim() == 3
+            and t.get_device() == k_pages.get_device())
 
 
 def _rows(t):
@@ -150,7 +178,9 @@ def _rows(t):
 
 
 def _offsets(what: str, offsets, tables) -> None:
-    _is(what, "offsets", offsets, 1, (torch.int32,), tables.device)
+    if not (isinstance(offsets, torch.Tensor) and offsets.dtype is torch.int32 and offsets.dim() == 1
+            and offsets.get_device() == tables.get_device()):
+        _check(what, "offsets", offsets, 1, (torch.int32,), tables.device)
     if offsets.shape[0] != tables.shape[0] + 1:
         raise RuntimeError(f"{what}: offsets must have {tables.shape[0] + 1} entries, got "
                            f"{offsets.shape[0]}")
@@ -173,7 +203,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     p = _pages(what, k_pages, v_pages, weights, tables, lengths)
     dev = k_pages.device
     for name, t in (("k", k), ("v", v)):
-        _is(what, name, t, 3, (k_pages.dtype,), dev)
+        if not _heads_on(t, k_pages):
+            _check(what, name, t, 3, (k_pages.dtype,), dev)
         if t.shape[1] != p.heads or t.shape[2] != p.dim:
             raise RuntimeError(f"{what}: {name} must have {p.heads} heads of {p.dim}, got "
                                f"{tuple(t.shape)}")
@@ -218,7 +249,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     tables, lengths, offsets = _rows(tables), _rows(lengths), _rows(offsets)
     p = _pages(what, k_pages, v_pages, weights, tables, lengths)
     dev = k_pages.device
-    _is(what, "q", q, 3, (k_pages.dtype,), dev)
+    if not _heads_on(q, k_pages):
+        _check(what, "q", q, 3, (k_pages.dtype,), dev)
     heads = q.shape[1]
     if q.shape[2] != p.dim:
         raise RuntimeError(f"{what}: q must have dimension {p.dim}, got {tuple(q.shape)}")
@@ -271,7 +303,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
         raise RuntimeError(f"{what}: weights must be a torch.Tensor, got NoneType")
     p = _pages(what, k_pages, v_pages, weights, tables, lengths)
     dev = k_pages.device
-    _is(what, "new_tables", new_tables, 2, (torch.int32,), dev)
+    _check(what, "new_tables", new_tables, 2, (torch.int32,), dev)
     keep, recent = int(keep), int(recent)
     if keep < 1 or not 0 <= recent <= keep:
         raise ValueError(f"{what}: keep must be at least 1 and recent from 0 to keep, got {keep} "

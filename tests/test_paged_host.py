@@ -135,12 +135,12 @@ def test_rows_that_overlap_are_found():
     assert not apart(t.as_strided((6, 5, 4, 8), (160, 32, 4, 1)))
     assert not apart(t.as_strided((6, 5, 4, 8), (160, 24, 8, 1)))
     assert not apart(t.as_strided((2, 2, 2, 8), (64, 32, 12, 1))) and not apart(t[..., ::2])
-    assert _pool_strides((1, 5, 1, 8), (0, 8, 3, 1)) == [0, 8, 0]
-    assert _pool_strides((6, 1, 4, 8), (32, 3, 8, 1)) == [32, 8, 8]
+    assert _pool_strides((1, 5, 1, 8), (0, 8, 3, 1)) == (0, 8, 0)
+    assert _pool_strides((6, 1, 4, 8), (32, 3, 8, 1)) == (32, 8, 8)
     assert _pool_strides((6, 5, 1, 8), (1 << 31, 8, 8, 1)) is None
     assert _pool_strides((6, 5, 1, 8), (1 << 30, 1 << 24, 8, 1)) is None
     w = t[..., 0]
-    assert _weight_strides(w.shape, w.stride()) == [160, 32, 8]
+    assert _weight_strides(w.shape, w.stride()) == (160, 32, 8)
     assert _weight_strides((6, 5, 4), (20, 4, 0)) is None and _weight_strides((6, 5, 4), (1, 6, 30))
     assert _weight_strides((6, 5, 4), (1 << 31, 4, 1)) is None
 
