@@ -48,9 +48,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(
 
 // --------------------------------------------------------------------- evict
 // A weight's place in the order of all floats: larger is larger, both zeros are one, NaN is above
-// infinity.
+// infinity.  No weight's is 0, nor kRecent, which is above all.
+constexpr uint32_t kRecent = 0xffffffffu, kLargest = 0xfffffffeu;
 __device__ __forceinline__ uint32_t order_of(float w) {
-    if (w != w) return 0xffffffffu;
+    if (w != w) return kLargest;
     const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f);  // -0 + 0 = 0
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
@@ -106,10 +107,13 @@ __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int
     const int rounds = rounds_of(filled);            // of a wave
     const int first = wave * rounds * kWave + lane;  // the lane's first slot
     const int more_pages = kWave / p.page_size, more_places = kWave - more_pages * p.page_size;
-    // f(slot, order) for the lane's slots in turn; the order of a slot that is not there is 0, which
-    // no weight has.  Pages and weights of BATCH slots are on their way at a time.
+    // f(slot, order) for the lane's slots in turn; the order of a slot that is not there is 0, that of
+    // a recent one kRecent.  Pages and weights of BATCH slots are on their way at a time.
     const auto from_memory = [&](auto f) {
         constexpr int BATCH = 16;
+        const auto put = [&](int slot, bool is, float w) {
+            f(slot, !is ? 0u : slot >= old ? kRecent : order_of(w));
+        };
         if constexpr (WHOLE) {
             // a lane looks for the page of a round's 64 slots
             for (int i0 = 0; i0 < rounds; i0 += kWave) {
@@ -130,7 +134,7 @@ __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int
 #pragma unroll
                     for (int j = 0; j < BATCH; ++j)
                         if (i0 + j0 + j < rounds)
-                            f(first + (i0 + j0 + j) * kWave, has[j] ? order_of(w[j]) : 0u);
+                            put(first + (i0 + j0 + j) * kWave, has[j], w[j]);
                 }
             }
         } else {
@@ -152,8 +156,7 @@ __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int
                     w[i] = pages[i] >= 0 ? weights[sum_at(p, pages[i], places[i], head)] : 0.0f;
 #pragma unroll
                 for (int i = 0; i < BATCH; ++i)
-                    if (i0 + i < rounds)
-                        f(first + (i0 + i) * kWave, pages[i] >= 0 ? order_of(w[i]) : 0u);
+                    if (i0 + i < rounds) put(first + (i0 + i) * kWave, pages[i] >= 0, w[i]);
             }
         }
     };
@@ -176,7 +179,7 @@ __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int
     uint32_t there = 0, there_old = 0;
     from_memory([&](int slot, uint32_t order) {
         if (HELD) orders[slot] = order;
-        const bool counts = order && slot < old;
+        const bool counts = order - 1 < kRecent - 1;
         there += __popcll(__ballot(order != 0));
         there_old += __popcll(__ballot(counts));
         if (counts) atomicAdd(&shared.histogram[order >> (32 - kDigit)], 1u);
@@ -186,11 +189,13 @@ __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int
     const uint32_t all = sum_of_waves(shared.waves[0], kPickWaves);
     const uint32_t all_old = sum_of_waves(shared.waves[1], kPickWaves);
     __syncthreads();
-    // `want` of the old slots stay: those whose digits under the mask are above the threshold's, and
-    // the first `need` with the threshold's
+    // `want` of the old slots stay: orders above `high`, and the first `need` from `low` to `high`
     const uint32_t want = min((uint32_t)keep - (all - all_old), all_old);
-    uint32_t threshold = 0, mask = 0, need = want;
+    uint32_t low = kLargest, high = kLargest, need = 0;  // none
+    if (want == all_old) low = high = 0;                 // all
     if (want > 0 && want < all_old) {
+        low = 0;
+        need = want;
         for (int shift = 32 - kDigit, digit = kDigit;;) {
             // bins from the largest down, two a thread: the one in which the count passes need
             const int bin = kBins - 1 - 2 * t;
@@ -207,30 +212,24 @@ __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int
                 shared.found[2] = second ? two : one;
             }
             __syncthreads();
-            threshold |= shared.found[0] << shift;
-            mask |= ((1u << digit) - 1) << shift;
+            low |= shared.found[0] << shift;
+            high = min(low | ((1u << shift) - 1), kLargest);
             need = shared.found[1];
             // (done too where all with these digits stay)
             if (shift == 0 || need == shared.found[2]) break;
             digit = min(shift, kDigit);
             shift -= digit;
-            each([&](int slot, uint32_t order) {
-                if (order && slot < old && (order & mask) == threshold)
+            each([&](int, uint32_t order) {
+                if (order - low <= high - low)
                     atomicAdd(&shared.histogram[order >> shift & ((1u << digit) - 1)], 1u);
             });
             __syncthreads();
         }
     }
-    const auto certain = [&](int slot, uint32_t order) {
-        return order && (slot >= old || (order & mask) > threshold);
-    };
-    const auto same = [&](int slot, uint32_t order) {
-        return order && slot < old && (order & mask) == threshold;
-    };
     uint32_t sure = 0, equal = 0;
-    each([&](int slot, uint32_t order) {
-        sure += __popcll(__ballot(certain(slot, order)));
-        equal += __popcll(__ballot(same(slot, order)));
+    each([&](int, uint32_t order) {
+        sure += __popcll(__ballot(order > high));
+        equal += __popcll(__ballot(order - low <= high - low));
     });
     __syncthreads();
     if (lane == 0) shared.waves[0][wave] = sure, shared.waves[1][wave] = equal;
@@ -238,10 +237,11 @@ __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int
     uint32_t equals = sum_of_waves(shared.waves[1], wave);
     uint32_t written = sum_of_waves(shared.waves[0], wave) + min(equals, need);
     each([&](int slot, uint32_t order) {
-        bool stays = certain(slot, order);
-        const uint64_t alike = __ballot(same(slot, order));
-        if (alike) {
-            stays = stays || ((alike >> lane & 1) && equals + lanes_before(alike) < need);
+        bool stays = order > high;
+        const bool same = order - low <= high - low;
+        const uint64_t alike = __ballot(same);
+        if (alike && equals < need) {
+            stays = stays || (same && equals + lanes_before(alike) < need);
             equals += __popcll(alike);
         }
         const uint64_t stay = __ballot(stays);
