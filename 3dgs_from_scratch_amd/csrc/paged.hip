@@ -92,12 +92,11 @@ __device__ __forceinline__ uint32_t lanes_before(uint64_t mask) {
 // that agree so far; then each wave counts what it keeps, and writes it behind what the waves before
 // it keep.
 //
-// Bound by the instructions of one CU: of 24 us for 32640 slots, 8 go to reading and the first
-// histogram, 4 to its scan, 3 to a second one, 2 to counting and 7 to writing.  64 heads of 2500 to
-// 32640 slots 29 us, 3 of 16320 in pages of 40 19, 18 of up to 60 10.  For the first, orders in registers,
-// whose loops have to be unrolled, took 64 us, and a page found for every slot 45.  Additions to
-// one place in LDS follow one another: with all weights alike the eviction takes 170 us, otherwise 106;
-// digits that a wave has in common counted at once cost every histogram twice its time.
+// Bound by the instructions of one CU: reading and the first histogram are a third of the time for
+// 32640 slots, then its scan, a second histogram, counting and writing.  64 heads of 2500 to 32640 slots
+// 25 us, 3 of 16320 in pages of 40 16, 18 of up to 60 10.  For the first, orders in registers, whose
+// loops have to be unrolled, took 64 us, a page found for every slot 45, and digits under masks, with the
+// recent slots told by their numbers, 29.
 template <bool HELD, bool WHOLE>
 __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int b, int head, int filled,
                                      int32_t keep, int32_t recent, int32_t *new_lengths, int32_t *out,
@@ -219,10 +218,27 @@ __device__ __forceinline__ void pick(const GsPages &p, const float *weights, int
             if (shift == 0 || need == shared.found[2]) break;
             digit = min(shift, kDigit);
             shift -= digit;
-            each([&](int, uint32_t order) {
-                if (order - low <= high - low)
-                    atomicAdd(&shared.histogram[order >> shift & ((1u << digit) - 1)], 1u);
-            });
+            const auto bin_of = [&](uint32_t order) { return order >> shift & ((1u << digit) - 1); };
+            if (shared.found[2] > all_old / 4) {
+                // (they may all be alike, such as zeros, and additions to one place follow one
+                // another: one for a wave whose lanes agree.  With all weights alike the eviction of
+                // up to 32640 slots takes 124 us and 167 without; taken always, this costs the others 5)
+                each([&](int, uint32_t order) {
+                    const bool counts = order - low <= high - low;
+                    const uint32_t mine = bin_of(order), first_bin = uniform((int)mine);
+                    const uint64_t some = __ballot(counts);
+                    if (!__ballot(counts && mine != first_bin)) {
+                        if (lane == 0 && some)
+                            atomicAdd(&shared.histogram[first_bin], (uint32_t)__popcll(some));
+                    } else if (counts) {
+                        atomicAdd(&shared.histogram[mine], 1u);
+                    }
+                });
+            } else {
+                each([&](int, uint32_t order) {
+                    if (order - low <= high - low) atomicAdd(&shared.histogram[bin_of(order)], 1u);
+                });
+            }
             __syncthreads();
         }
     }

@@ -589,6 +589,57 @@ def test_two_streams_at_once(gpu):
         assert all(same(x, y) for x, y in zip(got, want))
 
 
+# --------------------------------------------------------------------- layouts
+@pytest.mark.parametrize("layout", ["keys and values in turn", "a layer of several", "some of the heads",
+                                    "every other page", "weights in another order"])
+@pytest.mark.parametrize("page", [16, 64])
+def test_pools_in_larger_ones(gpu, layout, page):
+    """Pools, tables, lengths and offsets that are parts of other tensors, which stay as they are."""
+    dtype, heads, dim, lengths, new = torch.float16, 2, 64, [200, 33, 70], [30, 1, 0]
+    c = Cache(gpu, lengths, page, heads, dim, dtype, spare=3 * (-(-50 // page)))
+    pages = c.k.shape[0]
+    whole = {"keys and values in turn": (pages, 2, page, heads, dim),
+             "a layer of several": (pages, 5, page, heads, dim),
+             "some of the heads": (pages, page, heads + 3, dim),
+             "every other page": (2 * pages, page, heads, dim + 8),
+             "weights in another order": (pages, page, heads, dim)}[layout]
+    pools = [torch.full(whole, math.nan, dtype=dtype, device=gpu) for _ in range(2)]
+    if layout == "keys and values in turn":
+        pools[1] = pools[0]
+        k, v = pools[0][:, 0], pools[0][:, 1]
+    else:
+        k, v = {"a layer of several": lambda t: t[:, 3], "some of the heads": lambda t: t[:, :, 1:1 + heads],
+                "every other page": lambda t: t[::2, ..., :dim],
+                "weights in another order": lambda t: t}[layout](pools[0]), None
+        v = pools[1].as_strided(k.shape, k.stride(), k.storage_offset())
+    k.copy_(c.k), v.copy_(c.v)
+    outside = [t.clone() for t in pools]
+    w = c.w.clone()
+    if layout == "weights in another order":
+        w = torch.empty(heads, pages, page, device=gpu).permute(1, 2, 0).copy_(c.w)
+    wide = torch.full((3, c.tables.shape[1] + 5), 1 << 20, dtype=torch.int32, device=gpu)
+    tables = wide[:, 2:2 + c.tables.shape[1]].copy_(c.tables)
+    spread = torch.stack((c.lengths, c.lengths + 7), 1)[:, 0]
+    offsets = torch.stack((offsets_of(new, gpu),) * 3, 1)[:, 1]
+    fresh = torch.full((3, -(-50 // page) + 1), -1, dtype=torch.int32, device=gpu)
+    new_tables = fresh[:, :-1].copy_(c.spare.view(3, -1))
+    q, nk, nv = (queries(gpu, sum(new), h, dim, dtype, h) for h in (4, heads, heads))
+
+    def run(k, v, w, tables, lengths, offsets, new_tables):
+        cr.paged_append(nk, nv, k, v, tables, lengths, offsets, w)
+        out = cr.paged_attention(q, k, v, tables, lengths, offsets, True, weights=w)
+        return (out, *cr.paged_evict(k, v, w, tables, lengths, new_tables, 50, 20))
+
+    want = run(c.k, c.v, c.w, c.tables, c.lengths, offsets.contiguous(), new_tables.contiguous())
+    got = run(k, v, w, tables, spread, offsets, new_tables)
+    assert all(same(a, b) for a, b in zip(got, want))
+    assert same(k.contiguous(), c.k) and same(v.contiguous(), c.v) and same(w.contiguous(), c.w)
+    k.zero_(), v.zero_()
+    for t, before in zip(pools, outside):  # what is not the pool's
+        mask = t != 0
+        assert same(torch.where(mask, t, 0.0), torch.where(mask, before, 0.0))
+
+
 # -------------------------------------------------------------------- refusals
 def test_refusals(gpu):
     c = Cache(gpu, [40, 9], 16, 2, 64, torch.float16)
