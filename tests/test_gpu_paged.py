@@ -9,12 +9,15 @@ Tolerances, with u the unit roundoff of the pool's type (2^-11, 2^-8) and e = 2^
   float add (dim + 16) e of sum |q k|, relative to a probability;
 - a slot's weight: a probability exp(s - L) is off relatively by that of the score and of the
   log-sum, (dim + 16) e (sum |q k| + |L| + 1) each, and by 8 e of exp; sums are of chains of at
-  most n / 32 + 64 additions, n the queries and heads; what was there before is added once (e).
+  most n / 32 + 64 additions, n the queries and heads; what was there before is added once (e).  A
+  probability below 2^-126, the smallest normal float, may be 0: the hardware's exponential need not
+  give smaller ones.
 """
 
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
@@ -121,7 +124,8 @@ def check_attention(q, c, offsets, causal=True, scale=None):
     off = 2 * (dim + 16) * E * (reach + (float(size.max()) if size.numel() else 0.0) + 1) + 8 * E
     off = off + (ref["weights_terms"] / 32 + 64) * E
     want = before.double() + ref["weights"]
-    within(after[there], want[there], (off * ref["weights"])[there] + 2 * E * want[there], "weights")
+    off = off * ref["weights"] + 2 * E * want + 2.0 ** -126 * ref["weights_terms"]
+    within(after[there], want[there], off[there], "weights")
     assert same(after[~there], before[~there])
     assert out.is_contiguous() and out.shape == q.shape
     # without what is not asked for, and with it again
@@ -468,6 +472,41 @@ def test_evict_of_many_sequences(gpu):
     lengths = torch.randint(0, 90, (700,), generator=g).tolist()
     c = Cache(gpu, lengths, 16, 2, 16, torch.float16, spare=700 * 2)
     check_evict(c, c.spare.view(700, 2), 32, 8)
+
+
+# ---------------------------------------------------------------------- drawn
+@pytest.mark.parametrize("seed", range(48))
+def test_drawn_caches(gpu, seed):
+    """All three operators at sizes, layouts and masks that are drawn together."""
+    rng = random.Random(seed)
+
+    def log(low, high):
+        return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+    dtype, dim = TYPES[seed % 2], rng.choice([8, 24, 32, 64, 72, 96, 104, 128])
+    key_heads, group = rng.choice([1, 2, 3, 5]), rng.choice([1, 2, 3, 8, 17])
+    page = rng.choice([1, 2, 5, 13, 16, 24, 32, 63, 64, 65, 128, 192, 300])
+    sequences = rng.choice([1, 2, 3, 5, 20, 70])
+    longest, most = log(2, max(3, 4000 // sequences)), rng.choice([1, 1, 2, 8, 60, 300])
+    lengths = [rng.choice([0, log(1, longest), longest]) for _ in range(sequences)]
+    new = [rng.choice([0, min(n, most), rng.randint(0, most)]) for n in lengths]
+    keep = log(1, longest)
+    fresh = -(-keep // page)
+    c = Cache(gpu, lengths, page, key_heads, dim, dtype, rng.random() < 0.5, seed, rng.choice([0, 50]),
+              fresh * sequences + 1)
+    if rng.random() < 0.4:
+        g = torch.Generator(device=gpu).manual_seed(seed)
+        hide = torch.rand(c.tables.shape, generator=g, device=gpu) < rng.choice([0.05, 0.5, 0.95])
+        c.tables[hide] = rng.choice([-1, c.k.shape[0], 2 ** 31 - 1, -2 ** 31])
+    at = offsets_of(new, gpu)
+    k, v = (queries(gpu, sum(new), key_heads, dim, dtype, s + seed) for s in (1, 2))
+    check_append(c, k, v, at)
+    if sum(new):
+        check_attention(queries(gpu, sum(new), key_heads * group, dim, dtype, seed), c, at,
+                        rng.random() < 0.7, rng.choice([None, None, 1.0, -0.3, 0.0]))
+    if rng.random() < 0.3:
+        c.w.copy_(torch.floor(c.w * rng.choice([0.1, 1, 3])))
+    check_evict(c, c.spare[:fresh * sequences].view(sequences, fresh), keep, rng.randint(0, keep))
 
 
 # ------------------------------------------------------------------- together
