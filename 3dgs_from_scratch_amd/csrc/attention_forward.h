@@ -584,23 +584,57 @@ __device__ __forceinline__ void forward_shared(const GsAttention &a, const Sourc
         const int2 r = rows_of(a.offsets_q, a.sequences, a.rows_q, s);
         return (int)(((int64_t)(r.y - r.x) * group + F::kRows - 1) / F::kRows);
     };
+    // Of up to 128 sequences a lane keeps two and their tiles, so that offsets and lengths are read
+    // once; more are looked through again for every split.
+    constexpr int kHeld = 2;
+    const bool few = all <= kHeld * kWave;
+    int rows_held[kHeld], held[kHeld], upto[kHeld];
     float total = 0.0f;  // tiles of all (far below 2^24 where a split is more than one)
-    for (int first = 0; first < all; first += kWave) {
-        const int s = first + (int)__lane_id();
-        total += wave_sum(s < all ? (float)rows_tiles_of(s) * (float)tiles_of(s) : 0.0f);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int s = i * kWave + (int)__lane_id();
+        rows_held[i] = few && s < all ? rows_tiles_of(s) : 0;
+        held[i] = few && s < all ? tiles_of(s) : 0;
+        total += (float)rows_held[i] * (float)held[i];
     }
+    if (!few)
+        for (int s = (int)__lane_id(); s < all; s += kWave)
+            total += (float)rows_tiles_of(s) * (float)tiles_of(s);
+    total = wave_sum(total);
     const int least = uniform(max(4, (int)(total * (float)a.heads_k / (float)kSplits) + 1));
     const auto share_of = [&](int t) { return max(least, (t + partial.splits - 1) / partial.splits); };
     const auto splits_of = [&](int t) {
         const int share = share_of(t);
         return max((t + share - 1) / share, 1);
     };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        upto[i] = (int)lanes_sum_upto((uint32_t)(rows_held[i] * splits_of(held[i]) * a.heads_k));
     const auto count = [&](int s) { return rows_tiles_of(s) * splits_of(tiles_of(s)) * a.heads_k; };
-    int sequence, number;
-    for (int item = blockIdx.x; find_place(all, count, item, false, &sequence, &number);
-         item += gridDim.x) {
-        const int t = uniform(tiles_of(sequence)), splits = splits_of(t);
-        const int rest = number / a.heads_k;
+    // the sequence and the place in it of an item, and the sequence's tiles of keys
+    int sequence, number, t;
+    const auto find = [&](int item) {
+        if (!few) {
+            if (!find_place(all, count, item, false, &sequence, &number)) return false;
+            t = uniform(tiles_of(sequence));
+            return true;
+        }
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const uint64_t past = __ballot(upto[i] > item);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                sequence = i * kWave + l;
+                number = item - (l ? __builtin_amdgcn_readlane(upto[i], l - 1) : 0);
+                t = __builtin_amdgcn_readlane(held[i], l);
+                return true;
+            }
+            item -= __builtin_amdgcn_readlane(upto[i], kWave - 1);
+        }
+        return false;
+    };
+    for (int item = blockIdx.x; find(item); item += gridDim.x) {
+        const int splits = splits_of(t), rest = number / a.heads_k;
         forward_rows<T, DIM, BY_KEYS, true>(a, source, q, out, out_rest, log_sum, partial, lds,
                                             number % a.heads_k, sequence, rest / splits, rest % splits,
                                             share_of(t));

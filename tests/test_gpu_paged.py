@@ -461,10 +461,13 @@ def test_evict_without_some_pages(gpu):
 
 @pytest.mark.parametrize("length,keep", [(20_000, 9000), (32_768, 20_000), (32_769, 100), (70_000, 30_000),
                                          (140_001, 3), (40_000, 39_999)])
-def test_evict_of_long_sequences(gpu, length, keep):
-    fresh = -(-keep // 64)
-    c = Cache(gpu, [length, 500], 64, 2, 8, torch.float16, spare=2 * fresh)
+@pytest.mark.parametrize("page", [24, 64])
+def test_evict_of_long_sequences(gpu, length, keep, page):
+    fresh = -(-keep // page)
+    c = Cache(gpu, [length, 500], page, 2, 8, torch.float16, spare=2 * fresh)
     check_evict(c, c.spare.view(2, fresh), keep, min(keep, 1000))
+    c.w.copy_(torch.floor(c.w))  # most alike
+    check_evict(c, c.spare.view(2, fresh), keep, 0)
 
 
 def test_evict_of_many_sequences(gpu):
