@@ -76,6 +76,14 @@ def attention(q, k_pages, v_pages, tables, lengths, offsets, causal=False, scale
     return res | {"weights": got, "weights_terms": terms}
 
 
+def _column(weights, slots, head):
+    """The weights of (slot, page, place) of a head."""
+    if not slots:
+        return []
+    _, page, place = (torch.tensor(x, device=weights.device) for x in zip(*slots))
+    return weights[page, place, head].tolist()
+
+
 def evict(k_pages, v_pages, weights, tables, lengths, new_tables, keep, recent=0):
     """(new_lengths, kept, k_pages, v_pages, weights)."""
     out = [t.clone() for t in (k_pages, v_pages, weights)]
@@ -91,16 +99,20 @@ def evict(k_pages, v_pages, weights, tables, lengths, new_tables, keep, recent=0
         stay = min(keep - len(late), len(old))
         new_lengths[b] = stay + len(late)
         for h in range(heads):
+            lines = {x: w for x, w in zip(there, _column(weights, there, h))}
+
             def rank(x):
-                w = float(weights[x[1], x[2], h])
+                w = lines[x]
                 return (-math.inf, -1, x[0]) if w != w else (-w, 0, x[0])
             chosen = sorted(sorted(old, key=rank)[:stay] + late)
-            for j, (slot, page, place) in enumerate(chosen):
-                kept[b, h, j] = slot
-                to = int(new_tables[b, j // size])
-                if 0 <= to < pages:
-                    for x, y in zip(out, (k_pages, v_pages, weights)):
-                        x[to, j % size, h] = y[page, place, h]
+            kept[b, h, :len(chosen)] = torch.tensor([x[0] for x in chosen], dtype=torch.int32)
+            row = new_tables[b].tolist()
+            moves = [(x[1], x[2], row[j // size], j % size) for j, x in enumerate(chosen)
+                     if 0 <= row[j // size] < pages]
+            if moves:
+                page, place, to, at = (torch.tensor(m, device=weights.device) for m in zip(*moves))
+                for x, y in zip(out, (k_pages, v_pages, weights)):
+                    x[to, at, h] = y[page, place, h]
     return new_lengths, kept, *out
 
 
