@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(int64_t rows, int d
                                                              T *__restrict__ out_rest,
                                                              float *__restrict__ log_sum) {
     __shared__ f32x4 sums[8][32];
-    join_row<T>(rows, dim, partial, out, out_rest, log_sum, sums);
+    join_row<T>(blockIdx.x, rows, dim, partial, out, out_rest, log_sum, sums);
 }
 
 // ---------------------------------------------------------------- gradients

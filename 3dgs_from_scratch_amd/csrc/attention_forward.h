@@ -645,9 +645,8 @@ __device__ __forceinline__ void forward_shared(const GsAttention &a, const Sourc
 // Joins the splits of a row: a workgroup a row, four elements a thread, every eighth split
 // in each of its eight parts.  Bound by latency: 256 rows of 28 splits 4.8 us.
 template <typename T>
-__device__ __forceinline__ void join_row(int64_t rows, int dim, const Partial &partial, T *out,
-                                         T *out_rest, float *log_sum, f32x4 (*sums)[32]) {
-    const int64_t row = blockIdx.x;
+__device__ __forceinline__ void join_row(int64_t row, int64_t rows, int dim, const Partial &partial,
+                                         T *out, T *out_rest, float *log_sum, f32x4 (*sums)[32]) {
     const int lane = __lane_id(), column = threadIdx.x % 32 * 4, part = threadIdx.x / 32;
     const int splits = partial.count ? min(partial.count[row], partial.splits) : partial.splits;
     const float2 mine = lane < splits ? partial.max_sum[lane * rows + row]

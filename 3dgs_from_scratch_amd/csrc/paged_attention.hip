@@ -208,7 +208,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(int64_t rows, int dim, 
                                                          T *__restrict__ out,
                                                          float *__restrict__ log_sum) {
     __shared__ f32x4 sums[8][32];
-    join_row<T>(rows, dim, partial, out, (T *)nullptr, log_sum, sums);
+    join_row<T>(blockIdx.x, rows, dim, partial, out, (T *)nullptr, log_sum, sums);
 }
 
 // Many rows with few splits: 32 threads a row, four elements each; a lane has the maximum and the
@@ -332,10 +332,12 @@ struct SlotOperand {
     }
 };
 
-// f(sequence, tile, key head) for the tiles of SLOTS slots of all sequences that have queries.  The
-// workgroups take them in turn; most have one, and find it in one look through the sequences.
+// f(sequence, tile, key head) for the tiles of SLOTS slots of all sequences that have queries, from
+// number `item` on every `every`th.  Most workgroups have one, and find it in one look through the
+// sequences.
 template <int SLOTS, typename F>
-__device__ __forceinline__ void for_slot_tiles(const GsAttention &a, const GsPages &p, F f) {
+__device__ __forceinline__ void for_slot_tiles(const GsAttention &a, const GsPages &p, int item, int every,
+                                               F f) {
     const int lane = __lane_id();
     int upto = 0;  // places of 64 sequences up to and with the lane's
     const auto look = [&](int first) {  // all of them
@@ -348,7 +350,7 @@ __device__ __forceinline__ void for_slot_tiles(const GsAttention &a, const GsPag
         upto = (int)lanes_sum_upto((uint32_t)n);
         return __builtin_amdgcn_readlane(upto, kWave - 1);
     };
-    int item = blockIdx.x, first = 0, before = 0, here = look(0);
+    int first = 0, before = 0, here = look(0);
     for (;;) {
         while (item - before >= here) {
             before += here;
@@ -359,7 +361,7 @@ __device__ __forceinline__ void for_slot_tiles(const GsAttention &a, const GsPag
         const int l = __builtin_ctzll(__ballot(before + upto > item));
         const int place = item - before - (l ? __builtin_amdgcn_readlane(upto, l - 1) : 0);
         f(first + l + 1, place / a.heads_k, place % a.heads_k);
-        item += gridDim.x;
+        item += every;
     }
 }
 
@@ -379,7 +381,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
     const int wave = uniform(threadIdx.x / kWave);
     const float c = exponent_factor(a.scale);
     const auto copy = QTile::copy_of(wave, a.q_row, a.dim);
-    for_slot_tiles<kWeightSlots>(a, p, [&](int sequence, int tile, int kh) {
+    for_slot_tiles<kWeightSlots>(a, p, blockIdx.x, gridDim.x, [&](int sequence, int tile, int kh) {
         const int2 rows = rows_of(a.offsets_q, a.sequences, a.rows_q, sequence);
         const int q0 = uniform(rows.x), lq = uniform(rows.y - rows.x);
         const int filled = uniform(slots_of(p, sequence));
@@ -453,7 +455,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
 }
 
 // Few rows: a wave takes them from memory.  (Where the attention could not keep their scores.)  64 single
-// tokens over 12 to 2500 slots, 12 heads of 64: 32 us, and 8 from kept scores.
+// tokens over 12 to 2500 slots, 12 heads of 64: 32 us, and 11 from kept scores with the join.
 template <typename T, int DIM>
 __global__ __launch_bounds__(64 * kWaves) void paged_few_weights_kernel(
     GsAttention a, GsPages p, const T *__restrict__ q, const T *__restrict__ k,
@@ -461,7 +463,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_few_weights_kernel(
     const int group = a.heads_q / a.heads_k, lane = __lane_id(), half = lane >> 5;
     const int wave = uniform(threadIdx.x / kWave);
     const float c = exponent_factor(a.scale);
-    for_slot_tiles<kWeightSlots>(a, p, [&](int sequence, int tile, int kh) {
+    for_slot_tiles<kWeightSlots>(a, p, blockIdx.x, gridDim.x, [&](int sequence, int tile, int kh) {
         const int2 range = rows_of(a.offsets_q, a.sequences, a.rows_q, sequence);
         const int q0 = uniform(range.x), lq = uniform(range.y - range.x), rows = lq * group;
         const int filled = uniform(slots_of(p, sequence));
@@ -492,33 +494,63 @@ __global__ __launch_bounds__(64 * kWaves) void paged_few_weights_kernel(
     });
 }
 
-// Few rows whose scores the attention has kept: a thread a slot.  Bound by latency: the sequence, the
-// scores and the page, the weight.
+// Few rows whose scores the attention has kept: a thread a slot.  Rows in parts are joined by the last
+// `joins` workgroups of the same launch, a row each, and the slots' workgroups find a row's log-sum from
+// its parts for themselves: a launch less, 45 instead of 47 us for 64 single tokens over 12 to 2500 slots.
+// Bound by latency: the sequence, the log-sums, the scores and the page, the weight.
+template <typename T>
 __global__ __launch_bounds__(kScoreSlots) void paged_score_weights_kernel(
-    GsAttention a, GsPages p, const float *__restrict__ scores, int64_t score_slots,
-    const float *__restrict__ log_sum, float *__restrict__ weights) {
-    const int group = a.heads_q / a.heads_k;
+    GsAttention a, GsPages p, const float *__restrict__ scores, int64_t score_slots, Partial partial,
+    int joins, T *__restrict__ out, float *log_sum, float *__restrict__ weights) {
+    __shared__ f32x4 sums[8][32];
+    __shared__ float minus[kWave];  // -L of so many rows, in the exponent of two
+    const int64_t all_rows = a.rows_q * a.heads_q;
+    const int tiles = gridDim.x - joins;
+    if ((int)blockIdx.x >= tiles) {
+        join_row<T>(blockIdx.x - tiles, all_rows, a.dim, partial, out, (T *)nullptr, log_sum, sums);
+        return;
+    }
+    const int group = a.heads_q / a.heads_k, lane = __lane_id(), wave = uniform(threadIdx.x / kWave);
     const float c = exponent_factor(a.scale);
-    for_slot_tiles<kScoreSlots>(a, p, [&](int sequence, int tile, int kh) {
+    const auto minus_of = [&](int64_t row) {  // (every lane of a wave calls it)
+        if (partial.splits == 1) return minus_log(log_sum[row]);
+        const float2 part = lane < min(partial.count[row], partial.splits)
+                                ? partial.max_sum[lane * all_rows + row]
+                                : make_float2(-INFINITY, 0.0f);
+        const float top = wave_max(part.x);
+        const float share = part.x == -INFINITY ? 0.0f : part.y * __builtin_amdgcn_exp2f(part.x - top);
+        const float l = top == -INFINITY ? -INFINITY : top + __builtin_amdgcn_logf(wave_sum(share));
+        return l == -INFINITY ? -INFINITY : -l;
+    };
+    for_slot_tiles<kScoreSlots>(a, p, blockIdx.x, tiles, [&](int sequence, int tile, int kh) {
         const int2 range = rows_of(a.offsets_q, a.sequences, a.rows_q, sequence);
-        const int q0 = uniform(range.x), lq = uniform(range.y - range.x);
+        const int q0 = uniform(range.x), lq = uniform(range.y - range.x), rows = lq * group;
         const int filled = uniform(slots_of(p, sequence)), slot = tile * kScoreSlots + (int)threadIdx.x;
-        if (slot >= filled) return;
-        const int index = slot / p.page_size, page = page_of(p, sequence - 1, index);
+        const int index = slot / p.page_size;
+        const int page = slot < filled ? page_of(p, sequence - 1, index) : -1;
+        // the first row that sees the slot
+        const int least = slot >= filled ? rows : a.causal ? max(slot - (filled - lq), 0) * group : 0;
+        const auto row_of = [&](int r) {
+            const int i = r / group;
+            return (int64_t)(q0 + i) * a.heads_q + kh * group + (r - i * group);
+        };
         float sum = 0.0f;
-        for (int i = a.causal ? max(slot - (filled - lq), 0) : 0; i < lq; ++i) {
-            const int64_t row = (int64_t)(q0 + i) * a.heads_q + kh * group;
-            const float *line = scores + row * score_slots + slot;
-            for (int h0 = 0; h0 < group; h0 += 4) {
-                float s[4], l[4];
+        for (int r0 = 0; r0 < rows; r0 += kWave) {
+            const int end = min(r0 + kWave, rows);
+            __syncthreads();  // the rows before have been read
+            for (int r = r0 + wave; r < end; r += kScoreSlots / kWave) {
+                const float m = minus_of(row_of(r));
+                if (lane == 0) minus[r - r0] = m;
+            }
+            __syncthreads();
+            for (int r = max(r0, least); r < end; r += 4) {
+                float s[4], w[4];
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    s[h] = h0 + h < group ? line[(h0 + h) * score_slots] : 0.0f;
-                    l[h] = h0 + h < group ? minus_log(log_sum[row + h0 + h]) : -INFINITY;
-                }
-                float w[4];
+                for (int n = 0; n < 4; ++n)
+                    s[n] = r + n < end ? scores[row_of(r + n) * score_slots + slot] : 0.0f;
 #pragma unroll
-                for (int h = 0; h < 4; ++h) w[h] = __builtin_amdgcn_exp2f(fmaf(s[h], c, l[h]));
+                for (int n = 0; n < 4; ++n)
+                    w[n] = r + n < end ? __builtin_amdgcn_exp2f(fmaf(s[n], c, minus[r + n - r0])) : 0.0f;
                 sum += (w[0] + w[1]) + (w[2] + w[3]);
             }
         }
@@ -605,7 +637,7 @@ static int launch(const GsPages &p, const GsAttention &a, const ForwardPlan &f, 
         hipLaunchKernelGGL((paged_attention_kernel<T, DIM, false, WHOLE>), grid, dim3(64 * kWaves), 0,
                            stream, a, p, q, k, v, out, log_sum, partial);
     const int st = launch_status();
-    if (st || f.splits == 1) return st;
+    if (st || f.splits == 1 || scores) return st;  // (with scores the weights' launch joins)
     const int64_t rows = a.rows_q * a.heads_q;
     if (f.by_keys)
         hipLaunchKernelGGL((paged_join_kernel<T>), dim3((unsigned)rows), dim3(256), 0, stream, rows, a.dim,
@@ -665,7 +697,7 @@ extern "C" int gs_paged_attention(const GsPages *p, const GsPagedQueries *querie
                                                    scores, score_slots, stream)
                           : launch<T, kDim, false>(*p, a, f, tq, tk, tv, (T *)out, log_sum, partial,
                                                     scores, score_slots, stream);
-        if (s || !weights || p->sequences == 0 || p->table_width == 0) return s;
+        if (s || !weights || (!scores && (p->sequences == 0 || p->table_width == 0))) return s;
         // as many workgroups as there are tiles if no page is in two tables; the workgroups go on
         // while there are more
         const auto grid = [&](int64_t size) {
@@ -676,13 +708,16 @@ extern "C" int gs_paged_attention(const GsPages *p, const GsPagedQueries *querie
             return dim3((unsigned)(groups < 8192 ? groups : 8192));
         };
         const float *log = log_sum;
-        if (scores)
-            hipLaunchKernelGGL(paged_score_weights_kernel, grid(kScoreSlots), dim3(kScoreSlots), 0, stream, a,
-                               *p, (const float *)scores, score_slots, log, weights);
-        else if (f.by_keys)
+        const int joins = scores && f.splits > 1 ? (int)(a.rows_q * a.heads_q) : 0;
+        const unsigned both = joins + grid(kScoreSlots).x;
+        if (scores && both > 0)
+            hipLaunchKernelGGL((paged_score_weights_kernel<T>), dim3(both), dim3(kScoreSlots), 0, stream, a,
+                               *p, (const float *)scores, score_slots, partial, joins, (T *)out, log_sum,
+                               weights);
+        else if (f.by_keys && !scores)
             hipLaunchKernelGGL((paged_few_weights_kernel<T, kDim>), grid(kWeightSlots), dim3(64 * kWaves), 0,
                                stream, a, *p, tq, tk, log, weights);
-        else
+        else if (!scores)
             hipLaunchKernelGGL((paged_weights_kernel<T, kDim>), grid(kWeightSlots), dim3(64 * kWaves), 0,
                                stream, a, *p, tq, tk, log, weights);
         return launch_status();
