@@ -841,7 +841,7 @@ int gs_paged_attention(const GsPages *p, const GsPagedQueries *a, const void *q,
  *   there, the last `recent` slots and those with the largest weights among the others,
  *   `keep` in all or as many as there are (equal weights: the lower slot; NaN counts as
  *   the largest), move in their order to slots 0, 1, ... of the pages in new_tables
- *   (new_width >= keep / page_size entries a sequence), keys, values and weights.
+ *   (new_width entries a sequence, at least keep / page_size), keys, values and weights.
  *   kept (sequences, heads, keep) receives their slots, -1 behind the last, and
  *   new_lengths their number.  0 <= recent <= keep.  The old pages stay as they are; a page
  *   that the call moves to must be no sequence's old one, and one sequence's only.
