@@ -371,7 +371,7 @@ extern "C" int gs_paged_evict(const GsPages *p, void *k_pages, void *v_pages, fl
     if (!aligned16(k_pages) || !aligned16(v_pages)) return GS_ERR_UNSUPPORTED;
     const int64_t picks = (int64_t)p->sequences * p->heads;
     const int64_t groups = ((int64_t)keep * (p->dim / 8) * p->heads + 255) / 256;
-    if (picks > 0x7fffffffLL || groups > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
+    if (keep > kMaxSlots || picks > 0x7fffffffLL || groups > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
     // (by the slots that a table could hold: what is filled is not known here)
     const int64_t slots = (int64_t)p->page_size * p->table_width;
     const bool held = slots <= kHeld, whole = p->page_size % kWave == 0;

@@ -128,6 +128,9 @@ def _layout(what: str, shape, k_strides, v_shape, v_strides, w_shape, w_strides,
     sequences, width = tables
     if lengths[0] != sequences:
         raise RuntimeError(f"{what}: lengths must have {sequences} entries, got {lengths[0]}")
+    if max(sequences, page_size, heads) > MAX_SLOTS:
+        raise RuntimeError(f"{what}: {sequences} sequences and {heads} heads in pages of {page_size} are "
+                           "too many")
     if width * page_size > MAX_SLOTS:
         raise RuntimeError(f"{what}: at most {MAX_SLOTS} slots a sequence are supported, got "
                            f"{width} pages of {page_size}")
@@ -308,6 +311,8 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     if keep < 1 or not 0 <= recent <= keep:
         raise ValueError(f"{what}: keep must be at least 1 and recent from 0 to keep, got {keep} "
                          f"and {recent}")
+    if keep > MAX_SLOTS:
+        raise ValueError(f"{what}: at most {MAX_SLOTS} slots a sequence are supported, keep is {keep}")
     if new_tables.shape[0] != p.sequences or new_tables.shape[1] * p.page_size < keep:
         raise RuntimeError(f"{what}: new_tables must have {p.sequences} rows of "
                            f"{-(-keep // p.page_size)} pages at least, got {tuple(new_tables.shape)}")

@@ -843,8 +843,9 @@ int gs_paged_attention(const GsPages *p, const GsPagedQueries *a, const void *q,
  *   the largest), move in their order to slots 0, 1, ... of the pages in new_tables
  *   (new_width entries a sequence, at least keep / page_size), keys, values and weights.
  *   kept (sequences, heads, keep) receives their slots, -1 behind the last, and
- *   new_lengths their number.  0 <= recent <= keep.  The old pages stay as they are; a page
- *   that the call moves to must be no sequence's old one, and one sequence's only.
+ *   new_lengths their number.  0 <= recent <= keep < 2^31 - 65536 (GS_ERR_UNSUPPORTED above).
+ *   The old pages stay as they are; a page that the call moves to must be no sequence's old
+ *   one, and one sequence's only.
  */
 int gs_paged_evict(const GsPages *p, void *k_pages, void *v_pages, float *weights,
                    const int32_t *new_tables, int64_t new_stride, int32_t new_width, int32_t keep,

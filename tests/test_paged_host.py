@@ -13,7 +13,7 @@ import helpers  # noqa: F401
 import cuda_rasterizer as cr
 from cuda_rasterizer import _lib
 from cuda_rasterizer._lib import GsPagedQueries, GsPages
-from cuda_rasterizer.paged import _pool_strides, _weight_strides
+from cuda_rasterizer.paged import _layout, _pool_strides, _weight_strides
 from oracle import paged as op
 from oracle import tokens as ot
 
@@ -101,6 +101,24 @@ def test_refused_arguments(lib):
     assert evict(lib, pages(sum_page=-1)) == INVALID
     for stride in ("sum_page", "sum_slot", "sum_head"):
         assert evict(lib, pages(**{stride: 1 << 31})) == UNSUPPORTED
+
+
+def test_more_kept_than_slots_have_numbers(lib):
+    most = (1 << 31) - 1 - 65536
+    for keep in (most + 1, (1 << 31) - 1):
+        assert evict(lib, pages(), keep=keep, width=1 << 27) == UNSUPPORTED
+
+
+def test_counts_that_pass_32_bits():
+    """(Sizes alone: with a table of no pages they cost next to nothing.)"""
+    shape, w = (1, 16, 2, 64), (None, None)
+    strides = (2048, 128, 64, 1)
+    assert _layout("x", shape, strides, shape, strides, *w, (3, 0), (3,))
+    with pytest.raises(RuntimeError, match="too many"):
+        _layout("x", shape, strides, shape, strides, *w, ((1 << 32) + 3, 0), ((1 << 32) + 3,))
+    for shape, strides in (((1, 1 << 32, 1, 8), (1 << 35, 8, 8, 1)), ((1, 1, 1 << 32, 8), (8, 8, 8, 1))):
+        with pytest.raises(RuntimeError, match="too many|strides"):
+            _layout("x", shape, strides, shape, strides, *w, (3, 0), (3,))
 
 
 def test_nothing_to_do(lib):
