@@ -367,8 +367,8 @@ __device__ __forceinline__ void for_slot_tiles(const GsAttention &a, const GsPag
 
 // Many rows: tiles of a head's queries go through LDS, which the workgroup's waves share.  Bound by
 // issue: of a SIMD's time 44% are matrix instructions and 55% the others, an exponential, a
-// multiplication and an addition a score.  2 sequences, 8160 queries each over 28284 and 32640 slots, 16 heads on 4, dim
-// 128: 2.1 ms, 0.83 PFLOP/s.
+// multiplication and an addition a score.  2 sequences, 8160 queries each over 28284 and 32640 slots,
+// 16 heads on 4, dim 128: 2.1 ms, 0.83 PFLOP/s.
 template <typename T, int DIM>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
     GsAttention a, GsPages p, const T *__restrict__ q, const T *__restrict__ k,
@@ -386,7 +386,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
         const int q0 = uniform(rows.x), lq = uniform(rows.y - rows.x);
         const int filled = uniform(slots_of(p, sequence));
         const int slot0 = tile * kWeightSlots + 32 * wave, slot = slot0 + (lane & 31);
-        // query i sees slots up to i + shift
+        // query i sees slots up to i + shift (a sum that may pass 32 bits: i and slot - shift do not)
         const int shift = a.causal ? filled - lq : filled;
         const int first = max(tile * kWeightSlots - shift, 0) / kRows;
         const int tiles = (lq + kRows - 1) / kRows - first, steps = tiles * group;
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
                 }
             };
             const int row0 = now * kRows;
-            if (row0 + shift >= slot0 + 31 && row0 + kRows <= lq) {
+            if (row0 >= slot0 + 31 - shift && row0 + kRows <= lq) {
                 f32x16 s[2] = {};
 #pragma unroll
                 for (int i = 0; i < DIM / 16; ++i)
@@ -436,14 +436,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const int row = row0 + 32 * n;
-                    if (row >= lq || row + 31 + shift < slot0) continue;
+                    if (row >= lq || row + 31 < slot0 - shift) continue;
                     f32x16 s = {};
 #pragma unroll
                     for (int i = 0; i < DIM / 16; ++i) s = mfma(QTile::along(qt, 32 * n, i), mine.k.x[i], s);
                     float m[16];
                     minus_of(n, m);
                     sum += sum_of_weights<true>(
-                        s, c, m, [&](int i) { return row + i < lq && row + i + shift >= slot; });
+                        s, c, m, [&](int i) { return row + i < lq && row + i >= slot - shift; });
                 }
             }
             if (++now == first + tiles) now = first;
@@ -558,12 +558,16 @@ __global__ __launch_bounds__(kScoreSlots) void paged_score_weights_kernel(
     });
 }
 
-static int check_queries(const GsPages *p, const GsPagedQueries *a) {
+static int check_queries(const GsPages *p, const GsPagedQueries *a, bool weights) {
     if (!a || a->rows_q < 0 || a->row_stride < 0 || a->head_stride < 0 || a->heads_q < 1 ||
         a->heads_q % p->heads != 0 || !a->offsets || !(a->scale == a->scale))
         return GS_ERR_INVALID_ARGUMENT;
     if ((a->row_stride | a->head_stride) % 8 != 0 || !tile_stride(a->row_stride, p->dim) ||
         a->rows_q > kMaxRows / (a->heads_q / p->heads))
+        return GS_ERR_UNSUPPORTED;
+    // the numbers of the slots' tiles stay in 32 bits (as they do where each lies in its own memory)
+    const int64_t tiles = ((int64_t)p->page_size * p->table_width + kWeightSlots - 1) / kWeightSlots;
+    if (weights && tiles > 0 && (int64_t)p->sequences * p->heads > kMaxRows / tiles)
         return GS_ERR_UNSUPPORTED;
     return GS_OK;
 }
@@ -656,7 +660,7 @@ using namespace gs;
 extern "C" int gs_paged_attention_workspace_size(const GsPages *p, const GsPagedQueries *q,
                                                  int32_t weights, size_t *bytes) {
     int st = check_pages(p, weights != 0);
-    if (!st) st = check_queries(p, q);
+    if (!st) st = check_queries(p, q, weights != 0);
     if (st) return st;
     if (!bytes) return GS_ERR_INVALID_ARGUMENT;
     const GsAttention a = problem_of(*p, *q);

@@ -242,7 +242,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     With weights also adds to each slot's weight the probabilities that it gets, summed over
     the sequence's queries and the heads that share its key head, in float32 and in an order
     that depends on the sizes and tables alone.  A page that the tables hold twice gets its
-    weights from one of its places there, whichever.
+    weights from one of its places there, whichever.  With weights, sequences times key heads
+    times the slots that a table's row covers are below 2^38 - 2^23.
 
     scale defaults to dim ** -0.5.  With return_log_sum also the float32 (queries, heads)
     natural logarithm of each softmax's denominator.  Types, rounding and what is not finite

@@ -610,6 +610,39 @@ def test_on_another_stream_and_in_a_graph(gpu):
             assert same(getattr(held, t), getattr(fresh, t))
 
 
+def test_two_captured_calls_at_once(gpu):
+    """Two captured steps that need workspaces, replayed in turn and on two streams at once, with eager
+    calls between."""
+    held = []
+    for lengths, new, seed in (([9000, 300], [40, 40], 2), ([5000, 7000, 12], [1, 1, 1], 4)):
+        c = Cache(gpu, lengths, 64, 2, 128, torch.bfloat16, seed=seed)
+        q = queries(gpu, sum(new), 8, 128, torch.bfloat16, seed)
+        w = torch.zeros_like(c.w)
+
+        def step(c=c, q=q, w=w, at=offsets_of(new, gpu)):
+            w.zero_()
+            return cr.paged_attention(q, *c.args(), at, True, weights=w, return_log_sum=True)
+
+        want = [t.clone() for t in step()] + [w.clone()]
+        held.append((CapturedStep(step), step, w, want))
+    streams = [torch.cuda.Stream() for _ in held]
+    for at_once in (False, True, False, True):
+        for (captured, _, w, _), one in zip(held, streams):
+            for t in (*captured.output, w):
+                t.fill_(math.nan)
+        torch.cuda.synchronize()
+        for (captured, _, _, _), one in zip(held, streams):
+            with torch.cuda.stream(one):
+                captured.replay()
+            if not at_once:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        for captured, step, w, want in held:
+            assert all(same(a, b) for a, b in zip((*captured.output, w), want))
+            assert all(same(a, b) for a, b in zip(step(), want))
+        torch.cuda.synchronize()
+
+
 def test_two_streams_at_once(gpu):
     """Two calls of the same operators at once, each with its own workspace."""
     a, b = ([Cache(gpu, [9000, 300], 64, 2, 128, torch.bfloat16, seed=s), s] for s in (2, 4))

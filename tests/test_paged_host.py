@@ -109,6 +109,17 @@ def test_more_kept_than_slots_have_numbers(lib):
         assert evict(lib, pages(), keep=keep, width=1 << 27) == UNSUPPORTED
 
 
+def test_more_tiles_of_weights_than_have_numbers(lib):
+    """A tile of slots' weights is 128 of them: 2^24 - 520 in a table here, times sequences and heads."""
+    p = pages(page_size=1 << 10, table_width=(1 << 21) - 65, sequences=65)
+    assert attention(lib, p, queries()) == UNSUPPORTED
+    size = ctypes.c_size_t(0)
+    for sequences, weights, status in ((65, 1, UNSUPPORTED), (64, 1, 0), (1 << 16, 0, 0)):
+        p.sequences = sequences
+        assert lib.gs_paged_attention_workspace_size(ctypes.byref(p), ctypes.byref(queries()), weights,
+                                                     ctypes.byref(size)) == status
+
+
 def test_counts_that_pass_32_bits():
     """(Sizes alone: with a table of no pages they cost next to nothing.)"""
     shape, w = (1, 16, 2, 64), (None, None)
