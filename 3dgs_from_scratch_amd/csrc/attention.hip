@@ -624,7 +624,7 @@ extern "C" int gs_attention_forward(const GsAttention *a, const void *q, const v
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(out_rest))
         return GS_ERR_UNSUPPORTED;
     const ForwardPlan f = plan_forward(*a);
-    if (f.groups > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
+    if (!launchable(f.groups, 64 * kWaves)) return GS_ERR_UNSUPPORTED;
     const size_t need = partial_bytes(*a, f.splits);
     if (need && !workspace) return GS_ERR_INVALID_ARGUMENT;
     if (workspace_bytes < need) return GS_ERR_WORKSPACE_TOO_SMALL;

@@ -40,6 +40,9 @@ inline int launch_status() {
     return e == hipSuccess ? GS_OK : static_cast<int>(e);
 }
 
+// Whether a launch takes so many workgroups in a dimension: it has fewer than 2^32 threads there.
+inline bool launchable(int64_t groups, int threads) { return groups <= 0xffffffffLL / threads; }
+
 // Zero `bytes` of device memory on `stream` with a fill kernel (capi.hip).
 int zero_bytes(void *ptr, size_t bytes, hipStream_t stream);
 

@@ -349,7 +349,7 @@ extern "C" int gs_paged_append(const GsPages *p, const void *k, int64_t k_row, i
         (k_row | k_head | v_row | v_head) % 8 != 0)
         return GS_ERR_UNSUPPORTED;
     const int64_t groups = (rows * (p->dim / 8) * p->heads + 255) / 256;
-    if (rows > kMaxSlots || groups > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
+    if (rows > kMaxSlots || !launchable(groups, 256)) return GS_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)groups), dim3(256), 0, stream, *p,
                        (const uint16_t *)k, k_row, k_head, (const uint16_t *)v, v_row, v_head, rows,
                        offsets, (uint16_t *)k_pages, (uint16_t *)v_pages, weights);
@@ -371,7 +371,7 @@ extern "C" int gs_paged_evict(const GsPages *p, void *k_pages, void *v_pages, fl
     if (!aligned16(k_pages) || !aligned16(v_pages)) return GS_ERR_UNSUPPORTED;
     const int64_t picks = (int64_t)p->sequences * p->heads;
     const int64_t groups = ((int64_t)keep * (p->dim / 8) * p->heads + 255) / 256;
-    if (keep > kMaxSlots || picks > 0x7fffffffLL || groups > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
+    if (keep > kMaxSlots || !launchable(picks, kPick) || !launchable(groups, 256)) return GS_ERR_UNSUPPORTED;
     // (by the slots that a table could hold: what is filled is not known here)
     const int64_t slots = (int64_t)p->page_size * p->table_width;
     const bool held = slots <= kHeld, whole = p->page_size % kWave == 0;
@@ -380,6 +380,8 @@ extern "C" int gs_paged_evict(const GsPages *p, void *k_pages, void *v_pages, fl
                              : whole ? paged_pick_kernel<false, true> : paged_pick_kernel<false, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)picks), dim3(kPick), lds, stream, *p,
                        (const float *)weights, keep, recent, new_lengths, kept);
+    const int picked = launch_status();
+    if (picked) return picked;  // (what moves is what has been picked)
     const int32_t rows = p->sequences < 65535 ? p->sequences : 65535;  // of the grid's second dimension
     hipLaunchKernelGGL(paged_move_kernel,
                        dim3((unsigned)groups, (unsigned)rows, (unsigned)((p->sequences + rows - 1) / rows)),

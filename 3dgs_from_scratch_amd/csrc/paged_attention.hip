@@ -684,7 +684,7 @@ extern "C" int gs_paged_attention(const GsPages *p, const GsPagedQueries *querie
         return GS_ERR_UNSUPPORTED;
     const GsAttention a = problem_of(*p, *queries);
     const ForwardPlan f = plan_of(*p, a);
-    if (f.groups > 0x7fffffffLL) return GS_ERR_UNSUPPORTED;
+    if (!launchable(f.groups, 64 * kWaves)) return GS_ERR_UNSUPPORTED;
     if (need && !workspace) return GS_ERR_INVALID_ARGUMENT;
     if (workspace_bytes < need) return GS_ERR_WORKSPACE_TOO_SMALL;
     // the scores, whole lines, then the parts

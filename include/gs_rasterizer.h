@@ -804,7 +804,8 @@ typedef struct {
  * gs_paged_append: row offsets[b] + t of k and v (rows k_row and v_row apart, heads
  *   k_head and v_head, 16-byte aligned, multiples of 8) goes to slot lengths[b] -
  *   (offsets[b + 1] - offsets[b]) + t of sequence b, so lengths count the new slots;
- *   their weights become 0 where weights is set.  Rows of no sequence, and rows whose
+ *   their weights become 0 where weights is set.  rows * heads * dim / 8 is below 2^32 - 256
+ *   (GS_ERR_UNSUPPORTED otherwise).  Rows of no sequence, and rows whose
  *   slot is below 0, past the table or on no page, go nowhere.
  */
 int gs_paged_append(const GsPages *p, const void *k, int64_t k_row, int64_t k_head, const void *v,
@@ -844,7 +845,8 @@ int gs_paged_attention(const GsPages *p, const GsPagedQueries *a, const void *q,
  *   the largest), move in their order to slots 0, 1, ... of the pages in new_tables
  *   (new_width entries a sequence, at least keep / page_size), keys, values and weights.
  *   kept (sequences, heads, keep) receives their slots, -1 behind the last, and
- *   new_lengths their number.  0 <= recent <= keep < 2^31 - 65536 (GS_ERR_UNSUPPORTED above).
+ *   new_lengths their number.  0 <= recent <= keep < 2^31 - 65536, sequences * heads is below 2^22
+ *   and keep * heads * dim / 8 below 2^32 - 256 (GS_ERR_UNSUPPORTED above).
  *   The old pages stay as they are; a page that the call moves to must be no sequence's old
  *   one, and one sequence's only.
  */

@@ -137,6 +137,13 @@ def test_entry_points_reject_on_the_host():
                                     None, None, None, None, 0, None) == 0
 
 
+def test_attention_of_more_threads_than_a_launch_takes():
+    """256 for each tile of packed rows and key head, and a launch has fewer than 2^32."""
+    lib, some = _lib.load(), ctypes.c_void_p(4096)
+    a = _attention_problem(rows_q=(1 << 28) + 1, heads_q=2, heads_k=2, sequences=1 << 23)
+    assert lib.gs_attention_forward(ctypes.byref(a), some, some, some, some, None, None, None, 0, None) == -4
+
+
 def test_python_layer_refuses_cpu_tensors_and_other_things():
     x = torch.zeros(4, 2, 64, dtype=torch.float16)
     at = torch.tensor([0, 4], dtype=torch.int32)

@@ -120,6 +120,17 @@ def test_more_tiles_of_weights_than_have_numbers(lib):
                                                      ctypes.byref(size)) == status
 
 
+def test_more_threads_than_a_launch_takes(lib):
+    """A launch has fewer than 2^32 threads: 1024 for each sequence and head that an eviction chooses for,
+    one for each 8 elements that it moves or that are appended, 256 for each tile of attention."""
+    for change in (dict(sequences=1 << 21), dict(sequences=1 << 22, heads=1), dict(sequences=1 << 30)):
+        assert evict(lib, pages(**change)) == UNSUPPORTED
+    assert evict(lib, pages(), keep=1 << 28, width=1 << 24) == UNSUPPORTED
+    assert append(lib, pages(), rows=1 << 28) == UNSUPPORTED
+    p, a = pages(sequences=1 << 23), queries(rows_q=(1 << 27) + 1)
+    assert attention(lib, p, a, weights=None, log_sum=None) == UNSUPPORTED
+
+
 def test_counts_that_pass_32_bits():
     """(Sizes alone: with a table of no pages they cost next to nothing.)"""
     shape, w = (1, 16, 2, 64), (None, None)
