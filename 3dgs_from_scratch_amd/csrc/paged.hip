@@ -24,7 +24,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(
     const int rest = (int)(at - row * a_row), head = rest / chunks, chunk = rest - head * chunks;
     int low = 0, high = p.sequences + 1;  // offsets that are at most row
     while (low < high) {
-        const int middle = (low + high) / 2;
+        const int middle = low + (high - low) / 2;  // (the sum of both may pass 32 bits)
         if (offsets[middle] <= row)
             low = middle + 1;
         else

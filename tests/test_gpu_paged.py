@@ -215,6 +215,23 @@ def test_append_past_32_bits(gpu):
     assert same(v_pages[new_tables[0].long()].reshape(4, 1, 64)[:3], v[[1, 4, 5]])
 
 
+def test_append_to_more_than_2_30_sequences(gpu):
+    """(Of which the last three have a token: 4 GB of offsets, and as much of lengths.)"""
+    n = (1 << 30) + 100
+    offsets = torch.zeros(n + 1, dtype=torch.int32, device=gpu)
+    offsets[-3:] = torch.tensor([1, 2, 3], device=gpu)
+    lengths = torch.zeros(n, dtype=torch.int32, device=gpu)
+    lengths[-3:] = torch.tensor([5, 1, 3], device=gpu)
+    tables = torch.zeros(1, 1, dtype=torch.int32, device=gpu).expand(n, 1)
+    pool = [torch.zeros(1, 8, 2, 16, dtype=torch.float16, device=gpu) for _ in range(2)]
+    k, v = (queries(gpu, 3, 2, 16, torch.float16, s) for s in (1, 2))
+    cr.paged_append(k, v, *pool, tables, lengths, offsets)
+    for got, new in zip(pool, (k, v)):
+        want = torch.zeros_like(got)
+        want[0, [4, 0, 2]] = new
+        assert same(got, want)
+
+
 # ------------------------------------------------------------------ attention
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("causal", [False, True])
