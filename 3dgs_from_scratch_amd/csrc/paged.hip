@@ -325,6 +325,7 @@ int check_pages(const GsPages *p, bool weights) {
         return GS_ERR_UNSUPPORTED;
     if (p->type == GS_F32 || p->dim % 8 != 0 || p->dim > GS_MAX_HEAD_DIM ||
         p->pages > 0x7fffffffLL || (int64_t)p->page_size * p->table_width > kMaxSlots ||
+        p->sequences > kMaxSlots || p->page_size > kMaxSlots || (int64_t)p->heads * (p->dim / 8) > kMaxSlots ||
         p->slot_stride < p->dim || p->slot_stride > (1 << 23) ||
         (p->page_stride | p->slot_stride | p->head_stride) % 8 != 0)
         return GS_ERR_UNSUPPORTED;

@@ -788,7 +788,8 @@ int gs_attention_backward(const GsAttention *a, const void *q, const void *k, co
  * page_size * table_width.  tables, lengths and offsets are device memory.
  * dim is a multiple of 8 and at most GS_MAX_HEAD_DIM, type GS_F16 or GS_BF16; pools
  * are 16-byte aligned with strides that are multiples of 8, slot_stride from dim to
- * 2^23, all strides below 2^31; a table covers less than 2^31 - 65536 slots
+ * 2^23, all strides below 2^31; a table covers less than 2^31 - 65536 slots, and there
+ * are fewer sequences, places of a page and heads times dim / 8 than that
  * (GS_ERR_UNSUPPORTED otherwise).
  */
 typedef struct {

@@ -103,6 +103,15 @@ def test_refused_arguments(lib):
         assert evict(lib, pages(**{stride: 1 << 31})) == UNSUPPORTED
 
 
+@pytest.mark.parametrize("change", [dict(sequences=(1 << 31) - 1), dict(page_size=(1 << 31) - 1, table_width=0),
+                                    dict(heads=1 << 28)])
+def test_counts_near_2_31(lib, change):
+    """What is one more, or a row's heads in eights, stays in 32 bits."""
+    p = pages(**change)
+    assert append(lib, p, rows=1) == attention(lib, p, queries(heads_q=p.heads)) == UNSUPPORTED
+    assert evict(lib, p, keep=1) == UNSUPPORTED
+
+
 def test_more_kept_than_slots_have_numbers(lib):
     most = (1 << 31) - 1 - 65536
     for keep in (most + 1, (1 << 31) - 1):
