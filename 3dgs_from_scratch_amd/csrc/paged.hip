@@ -33,8 +33,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(
     const int b = low - 1;
     if (b < 0 || b >= p.sequences) return;
     const int64_t end = offsets[b + 1] < rows ? offsets[b + 1] : rows;
-    const int64_t slot = filled_slots(p, b) - (end - row);
-    if (slot < 0) return;
+    // (not by the length as the table clamps it, which would be an earlier token's slot)
+    const int64_t slot = p.lengths[b] - (end - row);
+    if (slot < 0 || slot >= (int64_t)p.page_size * p.table_width) return;
     const int index = (int)(slot / p.page_size), place = (int)(slot - (int64_t)index * p.page_size);
     const int page = page_of(p, b, index);
     if (page < 0) return;

@@ -804,7 +804,8 @@ typedef struct {
 /*
  * gs_paged_append: row offsets[b] + t of k and v (rows k_row and v_row apart, heads
  *   k_head and v_head, 16-byte aligned, multiples of 8) goes to slot lengths[b] -
- *   (offsets[b + 1] - offsets[b]) + t of sequence b, so lengths count the new slots;
+ *   (offsets[b + 1] - offsets[b]) + t of sequence b, so lengths count the new slots (here
+ *   they are not clamped to the table; offsets are to rows);
  *   their weights become 0 where weights is set.  rows * heads * dim / 8 is below 2^32 - 256
  *   (GS_ERR_UNSUPPORTED otherwise).  Rows of no sequence, and rows whose
  *   slot is below 0, past the table or on no page, go nowhere.

@@ -29,8 +29,8 @@ def append(k, v, k_pages, v_pages, tables, lengths, offsets, weights=None):
     for b in range(tables.shape[0]):
         end = min(at[b + 1], k.shape[0])
         for row in range(max(at[b], 0), end):
-            slot = filled(tables, lengths, b, size) - (end - row)
-            if slot < 0:
+            slot = int(lengths[b]) - (end - row)
+            if not 0 <= slot < tables.shape[1] * size:
                 continue
             page = int(tables[b, slot // size])
             if not 0 <= page < pages:

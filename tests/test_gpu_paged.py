@@ -215,6 +215,23 @@ def test_append_past_32_bits(gpu):
     assert same(v_pages[new_tables[0].long()].reshape(4, 1, 64)[:3], v[[1, 4, 5]])
 
 
+@pytest.mark.parametrize("page", [4, 64])
+def test_append_past_the_table(gpu, page):
+    """New tokens that the table has no slot for go nowhere, and the earlier ones stay."""
+    c = Cache(gpu, [64, 64, 64], page, 2, 64, torch.bfloat16)
+    before = [t.clone() for t in (c.k, c.v, c.w)]
+    c.lengths.copy_(torch.tensor([70, 64, 1000], device=gpu))
+    new = [10, 10, 10]
+    k, v = (queries(gpu, 30, 2, 64, torch.bfloat16, s) for s in (1, 2))
+    check_append(c, k, v, offsets_of(new, gpu))
+    for b, (first, n) in enumerate(((60, 4), (54, 10), (64, 0))):
+        slots = torch.arange(64, device=gpu)
+        at = c.tables[b, slots // page].long(), slots % page
+        for got, was, rows in zip((c.k, c.v, c.w), before, (k, v, torch.zeros(30, 2, device=gpu))):
+            assert same(got[at][:first], was[at][:first])
+            assert same(got[at][first:], rows[10 * b:10 * b + n])
+
+
 def test_append_to_more_than_2_30_sequences(gpu):
     """(Of which the last three have a token: 4 GB of offsets, and as much of lengths.)"""
     n = (1 << 30) + 100

@@ -215,6 +215,15 @@ def test_oracle_appends_to_the_last_slots():
     assert int((k2 != k).any(3).any(2).sum()) == 5 and int((w2 != w).any(2).sum()) == 5
 
 
+def test_oracle_appends_nothing_past_the_table():
+    k, v, w, tables = small()
+    lengths, offsets = torch.tensor([10, 13], dtype=torch.int32), torch.tensor([0, 0, 4], dtype=torch.int32)
+    new = torch.randn(4, 2, 8)
+    k2, _, w2 = op.append(new, new, k, v, tables, lengths, offsets, w)  # slots 9 to 12 of 12
+    assert torch.equal(k2[2, 1:], new[:3]) and bool((w2[2, 1:] == 0).all())
+    assert int((k2 != k).any(3).any(2).sum()) == 3
+
+
 def test_oracle_attention_is_that_of_packed_rows():
     k, v, _, tables = small()
     lengths = torch.tensor([7, 10], dtype=torch.int32)
