@@ -275,7 +275,9 @@ __global__ __launch_bounds__(32 * kJoinRows) void paged_join_rows_kernel(
 
 // ---------------------------------------------------------------- slots' weights
 // S = Q K^T once more, now that a row's log-sum L is known: a lane has a slot, and adds up
-// exp2(c S - L) over the rows in its registers.  No atomics: a slot and head is one wave's.
+// exp2(c S - L) over the rows in its registers.  A slot and head is one wave's, and its sum is added
+// to the weight at once: other sequences, or other places of the same, may have the page too.  Where
+// none has, that is one addition, the same in every call.
 // 16 rows of a tile are added in pairs, so that chains of additions grow by one for 32 rows.
 
 // Sum over the 16 rows of a 32x32 result that a lane holds; minus: -L of each, minus infinity for
@@ -302,14 +304,13 @@ __device__ __forceinline__ float minus_log(float log_sum) {
 }
 
 constexpr int kWeightSlots = 32 * kWaves;  // of a workgroup
-constexpr int kScoreSlots = 256;           // of one where the scores are there
+constexpr int kScoreSlots = 256;           // and heads, of one where the scores are there
 
 // The slots of a workgroup, and what its lanes have of them.
 template <typename T, int DIM>
 struct SlotOperand {
     RowOperand<T, DIM> k;
-    float *weight;        // null: no such slot
-    float before = 0.0f;  // what it is, read beside the key
+    float *weight;  // null: no such slot
     __device__ __forceinline__ SlotOperand(const GsPages &p, const T *keys, float *weights, int sequence,
                                            int slot, int filled, int kh, bool negate)
         : weight(nullptr) {
@@ -323,21 +324,20 @@ struct SlotOperand {
             }
         }
         k.load(row, p.dim, negate);
-        if (weight) before = *weight;
     }
     // sum: of the lane's rows, half of all
     __device__ __forceinline__ void add(float sum) const {
         sum = half_sum(sum);
-        if (__lane_id() < 32 && weight) *weight = before + sum;
+        if (__lane_id() < 32 && weight) unsafeAtomicAdd(weight, sum);
     }
 };
 
-// f(sequence, tile, key head) for the tiles of SLOTS slots of all sequences that have queries, from
-// number `item` on every `every`th.  Most workgroups have one, and find it in one look through the
-// sequences.
-template <int SLOTS, typename F>
-__device__ __forceinline__ void for_slot_tiles(const GsAttention &a, const GsPages &p, int item, int every,
-                                               F f) {
+// f(sequence, tile, part) for the tiles of so many slots of all sequences that have queries, each in
+// `parts` parts (of key heads), from number `item` on every `every`th.  Most workgroups have one, and find
+// it in one look through the sequences.
+template <typename F>
+__device__ __forceinline__ void for_slot_tiles(const GsAttention &a, const GsPages &p, int slots, int parts,
+                                               int item, int every, F f) {
     const int lane = __lane_id();
     int upto = 0;  // places of 64 sequences up to and with the lane's
     const auto look = [&](int first) {  // all of them
@@ -345,7 +345,7 @@ __device__ __forceinline__ void for_slot_tiles(const GsAttention &a, const GsPag
         int n = 0;
         if (s <= a.sequences) {
             const int2 q = rows_of(a.offsets_q, a.sequences, a.rows_q, s);
-            n = q.x == q.y ? 0 : (slots_of(p, s) + SLOTS - 1) / SLOTS * a.heads_k;
+            n = q.x == q.y ? 0 : (slots_of(p, s) + slots - 1) / slots * parts;
         }
         upto = (int)lanes_sum_upto((uint32_t)n);
         return __builtin_amdgcn_readlane(upto, kWave - 1);
@@ -360,7 +360,7 @@ __device__ __forceinline__ void for_slot_tiles(const GsAttention &a, const GsPag
         }
         const int l = __builtin_ctzll(__ballot(before + upto > item));
         const int place = item - before - (l ? __builtin_amdgcn_readlane(upto, l - 1) : 0);
-        f(first + l + 1, place / a.heads_k, place % a.heads_k);
+        f(first + l + 1, place / parts, place % parts);
         item += every;
     }
 }
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
     const int wave = uniform(threadIdx.x / kWave);
     const float c = exponent_factor(a.scale);
     const auto copy = QTile::copy_of(wave, a.q_row, a.dim);
-    for_slot_tiles<kWeightSlots>(a, p, blockIdx.x, gridDim.x, [&](int sequence, int tile, int kh) {
+    for_slot_tiles(a, p, kWeightSlots, a.heads_k, blockIdx.x, gridDim.x, [&](int sequence, int tile, int kh) {
         const int2 rows = rows_of(a.offsets_q, a.sequences, a.rows_q, sequence);
         const int q0 = uniform(rows.x), lq = uniform(rows.y - rows.x);
         const int filled = uniform(slots_of(p, sequence));
@@ -463,7 +463,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_few_weights_kernel(
     const int group = a.heads_q / a.heads_k, lane = __lane_id(), half = lane >> 5;
     const int wave = uniform(threadIdx.x / kWave);
     const float c = exponent_factor(a.scale);
-    for_slot_tiles<kWeightSlots>(a, p, blockIdx.x, gridDim.x, [&](int sequence, int tile, int kh) {
+    for_slot_tiles(a, p, kWeightSlots, a.heads_k, blockIdx.x, gridDim.x, [&](int sequence, int tile, int kh) {
         const int2 range = rows_of(a.offsets_q, a.sequences, a.rows_q, sequence);
         const int q0 = uniform(range.x), lq = uniform(range.y - range.x), rows = lq * group;
         const int filled = uniform(slots_of(p, sequence));
@@ -494,23 +494,28 @@ __global__ __launch_bounds__(64 * kWaves) void paged_few_weights_kernel(
     });
 }
 
-// Few rows whose scores the attention has kept: a thread a slot.  Rows in parts are joined by the last
-// `joins` workgroups of the same launch, a row each, and the slots' workgroups find a row's log-sum from
-// its parts for themselves: a launch less, 45 instead of 47 us for 64 single tokens over 12 to 2500 slots.
-// Bound by latency: the sequence, the log-sums, the scores and the page, the weight.
+// Few rows whose scores the attention has kept: a thread a slot and head, `beside` heads a workgroup.
+// Weights of neighbouring heads are neighbours in memory where heads are the last dimension, and a
+// workgroup adds them slot by slot, since additions go to memory a line at a time.  Rows in parts are joined
+// by the last `joins` workgroups of the same launch, a row each, and the slots' workgroups find a row's
+// log-sum from its parts for themselves: a launch less.  Bound by latency: the sequence, the log-sums, the
+// scores and the page.
 template <typename T>
 __global__ __launch_bounds__(kScoreSlots) void paged_score_weights_kernel(
     GsAttention a, GsPages p, const float *__restrict__ scores, int64_t score_slots, Partial partial,
-    int joins, T *__restrict__ out, float *log_sum, float *__restrict__ weights) {
+    int joins, int beside, T *__restrict__ out, float *log_sum, float *__restrict__ weights) {
     __shared__ f32x4 sums[8][32];
-    __shared__ float minus[kWave];  // -L of so many rows, in the exponent of two
+    __shared__ float minus[kScoreSlots / kWave][kWave];  // -L of so many rows of each head, in the exponent of two
     const int64_t all_rows = a.rows_q * a.heads_q;
     const int tiles = gridDim.x - joins;
     if ((int)blockIdx.x >= tiles) {
         join_row<T>(blockIdx.x - tiles, all_rows, a.dim, partial, out, (T *)nullptr, log_sum, sums);
         return;
     }
+    float *const sum_of = (float *)sums;  // of each thread
     const int group = a.heads_q / a.heads_k, lane = __lane_id(), wave = uniform(threadIdx.x / kWave);
+    // waves of the same head follow one another every `beside`
+    const int slots = kScoreSlots / beside, wave_slots = wave / beside, wave_head = wave % beside;
     const float c = exponent_factor(a.scale);
     const auto minus_of = [&](int64_t row) {  // (every lane of a wave calls it)
         if (partial.splits == 1) return minus_log(log_sum[row]);
@@ -522,25 +527,28 @@ __global__ __launch_bounds__(kScoreSlots) void paged_score_weights_kernel(
         const float l = top == -INFINITY ? -INFINITY : top + __builtin_amdgcn_logf(wave_sum(share));
         return l == -INFINITY ? -INFINITY : -l;
     };
-    for_slot_tiles<kScoreSlots>(a, p, blockIdx.x, tiles, [&](int sequence, int tile, int kh) {
+    for_slot_tiles(a, p, slots, a.heads_k / beside, blockIdx.x, tiles, [&](int sequence, int tile, int part) {
         const int2 range = rows_of(a.offsets_q, a.sequences, a.rows_q, sequence);
         const int q0 = uniform(range.x), lq = uniform(range.y - range.x), rows = lq * group;
-        const int filled = uniform(slots_of(p, sequence)), slot = tile * kScoreSlots + (int)threadIdx.x;
-        const int index = slot / p.page_size;
-        const int page = slot < filled ? page_of(p, sequence - 1, index) : -1;
+        const int filled = uniform(slots_of(p, sequence)), kh = part * beside + wave_head;
+        const int slot = tile * slots + wave_slots * kWave + lane;
         // the first row that sees the slot
         const int least = slot >= filled ? rows : a.causal ? max(slot - (filled - lq), 0) * group : 0;
         const auto row_of = [&](int r) {
             const int i = r / group;
             return (int64_t)(q0 + i) * a.heads_q + kh * group + (r - i * group);
         };
+        // the slot and head whose sum this thread adds to its weight
+        const int to = (int)threadIdx.x / beside, to_head = (int)threadIdx.x % beside;
+        const int to_slot = tile * slots + to, index = to_slot / p.page_size;
+        const int page = to_slot < filled ? page_of(p, sequence - 1, index) : -1;
         float sum = 0.0f;
         for (int r0 = 0; r0 < rows; r0 += kWave) {
             const int end = min(r0 + kWave, rows);
             __syncthreads();  // the rows before have been read
-            for (int r = r0 + wave; r < end; r += kScoreSlots / kWave) {
+            for (int r = r0 + wave_slots; r < end; r += kScoreSlots / kWave / beside) {
                 const float m = minus_of(row_of(r));
-                if (lane == 0) minus[r - r0] = m;
+                if (lane == 0) minus[wave_head][r - r0] = m;
             }
             __syncthreads();
             for (int r = max(r0, least); r < end; r += 4) {
@@ -550,11 +558,20 @@ __global__ __launch_bounds__(kScoreSlots) void paged_score_weights_kernel(
                     s[n] = r + n < end ? scores[row_of(r + n) * score_slots + slot] : 0.0f;
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
-                    w[n] = r + n < end ? __builtin_amdgcn_exp2f(fmaf(s[n], c, minus[r + n - r0])) : 0.0f;
+                    w[n] = r + n < end ? __builtin_amdgcn_exp2f(fmaf(s[n], c, minus[wave_head][r + n - r0]))
+                                       : 0.0f;
                 sum += (w[0] + w[1]) + (w[2] + w[3]);
             }
         }
-        if (page >= 0) weights[sum_at(p, page, slot - index * p.page_size, kh)] += sum;
+        if (beside > 1) {
+            sum_of[threadIdx.x] = sum;
+            __syncthreads();
+            sum = sum_of[(to / kWave * beside + to_head) * kWave + to % kWave];
+            __syncthreads();  // before the next tile's
+        }
+        if (page >= 0)
+            unsafeAtomicAdd(
+                &weights[sum_at(p, page, to_slot - index * p.page_size, part * beside + to_head)], sum);
     });
 }
 
@@ -704,26 +721,32 @@ extern "C" int gs_paged_attention(const GsPages *p, const GsPagedQueries *querie
         if (s || !weights || (!scores && (p->sequences == 0 || p->table_width == 0))) return s;
         // as many workgroups as there are tiles if no page is in two tables; the workgroups go on
         // while there are more
-        const auto grid = [&](int64_t size) {
+        const auto grid = [&](int64_t size, int parts) {
             const int64_t slots = (int64_t)p->page_size * p->table_width;
             const int64_t tables = (slots + size - 1) / size * p->sequences;
             const int64_t pool = p->pages * p->page_size / size + p->sequences;
-            const int64_t groups = (tables < pool ? tables : pool) * p->heads;
+            const int64_t groups = (tables < pool ? tables : pool) * parts;
             return dim3((unsigned)(groups < 8192 ? groups : 8192));
         };
         const float *log = log_sum;
         const int joins = scores && f.splits > 1 ? (int)(a.rows_q * a.heads_q) : 0;
-        const unsigned both = joins + grid(kScoreSlots).x;
+        // heads beside each other take fewer lines, and each row's log-sum more often: where a sequence has
+        // fewer rows on average than there are key heads.  Single tokens, a head by itself and beside others:
+        // 64 over 12 to 2500 slots, 12 heads 52 and 41 us, 48 heads on 12 54 and 46; 16 over 2500 to 32640, 16
+        // heads on 4, 118 and 122; 8 times 8 over 2500 to 8160 41 and 52
+        const bool few = a.rows_q * (a.heads_q / a.heads_k) < (int64_t)a.sequences * a.heads_k;
+        const int beside = !few ? 1 : p->heads % 4 == 0 ? 4 : p->heads % 2 == 0 ? 2 : 1;
+        const unsigned both = joins + grid(kScoreSlots / beside, p->heads / beside).x;
         if (scores && both > 0)
             hipLaunchKernelGGL((paged_score_weights_kernel<T>), dim3(both), dim3(kScoreSlots), 0, stream, a,
-                               *p, (const float *)scores, score_slots, partial, joins, (T *)out, log_sum,
-                               weights);
+                               *p, (const float *)scores, score_slots, partial, joins, beside, (T *)out,
+                               log_sum, weights);
         else if (f.by_keys && !scores)
-            hipLaunchKernelGGL((paged_few_weights_kernel<T, kDim>), grid(kWeightSlots), dim3(64 * kWaves), 0,
-                               stream, a, *p, tq, tk, log, weights);
+            hipLaunchKernelGGL((paged_few_weights_kernel<T, kDim>), grid(kWeightSlots, p->heads),
+                               dim3(64 * kWaves), 0, stream, a, *p, tq, tk, log, weights);
         else if (!scores)
-            hipLaunchKernelGGL((paged_weights_kernel<T, kDim>), grid(kWeightSlots), dim3(64 * kWaves), 0,
-                               stream, a, *p, tq, tk, log, weights);
+            hipLaunchKernelGGL((paged_weights_kernel<T, kDim>), grid(kWeightSlots, p->heads),
+                               dim3(64 * kWaves), 0, stream, a, *p, tq, tk, log, weights);
         return launch_status();
     };
     return p->type == GS_F16 ? with_tile(p->dim, [&](auto d) { return all(f16{}, d); })

@@ -10,7 +10,7 @@ no end; here their keys and values lie in pages of one pool:
     lengths            (sequences,), int32: the slots that it has filled
 
 Slot i of sequence b is place i % page_size of page tables[b, i // page_size].  Who owns
-which page is the caller's to say, and sequences may share pages that are only read.
+which page is the caller's to say, and sequences may share pages that nothing is appended to.
 
 - paged_append(k, v, k_pages, v_pages, tables, lengths, offsets, weights): new tokens' keys
   and values into the last slots of their sequences;
@@ -199,7 +199,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     token i goes to slot lengths[b] - Ln + i, so lengths already count them.  The slots'
     weights become 0 where weights is given.  Rows before the first offset or after the last,
     and tokens whose slot is below 0, past the table or on no page, go nowhere, so that no
-    earlier token is lost; offsets are clamped to the tokens.  Two tokens on one place of a page (a page that two tables have) leave either."""
+    earlier token is lost; offsets are clamped to the tokens.  Two tokens on one place of a page (a page that two tables have) leave a mixture."""
     what = "paged_append"
     _no_gradient(what, k, v, k_pages, v_pages, weights)
     tables, lengths, offsets = _rows(tables), _rows(lengths), _rows(offsets)
@@ -241,8 +241,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     With weights also adds to each slot's weight the probabilities that it gets, summed over
     the sequence's queries and the heads that share its key head, in float32 and in an order
-    that depends on the sizes and tables alone.  A page that the tables hold twice gets its
-    weights from one of its places there, whichever.  With weights, sequences times key heads
+    that depends on the sizes and tables alone.  A page that the tables hold several times, such
+    as one that sequences share, gets those of all its places there, in any order: only there
+    may the last bits of repeated calls differ.  With weights, sequences times key heads
     times the slots that a table's row covers are below 2^38 - 2^23.
 
     scale defaults to dim ** -0.5.  With return_log_sum also the float32 (queries, heads)

@@ -830,8 +830,10 @@ typedef struct {
  *   log_sum as gs_attention_forward's.  When weights is set, every slot's weight of
  *   head h grows by exp(scale q k^T - log_sum) summed over the sequence's queries that
  *   see it and the query heads that read head h; then log_sum has to be set.  Queries
- *   with a log-sum of -infinity add nothing.  Deterministic: no atomics.  With weights
- *   sequences * heads * the table's slots / 128 stays below 2^31 - 65536 too.
+ *   with a log-sum of -infinity add nothing.  A page that the tables hold several times gets
+ *   all of that, by atomic additions; where they hold every page once the result is the
+ *   same in every call.  With weights sequences * heads * the table's slots / 128 stays
+ *   below 2^31 - 65536 too.
  */
 int gs_paged_attention_workspace_size(const GsPages *p, const GsPagedQueries *q, int32_t weights,
                                       size_t *bytes);

@@ -71,8 +71,9 @@ def attention(q, k_pages, v_pages, tables, lengths, offsets, causal=False, scale
             p = torch.where(some, torch.exp(s - torch.where(some, lse, 0.0)), 0.0)
             res["out"][q0:q1, h], res["log_sum"][q0:q1, h] = p @ vh, lse[:, 0]
             res["out_slack"][q0:q1, h] = 2.5 * (p @ vh.abs())
-            got[page, place, h // group] += p.sum(0)
-            terms[page, place, h // group] += seen.sum(0)
+            at_head = page, place, torch.full_like(page, h // group)  # (a place may come twice)
+            got.index_put_(at_head, p.sum(0), accumulate=True)
+            terms.index_put_(at_head, seen.sum(0).double(), accumulate=True)
     return res | {"weights": got, "weights_terms": terms}
 
 

@@ -412,6 +412,59 @@ def test_attention_of_skewed_chunks(gpu, page):
             check_attention(queries(gpu, sum(new), 4, 64, dtype), c, offsets_of(new, gpu))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page", [24, 64])
+@pytest.mark.parametrize("new,width", [([1] * 6, 0), ([2] * 6, 0), ([1] * 6, (1 << 25) // 24), ([60] * 6, 0),
+                                       ([70, 1, 0, 200, 5, 90], 0)])
+def test_weights_of_shared_pages(gpu, new, width, page, dtype):
+    """A page of several sequences, or twice in a table, gets what each of its places adds.  The bound is
+    check_attention's, and a rounding (e of the sum) for each place that adds."""
+    lengths = [400, 300, 130, 500, 64, 200]
+    c = Cache(gpu, lengths, page, 2, 64, dtype, width=width)
+    pages = 128 // page
+    c.tables[1:, :pages] = c.tables[0, :pages]  # the first slots are all sequences'
+    c.tables[3, pages + 1:300 // page] = c.tables[3, pages]  # and one page is all over a table
+    q = queries(gpu, sum(new), 4, 64, dtype)
+    k, v, tables, lengths = c.args()
+    at = offsets_of(new, gpu)
+    for causal in (True, False):
+        ref = op.attention(q, k, v, tables, lengths, at, causal)
+        there = ref["weights_terms"] > 0
+        reach = 64 ** -0.5 * float(q.double().norm(dim=2).max()) * float(k.double().norm(dim=3)[there].max())
+        size = ref["log_sum"][~torch.isinf(ref["log_sum"])].abs()
+        off = 2 * (64 + 16) * E * (reach + float(size.max()) + 1) + 8 * E
+        off = off + (ref["weights_terms"] / 32 + 64) * E
+        places = 6 + 300 // page
+        for _ in range(3):
+            w = c.w.clone()
+            cr.paged_attention(q, k, v, tables, lengths, at, causal, weights=w)
+            want = c.w.double() + ref["weights"]
+            bound = off * ref["weights"] + (1 + places) * E * want + 2.0 ** -126 * ref["weights_terms"]
+            within(w[there], want[there], bound[there], "weights")
+            assert same(w[~there], c.w[~there])
+
+
+@pytest.mark.parametrize("page", [24, 64])
+def test_weights_below_the_smallest_normal_float(gpu, page):
+    """They stay as they are where nothing is added, as every other weight."""
+    for new in (1, 200):
+        c = Cache(gpu, [300], page, 1, 64, torch.float16)
+        slots = torch.arange(300, device=gpu)
+        at = c.tables[0, slots // page].long(), slots % page
+        c.k[at] = 0.0
+        seen = at[0][7], at[1][7]
+        c.k[seen] = 16.0  # its score is 2048, the others' 0: their probabilities are 0 in float
+        q = torch.full((new, 1, 64), 16.0, dtype=torch.float16, device=gpu)
+        for small in (1e-40, 2.0 ** -149, -3e-39):
+            c.w[at] = small
+            want = c.w.clone()
+            cr.paged_attention(q, *c.args(), offsets_of([new], gpu), weights=c.w)
+            # a probability of 1 from a score and a log-sum of 2048 each, as check_attention's bound has it
+            assert abs(float(c.w[seen]) - new) <= 2 * (64 + 16) * E * (2048 + 2048 + 1) * new
+            c.w[seen] = want[seen]
+            assert same(c.w, want)
+
+
 @pytest.mark.parametrize("page", [24, 64])
 @pytest.mark.parametrize("lengths,new", [([300], [300]), ([5000], [1]), ([3000], [100])])
 def test_attention_of_keys_that_all_score_minus_infinity(gpu, lengths, new, page):
