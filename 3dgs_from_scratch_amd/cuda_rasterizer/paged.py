@@ -303,6 +303,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     (sequences, key_heads, keep)) which, rising, -1 behind the last."""
     what = "paged_evict"
     _no_gradient(what, k_pages, v_pages, weights)
+    given = tables, new_tables
     tables, lengths, new_tables = _rows(tables), _rows(lengths), _rows(new_tables)
     if weights is None:
         raise RuntimeError(f"{what}: weights must be a torch.Tensor, got NoneType")
@@ -318,7 +319,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     if new_tables.shape[0] != p.sequences or new_tables.shape[1] * p.page_size < keep:
         raise RuntimeError(f"{what}: new_tables must have {p.sequences} rows of "
                            f"{-(-keep // p.page_size)} pages at least, got {tuple(new_tables.shape)}")
-    if new_tables.data_ptr() == tables.data_ptr() and tables.numel():
+    if given[0].data_ptr() == given[1].data_ptr() and tables.numel():  # (_rows may have copied them)
         raise ValueError(f"{what}: new_tables are the tables that are read; slots move to other pages")
     new_lengths = torch.empty(p.sequences, dtype=torch.int32, device=dev)
     kept = torch.empty((p.sequences, p.heads, keep), dtype=torch.int32, device=dev)

@@ -863,6 +863,17 @@ def test_refusals(gpu):
         torch.jit.trace(lambda x: cr.paged_attention(**{**calls["paged_attention"][1], "q": x}), q)
 
 
+def test_evict_refuses_the_tables_it_reads_in_any_layout(gpu):
+    c = Cache(gpu, [40, 9], 16, 2, 64, torch.float16)
+    by_page = c.tables.t().contiguous().t()  # neighbours in the first dimension
+    assert by_page.stride(1) != 1
+    for tables in (c.tables, by_page):
+        before = [t.clone() for t in (c.k, c.v, c.w)]
+        with pytest.raises(ValueError, match="other pages"):
+            cr.paged_evict(c.k, c.v, c.w, tables, c.lengths, tables, 16)
+        assert all(same(a, b) for a, b in zip(before, (c.k, c.v, c.w)))
+
+
 def test_what_autograd_saved_is_told_of_writes(gpu):
     """A cache that an earlier operation's gradient needs is not overwritten unnoticed."""
     c = Cache(gpu, [40], 16, 2, 64, torch.float16)
