@@ -31,14 +31,14 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 
 import torch
 from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import GsPagedQueries, GsPages
-from .tokens import _MAX_STRIDE, _TYPES, MAX_HEAD_DIM, _check, _laid_out, _ptr, _workspace
+from .tokens import (_MAX_STRIDE, _TYPES, MAX_HEAD_DIM, _check, _laid_out, _ptr, _scale_of,
+                     _workspace)
 
 _HALVES = (torch.float16, torch.bfloat16)
 MAX_SLOTS = (1 << 31) - 1 - 65536  # of a sequence
@@ -262,9 +262,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if heads < 1 or heads % p.heads:
         raise RuntimeError(f"{what}: {heads} heads are no multiple of {p.heads} key heads")
     _offsets(what, offsets, tables)
-    scale = p.dim ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"{what}: scale must be finite, got {scale}")
+    scale = _scale_of(what, scale, p.dim)
     q = _laid_out(q)
     a = GsPagedQueries(q.shape[0], q.stride(0), q.stride(1), offsets.data_ptr(), heads,
                        bool(causal), scale)

@@ -57,6 +57,14 @@ def _check(what: str, name: str, t, dims: int | None = None, types=_TYPES, devic
         raise RuntimeError(f"{what}: {name} must have {dims} dimensions, got {tuple(t.shape)}")
 
 
+def _scale_of(what: str, scale, dim: int) -> float:
+    scale = dim ** -0.5 if scale is None else float(scale)
+    # (the kernels multiply scores by it and by log2 e, in float)
+    if not math.isfinite(ctypes.c_float(scale * math.log2(math.e)).value):
+        raise ValueError(f"{what}: scale must be finite, in float32 and times log2(e) too, got {scale}")
+    return scale
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -415,9 +423,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets_
                                f"{'at least 1' if want is None else want}")
     offsets_q, offsets_k = offsets_q.contiguous(), offsets_k.contiguous()
     lengths_k = None if lengths_k is None else lengths_k.contiguous()
-    scale = dim ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"packed_attention: scale must be finite, got {scale}")
+    scale = _scale_of("packed_attention", scale, dim)
     args = (q, k, v, offsets_q, offsets_k, lengths_k, bool(causal), scale)
     if _differentiable("packed_attention", q, k, v):
         out, log_sum = _PackedAttention.apply(*args)

@@ -137,6 +137,14 @@ def test_entry_points_reject_on_the_host():
                                     None, None, None, None, 0, None) == 0
 
 
+@pytest.mark.parametrize("scale", [math.inf, -math.inf, math.nan, 1e39, -1e300, 3e38])
+def test_scales_that_are_not_finite_in_float32(scale):
+    from cuda_rasterizer.tokens import _scale_of
+    with pytest.raises(ValueError, match="x: scale must be finite"):
+        _scale_of("x", scale, 64)
+    assert _scale_of("x", None, 64) == 0.125 and _scale_of("x", -2, 64) == -2.0
+
+
 def test_attention_of_more_threads_than_a_launch_takes():
     """256 for each tile of packed rows and key head, and a launch has fewer than 2^32."""
     lib, some = _lib.load(), ctypes.c_void_p(4096)
