@@ -145,10 +145,17 @@ class PagedCache:
         self.tables.copy_(table)
 
     def grow(self, new):
-        """Room for `new` tokens of each scene."""
-        for b, n in enumerate(new):
-            self.filled[b] += n
-            self.owned[b] += self._take(self.filled[b] - len(self.owned[b]) * self.page)
+        """Room for `new` tokens of each scene, or an error that leaves everything as it is."""
+        filled = [n + more for n, more in zip(self.filled, new, strict=True)]
+        pages = [-(-n // self.page) for n in filled]
+        wanted = sum(pages) - sum(map(len, self.owned))
+        if wanted > len(self.free):
+            raise RuntimeError(f"{wanted} pages are wanted and {len(self.free)} are free")
+        if max(pages, default=0) > self.tables.shape[1]:
+            raise RuntimeError(f"a scene wants {max(pages)} pages and the tables have {self.tables.shape[1]}")
+        for owned, count in zip(self.owned, pages):
+            owned += self._take((count - len(owned)) * self.page)
+        self.filled = filled
         self._deal()
 
     def attend(self, layer, q, k, v, offsets):
