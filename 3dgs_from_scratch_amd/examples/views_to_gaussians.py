@@ -166,21 +166,28 @@ class PagedCache:
 
     def evict(self, keep, recent):
         """Scenes of more than `keep` tokens keep so many: the last `recent`, and those that got the
-        most attention so far, each layer and key head its own."""
+        most attention so far, each layer and key head its own.  They move to free pages, as many scenes
+        at a time as those suffice for, and their old ones are free for the next: with none for a single
+        scene it raises, and changes nothing."""
         full = [b for b, n in enumerate(self.filled) if n > keep]
-        if not full:
-            return
-        fresh = [self._take(keep) for _ in full]
-        rows = torch.tensor(full, device=self.tables.device)
-        new_tables = torch.tensor(fresh, dtype=torch.int32).to(self.tables.device)
-        for layer in range(self.k.shape[0]):
-            lengths, _ = paged_evict(self.k[layer], self.v[layer], self.weights[layer], self.tables[rows],
-                                     self.lengths[rows], new_tables, keep, recent)
-        self.lengths[rows] = lengths
-        for b, pages in zip(full, fresh):
-            self.free += self.owned[b]
-            self.owned[b], self.filled[b] = pages, keep
-        self._deal()
+        count = max(1, -(-keep // self.page))
+        while full:
+            some = min(len(full), len(self.free) // count)
+            if not some:
+                raise RuntimeError(f"{count} pages are wanted and {len(self.free)} are free")
+            now, full = full[:some], full[some:]
+            fresh = [self.free[i * count:(i + 1) * count] for i in range(some)]
+            rows = torch.tensor(now, device=self.tables.device)
+            new_tables = torch.tensor(fresh, dtype=torch.int32).to(self.tables.device)
+            for layer in range(self.k.shape[0]):
+                lengths, _ = paged_evict(self.k[layer], self.v[layer], self.weights[layer],
+                                         self.tables[rows], self.lengths[rows], new_tables, keep, recent)
+            self.lengths[rows] = lengths
+            self.free = self.free[some * count:]
+            for b, pages in zip(now, fresh):
+                self.free += self.owned[b]
+                self.owned[b], self.filled[b] = pages, keep
+            self._deal()
 
 
 # --------------------------------------------------------------- views and tokens

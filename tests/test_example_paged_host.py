@@ -72,3 +72,38 @@ def test_no_room_to_grow_changes_nothing(cache, pages, width, message):
     assert state(c) == before
     fill(c, [0, 4, 3])
     dealt(c)
+
+
+def test_an_eviction_without_room_changes_nothing(cache):
+    c = cache(9)
+    fill(c, [12, 12, 10])
+    before = state(c)
+    with pytest.raises(RuntimeError, match="free"):
+        c.evict(5, 2)
+    assert state(c) == before
+
+
+def test_an_eviction_that_is_refused_changes_nothing(cache):
+    c = cache(30)
+    fill(c, [12, 12, 10])
+    before = state(c)
+    for keep, recent in ((5, 6), (5, -1), (0, 0)):
+        with pytest.raises(ValueError, match="paged_evict"):
+            c.evict(keep, recent)
+        assert state(c) == before
+
+
+@pytest.mark.parametrize("pages", [11, 12, 13, 30])
+def test_scenes_leave_in_turn_where_few_pages_are_free(cache, pages):
+    c = cache(pages)
+    fill(c, [12, 12, 10])
+    c.evict(5, 2)
+    dealt(c)
+    assert c.filled == [5, 5, 5]
+    for b, n in enumerate((12, 12, 10)):
+        rank = sorted(range(n - 2), key=lambda s: (-((s * 7) % 5), s))[:3]
+        kept = sorted(rank) + [n - 2, n - 1]
+        for layer in range(2):
+            got = [int(c.v[layer, c.owned[b][i // 4], i % 4, 0, 0]) for i in range(5)]
+            assert got == [int(torch.tensor(100.0 * b + s).bfloat16()) for s in kept]
+    c.grow([3, 0, 1])
