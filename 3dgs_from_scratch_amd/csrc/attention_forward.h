@@ -718,6 +718,11 @@ inline ForwardPlan plan_forward(const GsAttention &a, int64_t longest, int64_t a
         f.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
         const int64_t items = (packed / 32 + a.sequences + 2) * f.splits * a.heads_k;
         f.groups = items < 1024 ? items : 1024;
+        // (items have numbers of 32 bits: past those, more workgroups than a launch takes, so that it is refused)
+        const int64_t tiles = a.rows_q * ((group + 31) / 32);  // at most, however many sequences have none
+        const int64_t numbers = (tiles < packed / 32 + a.sequences + 2 ? tiles : packed / 32 + a.sequences + 2) *
+                                f.splits * a.heads_k;
+        if (numbers > kMaxRows) f.groups = numbers;
         return f;
     }
     // Workgroups that will find rows, at least, and as many splits of the keys as run at a time

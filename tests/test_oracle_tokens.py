@@ -152,6 +152,13 @@ def test_attention_of_more_threads_than_a_launch_takes():
     assert lib.gs_attention_forward(ctypes.byref(a), some, some, some, some, None, None, None, 0, None) == -4
 
 
+def test_attention_of_more_items_than_have_numbers():
+    """Single tokens of 2^28 sequences, 16 key heads each: an item is a sequence's tile, split and head."""
+    lib, some = _lib.load(), ctypes.c_void_p(4096)
+    a = _attention_problem(rows_q=1 << 28, heads_q=16, heads_k=16, sequences=1 << 28)
+    assert lib.gs_attention_forward(ctypes.byref(a), some, some, some, some, None, None, None, 0, None) == -4
+
+
 def test_python_layer_refuses_cpu_tensors_and_other_things():
     x = torch.zeros(4, 2, 64, dtype=torch.float16)
     at = torch.tensor([0, 4], dtype=torch.int32)

@@ -140,6 +140,13 @@ def test_more_threads_than_a_launch_takes(lib):
     assert attention(lib, p, a, weights=None, log_sum=None) == UNSUPPORTED
 
 
+def test_more_items_of_few_rows_than_have_numbers(lib):
+    """Single tokens of 2^28 sequences, 16 key heads each: an item is a sequence's tile, split and head."""
+    a = queries(rows_q=1 << 28, heads_q=16, row_stride=16 * 64)
+    p = pages(sequences=1 << 28, heads=16, slot_stride=16 * 64, page_stride=16 * 16 * 64)
+    assert attention(lib, p, a, weights=None, log_sum=None) == UNSUPPORTED
+
+
 def test_counts_that_pass_32_bits():
     """(Sizes alone: with a table of no pages they cost next to nothing.)"""
     shape, w = (1, 16, 2, 64), (None, None)
