@@ -363,6 +363,32 @@ def test_attention_equals_packed(gpu):
             assert float((got.double() - want.double()).norm()) <= 2 * U[dtype] * float(want.double().norm())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,new,bits", [([640, 200], [130, 200], True), ([3000, 64], [1, 1], True),
+                                              ([9000, 500, 64], [1, 1, 1], True),
+                                              ([9000, 500], [300, 20], False)])
+def test_attention_equals_packed_element_by_element(gpu, lengths, new, bits, dtype):
+    """Pages one after another are packed rows.  Where both calls split the keys alike, which for few rows
+    and for tiles of rows over less than 2048 slots they do, the same to the bit; else each is within
+    check_attention's bound of the definition, and so within twice that of the other."""
+    c = Cache(gpu, lengths, 64, 2, 128, dtype)
+    q = queries(gpu, sum(new), 8, 128, dtype)
+    at = offsets_of(new, gpu)
+    packed = [torch.cat([t[c.tables[b, :-(-n // 64)].long()].flatten(0, 1)[:n]
+                         for b, n in enumerate(lengths)]) for t in (c.k, c.v)]
+    want = cr.packed_attention(q, *packed, at, offsets_of(lengths, gpu), causal=True)
+    got = cr.paged_attention(q, *c.args(), at, causal=True)
+    if bits:
+        assert same(got, want)
+        return
+    slack = op.attention(q, *c.args(), at, True)["out_slack"]
+    reach = 128 ** -0.5 * float(q.double().norm(dim=2).max()) * float(packed[0].double().norm(dim=2).max())
+    bound = U[dtype] * slack + 2 * (128 + 16) * E * reach * slack + 1e-30
+    if dtype == torch.float16:
+        bound = bound + E * max(lengths) * float(packed[1].double().abs().max())
+    within(got, want.double(), 2 * bound, "out")
+
+
 def test_attention_of_what_is_not_finite(gpu):
     """A NaN in a query makes its output and the weights that it gives NaN, and no other's; an
     infinity in a value that a query sees comes out in its column; values that it does not see
@@ -410,6 +436,29 @@ def test_attention_of_skewed_chunks(gpu, page):
                              ([6000, 300, 2500], [130, 1, 0])):
             c = Cache(gpu, lengths, page, 2, 64, dtype)
             check_attention(queries(gpu, sum(new), 4, 64, dtype), c, offsets_of(new, gpu))
+
+
+@pytest.mark.parametrize("page", [24, 64])
+@pytest.mark.parametrize("sequences", [63, 64, 65, 125, 126, 127, 128, 129, 300])
+def test_attention_of_many_sequences(gpu, sequences, page):
+    """Single tokens, and chunks: as many sequences as lanes hold, one more, and looks through many of them."""
+    rng = random.Random(sequences + page)
+    for dtype in TYPES:
+        lengths = [rng.choice([0, 1, 30, 64, 100, 300]) for _ in range(sequences)]
+        lengths[rng.randrange(sequences)] = 3000
+        for most in (1, 3, 40):
+            new = [rng.choice([0, min(n, most), most]) for n in lengths]
+            c = Cache(gpu, lengths, page, 2, 64, dtype, seed=most)
+            check_attention(queries(gpu, sum(new), 4, 64, dtype), c, offsets_of(new, gpu))
+
+
+@pytest.mark.parametrize("page", [24, 64])
+def test_attention_of_many_sequences_over_wide_tables(gpu, page):
+    """Few rows whose scores are not kept, of more sequences than a look through them takes."""
+    lengths, rng = [20, 300, 0, 64, 129] * 30, random.Random(page)
+    new = [rng.choice([0, 1, 1]) for _ in lengths]
+    c = Cache(gpu, lengths, page, 2, 64, torch.float16, width=(1 << 18) // page)
+    check_attention(queries(gpu, sum(new), 8, 64, torch.float16), c, offsets_of(new, gpu))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -562,6 +611,33 @@ def test_evict_of_many_sequences(gpu):
     lengths = torch.randint(0, 90, (700,), generator=g).tolist()
     c = Cache(gpu, lengths, 16, 2, 16, torch.float16, spare=700 * 2)
     check_evict(c, c.spare.view(700, 2), 32, 8)
+
+
+@pytest.mark.parametrize("sequences", [65_535, 65_536, 66_001, 140_000])
+def test_evict_of_more_sequences_than_a_grid_has_rows(gpu, sequences):
+    """Three slots on a page of four, down to two: slots and weights follow from the sequence's number."""
+    b = torch.arange(sequences, device=gpu)
+    slots = torch.arange(4, device=gpu)
+    k = torch.zeros(2 * sequences, 4, 1, 8, dtype=torch.float16, device=gpu)
+    k[:sequences] = ((b[:, None] * 4 + slots) % 2039)[..., None, None].to(torch.float16)
+    v = -k
+    w = torch.zeros(2 * sequences, 4, 1, device=gpu)
+    w[:sequences, :, 0] = ((b[:, None] * 7 + slots * 5) % 11).float()
+    tables, new_tables = b[:, None].to(torch.int32), (b[:, None] + sequences).to(torch.int32)
+    filled = b % 4  # none to three
+    order = torch.where(slots < filled[:, None], w[:sequences, :, 0], -1.0)
+    order = torch.sort(order, dim=1, descending=True, stable=True)[1][:, :2].sort(1)[0]
+    there = slots[:2] < filled.clamp(max=2)[:, None]
+    # (of fewer slots than two, the first)
+    order = torch.where(filled[:, None] < 2, slots[:2], order)
+    want = [t.clone() for t in (k, v, w)]
+    for t in want:
+        moved = t[b[:, None], order]
+        t[sequences:, :2] = torch.where(there.view(there.shape + (1,) * (t.dim() - 2)), moved, t[sequences:, :2])
+    lengths, kept = cr.paged_evict(k, v, w, tables, filled.to(torch.int32), new_tables, 2)
+    assert torch.equal(lengths.long(), filled.clamp(max=2))
+    assert torch.equal(kept[:, 0].long(), torch.where(there, order, -1))
+    assert all(same(a, x) for a, x in zip((k, v, w), want))
 
 
 # ---------------------------------------------------------------------- drawn
@@ -749,6 +825,29 @@ def test_two_streams_at_once(gpu):
                 got.append(cr.paged_attention(q, *c.args(), at, True, weights=c.w))
         torch.cuda.synchronize()
         assert all(same(x, y) for x, y in zip(got, want))
+
+
+def test_weights_on_two_streams_at_once(gpu):
+    """Two calls at once, with and without kept scores: outputs and weights as those of the calls alone."""
+    for new, heads in (([40, 40], 8), ([1, 1], 8), ([1, 1], 2)):
+        held = []
+        for s in (2, 4):
+            c = Cache(gpu, [9000, 300], 64, 2, 128, torch.bfloat16, seed=s)
+            q, at = queries(gpu, sum(new), heads, 128, torch.bfloat16, s), offsets_of(new, gpu)
+            w = c.w.clone()
+            out = cr.paged_attention(q, *c.args(), at, True, weights=w)
+            held.append((c, q, at, out, w))
+        streams = [torch.cuda.Stream() for _ in held]
+        for _ in range(4):
+            weights = [c.w.clone() for c, *_ in held]
+            torch.cuda.synchronize()
+            got = []
+            for (c, q, at, _, _), w, one in zip(held, weights, streams):
+                with torch.cuda.stream(one):
+                    got.append(cr.paged_attention(q, *c.args(), at, True, weights=w))
+            torch.cuda.synchronize()
+            for (_, _, _, out, w), mine, now in zip(held, weights, got):
+                assert same(now, out) and same(mine, w)
 
 
 # --------------------------------------------------------------------- layouts
