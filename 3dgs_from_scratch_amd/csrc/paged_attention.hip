@@ -365,10 +365,10 @@ __device__ __forceinline__ void for_slot_tiles(const GsAttention &a, const GsPag
     }
 }
 
-// Many rows: tiles of a head's queries go through LDS, which the workgroup's waves share.  Bound by
-// issue: of a SIMD's time 44% are matrix instructions and 55% the others, an exponential, a
-// multiplication and an addition a score.  2 sequences, 8160 queries each over 28284 and 32640 slots,
-// 16 heads on 4, dim 128: 2.1 ms, 0.83 PFLOP/s.
+// Many rows: tiles of a head's queries go through LDS, which the workgroup's waves share.  No unit is
+// full: of the busy time matrix instructions take 43%, the others 54%, an exponential, a multiplication
+// and an addition a score, and LDS 54%, 22 of them for conflicts; they overlap in part only.  2 sequences,
+// 8160 queries each over 28284 and 32640 slots, 16 heads on 4, dim 128: 2.0 to 2.1 ms, 0.83 to 0.88 PFLOP/s.
 template <typename T, int DIM>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
     GsAttention a, GsPages p, const T *__restrict__ q, const T *__restrict__ k,
@@ -455,7 +455,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_weights_kernel(
 }
 
 // Few rows: a wave takes them from memory.  (Where the attention could not keep their scores.)  64 single
-// tokens over 12 to 2500 slots, 12 heads of 64: 32 us, and 11 from kept scores with the join.
+// tokens over 12 to 2500 slots, 12 heads of 64: 24 us more than without weights, and 7 from kept scores.
 template <typename T, int DIM>
 __global__ __launch_bounds__(64 * kWaves) void paged_few_weights_kernel(
     GsAttention a, GsPages p, const T *__restrict__ q, const T *__restrict__ k,
@@ -611,7 +611,8 @@ static GsAttention problem_of(const GsPages &p, const GsPagedQueries &q) {
 // as many as the average.  5 sequences of up to 300 over 8044 to 16320 slots, 12 heads on 4, dim 72:
 // 85 us in equal splits of each sequence, 77 in equal splits of all; 1200 rows over 20000, 16 heads
 // on 4, dim 128: 393 in 1, 243.  Not over short tables (600 over 1000: 34 in 1, 44), and not where the
-// tiles fill the GPU once (2500 over 10000: 260 in 1, 434): a second workgroup on a CU adds little.
+// tiles fill the GPU once (2500 over 10000: 260 in 1, 434): then there are more items than run at a time,
+// and what the last ones and the join take is more than what the CUs without a second tile lose.
 static ForwardPlan plan_of(const GsPages &p, const GsAttention &a) {
     const int64_t slots = (int64_t)p.page_size * p.table_width;
     ForwardPlan f = plan_forward(a, slots, slots);
