@@ -237,7 +237,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     says where each sequence's queries begin: one token each, or chunks of any sizes.  causal:
     of Lq queries, query i sees slots j <= i + lengths[b] - Lq, so that new tokens, appended
     before, see all before them; else every filled slot.  A query that sees no slot, and a row
-    of no sequence, gives 0.  lengths are clamped to the tables, offsets to the queries.
+    of no sequence, gives 0.  lengths are clamped to the tables, as if a longer sequence ended
+    there, offsets to the queries.
 
     With weights also adds to each slot's weight the probabilities that it gets, summed over
     the sequence's queries and the heads that share its key head, in float32 and in an order

@@ -808,7 +808,8 @@ typedef struct {
  *   they are not clamped to the table; offsets are to rows);
  *   their weights become 0 where weights is set.  rows * heads * dim / 8 is below 2^32 - 256
  *   (GS_ERR_UNSUPPORTED otherwise).  Rows of no sequence, and rows whose
- *   slot is below 0, past the table or on no page, go nowhere.
+ *   slot is below 0, past the table or on no page, go nowhere; two rows for one place of a
+ *   page leave a mixture.
  */
 int gs_paged_append(const GsPages *p, const void *k, int64_t k_row, int64_t k_head, const void *v,
                     int64_t v_row, int64_t v_head, int64_t rows, const int32_t *offsets,
@@ -831,8 +832,9 @@ typedef struct {
  *   head h grows by exp(scale q k^T - log_sum) summed over the sequence's queries that
  *   see it and the query heads that read head h; then log_sum has to be set.  Queries
  *   with a log-sum of -infinity add nothing.  A page that the tables hold several times gets
- *   all of that, by atomic additions; where they hold every page once the result is the
- *   same in every call.  With weights sequences * heads * the table's slots / 128 stays
+ *   all of that, by atomic additions, which weights take in the device's own memory only, not
+ *   in managed or host memory; where they hold every page once the result is the same in
+ *   every call.  With weights sequences * heads * the table's slots / 128 stays
  *   below 2^31 - 65536 too.
  */
 int gs_paged_attention_workspace_size(const GsPages *p, const GsPagedQueries *q, int32_t weights,

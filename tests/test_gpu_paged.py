@@ -494,6 +494,18 @@ def test_weights_of_shared_pages(gpu, new, width, page, dtype):
 
 
 @pytest.mark.parametrize("page", [24, 64])
+@pytest.mark.parametrize("key_heads", [4, 5, 6, 8, 12])
+def test_weights_of_many_key_heads(gpu, key_heads, page):
+    """Few rows, fewer than the key heads or more: heads one by one, in pairs, in fours."""
+    lengths = [300, 0, 1, 65, 5000, 64, 129]
+    for dtype in TYPES:
+        for group, new in ((1, [1] * 7), (2, [1, 0, 1, 1, 2, 1, 0]), (3, [2] * 7), (8, [1] * 7),
+                           (1, [40, 0, 1, 1, 1, 1, 1])):
+            c = Cache(gpu, lengths, page, key_heads, 32, dtype, heads_first=group == 2)
+            check_attention(queries(gpu, sum(new), key_heads * group, 32, dtype), c, offsets_of(new, gpu))
+
+
+@pytest.mark.parametrize("page", [24, 64])
 def test_weights_below_the_smallest_normal_float(gpu, page):
     """They stay as they are where nothing is added, as every other weight."""
     for new in (1, 200):
