@@ -505,7 +505,7 @@ __global__ __launch_bounds__(kScoreSlots) void paged_score_weights_kernel(
     GsAttention a, GsPages p, const float *__restrict__ scores, int64_t score_slots, Partial partial,
     int joins, int beside, T *__restrict__ out, float *log_sum, float *__restrict__ weights) {
     __shared__ f32x4 sums[8][32];
-    __shared__ float minus[kScoreSlots / kWave][kWave];  // -L of so many rows of each head, in the exponent of two
+    __shared__ float minus[kScoreSlots / kWave][kWave];  // -L of so many rows a head, in the exponent of two
     const int64_t all_rows = a.rows_q * a.heads_q;
     const int tiles = gridDim.x - joins;
     if ((int)blockIdx.x >= tiles) {

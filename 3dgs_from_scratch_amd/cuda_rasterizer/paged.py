@@ -199,7 +199,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     token i goes to slot lengths[b] - Ln + i, so lengths already count them.  The slots'
     weights become 0 where weights is given.  Rows before the first offset or after the last,
     and tokens whose slot is below 0, past the table or on no page, go nowhere, so that no
-    earlier token is lost; offsets are clamped to the tokens.  Two tokens on one place of a page (a page that two tables have) leave a mixture."""
+    earlier token is lost; offsets are clamped to the tokens.  Two tokens on one place of a
+    page (a page that two tables have) leave a mixture of both."""
     what = "paged_append"
     _no_gradient(what, k, v, k_pages, v_pages, weights)
     tables, lengths, offsets = _rows(tables), _rows(lengths), _rows(offsets)
